@@ -474,6 +474,60 @@ int spion_project_backward(const float* dY, const float* const* W, const float* 
  * of the key-mask entry points (models/attention_blockcuda_mask.py:42-43).  Returns 0 on success. */
 int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, int seq_len, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Attention with a learned bias by buckets of relative position (no counterpart in the reference, whose encoder
+ * adds position embeddings to its input, models/model_transformer.py:17-52).  Forward and backward of
+ *
+ *   v_ij = (q_i . k_j) / sqrt(d) + weight[buckets[clamp(j - i - offset, -R, R) + R]][h],   R = max_distance
+ *   P_ij = exp(v_ij) / Z_i,   Out_i = sum_j P_ij v_j
+ *
+ * fp32 or bf16 tensors, sums and softmax in fp32; the probabilities are never written.  Sizes come with every call; there is no
+ * handle, nothing is kept between calls, and the workspace is the caller's: calls with workspaces of their own may overlap.
+ *   heads        [B][H][L][d] tensors or views, strides in elements, multiples of 16 bytes; pointers 16-byte aligned; d = 32 or 64.
+ *                The strides of tensors that are only read may be 0 (a head shared by others).
+ *   weight       [num_buckets][heads], of the heads' type; dweight alike.
+ *   buckets      [2 R + 1] ints in 0 .. num_buckets - 1 (anything else is read as the nearest of them); 1 <= R <= 1024.
+ *   offset       query i stands at position i + offset of the keys' count.
+ *   key_mask     null, or [batch][k_len] floats (mask_bytes 4) or bytes (1): keys with a 0 are left out, and nothing of their K and V
+ *                is used.  A row without any key has an Out of 0 and no gradients.
+ *   mat          null: Z_i is the sum over all keys that take part.  Else [nb][nb] floats, nb = ceil(k_len / block_size): pairs
+ *                in blocks that are 0 have P = 0 but count in Z_i with a logit of 0, masked or not, as in the other sparse
+ *                families; block_size a multiple of 32, q_len = k_len, offset 0.
+ *   Lse          [batch * heads][q_len] fp32, out of the forward and into the backward: log2 Z_i, +infinity for empty rows.
+ *   OutLow       bf16 heads: null, or [batch * heads][q_len][head_dim] bf16, out of the forward and into the backward: what the
+ *                rounding of Out left.  The backward's row sums dO.Out are then those of the unrounded output; without it the
+ *                table's gradient, a sum over many rows that nearly cancel, is off by some 2^-8.  Not read for fp32 heads.
+ *   Mean         null, or [q_len][k_len] fp32, out: the mean of P over batch and heads (spion_pattern_generate's Score input);
+ *                not with mat.
+ *   workspace    spion_bias_workspace(call, backward) floats, contents unspecified; a forward without it walks long rows in one
+ *                piece.  The backward's gradients come out the same in every call with the same inputs.
+ * Each returns 0 on success (spion_bias_workspace: -1 on failure).
+ * ---------------------------------------------------------------------------------------------- */
+#define SPION_BIAS_MAX_DISTANCE 1024
+typedef struct spion_heads {
+    void* p;
+    long long batch_stride, head_stride, row_stride;
+} spion_heads;
+typedef struct spion_bias_attention {
+    spion_heads Q, K, V, Out;      /* Out: written by the forward, read by the backward */
+    spion_heads dO, dQ, dK, dV;    /* backward only */
+    const void* weight;
+    void* dweight;                 /* backward only */
+    const int* buckets;
+    const void* key_mask;
+    const float* mat;
+    float* Lse;
+    void* OutLow;
+    float* Mean;                   /* forward only */
+    float* workspace;
+    long long workspace_floats;
+    int batch, heads, q_len, k_len, head_dim, bf16;
+    int num_buckets, max_distance, offset, block_size, mask_bytes;
+} spion_bias_attention;
+long long spion_bias_workspace(const spion_bias_attention* call, int backward);
+int spion_bias_attention_forward(const spion_bias_attention* call, void* stream);
+int spion_bias_attention_backward(const spion_bias_attention* call, void* stream);
+
 const char* spion_version(void);
 
 #ifdef __cplusplus

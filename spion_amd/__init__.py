@@ -19,6 +19,7 @@ from .pattern import (
     generate_pattern_ff,
     mean_score_map,
 )
+from .relative_bias import RelativeBiasAttention, relative_bias_attention, relative_position_buckets
 
 __all__ = [
     "Attention",
@@ -42,4 +43,7 @@ __all__ = [
     "generate_pattern_conv_ff",
     "generate_pattern_ff",
     "mean_score_map",
+    "RelativeBiasAttention",
+    "relative_bias_attention",
+    "relative_position_buckets",
 ]

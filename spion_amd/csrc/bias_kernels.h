@@ -1,0 +1,533 @@
+// Attention with a learned bias by buckets of relative position: no counterpart in the reference (its encoder knows positions
+// only from embeddings, models/model_transformer.py:17-52).  With t_ij = (q_i . k_j / sqrt(d) + w[bucket(j - i - off)]) log2(e)
+//   forward   P_ij = exp2(t_ij - lse_i),  O = P V
+//   backward  dP = dO V^T,  D_i = dO_i . O_i,  dS = P (dP - D),  dQ = dS K / sqrt(d),  dK = dS^T Q / sqrt(d),  dV = P^T dO,
+//             dw[k] = sum of dS over the pairs of bucket k
+// P is never written: the forward leaves lse, the backward forms P again.  Keys whose mask is 0 are left out; with a block
+// pattern the keys off the pattern count with a logit of 0, as in models/block_attn.cu:70-72.
+//
+// The kernels here give a work-group one strip of 32 rows, which is the lane index of every accumulator, and its four wavefronts
+// every fourth tile of the strip's list; each stages its tiles in its own part of LDS, so nothing waits for a barrier inside
+// the walk, and long strips (a global block row, a single query over a long sample) are shared by four wavefronts and, in the
+// forward, by several work-groups.
+#pragma once
+#include "bias_tile.h"
+
+namespace spion {
+
+constexpr float BIAS_LAZY = 8.f;  // the running maximum is raised only when a tile exceeds it by 2^8
+
+// floats a piece of a forward strip leaves for the merge: the unscaled sums, maxima, denominators, keys of the pattern
+template <int D>
+constexpr int bias_slot() { return 32 * D + 96; }
+
+__device__ __forceinline__ int key_bit(unsigned word, int key) { return (word >> key) & 1u; }
+
+// t[r] = logits (log2 domain) of a tile whose keys are the accumulator rows, query on the lane.  One number for the bias of a
+// tile far from the strip; NEG: keys that are left out get -infinity.
+template <bool MASKED>
+__device__ __forceinline__ void logits_of(const f32x16& s, float c2, const float* tab, int R, int rel0, int li, int h,
+                                          unsigned word, float (&t)[16]) {
+    if (rel0 + 31 > -R && rel0 - 31 < R) {
+        const float* at = tab + rel0 + R + BIAS_PAD - li + 4 * h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t[r] = fmaf(s[r], c2, at[8 * (r >> 2) + (r & 3)]);
+    } else {
+        const float c = tab[rel0 > 0 ? 2 * (R + BIAS_PAD) : 0];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t[r] = fmaf(s[r], c2, c);
+    }
+    if (MASKED) {
+        const unsigned mine = word >> (4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t[r] = (mine >> (8 * (r >> 2) + (r & 3))) & 1u ? t[r] : -__builtin_inff();
+    }
+}
+
+// Work-group -> (sample, head, strip, piece): the strips of a head follow each other on one XCD.
+struct BiasItem {
+    int b, h, bh, strip, split;
+    __device__ __forceinline__ BiasItem(const BiasCall& a, int total) {
+        int i = xcd_remap(blockIdx.x, total);
+        split = i % a.splits;
+        i /= a.splits;
+        strip = i % a.strips;
+        bh = i / a.strips;
+        b = bh / a.H;
+        h = bh - b * a.H;
+    }
+};
+
+template <class T, int D>
+constexpr int bias_tiles_bytes() {
+    const int tiles = 4 * 2 * BiasTile<T, D>::BYTES, merge = merge_floats<D>() * 4;
+    return tiles > merge ? tiles : merge;
+}
+
+// Eighth j of row q of the output
+template <class T, int D>
+__device__ __forceinline__ void store_out(const BiasCall& a, int b, int h, int bh, int q, int j, float (&x)[D / 8]) {
+    store_values<T, D / 8>(const_cast<char*>(a.o.head(b, h)) + q * a.o.row + j * (D / 8) * sizeof(T), x);
+    if (sizeof(T) == 2 && a.low) {
+        rounded_off(x);
+        store_values<T, D / 8>(a.low + (((size_t)bh * a.Lq + q) * D + j * (D / 8)) * sizeof(T), x);
+    }
+}
+
+// -------------------------------------------------------------------------------------------------
+// Forward
+// -------------------------------------------------------------------------------------------------
+// FINE (bf16 heads, ahead of a backward): the probabilities enter the output with 2^-17, and what the rounding of the output
+// leaves is stored beside it.  The backward's D = dO.O has to be sum_j P_ij dP_ij for the P that it forms itself: the table's
+// gradient adds up P (dP - D) over thousands of rows whose terms nearly cancel, and with P and O rounded to bf16 in D the buckets
+// of far keys come out wrong by 0.8 % (28 heads of 2923 tokens, 8 buckets), against 0.16 % of rounding at the end.
+template <class T, int D, bool FINE>
+__global__ __launch_bounds__(256, 2) void bias_forward_kernel(BiasCall a) {
+    typedef BiasTile<T, D> TL;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
+    ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
+    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const BiasItem it(a, gridDim.x);
+    fill_bias<T>(a, it.h, tab, tid, 256);
+    const int q0 = it.strip * 32;
+    const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + min(q0 + li, a.Lq - 1) * a.q.row, h, q0 + li < a.Lq);
+    const char *kh = a.k.head(it.b, it.h), *vh = a.v.head(it.b, it.h);
+    const typename TL::At at = TL::at(l);
+    char* tk = lds + w * 2 * TL::BYTES;
+    char* tv = tk + TL::BYTES;
+    const float c2 = a.scale * LOG2E;
+    const int qpos = q0 + a.off;
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) o[c] = splat16(0.f);
+    float m = -__builtin_inff(), z = 0.f;
+    int in_pattern = 0;
+    const int tiles = (a.Lk + 31) / 32;
+    const int t0 = it.split * a.per_split, t1 = min(tiles, t0 + a.per_split);
+    for (int first = t0; first < t1; first += CHUNK) {
+        const int n = scan_chunk<true>(a, sc, it.b, it.strip, first, min(CHUNK, t1 - first), tid, in_pattern);
+        TileInFlight<T, D> fk, fv;
+        auto fetch = [&](int i) __attribute__((always_inline)) {
+            const int j = (first + sc.list[i]) * 32;
+            fk.load(kh, a.k.row, j, a.Lk, l);
+            fv.load(vh, a.v.row, j, a.Lk, l);
+        };
+        if (w < n) fetch(w);
+        for (int i = w; i < n; i += 4) {
+            const int tile = uniform(sc.list[i]);
+            const unsigned word = uniform(sc.words[tile]);
+            wave_lds_order();
+            fk.store(tk, word, l);
+            fv.store(tv, word, l);
+            wave_lds_order();
+            if (i + 4 < n) fetch(i + 4);
+            const f32x16 s = TL::feat(TL::rows(tk, at), q);
+            float t[16];
+            const int rel0 = (first + tile) * 32 - qpos;
+            if (word == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word, t);
+            else logits_of<true>(s, c2, tab, a.R, rel0, li, h, word, t);
+            float mt = t[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mt = fmaxf(mt, t[r]);
+            mt = half_swap_max(mt);
+            if (__any(mt > m + BIAS_LAZY)) {
+                const float up = fmaxf(m, mt);
+                const float f = up == m ? 1.f : __builtin_amdgcn_exp2f(m - up);  // equal: also -infinity twice
+                m = up;
+                z *= f;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[c][r] *= f;
+            }
+            const float base = m == -__builtin_inff() ? 0.f : m;
+            float p[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                p[r] = __builtin_amdgcn_exp2f(t[r] - base);
+                z += p[r];
+            }
+            if constexpr (FINE) TL::add_t_fine(tv, at, p, o);
+            else TL::add_t(tv, at, p, o);
+        }
+    }
+    // the four wavefronts' parts
+    z = half_swap_sum(z);
+    if (h == 0) {
+        sc.ml[w][0][li] = m;
+        sc.ml[w][1][li] = z;
+    }
+    __syncthreads();
+    float M = sc.ml[0][0][li];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) M = fmaxf(M, sc.ml[k][0][li]);
+    const float base = M == -__builtin_inff() ? 0.f : M;
+    float Z = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) Z += sc.ml[k][1][li] * __builtin_amdgcn_exp2f(sc.ml[k][0][li] - base);
+    const float f = __builtin_amdgcn_exp2f(m - base);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[c][r] *= f;
+    float x[D / 8];
+    merge_waves<D>(o, reinterpret_cast<float*>(lds), tid, x);
+    const int row = tid >> 3, j = tid & 7;
+    if (a.splits > 1) {
+        float* slot = a.part + (size_t)((it.bh * (size_t)a.strips + it.strip) * a.splits + it.split) * bias_slot<D>();
+        store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
+        if (w == 0 && h == 0) {
+            slot[32 * D + li] = M;
+            slot[32 * D + 32 + li] = Z;
+            slot[32 * D + 64 + li] = __builtin_bit_cast(float, in_pattern);
+        }
+        return;
+    }
+    if (w == 0 && h == 0) {
+        const int off = a.mat ? a.Lk - in_pattern : 0;  // keys off the pattern: a logit of 0 each
+        float scale = 1.f;
+        if (off > 0) {
+            const float up = fmaxf(M, 0.f);
+            scale = __builtin_amdgcn_exp2f(M - up);
+            Z = Z * scale + off * __builtin_amdgcn_exp2f(-up);
+            M = up;
+        }
+        sc.row[li] = Z > 0.f ? scale / Z : 0.f;
+        if (q0 + li < a.Lq)
+            a.lse[(size_t)it.bh * a.Lq + q0 + li] = Z > 0.f ? M + __builtin_amdgcn_logf(Z) : __builtin_inff();
+    }
+    __syncthreads();
+    if (q0 + row < a.Lq) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) x[i] *= sc.row[row];
+        store_out<T, D>(a, it.b, it.h, it.bh, q0 + row, j, x);
+    }
+}
+
+// The pieces of a strip, in their order.
+template <class T, int D>
+__global__ __launch_bounds__(256) void bias_merge_kernel(BiasCall a) {
+    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7;
+    const int strip = blockIdx.x % a.strips, bh = blockIdx.x / a.strips, b = bh / a.H, ih = bh - b * a.H;
+    const float* slot = a.part + (size_t)blockIdx.x * a.splits * bias_slot<D>();
+    float M = -__builtin_inff();
+    int in_pattern = 0;
+    for (int k = 0; k < a.splits; ++k) {
+        M = fmaxf(M, slot[k * bias_slot<D>() + 32 * D + row]);
+        in_pattern += __builtin_bit_cast(int, slot[k * bias_slot<D>() + 32 * D + 64 + row]);
+    }
+    const int off = a.mat ? a.Lk - in_pattern : 0;
+    if (off > 0) M = fmaxf(M, 0.f);
+    const float base = M == -__builtin_inff() ? 0.f : M;
+    float Z = off > 0 ? off * __builtin_amdgcn_exp2f(-base) : 0.f, x[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
+    for (int k = 0; k < a.splits; ++k) {
+        const float* s = slot + k * bias_slot<D>();
+        const float f = __builtin_amdgcn_exp2f(s[32 * D + row] - base);
+        Z += s[32 * D + 32 + row] * f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(s + row * D + j * (D / 8) + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e] * f;
+        }
+    }
+    const int q = strip * 32 + row;
+    if (q >= a.Lq) return;
+    const float inv = Z > 0.f ? 1.f / Z : 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) x[i] *= inv;
+    store_out<T, D>(a, b, ih, bh, q, j, x);
+    if (j == 0) a.lse[(size_t)bh * a.Lq + q] = Z > 0.f ? M + __builtin_amdgcn_logf(Z) : __builtin_inff();
+}
+
+// -------------------------------------------------------------------------------------------------
+// Backward, strips of queries: dQ, D and the table's gradient
+// -------------------------------------------------------------------------------------------------
+// The table's gradient: a tile's dS of one accumulator register are 32 consecutive differences to either half-wave, so a tile that
+// touches (-R, R) adds its registers to a histogram by difference in LDS, one for each half-wave of each wavefront (no two lanes
+// of an instruction meet, and every histogram is added to in program order: the sums come out the same each time); of the others
+// only the sum is needed, which stays in a register.  The histograms of a strip are added up, folded into buckets and left
+// in the workspace, [strips][buckets] for every head.
+constexpr int BIAS_HISTS = 8;
+__device__ __forceinline__ void hist_add(float* at, float x) {
+    __hip_atomic_fetch_add(at, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void bias_backward_row_kernel(BiasCall a) {
+    typedef BiasTile<T, D> TL;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
+    ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
+    float* hist = reinterpret_cast<float*>(&sc + 1);
+    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const BiasItem it(a, gridDim.x);
+    const int entries = bias_entries(a.R);
+    fill_bias<T>(a, it.h, tab, tid, 256);
+    for (int i = tid; i < BIAS_HISTS * entries; i += 256) hist[i] = 0.f;
+    const int q0 = it.strip * 32, qi = min(q0 + li, a.Lq - 1);
+    const bool there = q0 + li < a.Lq;
+    const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + qi * a.q.row, h, there);
+    const typename TL::Row go = TL::load(a.dout.head(it.b, it.h) + qi * a.dout.row, h, there);
+    const size_t stat = (size_t)it.bh * a.Lq + qi;
+    const float lse = there ? a.lse[stat] : __builtin_inff();
+    float delta = TL::dot(go, TL::load(a.o.head(it.b, it.h) + qi * a.o.row, h, there));
+    if (sizeof(T) == 2 && a.low) delta += TL::dot(go, TL::load(a.low + stat * D * sizeof(T), h, there));
+    delta = half_swap_sum(delta);
+    if (w == 0 && h == 0 && there) a.delta[stat] = delta;
+    const char *kh = a.k.head(it.b, it.h), *vh = a.v.head(it.b, it.h);
+    const typename TL::At at = TL::at(l);
+    char* tk = lds + w * 2 * TL::BYTES;
+    char* tv = tk + TL::BYTES;
+    const float c2 = a.scale * LOG2E;
+    const int qpos = q0 + a.off;
+    float* mine = hist + (2 * w + h) * entries + a.R + BIAS_PAD - li + 4 * h;
+
+    f32x16 dq[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
+    float behind = 0.f, ahead = 0.f;
+    int in_pattern = 0;
+    const int tiles = (a.Lk + 31) / 32;
+    for (int first = 0; first < tiles; first += CHUNK) {
+        const int n = scan_chunk<true>(a, sc, it.b, it.strip, first, min(CHUNK, tiles - first), tid, in_pattern);
+        TileInFlight<T, D> fk, fv;
+        auto fetch = [&](int i) __attribute__((always_inline)) {
+            const int j = (first + sc.list[i]) * 32;
+            fk.load(kh, a.k.row, j, a.Lk, l);
+            fv.load(vh, a.v.row, j, a.Lk, l);
+        };
+        if (w < n) fetch(w);
+        for (int i = w; i < n; i += 4) {
+            const int tile = uniform(sc.list[i]);
+            const unsigned word = uniform(sc.words[tile]);
+            wave_lds_order();
+            fk.store(tk, word, l);
+            fv.store(tv, word, l);
+            wave_lds_order();
+            if (i + 4 < n) fetch(i + 4);
+            const f32x16 s = TL::feat(TL::rows(tk, at), q);
+            const f32x16 dp = TL::feat(TL::rows(tv, at), go);
+            float t[16];
+            const int rel0 = (first + tile) * 32 - qpos;
+            if (word == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word, t);
+            else logits_of<true>(s, c2, tab, a.R, rel0, li, h, word, t);
+            float ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(t[r] - lse) * (dp[r] - delta);
+            if (rel0 + 31 > -a.R && rel0 - 31 < a.R) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) hist_add(mine + rel0 + 8 * (r >> 2) + (r & 3), ds[r]);
+            } else {
+                float sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum += ds[r];
+                if (rel0 > 0) ahead += sum;
+                else behind += sum;
+            }
+            TL::add_t(tk, at, ds, dq);
+        }
+    }
+    __syncthreads();  // the tiles are done with
+    behind = wave_sum(behind);
+    ahead = wave_sum(ahead);
+    if (l == 0) {
+        hist[2 * w * entries] += behind;
+        hist[2 * w * entries + entries - 1] += ahead;
+    }
+    float x[D / 8];
+    merge_waves<D>(dq, reinterpret_cast<float*>(lds), tid, x);
+    const int row = tid >> 3, j = tid & 7;
+    if (q0 + row < a.Lq) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) x[i] *= a.scale;
+        store_values<T, D / 8>(const_cast<char*>(a.dq.head(it.b, it.h)) + (q0 + row) * a.dq.row + j * (D / 8) * sizeof(T), x);
+    }
+    // the eight histograms into the first, then by buckets: eight threads to a bucket, each every eighth entry
+    for (int i = tid; i < entries; i += 256) {
+        float s = hist[i];
+#pragma unroll
+        for (int k = 1; k < BIAS_HISTS; ++k) s += hist[k * entries + i];
+        hist[i] = s;
+    }
+    __syncthreads();
+    for (int k0 = 0; k0 < a.buckets; k0 += 32) {
+        const int k = k0 + (tid >> 3);
+        float s = 0.f;
+        if (k < a.buckets)
+            for (int i = tid & 7; i < entries; i += 8)
+                if (bucket_at(a, i - a.R - BIAS_PAD) == k) s += hist[i];
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor(s, o, 64);
+        if (k < a.buckets && (tid & 7) == 0)
+            a.part[((size_t)it.bh * a.strips + it.strip) * a.buckets + k] = s;
+    }
+}
+
+// dw[k][h]: the strips of all samples, 256 partial sums in a fixed order.
+template <class T>
+__global__ __launch_bounds__(256) void bias_table_kernel(BiasCall a, T* __restrict__ dw) {
+    __shared__ float red[4];
+    const int k = blockIdx.x % a.buckets, h = blockIdx.x / a.buckets, tid = threadIdx.x;
+    const int n = a.B * a.strips;
+    float s = 0.f;
+    for (int i = tid; i < n; i += 256) {
+        const int b = i / a.strips, strip = i - b * a.strips;
+        s += a.part[(((size_t)b * a.H + h) * a.strips + strip) * a.buckets + k];
+    }
+    s = wave_sum(s);
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    __syncthreads();
+    if (tid == 0) dw[(size_t)k * a.H + h] = (T)(red[0] + red[1] + red[2] + red[3]);
+}
+
+// -------------------------------------------------------------------------------------------------
+// Backward, strips of keys: dK and dV
+// -------------------------------------------------------------------------------------------------
+// The strip's keys are the lanes: what a key that is left out holds reaches its own lane only, whose results are zeros.
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void bias_backward_col_kernel(BiasCall a) {
+    typedef BiasTile<T, D> TL;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
+    ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
+    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const BiasItem it(a, gridDim.x);
+    fill_bias<T>(a, it.h, tab, tid, 256);
+    const int k0 = it.strip * 32, ki = min(k0 + li, a.Lk - 1);
+    const typename TL::Row k = TL::load(a.k.head(it.b, it.h) + ki * a.k.row, h, k0 + li < a.Lk);
+    const typename TL::Row v = TL::load(a.v.head(it.b, it.h) + ki * a.v.row, h, k0 + li < a.Lk);
+    const unsigned keys = (unsigned)__ballot(key_there(a, it.b, k0 + li));
+    const char *qh = a.q.head(it.b, it.h), *gh = a.dout.head(it.b, it.h);
+    const float *lseh = a.lse + (size_t)it.bh * a.Lq, *deltah = a.delta + (size_t)it.bh * a.Lq;
+    const typename TL::At at = TL::at(l);
+    char* tq = lds + w * 2 * TL::BYTES;
+    char* tg = tq + TL::BYTES;
+    float* stats = sc.ml[w][0];  // lse of the tile's 32 queries, then their D
+    const float c2 = a.scale * LOG2E;
+
+    f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = splat16(0.f);
+    int in_pattern = 0;
+    const int tiles = keys == 0 ? 0 : (a.Lq + 31) / 32;  // the same in every thread
+    for (int first = 0; first < tiles; first += CHUNK) {
+        const int n = scan_chunk<false>(a, sc, it.b, it.strip, first, min(CHUNK, tiles - first), tid, in_pattern);
+        TileInFlight<T, D> fq, fg;
+        float st = 0.f;
+        auto fetch = [&](int i) __attribute__((always_inline)) {
+            const int r = (first + sc.list[i]) * 32;
+            fq.load(qh, a.q.row, r, a.Lq, l);
+            fg.load(gh, a.dout.row, r, a.Lq, l);
+            st = r + li < a.Lq ? (h ? deltah : lseh)[r + li] : (h ? 0.f : __builtin_inff());
+        };
+        if (w < n) fetch(w);
+        for (int i = w; i < n; i += 4) {
+            const int tile = uniform(sc.list[i]);
+            const int r0 = (first + tile) * 32;
+            const unsigned word = a.Lq - r0 >= 32 ? ~0u : (1u << (a.Lq - r0)) - 1u;
+            wave_lds_order();
+            fq.store(tq, word, l);
+            fg.store(tg, word, l);
+            stats[l] = st;
+            wave_lds_order();
+            if (i + 4 < n) fetch(i + 4);
+            const f32x16 s = TL::feat(TL::rows(tq, at), k);
+            const f32x16 dp = TL::feat(TL::rows(tg, at), v);
+            const int rel0 = k0 - r0 - a.off;  // of the tile's corner: lane li, row r has rel0 + li - r
+            float p[16];
+            if (rel0 + 31 > -a.R && rel0 - 31 < a.R) {
+                const float* bias = tab + rel0 + a.R + BIAS_PAD + li - 4 * h;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] = fmaf(s[r], c2, bias[-(8 * (r >> 2) + (r & 3))]);
+            } else {
+                const float c = tab[rel0 > 0 ? 2 * (a.R + BIAS_PAD) : 0];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] = fmaf(s[r], c2, c);
+            }
+            float ds[16];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 e = *reinterpret_cast<const f32x4*>(stats + 8 * g + 4 * h);
+                const f32x4 d = *reinterpret_cast<const f32x4*>(stats + 32 + 8 * g + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[4 * g + j] = __builtin_amdgcn_exp2f(p[4 * g + j] - e[j]);
+                    ds[4 * g + j] = p[4 * g + j] * (dp[4 * g + j] - d[j]);
+                }
+            }
+            TL::add_t(tg, at, p, dv);
+            TL::add_t(tq, at, ds, dk);
+        }
+    }
+    __syncthreads();
+    const int row = tid >> 3, j = tid & 7;
+    const bool keep = key_bit(keys, row);
+    float x[D / 8];
+    merge_waves<D>(dv, reinterpret_cast<float*>(lds), tid, x);
+    if (k0 + row < a.Lk) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) x[i] = keep ? x[i] : 0.f;
+        store_values<T, D / 8>(const_cast<char*>(a.dv.head(it.b, it.h)) + (k0 + row) * a.dv.row + j * (D / 8) * sizeof(T), x);
+    }
+    __syncthreads();
+    merge_waves<D>(dk, reinterpret_cast<float*>(lds), tid, x);
+    if (k0 + row < a.Lk) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) x[i] = keep ? x[i] * a.scale : 0.f;
+        store_values<T, D / 8>(const_cast<char*>(a.dk.head(it.b, it.h)) + (k0 + row) * a.dk.row + j * (D / 8) * sizeof(T), x);
+    }
+}
+
+// -------------------------------------------------------------------------------------------------
+// Mean probability map of all samples and heads
+// -------------------------------------------------------------------------------------------------
+// A work-group has one 32 x 32 tile of the map and its wavefronts every fourth (sample, head); probabilities are formed from the
+// forward's lse, added up in registers and never written.
+template <class T, int D>
+__global__ __launch_bounds__(256) void bias_mean_kernel(BiasCall a) {
+    typedef BiasTile<T, D> TL;
+    __shared__ float red[4][16][64];
+    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const int kt = (a.Lk + 31) / 32, tile = xcd_remap(blockIdx.x, gridDim.x);
+    const int q0 = tile / kt * 32, k0 = tile % kt * 32;
+    const int qi = min(q0 + li, a.Lq - 1), ki = min(k0 + li, a.Lk - 1);
+    const float c2 = a.scale * LOG2E;
+    int bucket[16];  // of (query row r, key li)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bucket[r] = bucket_at(a, k0 + li - (q0 + acc_row(r, h)) - a.off) * a.H;
+    float sum[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[r] = 0.f;
+    for (int bh = w; bh < a.B * a.H; bh += 4) {
+        const int b = bh / a.H, ih = bh - b * a.H;
+        const bool key = key_there(a, b, k0 + li);
+        if (!__any(key)) continue;
+        const typename TL::Row q = TL::load(a.q.head(b, ih) + qi * a.q.row, h, q0 + li < a.Lq);
+        const typename TL::Row k = TL::load(a.k.head(b, ih) + ki * a.k.row, h, key);
+        const f32x16 s = TL::feat(q, k);
+        const float* lse = a.lse + (size_t)bh * a.Lq;
+        const T* wh = reinterpret_cast<const T*>(a.w) + ih;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float t = fmaf(s[r], c2, (float)wh[bucket[r]] * LOG2E - lse[min(q0 + acc_row(r, h), a.Lq - 1)]);
+            sum[r] += key ? __builtin_amdgcn_exp2f(t) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) red[w][r][l] = sum[r];
+    __syncthreads();
+    const float inv = 1.f / (a.B * a.H);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = 4 * w + i, qr = q0 + acc_row(r, h);
+        const float v = (red[0][r][l] + red[1][r][l]) + (red[2][r][l] + red[3][r][l]);
+        if (qr < a.Lq && k0 + li < a.Lk) a.mean[(size_t)qr * a.Lk + k0 + li] = v * inv;
+    }
+}
+
+}  // namespace spion

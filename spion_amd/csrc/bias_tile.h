@@ -1,0 +1,359 @@
+// What the kernels of the attention with a relative position bias share (bias_kernels.h): 32 x D tiles in LDS for bf16 and fp32
+// and the matrix operands read from them, the bias table of a head, and the list of the tiles a strip has to visit.
+#pragma once
+#include "bf16_kernels.h"
+
+namespace spion {
+
+// Heads of one tensor, [B][H][L][D] by strides in bytes.
+struct HeadsAt {
+    const char* p;
+    long long b, h, row;
+    __device__ __forceinline__ const char* head(int ib, int ih) const { return p + ib * b + ih * h; }
+};
+
+struct BiasCall {
+    HeadsAt q, k, v, o, dout, dq, dk, dv;
+    const void* w;      // [buckets][H], of the heads' type
+    const int* map;     // [2 R + 1]: bucket of every difference -R .. R
+    const void* mask;   // [B][Lk]: null, float (0 = left out) or bytes
+    const float* mat;   // [nb][nb] pattern of bs x bs blocks, or null
+    float* lse;         // [B*H][Lq]: log2 of the softmax denominator, +inf for rows that nothing enters
+    char* low;          // [B*H][Lq][D] bf16 or null: O before its rounding less O
+    float* delta;       // [B*H][Lq]: dO . O
+    float* part;        // workspace
+    float* mean;        // [Lq][Lk]
+    int B, H, Lq, Lk, R, buckets, off, bs, nb;
+    int mask_bytes;     // 4 or 1
+    int strips, splits, per_split;  // strips of 32 (or 128) rows, pieces of the other side, tiles of 32 to a piece
+    float scale;
+};
+
+// ---------------------------------------------------------------------------------------------------------------------
+// 32 x D tiles
+// ---------------------------------------------------------------------------------------------------------------------
+// Rows are stored as 16-byte pieces, piece c of row r at c ^ swz(r).  rows(): lane (li, h) has features h*D/2 .. of row li, the
+// operand of a product over the head dimension.  add_t(): out[c] += X^T . W, W given as the accumulator values of a 32 x 32
+// product whose rows are the tile's rows; the accumulator layout is then the other operand's, register for register (bf16: after
+// conversion).  W's rounding to bf16 is off by up to 2^-8 of each weight, as the outputs' own is; sums are fp32.
+template <class T, int D>
+struct BiasTile;
+
+template <int D>
+struct BiasTile<__bf16, D> {
+    typedef DmaTile<D> DT;
+    static constexpr int ROW = DT::ROW, BYTES = DT::TILE, CPR = DT::CPR;
+    struct Row {
+        bf16x8 x[D / 16];
+    };
+    struct At {
+        typename DT::RowAddr ra;
+        typename DT::TrAddr ta;
+    };
+    __device__ static __forceinline__ At at(int l) { return At{DT::row_addr(l & 31, l >> 5), DT::tr_addr(l)}; }
+    __device__ static __forceinline__ int swz(int r) { return DT::swz(r); }
+    __device__ static __forceinline__ Row rows(const char* t, const At& a) {
+        Row r;
+        DT::get_rows(t, a.ra, r.x);
+        return r;
+    }
+    // row `row` of a head, from global memory; zeros where `there` is false
+    __device__ static __forceinline__ Row load(const char* row, int h, bool there) {
+        Row r;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            u32x4 v = {0, 0, 0, 0};
+            if (there) v = *reinterpret_cast<const u32x4*>(row + h * D + 16 * i);
+            r.x[i] = __builtin_bit_cast(bf16x8, v);
+        }
+        return r;
+    }
+    __device__ static __forceinline__ float dot(const Row& a, const Row& b) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf((float)a.x[i][e], (float)b.x[i][e], s);
+        return s;
+    }
+    __device__ static __forceinline__ f32x16 feat(const Row& a, const Row& b) {
+        f32x16 acc = {0};
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) acc = mfma_bf16(a.x[i], b.x[i], acc);
+        return acc;
+    }
+    __device__ static __forceinline__ void add_t(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
+        bf16x8 xt[D / 32][2], wb[2];
+        DT::get_tile_t(t, a.ta, xt);
+        pack16(p, wb);
+        mma_tile_bf16<D>(xt, wb, out);
+    }
+    // the same with W to 2^-17: what its rounding leaves, rounded once more, in products of its own
+    __device__ static __forceinline__ void add_t_fine(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
+        bf16x8 xt[D / 32][2], wb[2];
+        DT::get_tile_t(t, a.ta, xt);
+        float low[16];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            u32x4 u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 8 * i + 2 * e;
+                u[e] = pack_bf16(p[r], p[r + 1]);
+                low[r] = p[r] - bf16_lo(u[e]);
+                low[r + 1] = p[r + 1] - bf16_hi(u[e]);
+            }
+            wb[i] = __builtin_bit_cast(bf16x8, u);
+        }
+        mma_tile_bf16<D>(xt, wb, out);
+        pack16(low, wb);
+        mma_tile_bf16<D>(xt, wb, out);
+    }
+};
+
+template <int D>
+struct BiasTile<float, D> {
+    static constexpr int ROW = D * 4, BYTES = 32 * ROW, CPR = D / 4;
+    struct Row {
+        float x[D / 2];
+    };
+    struct At {
+        int row, sw;         // of the row operand
+        int col, lane4, h4;  // of the transposed one
+    };
+    __device__ static __forceinline__ At at(int l) {
+        const int li = l & 31, h = l >> 5;
+        return At{li * ROW, swz(li), li >> 2, 4 * (li & 3), 4 * h};
+    }
+    __device__ static __forceinline__ int swz(int r) { return r & (CPR - 1); }
+    __device__ static __forceinline__ Row rows_of(const char* t, const At& a, int h) {
+        Row r;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(t + a.row + 16 * ((h * (CPR / 2) + i) ^ a.sw));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.x[4 * i + e] = v[e];
+        }
+        return r;
+    }
+    __device__ static __forceinline__ Row rows(const char* t, const At& a) { return rows_of(t, a, a.h4 >> 2); }
+    __device__ static __forceinline__ Row load(const char* row, int h, bool there) {
+        Row r;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            f32x4 v = {0, 0, 0, 0};
+            if (there) v = *reinterpret_cast<const f32x4*>(row + h * (2 * D) + 16 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.x[4 * i + e] = v[e];
+        }
+        return r;
+    }
+    __device__ static __forceinline__ float dot(const Row& a, const Row& b) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) s = fmaf(a.x[i], b.x[i], s);
+        return s;
+    }
+    __device__ static __forceinline__ f32x16 feat(const Row& a, const Row& b) { return mma_feat<D>(a.x, b.x); }
+    __device__ static __forceinline__ void add_t(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            float x[16];
+#pragma unroll
+            for (int s = 0; s < 16; ++s) {
+                const int row = 8 * (s >> 2) + (s & 3);  // and 4 h
+                const int sw = ((row & (CPR - 1)) ^ (a.h4 & (CPR - 1)));  // row + 4 h = row | 4 h: the bits are apart
+                x[s] = *reinterpret_cast<const float*>(t + (row + a.h4) * ROW + 16 * ((8 * c + a.col) ^ sw) + a.lane4);
+            }
+            out[c] = mma_chain(x, p, out[c]);
+        }
+    }
+    __device__ static __forceinline__ void add_t_fine(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
+        add_t(t, a, p, out);
+    }
+};
+
+// A wavefront's tile on its way from global memory to LDS: 16-byte piece n = 64 i + l of the tile is piece n % CPR of row n / CPR.
+template <class T, int D>
+struct TileInFlight {
+    typedef BiasTile<T, D> TL;
+    static constexpr int N = TL::CPR / 2;
+    u32x4 x[N];
+    // rows first .. first + 31 of a head of `rows` rows; behind its end the last one again, which store() leaves out
+    __device__ __forceinline__ void load(const char* head, long long ld, int first, int rows, int l) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int n = 64 * i + l, r = n / TL::CPR, c = n % TL::CPR;
+            x[i] = *reinterpret_cast<const u32x4*>(head + min(first + r, rows - 1) * ld + 16 * c);
+        }
+    }
+    // to LDS; rows whose bit of `word` is not set become zeros (whatever lies in a key that is left out: 0 times it is 0)
+    __device__ __forceinline__ void store(char* t, unsigned word, int l) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int n = 64 * i + l, r = n / TL::CPR, c = n % TL::CPR;
+            u32x4 v = x[i];
+            if (!((word >> r) & 1u)) v = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(t + r * TL::ROW + 16 * (c ^ TL::swz(r))) = v;
+        }
+    }
+};
+
+// Orders a wavefront's own LDS accesses (they complete in order; this is for the compiler).
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// The bias
+// ---------------------------------------------------------------------------------------------------------------------
+// A head's bias by position difference, log2 domain: entry i is difference i - R - BIAS_PAD; differences beyond R on either
+// side have the outermost buckets.  The padding is what tiles that touch (-R, R) reach beyond it (62), so their look-ups need
+// no clamping; tiles further out take one number for all their pairs.
+constexpr int BIAS_PAD = 64;
+__host__ __device__ inline int bias_entries(int R) { return 2 * (R + BIAS_PAD) + 1; }
+__host__ __device__ inline int bias_floats(int R) { return (bias_entries(R) + 3) & ~3; }
+
+__device__ __forceinline__ int bucket_at(const BiasCall& a, int diff) {
+    const int k = a.map[min(max(diff, -a.R), a.R) + a.R];
+    return min(max(k, 0), a.buckets - 1);
+}
+template <class T>
+__device__ __forceinline__ float bias_weight(const BiasCall& a, int bucket, int h) {
+    return (float)reinterpret_cast<const T*>(a.w)[(size_t)bucket * a.H + h] * LOG2E;
+}
+template <class T>
+__device__ __forceinline__ void fill_bias(const BiasCall& a, int h, float* tab, int tid, int threads) {
+    for (int i = tid; i < bias_entries(a.R); i += threads) tab[i] = bias_weight<T>(a, bucket_at(a, i - a.R - BIAS_PAD), h);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Tiles to visit
+// ---------------------------------------------------------------------------------------------------------------------
+// The other side of a strip is walked in chunks of CHUNK tiles of 32.  For a chunk the work-group makes, in LDS, the list of
+// the tiles that the strip has to visit, in order: those of the pattern that have a key which takes part.  words: which keys of
+// each tile do.  Everything is read from the mask and the pattern as they are at the call.
+constexpr int CHUNK = 512;
+struct ScanLds {
+    unsigned words[CHUNK];
+    unsigned short list[CHUNK];
+    int seg[8], pat[8];
+    float ml[4][2][32];
+    float row[32];
+};
+
+__device__ __forceinline__ bool key_there(const BiasCall& a, int b, int key) {
+    if (key >= a.Lk) return false;
+    if (a.mask == nullptr) return true;
+    const size_t i = (size_t)b * a.Lk + key;
+    return a.mask_bytes == 4 ? reinterpret_cast<const float*>(a.mask)[i] != 0.f : reinterpret_cast<const unsigned char*>(a.mask)[i] != 0;
+}
+
+// Tiles first .. first + count - 1 (count <= CHUNK) of the other side, for strip `own` of 32 rows.  KEYS: the other side is the
+// keys, else the queries.  Returns how many are listed; in_pattern grows by the keys of the pattern's tiles.  All threads of
+// the work-group call it; LDS that they still read must be done with.
+template <bool KEYS>
+__device__ __forceinline__ int scan_chunk(const BiasCall& a, ScanLds& s, int b, int own, int first, int count, int tid,
+                                          int& in_pattern) {
+    const int w = tid >> 6, l = tid & 63;
+    __syncthreads();
+    if (KEYS) {
+        for (int g = w; g < (count + 1) / 2; g += 4) {
+            const unsigned long long there = __ballot(key_there(a, b, (first + 2 * g) * 32 + l));
+            if (l == 0) {
+                s.words[2 * g] = (unsigned)there;
+                if (2 * g + 1 < CHUNK) s.words[2 * g + 1] = (unsigned)(there >> 32);
+            }
+        }
+        __syncthreads();
+    }
+    bool act[2];
+    unsigned long long votes[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int i = tid + 256 * r, tile = first + i;
+        bool in = i < count;
+        if (in && a.mat) {
+            const int o = own * 32 / a.bs, t = tile * 32 / a.bs;
+            in = a.mat[KEYS ? (size_t)o * a.nb + t : (size_t)t * a.nb + o] != 0.f;
+        }
+        const unsigned long long pat = __ballot(in);
+        const unsigned long long tail = KEYS ? __ballot(in && tile * 32 + 32 > a.Lk) : 0;
+        act[r] = in && (!KEYS || s.words[i] != 0);
+        votes[r] = __ballot(act[r]);
+        if (l == 0) {
+            s.seg[4 * r + w] = __popcll(votes[r]);
+            s.pat[4 * r + w] = 32 * __popcll(pat) - (tail ? 32 - (a.Lk & 31) : 0);
+        }
+    }
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        int before = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) before += k < 4 * r + w ? s.seg[k] : 0;
+        if (act[r]) s.list[before + __popcll(votes[r] & ((1ull << l) - 1))] = (unsigned short)(tid + 256 * r);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        total += s.seg[k];
+        in_pattern += s.pat[k];
+    }
+    __syncthreads();
+    return total;
+}
+
+// Wavefronts' 32 x D results acc[c][r] (lane (li, h): row li, feature 32 c + acc_row(r, h)) added up in the wavefronts' order in LDS
+// (4 x 32 x (D + 4) floats).  Afterwards thread t has the sums of features 8 j .. of row t / 8, j = t % 8 + 8 n, in x[n].
+template <int D>
+constexpr int merge_floats() { return 4 * 32 * (D + 4); }
+template <int D>
+__device__ __forceinline__ void merge_waves(const f32x16 (&acc)[D / 32], float* red, int tid, float (&x)[D / 8]) {
+    const int w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    float* mine = red + (w * 32 + li) * (D + 4);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(mine + 32 * c + 8 * g + 4 * h) =
+                f32x4{acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]};
+    __syncthreads();
+    const int row = tid >> 3, j = tid & 7;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(red + (k * 32 + row) * (D + 4) + j * (D / 8) + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e];
+        }
+}
+// What the rounding of x to bf16 leaves of it.
+template <int N>
+__device__ __forceinline__ void rounded_off(float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] -= (float)(__bf16)x[i];
+}
+// D / 8 consecutive values to memory, rounded once
+template <class T, int N>
+__device__ __forceinline__ void store_values(char* p, const float (&x)[N]) {
+    T* t = reinterpret_cast<T*>(p);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) *reinterpret_cast<f32x4*>(t + 4 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            bf16x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (__bf16)x[4 * i + e];
+            *reinterpret_cast<bf16x4*>(t + 4 * i) = v;
+        }
+    }
+}
+
+}  // namespace spion

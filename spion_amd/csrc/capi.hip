@@ -126,6 +126,9 @@ int project_backward_input(const float*, const float* const*, float*, long long,
 long long project_workspace(long long, int, int);
 int project_backward_weight(const float*, const float*, float*, float*, float*, long long, int, int, hipStream_t);
 int project_backward(const float*, const float* const*, const float*, float*, float*, float*, float*, long long, int, int, int, hipStream_t);
+long long bias_workspace(const spion_bias_attention*, int);
+int bias_forward(const spion_bias_attention*, hipStream_t);
+int bias_backward(const spion_bias_attention*, hipStream_t);
 int key_penalty(const float*, float*, int, int, int, hipStream_t);
 int pattern_generate_maps(const float* const*, int, int, int, int, int, double, float*, int, float*, float*, hipStream_t);
 int score_map_mean(const float*, int, int, int, int, float*, hipStream_t, float post = 1.0f);
@@ -302,6 +305,20 @@ int spion_project_backward(const float* dY, const float* const* W, const float* 
 int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, int seq_len, void* stream) {
     note_current_handle(nullptr);
     return key_penalty(mask, penalty, batch, heads, seq_len, static_cast<hipStream_t>(stream));
+}
+
+// ---- attention with a bias by relative position ---------------------------------------------------
+long long spion_bias_workspace(const spion_bias_attention* call, int backward) {
+    note_current_handle(nullptr);
+    return bias_workspace(call, backward);
+}
+int spion_bias_attention_forward(const spion_bias_attention* call, void* stream) {
+    note_current_handle(nullptr);
+    return bias_forward(call, static_cast<hipStream_t>(stream));
+}
+int spion_bias_attention_backward(const spion_bias_attention* call, void* stream) {
+    note_current_handle(nullptr);
+    return bias_backward(call, static_cast<hipStream_t>(stream));
 }
 
 // ---- pattern discovery ---------------------------------------------------------------------------

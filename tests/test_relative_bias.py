@@ -1,0 +1,110 @@
+"""Relative position buckets and what the bias operators refuse, without a GPU."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import spion_amd
+from spion_amd import _lib
+from spion_amd import relative_bias as rb
+
+
+@pytest.mark.parametrize("buckets,distance", [(4, 2), (8, 27), (32, 128), (64, 1000), (256, 100)])
+def test_buckets_by_their_definition(buckets, distance):
+    got = spion_amd.relative_position_buckets(buckets, distance)
+    assert got.dtype == torch.int32 and got.shape == (2 * distance + 1,)
+    half, exact = buckets // 2, buckets // 4
+    for diff in range(-distance, distance + 1):
+        n = abs(diff)
+        k = n
+        if n >= exact:
+            x = math.log(n / exact) / math.log(distance / exact) * (half - exact)
+            if abs(x - round(x)) < 1e-9:
+                x = round(x)  # a border: the logarithm may be off either way
+            k = min(half - 1, exact + int(x))
+        assert int(got[diff + distance]) == (half if diff > 0 else 0) + k, diff
+
+
+@pytest.mark.parametrize("buckets,distance", [(0, 10), (6, 10), (32, 8), (32, 1025), (-4, 10)])
+def test_buckets_refuse(buckets, distance):
+    with pytest.raises(ValueError):
+        spion_amd.relative_position_buckets(buckets, distance)
+
+
+def _ok():
+    x = torch.zeros(2, 3, 40, 32)
+    return dict(query=x, key=x, value=x, weight=torch.zeros(8, 3), buckets=spion_amd.relative_position_buckets(8, 20))
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(query=torch.zeros(3, 40, 32)), ValueError),
+    (dict(key=torch.zeros(2, 2, 40, 32)), ValueError),
+    (dict(value=torch.zeros(2, 3, 41, 32)), ValueError),
+    (dict(query=torch.zeros(2, 3, 40, 32).half()), TypeError),
+    (dict(key=torch.zeros(2, 3, 40, 32).bfloat16()), (TypeError, RuntimeError)),
+    (dict(weight=torch.zeros(8, 2)), ValueError),
+    (dict(weight=torch.zeros(0, 3)), ValueError),
+    (dict(buckets=torch.zeros(10, dtype=torch.int32)), ValueError),
+    (dict(buckets=torch.zeros(2051, dtype=torch.int32)), ValueError),
+    (dict(buckets=torch.zeros(41, dtype=torch.int64)), TypeError),
+    (dict(key_mask=torch.ones(2, 41)), ValueError),
+    (dict(offset=1 << 30), ValueError),
+    (dict(mat=torch.ones(2, 2)), ValueError),
+    (dict(mat=torch.ones(2, 2), block_size=16), ValueError),
+    (dict(mat=torch.ones(3, 3), block_size=32), ValueError),
+    (dict(mat=torch.ones(2, 2), block_size=32, offset=1), ValueError),
+    (dict(mat=torch.ones(2, 2), block_size=32, score_map=True), ValueError),
+    (dict(), RuntimeError),  # everything in order, but not on a GPU
+])
+def test_operator_refuses(change, error):
+    with pytest.raises(error):
+        spion_amd.relative_bias_attention(**{**_ok(), **change})
+
+
+def test_head_dimensions_other_than_32_and_64_are_refused():
+    x = torch.zeros(1, 1, 8, 48)
+    with pytest.raises(ValueError, match="head dimension"):
+        spion_amd.relative_bias_attention(x, x, x, torch.zeros(8, 1), spion_amd.relative_position_buckets(8, 20))
+
+
+def test_module_refuses_heads_of_another_shape():
+    mod = spion_amd.RelativeBiasAttention(dict(head_dim=32, num_head=2))
+    assert mod.weight.shape == (32, 2) and list(mod.state_dict()) == ["weight"]
+    with pytest.raises(ValueError, match="2 heads of 32"):
+        mod(*[torch.zeros(1, 3, 8, 32)] * 3, None)
+
+
+def test_c_entry_points_refuse_before_any_gpu_work():
+    lib = rb._lib_typed()
+    buf = (ctypes.c_char * 4096)()
+    at = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 16  # never read: every call below is refused
+
+    def call(**kw):
+        c = rb._Call(weight=at, dweight=at, buckets=at, Lse=at, workspace=at, workspace_floats=1 << 40, batch=1, heads=1, q_len=64,
+                     k_len=64, head_dim=32, num_buckets=8, max_distance=20)
+        for n in ("Q", "K", "V", "Out", "dO", "dQ", "dK", "dV"):
+            setattr(c, n, rb._Heads(at, 2048, 2048, 32))
+        for n, x in kw.items():
+            setattr(c, n, x)
+        return c
+
+    bad = [dict(batch=0), dict(q_len=0), dict(k_len=-1), dict(head_dim=48), dict(num_buckets=0), dict(max_distance=0),
+           dict(max_distance=1025), dict(offset=1 << 30), dict(q_len=(1 << 29) + 1), dict(batch=1 << 20, heads=1 << 10),
+           dict(mat=at, block_size=16), dict(mat=at, block_size=32, offset=1), dict(mat=at, block_size=32, k_len=65),
+           dict(key_mask=at, mask_bytes=2), dict(weight=None), dict(Lse=None), dict(buckets=None), dict(OutLow=at + 2),
+           dict(Q=rb._Heads(None, 0, 0, 32)), dict(K=rb._Heads(at + 4, 0, 0, 32)), dict(V=rb._Heads(at, 2, 0, 32)),
+           dict(Out=rb._Heads(at, 0, -32, 32))]
+    for kw in bad + [dict(Out=rb._Heads(at, 0, 0, 0)), dict(Mean=at, mat=at, block_size=32)]:
+        assert lib.spion_bias_attention_forward(ctypes.addressof(call(**kw)), None) != 0, kw
+        with pytest.raises(_lib.SpionLibraryError, match="spion_bias_attention_forward"):
+            _lib.check_error()
+    for kw in bad + [dict(dQ=rb._Heads(at, 0, 0, 28)), dict(dO=rb._Heads(None, 0, 0, 32)), dict(workspace=None), dict(dweight=None),
+                     dict(workspace_floats=63)]:
+        assert lib.spion_bias_attention_backward(ctypes.addressof(call(**kw)), None) != 0, kw
+        with pytest.raises(_lib.SpionLibraryError, match="spion_bias_attention_backward"):
+            _lib.check_error()
+    assert lib.spion_bias_attention_forward(None, None) != 0 and lib.spion_bias_workspace(None, 1) == -1
+    assert lib.spion_bias_workspace(ctypes.addressof(call(head_dim=16)), 0) == -1
+    _lib.core().spion_clear_error()
+    assert lib.spion_bias_workspace(ctypes.addressof(call()), 1) == 64 + 2 * 8
