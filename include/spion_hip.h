@@ -528,6 +528,38 @@ long long spion_bias_workspace(const spion_bias_attention* call, int backward);
 int spion_bias_attention_forward(const spion_bias_attention* call, void* stream);
 int spion_bias_attention_backward(const spion_bias_attention* call, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Root-mean-square norm of rows with the residual's addition (the reference's layer normalises with nn.LayerNorm,
+ * models/model_transformer.py:55-102):
+ *
+ *   h = x + residual (rounded to the tensors' type),  y = h / sqrt(mean(h^2) + eps) * weight
+ *
+ * fp32 or bf16 rows of any width; statistics and sums in fp32.  No handle; the workspace is the caller's.
+ *   forward    x, residual (may be null: h is x and not written), weight [width]; out: h [rows][width], and y [rows][width] or
+ *              codes [rows][width] with scales [rows]: y as 8-bit floats (e4m3: 4 bits of exponent, 3 of mantissa, largest 448)
+ *              times the row's scale, max|y| / 448 (at least 2^-126).  Rows with a NaN have a NaN for a scale.
+ *   backward   x: the stream h of the forward; dy, and dh (may be null), the gradients of y and of the stream; out: dx [rows][width],
+ *              the gradient of x and of the residual, and dweight [width].  workspace: spion_rms_norm_workspace(call)
+ *              floats, contents unspecified.  The same inputs give the same bits.
+ * Row strides in elements for what is read; what is written is contiguous and overlaps nothing that is read.  Each returns 0 on success (the workspace: -1 on failure).
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct spion_rms_norm {
+    const void *x, *residual, *weight;
+    void *y, *h;
+    unsigned char* codes;
+    float* scales;
+    const void *dy, *dh;
+    void *dx, *dweight;
+    float* workspace;
+    long long workspace_floats;
+    long long rows, x_stride, residual_stride, dy_stride, dh_stride;
+    int width, bf16;
+    float eps;
+} spion_rms_norm;
+long long spion_rms_norm_workspace(const spion_rms_norm* call);
+int spion_rms_norm_forward(const spion_rms_norm* call, void* stream);
+int spion_rms_norm_backward(const spion_rms_norm* call, void* stream);
+
 const char* spion_version(void);
 
 #ifdef __cplusplus

@@ -20,6 +20,7 @@ from .pattern import (
     mean_score_map,
 )
 from .relative_bias import RelativeBiasAttention, relative_bias_attention, relative_position_buckets
+from .norm import RMSNorm, rms_norm, rms_norm_fp8
 
 __all__ = [
     "Attention",
@@ -46,4 +47,7 @@ __all__ = [
     "RelativeBiasAttention",
     "relative_bias_attention",
     "relative_position_buckets",
+    "RMSNorm",
+    "rms_norm",
+    "rms_norm_fp8",
 ]

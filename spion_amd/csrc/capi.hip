@@ -129,6 +129,9 @@ int project_backward(const float*, const float* const*, const float*, float*, fl
 long long bias_workspace(const spion_bias_attention*, int);
 int bias_forward(const spion_bias_attention*, hipStream_t);
 int bias_backward(const spion_bias_attention*, hipStream_t);
+long long norm_workspace(const spion_rms_norm*);
+int norm_forward(const spion_rms_norm*, hipStream_t);
+int norm_backward(const spion_rms_norm*, hipStream_t);
 int key_penalty(const float*, float*, int, int, int, hipStream_t);
 int pattern_generate_maps(const float* const*, int, int, int, int, int, double, float*, int, float*, float*, hipStream_t);
 int score_map_mean(const float*, int, int, int, int, float*, hipStream_t, float post = 1.0f);
@@ -319,6 +322,20 @@ int spion_bias_attention_forward(const spion_bias_attention* call, void* stream)
 int spion_bias_attention_backward(const spion_bias_attention* call, void* stream) {
     note_current_handle(nullptr);
     return bias_backward(call, static_cast<hipStream_t>(stream));
+}
+
+// ---- root-mean-square norm -------------------------------------------------------------------------
+long long spion_rms_norm_workspace(const spion_rms_norm* call) {
+    note_current_handle(nullptr);
+    return norm_workspace(call);
+}
+int spion_rms_norm_forward(const spion_rms_norm* call, void* stream) {
+    note_current_handle(nullptr);
+    return norm_forward(call, static_cast<hipStream_t>(stream));
+}
+int spion_rms_norm_backward(const spion_rms_norm* call, void* stream) {
+    note_current_handle(nullptr);
+    return norm_backward(call, static_cast<hipStream_t>(stream));
 }
 
 // ---- pattern discovery ---------------------------------------------------------------------------

@@ -1,0 +1,48 @@
+"""What the norm refuses, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+import spion_amd
+from spion_amd import _lib
+from spion_amd import norm as rn
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(weight=torch.ones(7)), ValueError), (dict(weight=torch.ones(2, 4)), ValueError), (dict(residual=torch.ones(4, 8)), ValueError),
+    (dict(x=torch.ones(3, 8).double()), TypeError), (dict(x=torch.ones(())), ValueError), (dict(eps=-1.0), ValueError),
+    (dict(eps=float("nan")), ValueError), (dict(), RuntimeError)])
+@pytest.mark.parametrize("op", ["rms_norm", "rms_norm_fp8"])
+def test_refusals(op, change, error):
+    with pytest.raises(error):
+        getattr(spion_amd, op)(**{**dict(x=torch.ones(3, 8), weight=torch.ones(8)), **change})
+
+
+def test_c_entry_points_refuse_before_any_gpu_work():
+    lib = rn._lib_typed()
+    buf = (ctypes.c_char * 4096)()
+    at = ctypes.addressof(buf)  # never read: every call below is refused
+
+    def call(**kw):
+        c = rn._Call(x=at, weight=at, y=at, dy=at, dx=at, dweight=at, workspace=at, workspace_floats=1 << 40, rows=4, width=8, x_stride=8,
+                     dy_stride=8, eps=1e-6)
+        for n, v in kw.items():
+            setattr(c, n, v)
+        return c
+
+    sizes = [dict(rows=0), dict(width=0), dict(rows=(1 << 40) + 1), dict(width=(1 << 29) + 1), dict(x_stride=-8), dict(eps=-1.0),
+             dict(eps=float("nan"))]
+    for kw in sizes + [dict(x=None), dict(weight=None), dict(y=None), dict(residual=at), dict(codes=at), dict(codes=at, scales=at),
+                       dict(y=None, codes=at)]:
+        assert lib.spion_rms_norm_forward(ctypes.addressof(call(**kw)), None) != 0, kw
+        with pytest.raises(_lib.SpionLibraryError, match="spion_rms_norm_forward"):
+            _lib.check_error()
+    for kw in sizes + [dict(x=None), dict(weight=None), dict(dy=None), dict(dx=None), dict(dweight=None), dict(workspace=None),
+                       dict(workspace_floats=4 * 8 - 1)]:
+        assert lib.spion_rms_norm_backward(ctypes.addressof(call(**kw)), None) != 0, kw
+        with pytest.raises(_lib.SpionLibraryError, match="spion_rms_norm_backward"):
+            _lib.check_error()
+    assert lib.spion_rms_norm_forward(None, None) != 0 and lib.spion_rms_norm_backward(None, None) != 0
+    assert lib.spion_rms_norm_workspace(ctypes.addressof(call(rows=0))) == -1
+    _lib.core().spion_clear_error()
