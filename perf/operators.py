@@ -190,7 +190,8 @@ def _run_own(s):
         return spion_amd.rms_norm_fp8(s["x"], s["w"], s["res"], EPS)
     if s["op"] == "norm":
         if not s["train"]:
-            return spion_amd.rms_norm(s["x"], s["w"], s["res"], EPS)
+            out = spion_amd.rms_norm(s["x"], s["w"], s["res"], EPS)
+            return [out] if s["res"] is None else out
         leaves = [t.detach().requires_grad_() for t in (s["x"], s["w"], s["res"]) if t is not None]
         out = spion_amd.rms_norm(*leaves, eps=EPS)
         if s["res"] is None:
