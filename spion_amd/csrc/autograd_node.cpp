@@ -9,8 +9,10 @@
 // behaviour; tests run both and compare.
 #include <ATen/FuncTorchTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <climits>
 #include <stdexcept>
 #include <string>
 
@@ -815,6 +817,8 @@ Tensor bf16_attention(const Tensor& query, const Tensor& key, const Tensor& valu
     return BF16AttnNode::apply(query, key, value, keys.t, offsets, columns, sum_mat, handle, nnz, stream);
 }
 
+#include "operator_nodes.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -828,5 +832,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("sparse_layer", &sparse_layer, "forward of the attention layer in its sparse phase; returns [y, p_flat]");
     m.def("projections_fit", &projections_fit, "whether the projection kernels take this layer's linear layers");
     m.def("project_heads", &project_heads, "the three input projections; returns the [B, H, L, d] heads");
+    m.def("relative_bias_attention", &relative_bias_attention, "attention with a relative position bias; returns [out] or [out, mean map]");
+    m.def("rms_norm", &rms_norm, "norm of rows; returns [y] or [y, h]");
+    m.def("rms_norm_fp8", &rms_norm_fp8, "norm of rows in 8 bits; returns [codes, scales] or [codes, scales, h]");
     m.def("merge_heads", &merge_heads, "the output projection of [B, H, L, d] heads");
 }

@@ -134,9 +134,25 @@ class _RMSNormFunction(torch.autograd.Function):
         return dx, dw, dx if ctx.residual else None, None
 
 
+def _in_node(name, *args):
+    """The compiled form (csrc/operator_nodes.h: the same steps), or None where Python's is asked for."""
+    node = _lib.autograd_node()
+    if node is None or not _lib.plain_autograd():
+        return None
+    try:
+        return getattr(node, name)(*args)
+    except RuntimeError as e:
+        if str(e).startswith("spion_rms_norm"):
+            raise _lib.SpionLibraryError(str(e)) from None
+        raise
+
+
 def rms_norm(x, weight, residual=None, eps: float = 1e-6):
     """``y``, or ``(y, h)`` where there is a residual: see the module's head.  x and residual [..., width], weight [width], of one
     type; gradients for all three."""
+    out = _in_node("rms_norm", x, weight, residual, eps)
+    if out is not None:
+        return out[0] if residual is None else tuple(out)
     _check(x, weight, residual, eps)
     return _RMSNormFunction.apply(x, weight, residual, float(eps))
 
@@ -145,6 +161,9 @@ def rms_norm_fp8(x, weight, residual=None, eps: float = 1e-6):
     """``(codes, scales)``, or ``(codes, scales, h)`` where there is a residual: the norm as 8-bit floats (torch.float8_e4m3fn,
     [..., width]) times a scale for every row (fp32 [...]), max|y| / 448 and at least 2^-126.  For inference: it has no
     gradient and refuses tensors that ask for one."""
+    out = _in_node("rms_norm_fp8", x, weight, residual, eps)
+    if out is not None:
+        return tuple(out)
     _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")

@@ -242,6 +242,15 @@ def relative_bias_attention(query, key, value, weight, buckets, key_mask=None, m
     mat [nb, nb] with block_size: pairs in blocks that are 0 have probability 0 and count in the softmax with a logit of 0, as in
     the other sparse modules.  offset: query i stands at position i + offset (the last queries of a sequence: Lk - Lq).
     score_map: also return the mean of the probability maps over batch and heads, fp32 [Lq, Lk], without a gradient."""
+    node = _lib.autograd_node()
+    if node is not None and _lib.plain_autograd():  # csrc/operator_nodes.h: the same steps
+        try:
+            out = node.relative_bias_attention(query, key, value, weight, buckets, key_mask, mat, block_size or 0, offset, score_map)
+        except RuntimeError as e:
+            if str(e).startswith("spion_bias_"):
+                raise _lib.SpionLibraryError(str(e)) from None
+            raise
+        return tuple(out) if score_map else out[0]
     _check(query, key, value, weight, buckets, key_mask, mat, block_size, offset, score_map)
     if key_mask is not None:
         if key_mask.dtype not in (torch.float32, torch.bool, torch.uint8):

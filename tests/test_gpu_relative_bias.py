@@ -14,6 +14,13 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
 
+@pytest.fixture(params=["node", "python"], autouse=True)
+def both_nodes(request, monkeypatch):
+    """Every test runs through the compiled node and through the Python function."""
+    if request.param == "python":
+        monkeypatch.setitem(_lib._cache, "node", None)
+
+
 def _inputs(dtype, B, H, Lq, Lk, d, buckets=16, distance=40, seed=0, views=True):
     g = torch.Generator().manual_seed(seed)
 

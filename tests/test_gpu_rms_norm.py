@@ -17,6 +17,13 @@ pytestmark = pytest.mark.gpu
 DEV, U, EPS = "cuda", 2.0 ** -24, 1e-6
 
 
+@pytest.fixture(params=["node", "python"], autouse=True)
+def both_nodes(request, monkeypatch):
+    """Every test runs through the compiled node and through the Python function."""
+    if request.param == "python":
+        monkeypatch.setitem(_lib._cache, "node", None)
+
+
 def _close(name, got, value, bound):
     assert got.shape == value.shape and bool(torch.isfinite(got.float()).all()), name
     far = (got.detach().double() - value).abs() - bound

@@ -10,6 +10,13 @@ from spion_amd import _lib
 from spion_amd import relative_bias as rb
 
 
+@pytest.fixture(params=["node", "python"], autouse=True)
+def both_nodes(request, monkeypatch):
+    """Every test runs through the compiled node and through the Python function."""
+    if request.param == "python":
+        monkeypatch.setitem(_lib._cache, "node", None)
+
+
 @pytest.mark.parametrize("buckets,distance", [(4, 2), (8, 27), (32, 128), (64, 1000), (256, 100)])
 def test_buckets_by_their_definition(buckets, distance):
     got = spion_amd.relative_position_buckets(buckets, distance)

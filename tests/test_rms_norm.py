@@ -9,6 +9,13 @@ from spion_amd import _lib
 from spion_amd import norm as rn
 
 
+@pytest.fixture(params=["node", "python"], autouse=True)
+def both_nodes(request, monkeypatch):
+    """Every test runs through the compiled node and through the Python function."""
+    if request.param == "python":
+        monkeypatch.setitem(_lib._cache, "node", None)
+
+
 @pytest.mark.parametrize("change,error", [
     (dict(weight=torch.ones(7)), ValueError), (dict(weight=torch.ones(2, 4)), ValueError), (dict(residual=torch.ones(4, 8)), ValueError),
     (dict(x=torch.ones(3, 8).double()), TypeError), (dict(x=torch.ones(())), ValueError), (dict(eps=-1.0), ValueError),
