@@ -485,7 +485,7 @@ int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, i
  * handle, nothing is kept between calls, and the workspace is the caller's: calls with workspaces of their own may overlap.
  *   heads        [B][H][L][d] tensors or views, strides in elements, multiples of 16 bytes; pointers 16-byte aligned; d = 32 or 64.
  *                The strides of tensors that are only read may be 0 (a head shared by others).
- *   weight       [num_buckets][heads], of the heads' type; dweight alike.
+ *   weight       [num_buckets][heads], of the heads' type, up to 32767 buckets; dweight alike.
  *   buckets      [2 R + 1] ints in 0 .. num_buckets - 1 (anything else is read as the nearest of them); 1 <= R <= 1024.
  *   offset       query i stands at position i + offset of the keys' count.
  *   key_mask     null, or [batch][k_len] floats (mask_bytes 4) or bytes (1): keys with a 0 are left out, and nothing of their K and V

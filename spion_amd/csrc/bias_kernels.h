@@ -58,6 +58,10 @@ struct BiasItem {
     }
 };
 
+// Wavefronts a SIMD that the registers are for.  fp32 heads of 64 features have one work-group's tiles in a CU's LDS.
+template <class T, int D>
+constexpr int bias_waves() { return sizeof(T) == 4 && D == 64 ? 1 : 2; }
+
 template <class T, int D>
 constexpr int bias_tiles_bytes() {
     const int tiles = 4 * 2 * BiasTile<T, D>::BYTES, merge = merge_floats<D>() * 4;
@@ -82,14 +86,14 @@ __device__ __forceinline__ void store_out(const BiasCall& a, int b, int h, int b
 // gradient adds up P (dP - D) over thousands of rows whose terms nearly cancel, and with P and O rounded to bf16 in D the buckets
 // of far keys come out wrong by 0.8 % (28 heads of 2923 tokens, 8 buckets), against 0.16 % of rounding at the end.
 template <class T, int D, bool FINE>
-__global__ __launch_bounds__(256, 2) void bias_forward_kernel(BiasCall a) {
+__global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
-    fill_bias<T>(a, it.h, tab, tid, 256);
+    fill_bias<T>(a, it.h, tab, tid);
     const int q0 = it.strip * 32;
     const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + min(q0 + li, a.Lq - 1) * a.q.row, h, q0 + li < a.Lq);
     const char *kh = a.k.head(it.b, it.h), *vh = a.v.head(it.b, it.h);
@@ -247,28 +251,78 @@ __global__ __launch_bounds__(256) void bias_merge_kernel(BiasCall a) {
 // -------------------------------------------------------------------------------------------------
 // Backward, strips of queries: dQ, D and the table's gradient
 // -------------------------------------------------------------------------------------------------
-// The table's gradient: a tile's dS of one accumulator register are 32 consecutive differences to either half-wave, so a tile that
-// touches (-R, R) adds its registers to a histogram by difference in LDS, one for each half-wave of each wavefront (no two lanes
-// of an instruction meet, and every histogram is added to in program order: the sums come out the same each time); of the others
-// only the sum is needed, which stays in a register.  The histograms of a strip are added up, folded into buckets and left
-// in the workspace, [strips][buckets] for every head.
-constexpr int BIAS_HISTS = 8;
-__device__ __forceinline__ void hist_add(float* at, float x) {
-    __hip_atomic_fetch_add(at, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+// The table's gradient: dS summed by difference.  Of a tile outside (-R, R) only its sum is needed, which stays in a register.  A
+// tile that touches the range is summed along its diagonals: the wavefront writes 16 of its rows to LDS so that a diagonal is
+// a column, four rows to a 16-byte piece, reads the columns back, a lane each, and adds their sums to its histogram of differences
+// (an LDS atomic per register and lane instead takes a third of the kernel: 735 us against 490 without any sums, 128 padded
+// heads of 2048, where a seventh of the tiles touch the range).  Every histogram is added to by one wavefront in program order, no
+// two lanes of an instruction meet: the sums come out the same each time.  The histograms of a strip are added up, folded into
+// buckets and left in the workspace, [strips][buckets] for every head.
+constexpr int BIAS_HISTS = 4, DIAG_COLS = 48, DIAG_FLOATS = 4 * DIAG_COLS * 4;
+// ds: rows are keys, lanes queries; hist: at difference rel0 (of the tile's first key and query); buf: the wavefront's, places that
+// are never written are zeros
+__device__ __forceinline__ void add_diagonals(float* buf, float* hist, const float (&ds)[16], int li, int h) {
+    const int l = li + 32 * h;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        wave_lds_order();
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                buf[((2 * g + h) * DIAG_COLS + 8 * g + 4 * h + e - li + 31) * 4 + e] = ds[8 * half + 4 * g + e];
+        wave_lds_order();
+        if (l < DIAG_COLS - 1) {
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(buf + (k * DIAG_COLS + l) * 4);
+                s += (v[0] + v[1]) + (v[2] + v[3]);
+            }
+            __hip_atomic_fetch_add(hist + 16 * half - 31 + l, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+    }
 }
+// The wavefronts' histograms into buckets: eight threads to a bucket, each every eighth entry.  LDS behind a barrier.
+__device__ __forceinline__ void fold_hists(float* hist, const unsigned short* bucket, int entries, int buckets, int tid, float* part) {
+    for (int i = tid; i < entries; i += 256) hist[i] = (hist[i] + hist[entries + i]) + (hist[2 * entries + i] + hist[3 * entries + i]);
+    __syncthreads();
+    for (int k0 = 0; k0 < buckets; k0 += 32) {
+        const int k = k0 + (tid >> 3);
+        float s = 0.f;
+#pragma unroll 4
+        for (int i = tid & 7; i < entries; i += 8) s += bucket[i] == k ? hist[i] : 0.f;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor(s, o, 64);
+        if (k < buckets && (tid & 7) == 0) part[k] = s;
+    }
+}
+// LDS of the kernels that make the table's gradient, behind the scan's: the wavefronts' diagonals, their histograms, the entries'
+// buckets
+struct HistLds {
+    float *diag, *hist;
+    unsigned short* bucket;
+    __device__ __forceinline__ HistLds(ScanLds& sc, int R)
+        : diag(reinterpret_cast<float*>(&sc + 1)), hist(diag + BIAS_HISTS * DIAG_FLOATS),
+          bucket(reinterpret_cast<unsigned short*>(hist + BIAS_HISTS * bias_entries(R))) {}
+    __device__ __forceinline__ void clear(int R, int tid) {
+        for (int i = tid; i < BIAS_HISTS * (DIAG_FLOATS + bias_entries(R)); i += 256) diag[i] = 0.f;
+    }
+    static int bytes(int R) { return BIAS_HISTS * (DIAG_FLOATS + bias_entries(R)) * 4 + ((bias_entries(R) * 2 + 15) & ~15); }
+};
 
 template <class T, int D>
-__global__ __launch_bounds__(256, 2) void bias_backward_row_kernel(BiasCall a) {
+__global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
-    float* hist = reinterpret_cast<float*>(&sc + 1);
+    HistLds hl(sc, a.R);
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
     const int entries = bias_entries(a.R);
-    fill_bias<T>(a, it.h, tab, tid, 256);
-    for (int i = tid; i < BIAS_HISTS * entries; i += 256) hist[i] = 0.f;
+    fill_bias<T>(a, it.h, tab, tid, hl.bucket);
+    hl.clear(a.R, tid);
     const int q0 = it.strip * 32, qi = min(q0 + li, a.Lq - 1);
     const bool there = q0 + li < a.Lq;
     const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + qi * a.q.row, h, there);
@@ -285,8 +339,9 @@ __global__ __launch_bounds__(256, 2) void bias_backward_row_kernel(BiasCall a) {
     char* tv = tk + TL::BYTES;
     const float c2 = a.scale * LOG2E;
     const int qpos = q0 + a.off;
-    float* mine = hist + (2 * w + h) * entries + a.R + BIAS_PAD - li + 4 * h;
+    float *mine = hl.hist + w * entries + a.R + BIAS_PAD, *diag = hl.diag + w * DIAG_FLOATS;
 
+    const f32x16 minus = splat16(-delta);
     f32x16 dq[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
@@ -311,17 +366,16 @@ __global__ __launch_bounds__(256, 2) void bias_backward_row_kernel(BiasCall a) {
             wave_lds_order();
             if (i + 4 < n) fetch(i + 4);
             const f32x16 s = TL::feat(TL::rows(tk, at), q);
-            const f32x16 dp = TL::feat(TL::rows(tv, at), go);
+            const f32x16 dp = TL::feat(TL::rows(tv, at), go, minus);  // dP - D
             float t[16];
             const int rel0 = (first + tile) * 32 - qpos;
             if (word == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word, t);
             else logits_of<true>(s, c2, tab, a.R, rel0, li, h, word, t);
             float ds[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(t[r] - lse) * (dp[r] - delta);
+            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(t[r] - lse) * dp[r];
             if (rel0 + 31 > -a.R && rel0 - 31 < a.R) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) hist_add(mine + rel0 + 8 * (r >> 2) + (r & 3), ds[r]);
+                add_diagonals(diag, mine + rel0, ds, li, h);
             } else {
                 float sum = 0.f;
 #pragma unroll
@@ -336,8 +390,8 @@ __global__ __launch_bounds__(256, 2) void bias_backward_row_kernel(BiasCall a) {
     behind = wave_sum(behind);
     ahead = wave_sum(ahead);
     if (l == 0) {
-        hist[2 * w * entries] += behind;
-        hist[2 * w * entries + entries - 1] += ahead;
+        hl.hist[w * entries] += behind;
+        hl.hist[w * entries + entries - 1] += ahead;
     }
     float x[D / 8];
     merge_waves<D>(dq, reinterpret_cast<float*>(lds), tid, x);
@@ -347,25 +401,7 @@ __global__ __launch_bounds__(256, 2) void bias_backward_row_kernel(BiasCall a) {
         for (int i = 0; i < D / 8; ++i) x[i] *= a.scale;
         store_values<T, D / 8>(const_cast<char*>(a.dq.head(it.b, it.h)) + (q0 + row) * a.dq.row + j * (D / 8) * sizeof(T), x);
     }
-    // the eight histograms into the first, then by buckets: eight threads to a bucket, each every eighth entry
-    for (int i = tid; i < entries; i += 256) {
-        float s = hist[i];
-#pragma unroll
-        for (int k = 1; k < BIAS_HISTS; ++k) s += hist[k * entries + i];
-        hist[i] = s;
-    }
-    __syncthreads();
-    for (int k0 = 0; k0 < a.buckets; k0 += 32) {
-        const int k = k0 + (tid >> 3);
-        float s = 0.f;
-        if (k < a.buckets)
-            for (int i = tid & 7; i < entries; i += 8)
-                if (bucket_at(a, i - a.R - BIAS_PAD) == k) s += hist[i];
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor(s, o, 64);
-        if (k < a.buckets && (tid & 7) == 0)
-            a.part[((size_t)it.bh * a.strips + it.strip) * a.buckets + k] = s;
-    }
+    fold_hists(hl.hist, hl.bucket, entries, a.buckets, tid, a.part + ((size_t)it.bh * a.strips + it.strip) * a.buckets);
 }
 
 // dw[k][h]: the strips of all samples, 256 partial sums in a fixed order.
@@ -390,14 +426,14 @@ __global__ __launch_bounds__(256) void bias_table_kernel(BiasCall a, T* __restri
 // -------------------------------------------------------------------------------------------------
 // The strip's keys are the lanes: what a key that is left out holds reaches its own lane only, whose results are zeros.
 template <class T, int D>
-__global__ __launch_bounds__(256, 2) void bias_backward_col_kernel(BiasCall a) {
+__global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
-    fill_bias<T>(a, it.h, tab, tid, 256);
+    fill_bias<T>(a, it.h, tab, tid);
     const int k0 = it.strip * 32, ki = min(k0 + li, a.Lk - 1);
     const typename TL::Row k = TL::load(a.k.head(it.b, it.h) + ki * a.k.row, h, k0 + li < a.Lk);
     const typename TL::Row v = TL::load(a.v.head(it.b, it.h) + ki * a.v.row, h, k0 + li < a.Lk);

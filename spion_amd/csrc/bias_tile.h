@@ -32,66 +32,139 @@ struct BiasCall {
 // ---------------------------------------------------------------------------------------------------------------------
 // 32 x D tiles
 // ---------------------------------------------------------------------------------------------------------------------
-// Rows are stored as 16-byte pieces, piece c of row r at c ^ swz(r).  rows(): lane (li, h) has features h*D/2 .. of row li, the
-// operand of a product over the head dimension.  add_t(): out[c] += X^T . W, W given as the accumulator values of a 32 x 32
-// product whose rows are the tile's rows; the accumulator layout is then the other operand's, register for register (bf16: after
-// conversion).  W's rounding to bf16 is off by up to 2^-8 of each weight, as the outputs' own is; sums are fp32.
+// A tile in LDS is one bf16 image, or three for fp32 heads: every value as the sum of three bf16 numbers, split by the thread that
+// stages it (Split3 in tile_ops.h: six products of the parts give fp32 accuracy at 2.7 times the rate of the fp32 matrix
+// instructions; an infinite operand, or one of 2^127 and more, makes sums that it enters NaN).  Rows are stored as 16-byte pieces of
+// eight values, piece c of row r at c ^ swz(r): sixteen rows' reads of one piece, and the transposing reads of four rows, meet every
+// bank once.
+//   rows()   lane (li, h) has features h*D/2 .. of row li, the operand of a product over the head dimension
+//   add_t()  out[c] += X^T . W, W given as the accumulator values of a 32 x 32 product whose rows are the tile's rows; the
+//            accumulator layout is then the other operand's, register for register after conversion.  With bf16 heads W's rounding
+//            is off by up to 2^-8 of each weight, as the outputs' own is; sums are fp32.
 template <class T, int D>
-struct BiasTile;
-
-template <int D>
-struct BiasTile<__bf16, D> {
-    typedef DmaTile<D> DT;
-    static constexpr int ROW = DT::ROW, BYTES = DT::TILE, CPR = DT::CPR;
+struct BiasTile {
+    static constexpr int IM = sizeof(T) == 4 ? 3 : 1;
+    static constexpr int ROW = D * 2, IMAGE = 32 * ROW, BYTES = IM * IMAGE, CPR = D / 8;
     struct Row {
-        bf16x8 x[D / 16];
+        bf16x8 x[IM][D / 16];
     };
     struct At {
-        typename DT::RowAddr ra;
-        typename DT::TrAddr ta;
+        int row[D / 16], col[D / 32][2];
     };
-    __device__ static __forceinline__ At at(int l) { return At{DT::row_addr(l & 31, l >> 5), DT::tr_addr(l)}; }
-    __device__ static __forceinline__ int swz(int r) { return DT::swz(r); }
+    __device__ static __forceinline__ int swz(int r) {
+        if constexpr (D == 64) return ((r << 1) & 4) | ((r >> 1) & 2) | ((r >> 3) & 1);  // even (odd) rows of 16: all eight, r and r + 2 differ in 4
+        else return (r >> 2) & 3;
+    }
+    __device__ static __forceinline__ At at(int l) {
+        const int li = l & 31, h = l >> 5, gm = (l >> 4) & 1, j = l & 15, r = 4 * h + (j >> 2);
+        At a;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) a.row[t] = li * ROW + 16 * ((h * (CPR / 2) + t) ^ swz(li));
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                a.col[c][u] = (r + 8 * u) * ROW + 16 * ((4 * c + 2 * gm + ((j & 3) >> 1)) ^ swz(r + 8 * u)) + 8 * (j & 1);
+        return a;
+    }
     __device__ static __forceinline__ Row rows(const char* t, const At& a) {
         Row r;
-        DT::get_rows(t, a.ra, r.x);
+#pragma unroll
+        for (int m = 0; m < IM; ++m)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+                r.x[m][i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(t + m * IMAGE + a.row[i]));
         return r;
+    }
+    // eight values from memory, split
+    __device__ static __forceinline__ void split_piece(const char* p, u32x4 (&x)[IM]) {
+        if constexpr (IM == 1) {
+            x[0] = *reinterpret_cast<const u32x4*>(p);
+        } else {
+            split_values(*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 16), x);
+        }
+    }
+    __device__ static __forceinline__ void split_values(f32x4 a, f32x4 b, u32x4 (&x)[IM]) {
+        const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        const Split3<8> s = split3(v);
+#pragma unroll
+        for (int m = 0; m < IM; ++m) x[m] = __builtin_bit_cast(u32x4, s.p[m][0]);
     }
     // row `row` of a head, from global memory; zeros where `there` is false
     __device__ static __forceinline__ Row load(const char* row, int h, bool there) {
         Row r;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-            u32x4 v = {0, 0, 0, 0};
-            if (there) v = *reinterpret_cast<const u32x4*>(row + h * D + 16 * i);
-            r.x[i] = __builtin_bit_cast(bf16x8, v);
+            u32x4 v[IM];
+#pragma unroll
+            for (int m = 0; m < IM; ++m) v[m] = u32x4{0, 0, 0, 0};
+            if (there) split_piece(row + (h * (D / 2) + 8 * i) * sizeof(T), v);
+#pragma unroll
+            for (int m = 0; m < IM; ++m) r.x[m][i] = __builtin_bit_cast(bf16x8, v[m]);
         }
         return r;
+    }
+    __device__ static __forceinline__ float value(const Row& r, int i, int e) {
+        float v = (float)r.x[0][i][e];
+        if constexpr (IM == 3) v += (float)r.x[1][i][e] + (float)r.x[2][i][e];
+        return v;
     }
     __device__ static __forceinline__ float dot(const Row& a, const Row& b) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s = fmaf((float)a.x[i][e], (float)b.x[i][e], s);
+            for (int e = 0; e < 8; ++e) s = fmaf(value(a, i, e), value(b, i, e), s);
         return s;
     }
-    __device__ static __forceinline__ f32x16 feat(const Row& a, const Row& b) {
-        f32x16 acc = {0};
+    __device__ static __forceinline__ f32x16 feat(const Row& a, const Row& b, f32x16 acc = splat16(0.f)) {
+        if constexpr (IM == 3) {
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) acc = mfma_bf16(a.x[i], b.x[i], acc);
+            for (int i = 0; i < D / 16; ++i) {
+                acc = mfma_bf16(a.x[2][i], b.x[0][i], acc);
+                acc = mfma_bf16(a.x[0][i], b.x[2][i], acc);
+                acc = mfma_bf16(a.x[1][i], b.x[1][i], acc);
+                acc = mfma_bf16(a.x[1][i], b.x[0][i], acc);
+                acc = mfma_bf16(a.x[0][i], b.x[1][i], acc);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) acc = mfma_bf16(a.x[0][i], b.x[0][i], acc);
         return acc;
     }
-    __device__ static __forceinline__ void add_t(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
-        bf16x8 xt[D / 32][2], wb[2];
-        DT::get_tile_t(t, a.ta, xt);
-        pack16(p, wb);
-        mma_tile_bf16<D>(xt, wb, out);
+    // the tile feature-major, with the transposing LDS read
+    __device__ static __forceinline__ void columns(const char* t, const At& a, bf16x8 (&xt)[IM][D / 32][2]) {
+        typedef s16x4 __attribute__((address_space(3))) * lds_ptr;
+#pragma unroll
+        for (int m = 0; m < IM; ++m)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + m * IMAGE + a.col[c][0] + 16 * i * ROW));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + m * IMAGE + a.col[c][1] + 16 * i * ROW));
+                    xt[m][c][i] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+                }
     }
-    // the same with W to 2^-17: what its rounding leaves, rounded once more, in products of its own
+    __device__ static __forceinline__ void add_t(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
+        bf16x8 xt[IM][D / 32][2];
+        columns(t, a, xt);
+        if constexpr (IM == 1) {
+            bf16x8 wb[2];
+            pack16(p, wb);
+            mma_tile_bf16<D>(xt[0], wb, out);
+        } else {
+            const Split3<16> w = split3(p);
+            constexpr int PAIRS[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+#pragma unroll
+            for (int k = 0; k < 6; ++k) mma_tile_bf16<D>(xt[PAIRS[k][0]], w.p[PAIRS[k][1]], out);
+        }
+    }
+    // the same with bf16 heads and W to 2^-17: what its rounding leaves, rounded once more, in products of its own
     __device__ static __forceinline__ void add_t_fine(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
-        bf16x8 xt[D / 32][2], wb[2];
-        DT::get_tile_t(t, a.ta, xt);
+        static_assert(IM == 1, "fp32 heads have their weights whole");
+        bf16x8 xt[IM][D / 32][2], wb[2];
+        columns(t, a, xt);
         float low[16];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -99,102 +172,62 @@ struct BiasTile<__bf16, D> {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 8 * i + 2 * e;
-                u[e] = pack_bf16(p[r], p[r + 1]);
-                low[r] = p[r] - bf16_lo(u[e]);
-                low[r + 1] = p[r + 1] - bf16_hi(u[e]);
+                const unsigned both = pack_bf16(p[r], p[r + 1]);
+                u[e] = both;
+                low[r] = p[r] - bf16_lo(both);
+                low[r + 1] = p[r + 1] - bf16_hi(both);
             }
             wb[i] = __builtin_bit_cast(bf16x8, u);
         }
-        mma_tile_bf16<D>(xt, wb, out);
+        mma_tile_bf16<D>(xt[0], wb, out);
         pack16(low, wb);
-        mma_tile_bf16<D>(xt, wb, out);
+        mma_tile_bf16<D>(xt[0], wb, out);
     }
 };
 
-template <int D>
-struct BiasTile<float, D> {
-    static constexpr int ROW = D * 4, BYTES = 32 * ROW, CPR = D / 4;
-    struct Row {
-        float x[D / 2];
-    };
-    struct At {
-        int row, sw;         // of the row operand
-        int col, lane4, h4;  // of the transposed one
-    };
-    __device__ static __forceinline__ At at(int l) {
-        const int li = l & 31, h = l >> 5;
-        return At{li * ROW, swz(li), li >> 2, 4 * (li & 3), 4 * h};
+// Eight values on their way from global memory to LDS.
+template <class T>
+struct PieceInFlight {
+    u32x4 x[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const char* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) x[i] = *reinterpret_cast<const u32x4*>(p + 16 * i);
     }
-    __device__ static __forceinline__ int swz(int r) { return r & (CPR - 1); }
-    __device__ static __forceinline__ Row rows_of(const char* t, const At& a, int h) {
-        Row r;
+    // piece c of row r of tile t; a row that is left out becomes zeros (whatever lies in it: 0 times it is 0)
+    template <int D>
+    __device__ __forceinline__ void store(char* t, int r, int c, bool there) const {
+        typedef BiasTile<T, D> TL;
+        u32x4 v[TL::IM];
+        if constexpr (TL::IM == 1) v[0] = x[0];
+        else TL::split_values(__builtin_bit_cast(f32x4, x[0]), __builtin_bit_cast(f32x4, x[1]), v);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(t + a.row + 16 * ((h * (CPR / 2) + i) ^ a.sw));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r.x[4 * i + e] = v[e];
+        for (int m = 0; m < TL::IM; ++m) {
+            if (!there) v[m] = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(t + m * TL::IMAGE + r * TL::ROW + 16 * (c ^ TL::swz(r))) = v[m];
         }
-        return r;
-    }
-    __device__ static __forceinline__ Row rows(const char* t, const At& a) { return rows_of(t, a, a.h4 >> 2); }
-    __device__ static __forceinline__ Row load(const char* row, int h, bool there) {
-        Row r;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            f32x4 v = {0, 0, 0, 0};
-            if (there) v = *reinterpret_cast<const f32x4*>(row + h * (2 * D) + 16 * i);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r.x[4 * i + e] = v[e];
-        }
-        return r;
-    }
-    __device__ static __forceinline__ float dot(const Row& a, const Row& b) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i) s = fmaf(a.x[i], b.x[i], s);
-        return s;
-    }
-    __device__ static __forceinline__ f32x16 feat(const Row& a, const Row& b) { return mma_feat<D>(a.x, b.x); }
-    __device__ static __forceinline__ void add_t(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-            float x[16];
-#pragma unroll
-            for (int s = 0; s < 16; ++s) {
-                const int row = 8 * (s >> 2) + (s & 3);  // and 4 h
-                const int sw = ((row & (CPR - 1)) ^ (a.h4 & (CPR - 1)));  // row + 4 h = row | 4 h: the bits are apart
-                x[s] = *reinterpret_cast<const float*>(t + (row + a.h4) * ROW + 16 * ((8 * c + a.col) ^ sw) + a.lane4);
-            }
-            out[c] = mma_chain(x, p, out[c]);
-        }
-    }
-    __device__ static __forceinline__ void add_t_fine(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
-        add_t(t, a, p, out);
     }
 };
 
-// A wavefront's tile on its way from global memory to LDS: 16-byte piece n = 64 i + l of the tile is piece n % CPR of row n / CPR.
+// A wavefront's tile on its way from global memory to LDS: piece n = 64 i + l of the tile is piece n % CPR of row n / CPR.
 template <class T, int D>
 struct TileInFlight {
     typedef BiasTile<T, D> TL;
     static constexpr int N = TL::CPR / 2;
-    u32x4 x[N];
+    PieceInFlight<T> x[N];
     // rows first .. first + 31 of a head of `rows` rows; behind its end the last one again, which store() leaves out
     __device__ __forceinline__ void load(const char* head, long long ld, int first, int rows, int l) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int n = 64 * i + l, r = n / TL::CPR, c = n % TL::CPR;
-            x[i] = *reinterpret_cast<const u32x4*>(head + min(first + r, rows - 1) * ld + 16 * c);
+            x[i].load(head + min(first + r, rows - 1) * ld + 8 * c * sizeof(T));
         }
     }
-    // to LDS; rows whose bit of `word` is not set become zeros (whatever lies in a key that is left out: 0 times it is 0)
+    // to LDS; rows whose bit of `word` is not set are left out
     __device__ __forceinline__ void store(char* t, unsigned word, int l) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int n = 64 * i + l, r = n / TL::CPR, c = n % TL::CPR;
-            u32x4 v = x[i];
-            if (!((word >> r) & 1u)) v = u32x4{0, 0, 0, 0};
-            *reinterpret_cast<u32x4*>(t + r * TL::ROW + 16 * (c ^ TL::swz(r))) = v;
+            x[i].template store<D>(t, r, c, (word >> r) & 1u);
         }
     }
 };
@@ -223,9 +256,15 @@ template <class T>
 __device__ __forceinline__ float bias_weight(const BiasCall& a, int bucket, int h) {
     return (float)reinterpret_cast<const T*>(a.w)[(size_t)bucket * a.H + h] * LOG2E;
 }
+// The table, and with `buckets` what bucket each entry is of.
 template <class T>
-__device__ __forceinline__ void fill_bias(const BiasCall& a, int h, float* tab, int tid, int threads) {
-    for (int i = tid; i < bias_entries(a.R); i += threads) tab[i] = bias_weight<T>(a, bucket_at(a, i - a.R - BIAS_PAD), h);
+__device__ __forceinline__ void fill_bias(const BiasCall& a, int h, float* tab, int tid, unsigned short* buckets = nullptr) {
+#pragma unroll 2
+    for (int i = tid; i < bias_entries(a.R); i += 256) {
+        const int k = bucket_at(a, i - a.R - BIAS_PAD);
+        tab[i] = bias_weight<T>(a, k, h);
+        if (buckets) buckets[i] = (unsigned short)k;
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -242,6 +281,7 @@ struct ScanLds {
     float ml[4][2][32];
     float row[32];
 };
+static_assert(sizeof(ScanLds) % 16 == 0, "what follows it is aligned");
 
 __device__ __forceinline__ bool key_there(const BiasCall& a, int b, int key) {
     if (key >= a.Lk) return false;
@@ -250,21 +290,28 @@ __device__ __forceinline__ bool key_there(const BiasCall& a, int b, int key) {
     return a.mask_bytes == 4 ? reinterpret_cast<const float*>(a.mask)[i] != 0.f : reinterpret_cast<const unsigned char*>(a.mask)[i] != 0;
 }
 
-// Tiles first .. first + count - 1 (count <= CHUNK) of the other side, for strip `own` of 32 rows.  KEYS: the other side is the
-// keys, else the queries.  Returns how many are listed; in_pattern grows by the keys of the pattern's tiles.  All threads of
-// the work-group call it; LDS that they still read must be done with.
-template <bool KEYS>
+// Which of the 32 keys of a tile there are, without a mask.
+__device__ __forceinline__ unsigned tail_word(int left) { return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u; }
+
+// Units of SUBS tiles, from tile `first` on, `count` (<= CHUNK) tiles of the other side, for strip `own` of 32 rows (patterns: SUBS is
+// 1).  KEYS: the other side is the keys, else the queries.  Returns how many units are listed; in_pattern grows by the keys of
+// the pattern's tiles.  All threads of the work-group call it; LDS that they still read must be done with.
+template <bool KEYS, int SUBS = 1>
 __device__ __forceinline__ int scan_chunk(const BiasCall& a, ScanLds& s, int b, int own, int first, int count, int tid,
                                           int& in_pattern) {
     const int w = tid >> 6, l = tid & 63;
     __syncthreads();
     if (KEYS) {
-        for (int g = w; g < (count + 1) / 2; g += 4) {
-            const unsigned long long there = __ballot(key_there(a, b, (first + 2 * g) * 32 + l));
-            if (l == 0) {
-                s.words[2 * g] = (unsigned)there;
-                if (2 * g + 1 < CHUNK) s.words[2 * g + 1] = (unsigned)(there >> 32);
+        if (a.mask) {
+            for (int g = w; g < (count + 1) / 2; g += 4) {
+                const unsigned long long there = __ballot(key_there(a, b, (first + 2 * g) * 32 + l));
+                if (l == 0) {
+                    s.words[2 * g] = (unsigned)there;
+                    if (2 * g + 1 < CHUNK) s.words[2 * g + 1] = (unsigned)(there >> 32);
+                }
             }
+        } else {
+            for (int i = tid; i < CHUNK; i += 256) s.words[i] = i < count ? tail_word(a.Lk - (first + i) * 32) : 0;
         }
         __syncthreads();
     }
@@ -272,15 +319,20 @@ __device__ __forceinline__ int scan_chunk(const BiasCall& a, ScanLds& s, int b, 
     unsigned long long votes[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        const int i = tid + 256 * r, tile = first + i;
+        const int i = (tid + 256 * r) * SUBS, tile = first + i;
         bool in = i < count;
-        if (in && a.mat) {
+        if (SUBS == 1 && in && a.mat) {
             const int o = own * 32 / a.bs, t = tile * 32 / a.bs;
             in = a.mat[KEYS ? (size_t)o * a.nb + t : (size_t)t * a.nb + o] != 0.f;
         }
         const unsigned long long pat = __ballot(in);
         const unsigned long long tail = KEYS ? __ballot(in && tile * 32 + 32 > a.Lk) : 0;
-        act[r] = in && (!KEYS || s.words[i] != 0);
+        act[r] = in;
+        if (KEYS && in) {
+            unsigned any = s.words[i];
+            if (SUBS == 2 && i + 1 < count) any |= s.words[i + 1];
+            act[r] = any != 0;
+        }
         votes[r] = __ballot(act[r]);
         if (l == 0) {
             s.seg[4 * r + w] = __popcll(votes[r]);

@@ -41,6 +41,10 @@ static bool sizes_ok(const char* who, const Call& c) {
         set_error("%s: max_distance %d, 1 to %d expected", who, c.max_distance, SPION_BIAS_MAX_DISTANCE);
         return false;
     }
+    if (c.num_buckets > 32767) {
+        set_error("%s: up to 32767 buckets", who);
+        return false;
+    }
     if (c.q_len > (1 << 29) || c.k_len > (1 << 29) || c.offset > (1 << 29) || c.offset < -(1 << 29)) {
         set_error("%s: lengths and offset up to 2^29", who);
         return false;
@@ -140,7 +144,7 @@ static bool backward(const Call& c, hipStream_t stream) {
     a.delta = c.workspace;
     a.part = c.workspace + nb * a.Lq;
     a.strips = (int)strips_of(a.Lq);
-    const size_t hist = (size_t)BIAS_HISTS * bias_entries(a.R) * 4;
+    const size_t hist = HistLds::bytes(a.R);
     if (!launch("bias_backward_row_kernel", bias_backward_row_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a) + hist, stream, a)) return false;
     hipLaunchKernelGGL((bias_table_kernel<T>), dim3((unsigned)(a.buckets * a.H)), dim3(256), 0, stream, a, reinterpret_cast<T*>(c.dweight));
     if (!check_launch("bias_table_kernel")) return false;
