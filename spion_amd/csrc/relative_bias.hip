@@ -1,6 +1,6 @@
 // Host side of the attention with a learned bias by buckets of relative position (kernels: bias_kernels.h): argument checks,
 // launch shapes, workspaces.  No handle: sizes come with the call, and nothing is kept from one call for another.
-#include "bias_kernels.h"
+#include "bias_dense_kernels.h"
 #include "common.h"
 #include "../../include/spion_hip.h"
 
@@ -112,15 +112,36 @@ static bool launch(const char* name, K kernel, long long groups, size_t lds, hip
     return check_launch(name);
 }
 
+// Whether a side of `rows` rows is walked in strips of 128: without a pattern, and with strips enough for the machine.
+static bool dense_strips(const Call& c, int rows) {
+    return !c.mat && (long long)c.batch * c.heads * ((rows + 127) / 128) >= 2 * device_cus();
+}
+template <class T, int D>
+static size_t stages_lds(const BiasCall& a) {
+    return bias_stages_bytes<T, D>() + bias_floats(a.R) * 4 + sizeof(ScanLds);
+}
+
 template <class T, int D>
 static size_t walk_lds(const BiasCall& a) {
     return bias_tiles_bytes<T, D>() + bias_floats(a.R) * 4 + sizeof(ScanLds);
 }
 
 template <class T, int D>
+static bool mean_map(const Call& c, const BiasCall& a, hipStream_t stream) {
+    return !c.Mean || launch("bias_mean_kernel", bias_mean_kernel<T, D>, strips_of(a.Lq) * strips_of(a.Lk), 0, stream, a);
+}
+
+template <class T, int D>
 static bool forward(const Call& c, hipStream_t stream) {
     BiasCall a = device_call(c);
     const long long nb = (long long)a.B * a.H, tiles = strips_of(a.Lk);
+    if (dense_strips(c, a.Lq)) {
+        auto kernel = bias_forward_dense_kernel<T, D, false>;
+        if constexpr (sizeof(T) == 2)
+            if (a.low) kernel = bias_forward_dense_kernel<T, D, true>;
+        a.strips = (a.Lq + 127) / 128;
+        return launch("bias_forward_dense_kernel", kernel, nb * a.strips, stages_lds<T, D>(a), stream, a) && mean_map<T, D>(c, a, stream);
+    }
     a.strips = (int)strips_of(a.Lq);
     a.splits = forward_splits(c);
     if (a.splits > 1 && (!c.workspace || c.workspace_floats < workspace_floats(c, false))) a.splits = 1;
@@ -132,9 +153,7 @@ static bool forward(const Call& c, hipStream_t stream) {
         if (a.low) kernel = bias_forward_kernel<T, D, true>;
     if (!launch("bias_forward_kernel", kernel, nb * a.strips * a.splits, walk_lds<T, D>(a), stream, a)) return false;
     if (a.splits > 1 && !launch("bias_merge_kernel", bias_merge_kernel<T, D>, nb * a.strips, 0, stream, a)) return false;
-    if (c.Mean)
-        return launch("bias_mean_kernel", bias_mean_kernel<T, D>, strips_of(a.Lq) * strips_of(a.Lk), 0, stream, a);
-    return true;
+    return mean_map<T, D>(c, a, stream);
 }
 
 template <class T, int D>
@@ -143,11 +162,18 @@ static bool backward(const Call& c, hipStream_t stream) {
     const long long nb = (long long)a.B * a.H;
     a.delta = c.workspace;
     a.part = c.workspace + nb * a.Lq;
-    a.strips = (int)strips_of(a.Lq);
     const size_t hist = HistLds::bytes(a.R);
-    if (!launch("bias_backward_row_kernel", bias_backward_row_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a) + hist, stream, a)) return false;
+    const bool dense = dense_strips(c, a.Lq);
+    a.strips = dense ? (a.Lq + 127) / 128 : (int)strips_of(a.Lq);
+    if (!(dense ? launch("bias_backward_row_dense_kernel", bias_backward_row_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a) + hist, stream, a)
+                : launch("bias_backward_row_kernel", bias_backward_row_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a) + hist, stream, a)))
+        return false;
     hipLaunchKernelGGL((bias_table_kernel<T>), dim3((unsigned)(a.buckets * a.H)), dim3(256), 0, stream, a, reinterpret_cast<T*>(c.dweight));
     if (!check_launch("bias_table_kernel")) return false;
+    if (dense_strips(c, a.Lk)) {
+        a.strips = (a.Lk + 127) / 128;
+        return launch("bias_backward_col_dense_kernel", bias_backward_col_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a) + 2048, stream, a);
+    }
     a.strips = (int)strips_of(a.Lk);
     return launch("bias_backward_col_kernel", bias_backward_col_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a), stream, a);
 }

@@ -78,6 +78,28 @@ def test_long_sides(Lq, Lk, dtype):
     _compare(_run(q, k, v, w, buckets, do, key_mask=mask, offset=100), bias_reference(q, k, v, w, buckets, mask, offset=100, do=do))
 
 
+# calls that fill the machine take strips of 128 rows: ragged strips and stages, wavefronts without rows, few or many other rows,
+# ranges of differences that tiles lie within, across and outside of
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,Lq,Lk,d,distance,offset", [(32, 16, 60, 60, 32, 40, 0), (64, 4, 200, 130, 64, 9, -50), (32, 4, 500, 700, 32, 100, 200),
+                                                         (128, 4, 33, 1, 64, 40, 0), (16, 8, 512, 520, 64, 200, 0), (43, 12, 128, 96, 32, 4, 5)])
+@pytest.mark.parametrize("kind", [None, "lengths", "holes"])
+def test_calls_that_fill_the_machine(B, H, Lq, Lk, d, distance, offset, kind, dtype):
+    q, k, v, w, buckets, do = _inputs(dtype, B, H, Lq, Lk, d, 12, distance)
+    mask = None if kind is None else _lengths_mask(B, Lk, 7, kind)
+    if mask is not None:  # whatever lies in keys that are left out
+        hidden = ~mask[:, None, :, None].expand_as(k)
+        k = torch.where(hidden, torch.tensor(math.nan, dtype=dtype, device=DEV), k)
+        v = torch.where(hidden, torch.tensor(math.inf, dtype=dtype, device=DEV), v)
+    ref = bias_reference(q, k, v, w, buckets, mask, offset=offset, do=do)
+    _compare(_run(q, k, v, w, buckets, do, key_mask=mask, offset=offset), ref)
+    with torch.no_grad():
+        out, mean = spion_amd.relative_bias_attention(q, k, v, w, buckets, key_mask=mask, offset=offset, score_map=True)
+    check("out", out, ref["out"])
+    p, bound = ref["p"]
+    check("mean", mean, (p.mean((0, 1)), (bound + p * (B * H + 2) * 2.0 ** -24).mean((0, 1))))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("buckets,distance", [(4, 2), (8, 33), (32, 128), (64, 1024), (1024, 1000)])
 @pytest.mark.parametrize("offset", [-700, 0, 23])
@@ -202,9 +224,10 @@ def test_gradient_against_differences():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_the_same_call_gives_the_same_bits(dtype):
-    q, k, v, w, buckets, do = _inputs(dtype, 3, 2, 300, 300, 64)
-    mask = _lengths_mask(3, 300, 5, "holes")
+@pytest.mark.parametrize("B", [3, 128])
+def test_the_same_call_gives_the_same_bits(B, dtype):
+    q, k, v, w, buckets, do = _inputs(dtype, B, 2, 300, 300, 64)
+    mask = _lengths_mask(B, 300, 5, "holes")
     a, b = (_run(q, k, v, w, buckets, do, key_mask=mask) for _ in range(2))
     for n in a:
         assert torch.equal(a[n], b[n]), n
