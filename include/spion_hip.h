@@ -494,9 +494,6 @@ int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, i
  *                in blocks that are 0 have P = 0 but count in Z_i with a logit of 0, masked or not, as in the other sparse
  *                families; block_size a multiple of 32, q_len = k_len, offset 0.
  *   Lse          [batch * heads][q_len] fp32, out of the forward and into the backward: log2 Z_i, +infinity for empty rows.
- *   OutLow       bf16 heads: null, or [batch * heads][q_len][head_dim] bf16, out of the forward and into the backward: what the
- *                rounding of Out left.  The backward's row sums dO.Out are then those of the unrounded output; without it the
- *                table's gradient, a sum over many rows that nearly cancel, is off by some 2^-8.  Not read for fp32 heads.
  *   Mean         null, or [q_len][k_len] fp32, out: the mean of P over batch and heads (spion_pattern_generate's Score input);
  *                not with mat.
  *   workspace    spion_bias_workspace(call, backward) floats, contents unspecified; a forward without it walks long rows in one
@@ -517,7 +514,6 @@ typedef struct spion_bias_attention {
     const void* key_mask;
     const float* mat;
     float* Lse;
-    void* OutLow;
     float* Mean;                   /* forward only */
     float* workspace;
     long long workspace_floats;

@@ -115,7 +115,7 @@ __device__ __forceinline__ void store_strip(const f32x16 (&acc)[D / 32], float f
     }
 }
 
-template <class T, int D, bool FINE>
+template <class T, int D>
 __global__ __launch_bounds__(256, 2) void bias_forward_dense_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     typedef BiasStage<T, D> ST;
@@ -188,9 +188,7 @@ __global__ __launch_bounds__(256, 2) void bias_forward_dense_kernel(BiasCall a) 
                     p[r] = __builtin_amdgcn_exp2f(fmaf(t[u][r], mul, add));
                     z += p[r];
                 }
-                const char* tv = buf + (SUBS + u) * TL::BYTES;
-                if constexpr (FINE) TL::add_t_fine(tv, at, p, o);
-                else TL::add_t(tv, at, p, o);
+                TL::add_t(buf + (SUBS + u) * TL::BYTES, at, p, o);
             }
         });
     z = half_swap_sum(z);
@@ -199,7 +197,7 @@ __global__ __launch_bounds__(256, 2) void bias_forward_dense_kernel(BiasCall a) 
     if (h == 0 && q0 + li < a.Lq)
         a.lse[(size_t)it.bh * a.Lq + q0 + li] = z > 0.f ? m + __builtin_amdgcn_logf(z) : __builtin_inff();
     store_strip<D>(o, z > 0.f ? 1.f / z : 0.f, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
-        if (q0 + row < a.Lq) store_out<T, D>(a, it.b, it.h, it.bh, q0 + row, j, x);
+        if (q0 + row < a.Lq) store_eighth<T, D>(a.o, it.b, it.h, q0 + row, j, x);
     });
 }
 
@@ -211,31 +209,24 @@ __global__ __launch_bounds__(256, 2) void bias_backward_row_dense_kernel(BiasCal
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_stages_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
-    HistLds hl(sc, a.R);
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
-    const int entries = bias_entries(a.R);
-    fill_bias<T>(a, it.h, tab, tid, hl.bucket);
-    hl.clear(a.R, tid);
+    fill_bias<T>(a, it.h, tab, tid);
     const int q0 = it.strip * 128 + w * 32, qi = min(q0 + li, a.Lq - 1);
     const bool some = q0 < a.Lq, there = q0 + li < a.Lq;
     const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + qi * a.q.row, h, there);
     const typename TL::Row go = TL::load(a.dout.head(it.b, it.h) + qi * a.dout.row, h, there);
     const size_t stat = (size_t)it.bh * a.Lq + qi;
     const float lse = there ? a.lse[stat] : __builtin_inff();
-    float delta = TL::dot(go, TL::load(a.o.head(it.b, it.h) + qi * a.o.row, h, there));
-    if (sizeof(T) == 2 && a.low) delta += TL::dot(go, TL::load(a.low + stat * D * sizeof(T), h, there));
-    delta = half_swap_sum(delta);
-    if (h == 0 && there) a.delta[stat] = delta;
+    const float delta = half_swap_sum(TL::dot(go, TL::load(a.o.head(it.b, it.h) + qi * a.o.row, h, there)));
     const typename TL::At at = TL::at(l);
     const float c2 = a.scale * LOG2E;
     const int qpos = q0 + a.off;
-    float *mine = hl.hist + w * entries + a.R + BIAS_PAD, *diag = hl.diag + w * DIAG_FLOATS;
     const f32x16 minus = splat16(-delta);
     f32x16 dq[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
-    float behind = 0.f, ahead = 0.f;
+    float sum = 0.f;
     walk_stages<T, D, true>(a, sc, it.b, a.Lk, a.k.head(it.b, it.h), a.k.row, a.v.head(it.b, it.h), a.v.row, lds, tid, NothingElse(),
         [&](int k0, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
             if (!some) return;
@@ -246,49 +237,29 @@ __global__ __launch_bounds__(256, 2) void bias_backward_row_dense_kernel(BiasCal
                 const f32x16 s = TL::feat(TL::rows(tk, at), q);
                 const f32x16 dp = TL::feat(TL::rows(tv, at), go, minus);  // dP - D
                 const int rel0 = k0 + 32 * u - qpos;
-                const bool near = rel0 + 31 > -a.R && rel0 - 31 < a.R;
                 float ds[16];
-                if (!near && word[u] == ~0u) {
+                if (word[u] == ~0u && (rel0 - 31 >= a.R || rel0 + 31 <= -a.R)) {
                     const float add = tab[rel0 > 0 ? 2 * (a.R + BIAS_PAD) : 0] - lse;
-                    float sum = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, add)) * dp[r];
-                        sum += ds[r];
-                    }
-                    if (rel0 > 0) ahead += sum;
-                    else behind += sum;
+                    for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, add)) * dp[r];
                 } else {
                     float t[16];
                     logits_of<true>(s, c2, tab, a.R, rel0, li, h, word[u], t);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(t[r] - lse) * dp[r];
-                    if (near) {
-                        add_diagonals(diag, mine + rel0, ds, li, h);
-                    } else {
-                        float sum = 0.f;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) sum += ds[r];
-                        if (rel0 > 0) ahead += sum;
-                        else behind += sum;
-                    }
                 }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum += ds[r];
                 TL::add_t(tk, at, ds, dq);
             }
         });
-    behind = wave_sum(behind);
-    ahead = wave_sum(ahead);
-    if (l == 0) {
-        hl.hist[w * entries] += behind;
-        hl.hist[w * entries + entries - 1] += ahead;
-    }
-    __syncthreads();  // the stages are done with, the histograms whole
+    sum = half_swap_sum(sum);
+    if (h == 0 && there) a.delta[stat] = delta + sum;
+    __syncthreads();  // the stages are done with
     if (some)
         store_strip<D>(dq, a.scale, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
-            if (q0 + row < a.Lq)
-                store_values<T, D / 8>(const_cast<char*>(a.dq.head(it.b, it.h)) + (q0 + row) * a.dq.row + j * (D / 8) * sizeof(T), x);
+            if (q0 + row < a.Lq) store_eighth<T, D>(a.dq, it.b, it.h, q0 + row, j, x);
         });
-    fold_hists(hl.hist, hl.bucket, entries, a.buckets, tid, a.part + ((size_t)it.bh * a.strips + it.strip) * a.buckets);
 }
 
 // The stage's queries' lse, -D and, for tiles far behind and far ahead, what the outermost buckets' bias leaves of lse.
@@ -324,14 +295,17 @@ __global__ __launch_bounds__(256, 2) void bias_backward_col_dense_kernel(BiasCal
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_stages_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
-    float* stats = reinterpret_cast<float*>(&sc + 1);
+    HistLds hl(sc, a.R);
+    float* stats = reinterpret_cast<float*>(lds + bias_stages_bytes<T, D>() + bias_floats(a.R) * 4 + sizeof(ScanLds) + HistLds::bytes(a.R));
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
-    fill_bias<T>(a, it.h, tab, tid);
+    fill_bias<T>(a, it.h, tab, tid, hl.bucket);
+    hl.clear(a.R, tid);
     const int k0 = it.strip * 128 + w * 32, ki = min(k0 + li, a.Lk - 1);
     const bool key = key_there(a, it.b, k0 + li), some = __any(key);  // false behind the last key
     const typename TL::Row k = TL::load(a.k.head(it.b, it.h) + ki * a.k.row, h, k0 + li < a.Lk);
     const typename TL::Row v = TL::load(a.v.head(it.b, it.h) + ki * a.v.row, h, k0 + li < a.Lk);
+    DifferenceSums sums(hl, w, a.R, key);
     const typename TL::At at = TL::at(l);
     const float c2 = a.scale * LOG2E;
     f32x16 dk[D / 32], dv[D / 32];
@@ -358,8 +332,9 @@ __global__ __launch_bounds__(256, 2) void bias_backward_col_dense_kernel(BiasCal
                     const f32x16 s = TL::feat(TL::rows(tq, at), k);
                     dp = TL::feat(TL::rows(tg, at), v, dp);  // dP - D
                     const int rel0 = k0 - r0 - 32 * u - a.off;  // of the tile's corner: lane li, row r has rel0 + li - r
+                    const bool near = sums.touches(rel0);
                     float p[16], ds[16];
-                    if (rel0 + 31 > -a.R && rel0 - 31 < a.R) {
+                    if (near) {
                         const float* bias = tab + rel0 + a.R + BIAS_PAD + li - 4 * h;
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {
@@ -381,28 +356,30 @@ __global__ __launch_bounds__(256, 2) void bias_backward_col_dense_kernel(BiasCal
                         p[r] = __builtin_amdgcn_exp2f(p[r]);
                         ds[r] = p[r] * dp[r];
                     }
+                    if (near) sums.near(rel0, ds, li, h);
+                    else sums.far(rel0, ds);
                     TL::add_t(tg, at, p, dv);
                     TL::add_t(tq, at, ds, dk);
                 }
             });
-    __syncthreads();
-    if (k0 >= a.Lk) return;
+    sums.finish(l);
+    __syncthreads();  // the stages are done with, the histograms whole
     float* red = reinterpret_cast<float*>(lds);
     const unsigned keys = (unsigned)__ballot(key);
+    // (a key that is left out: what it holds has reached its own lane, and nothing else)
     store_strip<D>(dv, 1.f, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
         if (k0 + row >= a.Lk) return;
-        if (!key_bit(keys, row))  // a key that is left out: what it holds has reached its own lane, and nothing else
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
-        store_values<T, D / 8>(const_cast<char*>(a.dv.head(it.b, it.h)) + (k0 + row) * a.dv.row + j * (D / 8) * sizeof(T), x);
+        for (int i = 0; i < D / 8; ++i) x[i] = key_bit(keys, row) ? x[i] : 0.f;
+        store_eighth<T, D>(a.dv, it.b, it.h, k0 + row, j, x);
     });
     store_strip<D>(dk, a.scale, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
         if (k0 + row >= a.Lk) return;
-        if (!key_bit(keys, row))
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
-        store_values<T, D / 8>(const_cast<char*>(a.dk.head(it.b, it.h)) + (k0 + row) * a.dk.row + j * (D / 8) * sizeof(T), x);
+        for (int i = 0; i < D / 8; ++i) x[i] = key_bit(keys, row) ? x[i] : 0.f;
+        store_eighth<T, D>(a.dk, it.b, it.h, k0 + row, j, x);
     });
+    fold_hists(hl.hist, hl.bucket, bias_entries(a.R), a.buckets, tid, a.part + ((size_t)it.bh * a.strips + it.strip) * a.buckets);
 }
 
 }  // namespace spion

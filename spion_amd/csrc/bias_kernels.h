@@ -1,7 +1,7 @@
 // Attention with a learned bias by buckets of relative position: no counterpart in the reference (its encoder knows positions
 // only from embeddings, models/model_transformer.py:17-52).  With t_ij = (q_i . k_j / sqrt(d) + w[bucket(j - i - off)]) log2(e)
 //   forward   P_ij = exp2(t_ij - lse_i),  O = P V
-//   backward  dP = dO V^T,  D_i = dO_i . O_i,  dS = P (dP - D),  dQ = dS K / sqrt(d),  dK = dS^T Q / sqrt(d),  dV = P^T dO,
+//   backward  dP = dO V^T,  D_i = sum_j P_ij dP_ij,  dS = P (dP - D),  dQ = dS K / sqrt(d),  dK = dS^T Q / sqrt(d),  dV = P^T dO,
 //             dw[k] = sum of dS over the pairs of bucket k
 // P is never written: the forward leaves lse, the backward forms P again.  Keys whose mask is 0 are left out; with a block
 // pattern the keys off the pattern count with a logit of 0, as in models/block_attn.cu:70-72.
@@ -44,11 +44,21 @@ __device__ __forceinline__ void logits_of(const f32x16& s, float c2, const float
     }
 }
 
-// Work-group -> (sample, head, strip, piece): the strips of a head follow each other on one XCD.
+// Work-group -> (sample, head, strip, piece).  The hardware deals work-groups round-robin over the XCDs; the strips of a head follow
+// each other on one of them, whose L2 then holds its K and V, and the heads go round-robin, so that every XCD has heads of
+// every sample: with key masks samples differ in length (consecutive heads on an XCD instead: 8 heads each of 16 samples of
+// 1024 to 2048 tokens take 803 us a step against NEW).  What is left of eight heads is spread evenly.
 struct BiasItem {
     int b, h, bh, strip, split;
     __device__ __forceinline__ BiasItem(const BiasCall& a, int total) {
-        int i = xcd_remap(blockIdx.x, total);
+        const int each = a.strips * a.splits, whole = a.B * a.H / 8 * 8 * each;  // work-groups of a head, of the whole rounds
+        int i = blockIdx.x;
+        if (i < whole) {
+            const int n = i / 8;
+            i = (n / each * 8 + i % 8) * each + n % each;
+        } else {
+            i = whole + xcd_remap(i - whole, total - whole);
+        }
         split = i % a.splits;
         i /= a.splits;
         strip = i % a.strips;
@@ -68,24 +78,16 @@ constexpr int bias_tiles_bytes() {
     return tiles > merge ? tiles : merge;
 }
 
-// Eighth j of row q of the output
+// Eighth j of row i of a tensor
 template <class T, int D>
-__device__ __forceinline__ void store_out(const BiasCall& a, int b, int h, int bh, int q, int j, float (&x)[D / 8]) {
-    store_values<T, D / 8>(const_cast<char*>(a.o.head(b, h)) + q * a.o.row + j * (D / 8) * sizeof(T), x);
-    if (sizeof(T) == 2 && a.low) {
-        rounded_off(x);
-        store_values<T, D / 8>(a.low + (((size_t)bh * a.Lq + q) * D + j * (D / 8)) * sizeof(T), x);
-    }
+__device__ __forceinline__ void store_eighth(const HeadsAt& t, int b, int h, int i, int j, const float (&x)[D / 8]) {
+    store_values<T, D / 8>(const_cast<char*>(t.head(b, h)) + i * t.row + j * (D / 8) * sizeof(T), x);
 }
 
 // -------------------------------------------------------------------------------------------------
 // Forward
 // -------------------------------------------------------------------------------------------------
-// FINE (bf16 heads, ahead of a backward): the probabilities enter the output with 2^-17, and what the rounding of the output
-// leaves is stored beside it.  The backward's D = dO.O has to be sum_j P_ij dP_ij for the P that it forms itself: the table's
-// gradient adds up P (dP - D) over thousands of rows whose terms nearly cancel, and with P and O rounded to bf16 in D the buckets
-// of far keys come out wrong by 0.8 % (28 heads of 2923 tokens, 8 buckets), against 0.16 % of rounding at the end.
-template <class T, int D, bool FINE>
+template <class T, int D>
 __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -153,8 +155,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
                 p[r] = __builtin_amdgcn_exp2f(t[r] - base);
                 z += p[r];
             }
-            if constexpr (FINE) TL::add_t_fine(tv, at, p, o);
-            else TL::add_t(tv, at, p, o);
+            TL::add_t(tv, at, p, o);
         }
     }
     // the four wavefronts' parts
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
     if (q0 + row < a.Lq) {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) x[i] *= sc.row[row];
-        store_out<T, D>(a, it.b, it.h, it.bh, q0 + row, j, x);
+        store_eighth<T, D>(a.o, it.b, it.h, q0 + row, j, x);
     }
 }
 
@@ -244,22 +245,114 @@ __global__ __launch_bounds__(256) void bias_merge_kernel(BiasCall a) {
     const float inv = Z > 0.f ? 1.f / Z : 0.f;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) x[i] *= inv;
-    store_out<T, D>(a, b, ih, bh, q, j, x);
+    store_eighth<T, D>(a.o, b, ih, q, j, x);
     if (j == 0) a.lse[(size_t)bh * a.Lq + q] = Z > 0.f ? M + __builtin_amdgcn_logf(Z) : __builtin_inff();
 }
 
 // -------------------------------------------------------------------------------------------------
-// Backward, strips of queries: dQ, D and the table's gradient
+// Backward, strips of queries: dQ and D
 // -------------------------------------------------------------------------------------------------
+// D = dO . O to begin with, from the output as it was rounded (and summed with rounded weights): good for dQ, whose own rounding is
+// larger.  The strip's sum of P (dP - dO.O) then gives what is left to D = sum_j P_ij dP_ij of the P that the backward itself forms,
+// and the column pass has that.  (The table's gradient adds up P (dP - D) over thousands of rows whose terms nearly cancel:
+// with dO.O for D the buckets of far keys come out wrong by 0.8 %, 28 heads of 2923 tokens in bf16, 8 buckets, against 0.16 % of
+// rounding at the end.)
+// What the strip's probabilities add up to: keys off the pattern have the rest.
+__device__ __forceinline__ float probabilities_of(float lse, int off) { return 1.f - (off > 0 ? off * __builtin_amdgcn_exp2f(-lse) : 0.f); }
+
+template <class T, int D>
+__global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_kernel(BiasCall a) {
+    typedef BiasTile<T, D> TL;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
+    ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
+    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const BiasItem it(a, gridDim.x);
+    fill_bias<T>(a, it.h, tab, tid);
+    const int q0 = it.strip * 32, qi = min(q0 + li, a.Lq - 1);
+    const bool there = q0 + li < a.Lq;
+    const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + qi * a.q.row, h, there);
+    const typename TL::Row go = TL::load(a.dout.head(it.b, it.h) + qi * a.dout.row, h, there);
+    const size_t stat = (size_t)it.bh * a.Lq + qi;
+    const float lse = there ? a.lse[stat] : __builtin_inff();
+    const float delta = half_swap_sum(TL::dot(go, TL::load(a.o.head(it.b, it.h) + qi * a.o.row, h, there)));
+    const char *kh = a.k.head(it.b, it.h), *vh = a.v.head(it.b, it.h);
+    const typename TL::At at = TL::at(l);
+    char* tk = lds + w * 2 * TL::BYTES;
+    char* tv = tk + TL::BYTES;
+    const float c2 = a.scale * LOG2E;
+    const int qpos = q0 + a.off;
+
+    const f32x16 minus = splat16(-delta);
+    f32x16 dq[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
+    float sum = 0.f;
+    int in_pattern = 0;
+    const int tiles = (a.Lk + 31) / 32;
+    for (int first = 0; first < tiles; first += CHUNK) {
+        const int n = scan_chunk<true>(a, sc, it.b, it.strip, first, min(CHUNK, tiles - first), tid, in_pattern);
+        TileInFlight<T, D> fk, fv;
+        auto fetch = [&](int i) __attribute__((always_inline)) {
+            const int j = (first + sc.list[i]) * 32;
+            fk.load(kh, a.k.row, j, a.Lk, l);
+            fv.load(vh, a.v.row, j, a.Lk, l);
+        };
+        if (w < n) fetch(w);
+        for (int i = w; i < n; i += 4) {
+            const int tile = uniform(sc.list[i]);
+            const unsigned word = uniform(sc.words[tile]);
+            wave_lds_order();
+            fk.store(tk, word, l);
+            fv.store(tv, word, l);
+            wave_lds_order();
+            if (i + 4 < n) fetch(i + 4);
+            const f32x16 s = TL::feat(TL::rows(tk, at), q);
+            const f32x16 dp = TL::feat(TL::rows(tv, at), go, minus);  // dP - D
+            float t[16];
+            const int rel0 = (first + tile) * 32 - qpos;
+            if (word == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word, t);
+            else logits_of<true>(s, c2, tab, a.R, rel0, li, h, word, t);
+            float ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                ds[r] = __builtin_amdgcn_exp2f(t[r] - lse) * dp[r];
+                sum += ds[r];
+            }
+            TL::add_t(tk, at, ds, dq);
+        }
+    }
+    sum = half_swap_sum(sum);
+    if (h == 0) sc.ml[w][0][li] = sum;
+    __syncthreads();  // the tiles are done with
+    if (w == 0 && h == 0 && there) {
+        const float all = (sc.ml[0][0][li] + sc.ml[1][0][li]) + (sc.ml[2][0][li] + sc.ml[3][0][li]);
+        a.delta[stat] = fmaf(delta, probabilities_of(lse, a.mat ? a.Lk - in_pattern : 0), all);
+    }
+    float x[D / 8];
+    merge_waves<D>(dq, reinterpret_cast<float*>(lds), tid, x);
+    const int row = tid >> 3, j = tid & 7;
+    if (q0 + row < a.Lq) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) x[i] *= a.scale;
+        store_eighth<T, D>(a.dq, it.b, it.h, q0 + row, j, x);
+    }
+}
+
+// -------------------------------------------------------------------------------------------------
+// Backward, strips of keys: dK, dV and the table's gradient
+// -------------------------------------------------------------------------------------------------
+// The strip's keys are the lanes: what a key that is left out holds reaches its own lane only, whose results are zeros.
+//
 // The table's gradient: dS summed by difference.  Of a tile outside (-R, R) only its sum is needed, which stays in a register.  A
 // tile that touches the range is summed along its diagonals: the wavefront writes 16 of its rows to LDS so that a diagonal is
 // a column, four rows to a 16-byte piece, reads the columns back, a lane each, and adds their sums to its histogram of differences
-// (an LDS atomic per register and lane instead takes a third of the kernel: 735 us against 490 without any sums, 128 padded
-// heads of 2048, where a seventh of the tiles touch the range).  Every histogram is added to by one wavefront in program order, no
-// two lanes of an instruction meet: the sums come out the same each time.  The histograms of a strip are added up, folded into
-// buckets and left in the workspace, [strips][buckets] for every head.
+// (an LDS atomic per register and lane instead took a third of the kernel that had it: 735 us against 490 without any sums,
+// 128 padded heads of 2048, where a seventh of the tiles touch the range).  Every histogram is added to by one wavefront in
+// program order, no two lanes of an instruction meet: the sums come out the same each time.  The histograms of a strip are added
+// up, folded into buckets and left in the workspace, [strips][buckets] for every head.
 constexpr int BIAS_HISTS = 4, DIAG_COLS = 48, DIAG_FLOATS = 4 * DIAG_COLS * 4;
-// ds: rows are keys, lanes queries; hist: at difference rel0 (of the tile's first key and query); buf: the wavefront's, places that
+// ds: rows are queries, lanes keys; hist: at difference rel0 (of the tile's first key and query); buf: the wavefront's, places that
 // are never written are zeros
 __device__ __forceinline__ void add_diagonals(float* buf, float* hist, const float (&ds)[16], int li, int h) {
     const int l = li + 32 * h;
@@ -270,7 +363,7 @@ __device__ __forceinline__ void add_diagonals(float* buf, float* hist, const flo
         for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                buf[((2 * g + h) * DIAG_COLS + 8 * g + 4 * h + e - li + 31) * 4 + e] = ds[8 * half + 4 * g + e];
+                buf[((2 * g + h) * DIAG_COLS + li - (8 * g + 4 * h + e) + 15) * 4 + e] = ds[8 * half + 4 * g + e];
         wave_lds_order();
         if (l < DIAG_COLS - 1) {
             float s = 0.f;
@@ -279,7 +372,7 @@ __device__ __forceinline__ void add_diagonals(float* buf, float* hist, const flo
                 const f32x4 v = *reinterpret_cast<const f32x4*>(buf + (k * DIAG_COLS + l) * 4);
                 s += (v[0] + v[1]) + (v[2] + v[3]);
             }
-            __hip_atomic_fetch_add(hist + 16 * half - 31 + l, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            __hip_atomic_fetch_add(hist - 16 * half - 15 + l, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
     }
 }
@@ -308,11 +401,45 @@ struct HistLds {
     __device__ __forceinline__ void clear(int R, int tid) {
         for (int i = tid; i < BIAS_HISTS * (DIAG_FLOATS + bias_entries(R)); i += 256) diag[i] = 0.f;
     }
-    static int bytes(int R) { return BIAS_HISTS * (DIAG_FLOATS + bias_entries(R)) * 4 + ((bias_entries(R) * 2 + 15) & ~15); }
+    __host__ __device__ static int bytes(int R) { return BIAS_HISTS * (DIAG_FLOATS + bias_entries(R)) * 4 + ((bias_entries(R) * 2 + 15) & ~15); }
+};
+// A wavefront's sums: dS of a tile, whose lanes are keys of which `key` says whether they take part
+struct DifferenceSums {
+    float *hist, *diag;
+    int R;
+    bool key, some_out;  // some_out: a key of the strip is left out
+    float behind = 0.f, ahead = 0.f;
+    __device__ __forceinline__ DifferenceSums(const HistLds& hl, int w, int R_, bool key_)
+        : hist(hl.hist + w * bias_entries(R_) + R_ + BIAS_PAD), diag(hl.diag + w * DIAG_FLOATS), R(R_), key(key_), some_out(!__all(key_)) {}
+    __device__ __forceinline__ bool touches(int rel0) const { return rel0 + 31 > -R && rel0 - 31 < R; }
+    __device__ __forceinline__ void near(int rel0, const float (&ds)[16], int li, int h) {
+        if (some_out) {
+            float kept[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) kept[r] = key ? ds[r] : 0.f;
+            add_diagonals(diag, hist + rel0, kept, li, h);
+        } else {
+            add_diagonals(diag, hist + rel0, ds, li, h);
+        }
+    }
+    __device__ __forceinline__ void far(int rel0, const float (&ds)[16]) {
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += ds[r];
+        if (rel0 > 0) ahead += sum;
+        else behind += sum;
+    }
+    __device__ __forceinline__ void finish(int l) {
+        const float b = wave_sum(key ? behind : 0.f), f = wave_sum(key ? ahead : 0.f);
+        if (l == 0) {
+            hist[-R - BIAS_PAD] += b;
+            hist[R + BIAS_PAD] += f;
+        }
+    }
 };
 
 template <class T, int D>
-__global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_kernel(BiasCall a) {
+__global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
@@ -320,130 +447,20 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_k
     HistLds hl(sc, a.R);
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
-    const int entries = bias_entries(a.R);
     fill_bias<T>(a, it.h, tab, tid, hl.bucket);
     hl.clear(a.R, tid);
-    const int q0 = it.strip * 32, qi = min(q0 + li, a.Lq - 1);
-    const bool there = q0 + li < a.Lq;
-    const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + qi * a.q.row, h, there);
-    const typename TL::Row go = TL::load(a.dout.head(it.b, it.h) + qi * a.dout.row, h, there);
-    const size_t stat = (size_t)it.bh * a.Lq + qi;
-    const float lse = there ? a.lse[stat] : __builtin_inff();
-    float delta = TL::dot(go, TL::load(a.o.head(it.b, it.h) + qi * a.o.row, h, there));
-    if (sizeof(T) == 2 && a.low) delta += TL::dot(go, TL::load(a.low + stat * D * sizeof(T), h, there));
-    delta = half_swap_sum(delta);
-    if (w == 0 && h == 0 && there) a.delta[stat] = delta;
-    const char *kh = a.k.head(it.b, it.h), *vh = a.v.head(it.b, it.h);
-    const typename TL::At at = TL::at(l);
-    char* tk = lds + w * 2 * TL::BYTES;
-    char* tv = tk + TL::BYTES;
-    const float c2 = a.scale * LOG2E;
-    const int qpos = q0 + a.off;
-    float *mine = hl.hist + w * entries + a.R + BIAS_PAD, *diag = hl.diag + w * DIAG_FLOATS;
-
-    const f32x16 minus = splat16(-delta);
-    f32x16 dq[D / 32];
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
-    float behind = 0.f, ahead = 0.f;
-    int in_pattern = 0;
-    const int tiles = (a.Lk + 31) / 32;
-    for (int first = 0; first < tiles; first += CHUNK) {
-        const int n = scan_chunk<true>(a, sc, it.b, it.strip, first, min(CHUNK, tiles - first), tid, in_pattern);
-        TileInFlight<T, D> fk, fv;
-        auto fetch = [&](int i) __attribute__((always_inline)) {
-            const int j = (first + sc.list[i]) * 32;
-            fk.load(kh, a.k.row, j, a.Lk, l);
-            fv.load(vh, a.v.row, j, a.Lk, l);
-        };
-        if (w < n) fetch(w);
-        for (int i = w; i < n; i += 4) {
-            const int tile = uniform(sc.list[i]);
-            const unsigned word = uniform(sc.words[tile]);
-            wave_lds_order();
-            fk.store(tk, word, l);
-            fv.store(tv, word, l);
-            wave_lds_order();
-            if (i + 4 < n) fetch(i + 4);
-            const f32x16 s = TL::feat(TL::rows(tk, at), q);
-            const f32x16 dp = TL::feat(TL::rows(tv, at), go, minus);  // dP - D
-            float t[16];
-            const int rel0 = (first + tile) * 32 - qpos;
-            if (word == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word, t);
-            else logits_of<true>(s, c2, tab, a.R, rel0, li, h, word, t);
-            float ds[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(t[r] - lse) * dp[r];
-            if (rel0 + 31 > -a.R && rel0 - 31 < a.R) {
-                add_diagonals(diag, mine + rel0, ds, li, h);
-            } else {
-                float sum = 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) sum += ds[r];
-                if (rel0 > 0) ahead += sum;
-                else behind += sum;
-            }
-            TL::add_t(tk, at, ds, dq);
-        }
-    }
-    __syncthreads();  // the tiles are done with
-    behind = wave_sum(behind);
-    ahead = wave_sum(ahead);
-    if (l == 0) {
-        hl.hist[w * entries] += behind;
-        hl.hist[w * entries + entries - 1] += ahead;
-    }
-    float x[D / 8];
-    merge_waves<D>(dq, reinterpret_cast<float*>(lds), tid, x);
-    const int row = tid >> 3, j = tid & 7;
-    if (q0 + row < a.Lq) {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) x[i] *= a.scale;
-        store_values<T, D / 8>(const_cast<char*>(a.dq.head(it.b, it.h)) + (q0 + row) * a.dq.row + j * (D / 8) * sizeof(T), x);
-    }
-    fold_hists(hl.hist, hl.bucket, entries, a.buckets, tid, a.part + ((size_t)it.bh * a.strips + it.strip) * a.buckets);
-}
-
-// dw[k][h]: the strips of all samples, 256 partial sums in a fixed order.
-template <class T>
-__global__ __launch_bounds__(256) void bias_table_kernel(BiasCall a, T* __restrict__ dw) {
-    __shared__ float red[4];
-    const int k = blockIdx.x % a.buckets, h = blockIdx.x / a.buckets, tid = threadIdx.x;
-    const int n = a.B * a.strips;
-    float s = 0.f;
-    for (int i = tid; i < n; i += 256) {
-        const int b = i / a.strips, strip = i - b * a.strips;
-        s += a.part[(((size_t)b * a.H + h) * a.strips + strip) * a.buckets + k];
-    }
-    s = wave_sum(s);
-    if ((tid & 63) == 0) red[tid >> 6] = s;
-    __syncthreads();
-    if (tid == 0) dw[(size_t)k * a.H + h] = (T)(red[0] + red[1] + red[2] + red[3]);
-}
-
-// -------------------------------------------------------------------------------------------------
-// Backward, strips of keys: dK and dV
-// -------------------------------------------------------------------------------------------------
-// The strip's keys are the lanes: what a key that is left out holds reaches its own lane only, whose results are zeros.
-template <class T, int D>
-__global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_kernel(BiasCall a) {
-    typedef BiasTile<T, D> TL;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
-    ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
-    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
-    const BiasItem it(a, gridDim.x);
-    fill_bias<T>(a, it.h, tab, tid);
     const int k0 = it.strip * 32, ki = min(k0 + li, a.Lk - 1);
     const typename TL::Row k = TL::load(a.k.head(it.b, it.h) + ki * a.k.row, h, k0 + li < a.Lk);
     const typename TL::Row v = TL::load(a.v.head(it.b, it.h) + ki * a.v.row, h, k0 + li < a.Lk);
-    const unsigned keys = (unsigned)__ballot(key_there(a, it.b, k0 + li));
+    const bool key = key_there(a, it.b, k0 + li);
+    const unsigned keys = (unsigned)__ballot(key);
+    DifferenceSums sums(hl, w, a.R, key);
     const char *qh = a.q.head(it.b, it.h), *gh = a.dout.head(it.b, it.h);
     const float *lseh = a.lse + (size_t)it.bh * a.Lq, *deltah = a.delta + (size_t)it.bh * a.Lq;
     const typename TL::At at = TL::at(l);
     char* tq = lds + w * 2 * TL::BYTES;
     char* tg = tq + TL::BYTES;
-    float* stats = sc.ml[w][0];  // lse of the tile's 32 queries, then their D
+    float* stats = sc.ml[w][0];  // lse of the tile's 32 queries, then their -D
     const float c2 = a.scale * LOG2E;
 
     f32x16 dk[D / 32], dv[D / 32];
@@ -459,24 +476,32 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_k
             const int r = (first + sc.list[i]) * 32;
             fq.load(qh, a.q.row, r, a.Lq, l);
             fg.load(gh, a.dout.row, r, a.Lq, l);
-            st = r + li < a.Lq ? (h ? deltah : lseh)[r + li] : (h ? 0.f : __builtin_inff());
+            st = r + li < a.Lq ? (h ? -deltah[r + li] : lseh[r + li]) : (h ? 0.f : __builtin_inff());
         };
         if (w < n) fetch(w);
         for (int i = w; i < n; i += 4) {
             const int tile = uniform(sc.list[i]);
             const int r0 = (first + tile) * 32;
-            const unsigned word = a.Lq - r0 >= 32 ? ~0u : (1u << (a.Lq - r0)) - 1u;
+            const unsigned word = tail_word(a.Lq - r0);
             wave_lds_order();
             fq.store(tq, word, l);
             fg.store(tg, word, l);
             stats[l] = st;
             wave_lds_order();
             if (i + 4 < n) fetch(i + 4);
+            f32x16 dp;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 d = *reinterpret_cast<const f32x4*>(stats + 32 + 8 * g + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dp[4 * g + j] = d[j];
+            }
             const f32x16 s = TL::feat(TL::rows(tq, at), k);
-            const f32x16 dp = TL::feat(TL::rows(tg, at), v);
+            dp = TL::feat(TL::rows(tg, at), v, dp);  // dP - D
             const int rel0 = k0 - r0 - a.off;  // of the tile's corner: lane li, row r has rel0 + li - r
+            const bool near = sums.touches(rel0);
             float p[16];
-            if (rel0 + 31 > -a.R && rel0 - 31 < a.R) {
+            if (near) {
                 const float* bias = tab + rel0 + a.R + BIAS_PAD + li - 4 * h;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) p[r] = fmaf(s[r], c2, bias[-(8 * (r >> 2) + (r & 3))]);
@@ -489,17 +514,20 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_k
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 e = *reinterpret_cast<const f32x4*>(stats + 8 * g + 4 * h);
-                const f32x4 d = *reinterpret_cast<const f32x4*>(stats + 32 + 8 * g + 4 * h);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     p[4 * g + j] = __builtin_amdgcn_exp2f(p[4 * g + j] - e[j]);
-                    ds[4 * g + j] = p[4 * g + j] * (dp[4 * g + j] - d[j]);
+                    ds[4 * g + j] = p[4 * g + j] * dp[4 * g + j];
                 }
             }
+            if (near) sums.near(rel0, ds, li, h);
+            else sums.far(rel0, ds);
             TL::add_t(tg, at, p, dv);
             TL::add_t(tq, at, ds, dk);
         }
     }
+    if (keys == 0) __syncthreads();  // the tables are there (a scan has seen to it otherwise)
+    sums.finish(l);
     __syncthreads();
     const int row = tid >> 3, j = tid & 7;
     const bool keep = key_bit(keys, row);
@@ -508,15 +536,34 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_k
     if (k0 + row < a.Lk) {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) x[i] = keep ? x[i] : 0.f;
-        store_values<T, D / 8>(const_cast<char*>(a.dv.head(it.b, it.h)) + (k0 + row) * a.dv.row + j * (D / 8) * sizeof(T), x);
+        store_eighth<T, D>(a.dv, it.b, it.h, k0 + row, j, x);
     }
     __syncthreads();
     merge_waves<D>(dk, reinterpret_cast<float*>(lds), tid, x);
     if (k0 + row < a.Lk) {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) x[i] = keep ? x[i] * a.scale : 0.f;
-        store_values<T, D / 8>(const_cast<char*>(a.dk.head(it.b, it.h)) + (k0 + row) * a.dk.row + j * (D / 8) * sizeof(T), x);
+        store_eighth<T, D>(a.dk, it.b, it.h, k0 + row, j, x);
     }
+    fold_hists(hl.hist, hl.bucket, bias_entries(a.R), a.buckets, tid, a.part + ((size_t)it.bh * a.strips + it.strip) * a.buckets);
+}
+
+// dw[k][h]: the strips of all samples, 256 partial sums in a fixed order.
+template <class T>
+__global__ __launch_bounds__(256) void bias_table_kernel(BiasCall a, T* __restrict__ dw) {
+    __shared__ float red[4];
+    const int k = blockIdx.x % a.buckets, h = blockIdx.x / a.buckets, tid = threadIdx.x;
+    const int n = a.B * a.strips;
+    float s = 0.f;
+#pragma unroll 4
+    for (int i = tid; i < n; i += 256) {
+        const int b = i / a.strips, strip = i - b * a.strips;
+        s += a.part[(((size_t)b * a.H + h) * a.strips + strip) * a.buckets + k];
+    }
+    s = wave_sum(s);
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    __syncthreads();
+    if (tid == 0) dw[(size_t)k * a.H + h] = (T)(red[0] + red[1] + red[2] + red[3]);
 }
 
 // -------------------------------------------------------------------------------------------------

@@ -19,8 +19,7 @@ struct BiasCall {
     const void* mask;   // [B][Lk]: null, float (0 = left out) or bytes
     const float* mat;   // [nb][nb] pattern of bs x bs blocks, or null
     float* lse;         // [B*H][Lq]: log2 of the softmax denominator, +inf for rows that nothing enters
-    char* low;          // [B*H][Lq][D] bf16 or null: O before its rounding less O
-    float* delta;       // [B*H][Lq]: dO . O
+    float* delta;       // [B*H][Lq]: sum over the keys of P dP
     float* part;        // workspace
     float* mean;        // [Lq][Lk]
     int B, H, Lq, Lk, R, buckets, off, bs, nb;
@@ -159,29 +158,6 @@ struct BiasTile {
 #pragma unroll
             for (int k = 0; k < 6; ++k) mma_tile_bf16<D>(xt[PAIRS[k][0]], w.p[PAIRS[k][1]], out);
         }
-    }
-    // the same with bf16 heads and W to 2^-17: what its rounding leaves, rounded once more, in products of its own
-    __device__ static __forceinline__ void add_t_fine(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
-        static_assert(IM == 1, "fp32 heads have their weights whole");
-        bf16x8 xt[IM][D / 32][2], wb[2];
-        columns(t, a, xt);
-        float low[16];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            u32x4 u;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = 8 * i + 2 * e;
-                const unsigned both = pack_bf16(p[r], p[r + 1]);
-                u[e] = both;
-                low[r] = p[r] - bf16_lo(both);
-                low[r + 1] = p[r + 1] - bf16_hi(both);
-            }
-            wb[i] = __builtin_bit_cast(bf16x8, u);
-        }
-        mma_tile_bf16<D>(xt[0], wb, out);
-        pack16(low, wb);
-        mma_tile_bf16<D>(xt[0], wb, out);
     }
 };
 
@@ -383,12 +359,6 @@ __device__ __forceinline__ void merge_waves(const f32x16 (&acc)[D / 32], float* 
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e];
         }
-}
-// What the rounding of x to bf16 leaves of it.
-template <int N>
-__device__ __forceinline__ void rounded_off(float (&x)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] -= (float)(__bf16)x[i];
 }
 // D / 8 consecutive values to memory, rounded once
 template <class T, int N>

@@ -73,7 +73,7 @@ Tensor empty_like_heads(const Tensor& t) { return empty_heads(t.sizes(), t.strid
 spion_heads heads_of(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 
 spion_bias_attention bias_call(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& w, const Tensor& buckets,
-                               const Tensor& mask, const Tensor& mat, const Tensor& lse, const Tensor& low, int64_t block, int64_t offset) {
+                               const Tensor& mask, const Tensor& mat, const Tensor& lse, int64_t block, int64_t offset) {
     spion_bias_attention c{};
     c.Q = heads_of(q);
     c.K = heads_of(k);
@@ -87,7 +87,6 @@ spion_bias_attention bias_call(const Tensor& q, const Tensor& k, const Tensor& v
     }
     c.mat = fp(mat);
     c.Lse = static_cast<float*>(lse.data_ptr());
-    if (low.defined()) c.OutLow = low.data_ptr();
     c.batch = (int)q.size(0);
     c.heads = (int)q.size(1);
     c.q_len = (int)q.size(2);
@@ -111,10 +110,10 @@ Tensor bias_workspace(spion_bias_attention& c, bool backward, const Tensor& q) {
 }
 
 struct BiasForward {
-    Tensor q, k, v, w, buckets, out, lse, low, mean;
+    Tensor q, k, v, w, buckets, out, lse, mean;
 };
 BiasForward bias_forward(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& weight, const Tensor& buckets,
-                         const Tensor& mask, const Tensor& mat, int64_t block, int64_t offset, bool score_map, bool fine) {
+                         const Tensor& mask, const Tensor& mat, int64_t block, int64_t offset, bool score_map) {
     BiasForward r;
     r.q = readable_heads(query);
     r.k = readable_heads(key);
@@ -124,10 +123,8 @@ BiasForward bias_forward(const Tensor& query, const Tensor& key, const Tensor& v
     r.out = empty_like_heads(query);
     const auto fp32 = query.options().dtype(torch::kFloat32);
     r.lse = torch::empty({query.size(0) * query.size(1), query.size(2)}, fp32);
-    if (fine && query.scalar_type() == torch::kBFloat16)  // what the rounding of out leaves
-        r.low = torch::empty({query.size(0) * query.size(1), query.size(2), query.size(3)}, query.options());
     if (score_map) r.mean = torch::empty({query.size(2), key.size(2)}, fp32);
-    spion_bias_attention c = bias_call(r.q, r.k, r.v, r.out, r.w, r.buckets, mask, mat, r.lse, r.low, block, offset);
+    spion_bias_attention c = bias_call(r.q, r.k, r.v, r.out, r.w, r.buckets, mask, mat, r.lse, block, offset);
     if (score_map) c.Mean = fpm(r.mean);
     const Tensor ws = bias_workspace(c, false, query);
     spion_bias_attention_forward(&c, reinterpret_cast<void*>(current_stream(query.device().index())));
@@ -140,11 +137,11 @@ struct BiasNode : public torch::autograd::Function<BiasNode> {
                           c10::optional<Tensor> mask, c10::optional<Tensor> mat, int64_t block, int64_t offset, bool score_map,
                           Tensor* mean) {
         const Tensor m = mask.value_or(Tensor()), p = mat.value_or(Tensor());
-        const BiasForward r = bias_forward(query, key, value, weight, buckets, m, p, block, offset, score_map, true);
+        const BiasForward r = bias_forward(query, key, value, weight, buckets, m, p, block, offset, score_map);
         *mean = r.mean;
         ctx->saved_data["block"] = block;
         ctx->saved_data["offset"] = offset;
-        save_as_is(ctx, {r.q, r.k, r.v, r.w, r.out, r.lse, r.buckets, r.low, m, p});
+        save_as_is(ctx, {r.q, r.k, r.v, r.w, r.out, r.lse, r.buckets, m, p});
         return r.out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -153,7 +150,7 @@ struct BiasNode : public torch::autograd::Function<BiasNode> {
         const Tensor q = readable_heads(s[0]), k = readable_heads(s[1]), v = readable_heads(s[2]), out = readable_heads(s[4]);
         const Tensor w = s[3].contiguous(), lse = s[5].contiguous(), buckets = s[6].contiguous();
         const auto rest = [&](size_t i) { return s[i].defined() ? s[i].contiguous() : Tensor(); };
-        const Tensor low = rest(7), mask = rest(8), mat = rest(9);
+        const Tensor mask = rest(7), mat = rest(8);
         const Tensor go = readable_heads(grads[0].to(q.scalar_type()));
         variable_list g(11);
         if (q.scalar_type() == torch::kFloat32 && q.sizes() == k.sizes() && adjacent_head_views(q, k, v)) {
@@ -166,7 +163,7 @@ struct BiasNode : public torch::autograd::Function<BiasNode> {
             g[2] = empty_like_heads(v);
         }
         g[3] = torch::empty_like(w);
-        spion_bias_attention c = bias_call(q, k, v, out, w, buckets, mask, mat, lse, low, ctx->saved_data["block"].toInt(),
+        spion_bias_attention c = bias_call(q, k, v, out, w, buckets, mask, mat, lse, ctx->saved_data["block"].toInt(),
                                            ctx->saved_data["offset"].toInt());
         c.dO = heads_of(go);
         c.dQ = heads_of(g[0]);
@@ -233,7 +230,7 @@ std::vector<Tensor> relative_bias_attention(const Tensor& query, const Tensor& k
         return {out, torch::zeros({Lq, Lk}, query.options().dtype(torch::kFloat32))};
     }
     if (without_node({&query, &key, &value, &weight})) {
-        const BiasForward r = bias_forward(query, key, value, weight, buckets, mask, mat, block, offset, score_map, false);
+        const BiasForward r = bias_forward(query, key, value, weight, buckets, mask, mat, block, offset, score_map);
         return score_map ? std::vector<Tensor>{r.out, r.mean} : std::vector<Tensor>{r.out};
     }
     const auto given = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };

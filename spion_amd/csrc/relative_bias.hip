@@ -22,10 +22,10 @@ static int forward_splits(const Call& c) {
 }
 
 static long long workspace_floats(const Call& c, bool backward) {
-    const long long nb = (long long)c.batch * c.heads, strips = strips_of(c.q_len);
-    if (backward) return nb * c.q_len + nb * strips * c.num_buckets;
+    const long long nb = (long long)c.batch * c.heads;
+    if (backward) return nb * c.q_len + nb * strips_of(c.k_len) * c.num_buckets;
     const int s = forward_splits(c);
-    return s > 1 ? nb * strips * s * (32 * c.head_dim + 96) : 0;
+    return s > 1 ? nb * strips_of(c.q_len) * s * (32 * c.head_dim + 96) : 0;
 }
 
 static bool sizes_ok(const char* who, const Call& c) {
@@ -90,7 +90,7 @@ static BiasCall device_call(const Call& c) {
     a.q = heads_at(c, c.Q), a.k = heads_at(c, c.K), a.v = heads_at(c, c.V), a.o = heads_at(c, c.Out);
     a.dout = heads_at(c, c.dO), a.dq = heads_at(c, c.dQ), a.dk = heads_at(c, c.dK), a.dv = heads_at(c, c.dV);
     a.w = c.weight, a.map = c.buckets, a.mask = c.key_mask, a.mat = c.mat;
-    a.lse = c.Lse, a.mean = c.Mean, a.low = c.bf16 ? reinterpret_cast<char*>(c.OutLow) : nullptr;
+    a.lse = c.Lse, a.mean = c.Mean;
     a.B = c.batch, a.H = c.heads, a.Lq = c.q_len, a.Lk = c.k_len, a.R = c.max_distance, a.buckets = c.num_buckets;
     a.off = c.offset, a.bs = c.block_size, a.nb = c.mat ? (c.k_len + c.block_size - 1) / c.block_size : 0;
     a.mask_bytes = c.mask_bytes;
@@ -136,11 +136,8 @@ static bool forward(const Call& c, hipStream_t stream) {
     BiasCall a = device_call(c);
     const long long nb = (long long)a.B * a.H, tiles = strips_of(a.Lk);
     if (dense_strips(c, a.Lq)) {
-        auto kernel = bias_forward_dense_kernel<T, D, false>;
-        if constexpr (sizeof(T) == 2)
-            if (a.low) kernel = bias_forward_dense_kernel<T, D, true>;
         a.strips = (a.Lq + 127) / 128;
-        return launch("bias_forward_dense_kernel", kernel, nb * a.strips, stages_lds<T, D>(a), stream, a) && mean_map<T, D>(c, a, stream);
+        return launch("bias_forward_dense_kernel", bias_forward_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a), stream, a) && mean_map<T, D>(c, a, stream);
     }
     a.strips = (int)strips_of(a.Lq);
     a.splits = forward_splits(c);
@@ -148,10 +145,7 @@ static bool forward(const Call& c, hipStream_t stream) {
     a.per_split = (int)((tiles + a.splits - 1) / a.splits);
     a.splits = (int)((tiles + a.per_split - 1) / a.per_split);  // none of them empty
     a.part = c.workspace;
-    auto kernel = bias_forward_kernel<T, D, false>;
-    if constexpr (sizeof(T) == 2)
-        if (a.low) kernel = bias_forward_kernel<T, D, true>;
-    if (!launch("bias_forward_kernel", kernel, nb * a.strips * a.splits, walk_lds<T, D>(a), stream, a)) return false;
+    if (!launch("bias_forward_kernel", bias_forward_kernel<T, D>, nb * a.strips * a.splits, walk_lds<T, D>(a), stream, a)) return false;
     if (a.splits > 1 && !launch("bias_merge_kernel", bias_merge_kernel<T, D>, nb * a.strips, 0, stream, a)) return false;
     return mean_map<T, D>(c, a, stream);
 }
@@ -162,20 +156,18 @@ static bool backward(const Call& c, hipStream_t stream) {
     const long long nb = (long long)a.B * a.H;
     a.delta = c.workspace;
     a.part = c.workspace + nb * a.Lq;
+    const bool rows = dense_strips(c, a.Lq), cols = dense_strips(c, a.Lk);
+    a.strips = rows ? (a.Lq + 127) / 128 : (int)strips_of(a.Lq);
+    if (!(rows ? launch("bias_backward_row_dense_kernel", bias_backward_row_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a), stream, a)
+               : launch("bias_backward_row_kernel", bias_backward_row_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a), stream, a)))
+        return false;
+    a.strips = cols ? (a.Lk + 127) / 128 : (int)strips_of(a.Lk);
     const size_t hist = HistLds::bytes(a.R);
-    const bool dense = dense_strips(c, a.Lq);
-    a.strips = dense ? (a.Lq + 127) / 128 : (int)strips_of(a.Lq);
-    if (!(dense ? launch("bias_backward_row_dense_kernel", bias_backward_row_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a) + hist, stream, a)
-                : launch("bias_backward_row_kernel", bias_backward_row_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a) + hist, stream, a)))
+    if (!(cols ? launch("bias_backward_col_dense_kernel", bias_backward_col_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a) + hist + 2048, stream, a)
+               : launch("bias_backward_col_kernel", bias_backward_col_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a) + hist, stream, a)))
         return false;
     hipLaunchKernelGGL((bias_table_kernel<T>), dim3((unsigned)(a.buckets * a.H)), dim3(256), 0, stream, a, reinterpret_cast<T*>(c.dweight));
-    if (!check_launch("bias_table_kernel")) return false;
-    if (dense_strips(c, a.Lk)) {
-        a.strips = (a.Lk + 127) / 128;
-        return launch("bias_backward_col_dense_kernel", bias_backward_col_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a) + 2048, stream, a);
-    }
-    a.strips = (int)strips_of(a.Lk);
-    return launch("bias_backward_col_kernel", bias_backward_col_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a), stream, a);
+    return check_launch("bias_table_kernel");
 }
 
 long long bias_workspace(const Call* c, int backward) {
@@ -196,10 +188,6 @@ int bias_forward(const Call* c, hipStream_t stream) {
     if (!sizes_ok(who, *c) || !heads_ok(who, "Q", *c, c->Q, false) || !heads_ok(who, "K", *c, c->K, false) ||
         !heads_ok(who, "V", *c, c->V, false) || !heads_ok(who, "Out", *c, c->Out, true))
         return 1;
-    if (reinterpret_cast<uintptr_t>(c->OutLow) % 16) {
-        set_error("%s: OutLow is not 16-byte aligned", who);
-        return 1;
-    }
     if (c->Mean && c->mat) {
         set_error("%s: the mean map is of the dense phase, without a pattern", who);
         return 1;
@@ -223,10 +211,6 @@ int bias_backward(const Call* c, hipStream_t stream) {
         !heads_ok(who, "V", *c, c->V, false) || !heads_ok(who, "Out", *c, c->Out, false) || !heads_ok(who, "dO", *c, c->dO, false) ||
         !heads_ok(who, "dQ", *c, c->dQ, true) || !heads_ok(who, "dK", *c, c->dK, true) || !heads_ok(who, "dV", *c, c->dV, true))
         return 1;
-    if (reinterpret_cast<uintptr_t>(c->OutLow) % 16) {
-        set_error("%s: OutLow is not 16-byte aligned", who);
-        return 1;
-    }
     if (c->workspace_floats < workspace_floats(*c, true)) {
         set_error("%s: workspace of %lld floats, %lld expected", who, c->workspace_floats, workspace_floats(*c, true));
         return 1;

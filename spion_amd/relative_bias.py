@@ -62,7 +62,7 @@ class _Call(ctypes.Structure):
     """``spion_bias_attention``."""
 
     _fields_ = ([(n, _Heads) for n in ("Q", "K", "V", "Out", "dO", "dQ", "dK", "dV")]
-                + [(n, ctypes.c_void_p) for n in ("weight", "dweight", "buckets", "key_mask", "mat", "Lse", "OutLow", "Mean", "workspace")]
+                + [(n, ctypes.c_void_p) for n in ("weight", "dweight", "buckets", "key_mask", "mat", "Lse", "Mean", "workspace")]
                 + [("workspace_floats", ctypes.c_longlong)]
                 + [(n, ctypes.c_int) for n in ("batch", "heads", "q_len", "k_len", "head_dim", "bf16", "num_buckets",
                                                "max_distance", "offset", "block_size", "mask_bytes")])
@@ -135,23 +135,18 @@ class _RelativeBiasFunction(torch.autograd.Function):
         q, k, v, w = _readable(query), _readable(key), _readable(value), weight.contiguous()
         out = _empty_like_heads(query)
         lse = torch.empty((B * H, Lq), dtype=torch.float32, device=dev)
-        low = None
-        if query.dtype == torch.bfloat16 and any(ctx.needs_input_grad[:4]):
-            low = torch.empty((B * H, Lq, d), dtype=torch.bfloat16, device=dev)  # what the rounding of out leaves
         mean = torch.empty((Lq, Lk), dtype=torch.float32, device=dev) if score_map else None
         with torch.cuda.device(dev):
             call = _call_of(q, k, w, buckets, key_mask, mat, block_size, offset)
             call.Q, call.K, call.V, call.Out = (_heads(t) for t in (q, k, v, out))
             call.Lse = lse.data_ptr()
-            if low is not None:
-                call.OutLow = low.data_ptr()
             if mean is not None:
                 call.Mean = mean.data_ptr()
             ws = _workspace(lib, call, False, dev)
             _raise(lib.spion_bias_attention_forward(ctypes.addressof(call), _lib._raw_stream(dev.index)),
                    "spion_bias_attention_forward")
             del ws
-        optional = {"low": low, "key_mask": key_mask, "mat": mat}
+        optional = {"key_mask": key_mask, "mat": mat}
         ctx.given = [n for n, t in optional.items() if t is not None]
         ctx.numbers = (block_size, offset)
         _lib.save_for_backward(ctx, q, k, v, w, out, lse, buckets, *(optional[n] for n in ctx.given))
@@ -180,8 +175,6 @@ class _RelativeBiasFunction(torch.autograd.Function):
         with torch.cuda.device(dev):
             call = _call_of(q, k, w, buckets, rest.get("key_mask"), rest.get("mat"), block_size, offset)
             call.Q, call.K, call.V, call.Out = (_heads(t) for t in (q, k, v, out))
-            if "low" in rest:
-                call.OutLow = rest["low"].data_ptr()
             call.dO, call.dQ, call.dK, call.dV = (_heads(t) for t in (go, dq, dk, dv))
             call.Lse, call.dweight = lse.data_ptr(), dw.data_ptr()
             ws = _workspace(lib, call, True, dev)

@@ -5,7 +5,8 @@ most n u32 of the sum of magnitudes.  With t the logits, P = exp(t) / Z:
   dt    = (d + 8) u32 (|q|.|k| scale + |bias|)                 product, scale, bias, subtraction of the maximum, exp2's argument
   rP    = 2 max_j dt + (Lk + 64) u32                           of numerator and denominator, exp2, the sum of the denominator
   out   : sum_j P |v| (rP + wP + Lk u32) + r |out|             wP: rounding of the weights P to bf16 in the product, r: of the output
-  D     : sum_f |dO| (P |v|) (rP + wD + Lk u32) + d u32 |dO|.|out|   wD = 2^-15: P and out enter with 2^-16 each (bf16), 0 (fp32)
+  D     : for dQ dO.out of the output as rounded: sum_f |dO| (P |v|) (rP + wP + Lk u32) + (r + d u32) |dO|.|out|; for dK and dw the sum
+          over the keys of P dP: (rP + (Lk + 8) u32) (sum_j P |dP| + |D|) + sum_j P d u32 |dO|.|v|
   dS    : |dS| (rP + 4 u32) + P (d u32 |dO|.|v| + d(D))
   dQ    : scale sum_j (d(dS) + |dS| (wP + Lk u32)) |k| + r |dQ|, dK alike; dV: sum_i P |dO| (rP + wP + Lq u32) + r |dV|
   dw    : sum over the bucket of d(dS) + |dS| (Lq + Lk + B) u32, + r |dw|
@@ -20,7 +21,7 @@ U32 = 2.0 ** -24
 def bias_reference(q, k, v, w, buckets, mask=None, mat=None, block=0, offset=0, do=None):
     """Returns {"out", "p", and with do "dq", "dk", "dv", "dw"}: each (value, bound) in float64 on the inputs' device."""
     bf = q.dtype == torch.bfloat16
-    r, wP, wD = (2.0 ** -8, 2.0 ** -8, 2.0 ** -15) if bf else (2 * U32, 0.0, 0.0)
+    r, wP = (2.0 ** -8, 2.0 ** -8) if bf else (2 * U32, 2 * U32)
     q, k, v, w = (x.detach().double() for x in (q, k, v, w))
     B, H, Lq, d = q.shape
     Lk = k.shape[2]
@@ -59,10 +60,13 @@ def bias_reference(q, k, v, w, buckets, mask=None, mat=None, block=0, offset=0, 
     dp = do @ v.transpose(-1, -2).contiguous()
     D = (do * out).sum(-1, keepdim=True)
     ds = p * (dp - D)
-    dD = (do.abs() * pv).sum(-1, keepdim=True) * (rP + wD + Lk * U32) + d * U32 * (do.abs() * out.abs()).sum(-1, keepdim=True)
-    dds = ds.abs() * (rP + 4 * U32) + p * (d * U32 * (do.abs() @ v.abs().transpose(-1, -2).contiguous()) + dD)
+    ddp = d * U32 * (do.abs() @ v.abs().transpose(-1, -2).contiguous())
+    dD = (do.abs() * pv).sum(-1, keepdim=True) * (rP + wP + Lk * U32) + (r + d * U32) * (do.abs() * out.abs()).sum(-1, keepdim=True)
+    dds = ds.abs() * (rP + 4 * U32) + p * (ddp + dD)
     dq = scale * ds @ k
     res["dq"] = dq, scale * ((dds + ds.abs() * (wP + Lk * U32)) @ k.abs()) + r * dq.abs()
+    dD = (rP + (Lk + 8) * U32) * ((p * dp.abs()).sum(-1, keepdim=True) + D.abs()) + (p * ddp).sum(-1, keepdim=True)
+    dds = ds.abs() * (rP + 4 * U32) + p * (ddp + dD)
     tr = lambda x: x.transpose(-1, -2).contiguous()  # noqa: E731
     dk = scale * tr(ds) @ q
     res["dk"] = dk, scale * (tr(dds + ds.abs() * (wP + Lq * U32)) @ q.abs()) + r * dk.abs()

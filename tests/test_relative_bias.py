@@ -99,7 +99,7 @@ def test_c_entry_points_refuse_before_any_gpu_work():
     bad = [dict(batch=0), dict(q_len=0), dict(k_len=-1), dict(head_dim=48), dict(num_buckets=0), dict(num_buckets=32768), dict(max_distance=0),
            dict(max_distance=1025), dict(offset=1 << 30), dict(q_len=(1 << 29) + 1), dict(batch=1 << 20, heads=1 << 10),
            dict(mat=at, block_size=16), dict(mat=at, block_size=32, offset=1), dict(mat=at, block_size=32, k_len=65),
-           dict(key_mask=at, mask_bytes=2), dict(weight=None), dict(Lse=None), dict(buckets=None), dict(OutLow=at + 2),
+           dict(key_mask=at, mask_bytes=2), dict(weight=None), dict(Lse=None), dict(buckets=None),
            dict(Q=rb._Heads(None, 0, 0, 32)), dict(K=rb._Heads(at + 4, 0, 0, 32)), dict(V=rb._Heads(at, 2, 0, 32)),
            dict(Out=rb._Heads(at, 0, -32, 32))]
     for kw in bad + [dict(Out=rb._Heads(at, 0, 0, 0)), dict(Mean=at, mat=at, block_size=32)]:
