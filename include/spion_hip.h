@@ -484,7 +484,8 @@ int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, i
  * fp32 or bf16 tensors, sums and softmax in fp32; the probabilities are never written.  Sizes come with every call; there is no
  * handle, nothing is kept between calls, and the workspace is the caller's: calls with workspaces of their own may overlap.
  *   heads        [B][H][L][d] tensors or views, strides in elements, multiples of 16 bytes; pointers 16-byte aligned; d = 32 or 64.
- *                The strides of tensors that are only read may be 0 (a head shared by others).
+ *                The strides of tensors that are only read may be 0 (a head shared by others).  Rows lie up to 2^24 bytes apart,
+ *                a head within 2^31 bytes.
  *   weight       [num_buckets][heads], of the heads' type, up to 32767 buckets; dweight alike.
  *   buckets      [2 R + 1] ints in 0 .. num_buckets - 1 (anything else is read as the nearest of them); 1 <= R <= 1024.
  *   offset       query i stands at position i + offset of the keys' count.
@@ -496,8 +497,8 @@ int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, i
  *   Lse          [batch * heads][q_len] fp32, out of the forward and into the backward: log2 Z_i, +infinity for empty rows.
  *   Mean         null, or [q_len][k_len] fp32, out: the mean of P over batch and heads (spion_pattern_generate's Score input);
  *                not with mat.
- *   workspace    spion_bias_workspace(call, backward) floats, contents unspecified; a forward without it walks long rows in one
- *                piece.  The backward's gradients come out the same in every call with the same inputs.
+ *   workspace    spion_bias_workspace(call, backward) floats, 16-byte aligned, contents unspecified; a forward without it walks
+ *                long rows in one piece.  The backward's gradients come out the same in every call with the same inputs.
  * Each returns 0 on success (spion_bias_workspace: -1 on failure).
  * ---------------------------------------------------------------------------------------------- */
 #define SPION_BIAS_MAX_DISTANCE 1024

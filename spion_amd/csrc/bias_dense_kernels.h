@@ -1,7 +1,9 @@
 // The kernels of bias_kernels.h for calls without a pattern that have queries (column pass: keys) enough to fill the machine with
 // strips of 128 rows: each of a work-group's four wavefronts has 32 rows of its own, and the tiles of the other side are staged once
-// for all four, in two buffers taken in turn (one barrier a stage).  That is a quarter of the reads from L2, and of the work-groups
-// whose tables are set up and folded, and nothing is merged at the end.
+// for all four, in two buffers taken in turn (one barrier a stage).  That is a quarter of the reads from L2 and of the splitting of
+// fp32 values, and of the work-groups whose tables are set up and folded.  Where the strips alone do not fill the machine the
+// other side is cut into pieces; each leaves its sums in a slot of the workspace for every 32 rows, and a second launch adds the
+// pieces of a strip up in their order.
 #pragma once
 #include "bias_kernels.h"
 
@@ -17,22 +19,27 @@ struct BiasStage {
     static constexpr int N = ROWS * TL::CPR / 256;      // pieces of each tensor a thread moves
     static_assert(N * 256 == ROWS * TL::CPR, "whole pieces");
     PieceInFlight<T> x[N], y[N];
-    __device__ __forceinline__ void load(const char* xh, long long xld, const char* yh, long long yld, int first, int rows, int tid) {
+    __device__ __forceinline__ void load(const HeadBuf& xh, const HeadBuf& yh, int first, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int n = 256 * i + tid, r = min(first + n / TL::CPR, rows - 1), c = n % TL::CPR;
-            x[i].load(xh + r * xld + 8 * c * sizeof(T));
-            y[i].load(yh + r * yld + 8 * c * sizeof(T));
+            const int n = 256 * i + tid, r = n / TL::CPR, c = n % TL::CPR;
+            x[i].load(xh.r, xh.at(first, xh.at(r, 8 * c * (int)sizeof(T))));
+            y[i].load(yh.r, yh.at(first, yh.at(r, 8 * c * (int)sizeof(T))));
         }
     }
     // word[s]: which rows of tile s take part
     __device__ __forceinline__ void store(char* buf, const unsigned (&word)[SUBS], int tid) const {
+        if ((word[0] & word[SUBS - 1]) == ~0u) put<true>(buf, word, tid);
+        else put<false>(buf, word, tid);
+    }
+    template <bool ALL>
+    __device__ __forceinline__ void put(char* buf, const unsigned (&word)[SUBS], int tid) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int n = 256 * i + tid, r = n / TL::CPR, c = n % TL::CPR, s = r >> 5;
             const bool there = ((SUBS == 2 && s ? word[SUBS - 1] : word[0]) >> (r & 31)) & 1u;
-            x[i].template store<D>(buf + s * TL::BYTES, r & 31, c, there);
-            y[i].template store<D>(buf + (SUBS + s) * TL::BYTES, r & 31, c, there);
+            x[i].template store<D, ALL>(buf + s * TL::BYTES, r & 31, c, there);
+            y[i].template store<D, ALL>(buf + (SUBS + s) * TL::BYTES, r & 31, c, there);
         }
     }
 };
@@ -43,40 +50,58 @@ constexpr int bias_stages_bytes() {
     return stages > merge ? stages : merge;
 }
 
-// The stages of the other side, one after the other: the list's with a key mask, all of them without.  body(stage's first row, words).
+// The stages of a piece of the other side, one after the other: the list's with a key mask, all of them without.
+// body(stage's first row, words, buffer, its parity).
 template <class T, int D, bool KEYS, class Store, class Body>
-__device__ __forceinline__ void walk_stages(const BiasCall& a, ScanLds& sc, int b, int rows, const char* xh, long long xld,
-                                            const char* yh, long long yld, char* lds, int tid, Store&& fetched, Body&& body) {
+__device__ __forceinline__ void walk_stages(const BiasCall& a, ScanLds& sc, const BiasItem& it, int rows, const HeadBuf& xh,
+                                            const HeadBuf& yh, char* lds, int tid, Store&& fetched, Body&& body) {
     typedef BiasStage<T, D> ST;
     const bool listed = KEYS && a.mask;
-    const int tiles = (rows + 31) / 32, chunk = listed ? CHUNK : tiles;
+    const int from = it.split * a.per_split, to = min((rows + 31) / 32, from + a.per_split), chunk = listed ? CHUNK : a.per_split;
     int parity = 0, none = 0;
     if (!listed) __syncthreads();  // the tables are there
-    for (int first = 0; first < tiles; first += chunk) {
-        const int count = min(chunk, tiles - first);
-        const int n = listed ? scan_chunk<true, ST::SUBS>(a, sc, b, 0, first, count, tid, none) : (count + ST::SUBS - 1) / ST::SUBS;
-        auto unit = [&](int i) __attribute__((always_inline)) { return (listed ? uniform(sc.list[i]) : i) * ST::SUBS; };
+    for (int first = from; first < to; first += chunk) {
+        const int count = min(chunk, to - first);
+        const int n = listed ? scan_chunk<true, ST::SUBS>(a, sc, it.b, 0, first, count, tid, none) : (count + ST::SUBS - 1) / ST::SUBS;
+        // Which stage comes after next, and its words, are read from LDS while a stage is worked on.
+        struct Next {
+            int unit;
+            unsigned word[ST::SUBS];
+        };
+        auto look_up = [&](int i) __attribute__((always_inline)) {
+            Next x;
+            x.unit = listed ? (int)sc.list[min(i, n - 1)] : i;
+            if (listed) {
+#pragma unroll
+                for (int s = 0; s < ST::SUBS; ++s) x.word[s] = sc.words[x.unit * ST::SUBS + s];
+            }
+            return x;
+        };
         ST st;
-        int u = 0;
+        Next next, after;
         if (n > 0) {
-            u = unit(0);
-            st.load(xh, xld, yh, yld, (first + u) * 32, rows, tid);
-            fetched.load((first + u) * 32);
+            next = look_up(0);
+            next.unit = uniform(next.unit);
+            st.load(xh, yh, (first + next.unit * ST::SUBS) * 32, tid);
+            fetched.load((first + next.unit * ST::SUBS) * 32);
+            after = look_up(1);
         }
         for (int i = 0; i < n; ++i, parity ^= 1) {
+            const int u = next.unit * ST::SUBS, row0 = (first + u) * 32;
             unsigned word[ST::SUBS];
 #pragma unroll
             for (int s = 0; s < ST::SUBS; ++s)
-                word[s] = listed ? (u + s < count ? uniform(sc.words[u + s]) : 0u) : tail_word(rows - (first + u + s) * 32);
+                word[s] = listed ? (u + s < count ? (unsigned)uniform((int)next.word[s]) : 0u) : tail_word(rows - row0 - 32 * s);
             char* buf = lds + parity * ST::BYTES;
             st.store(buf, word, tid);
             fetched.store(parity);
             __syncthreads();
-            const int row0 = (first + u) * 32;
             if (i + 1 < n) {
-                u = unit(i + 1);
-                st.load(xh, xld, yh, yld, (first + u) * 32, rows, tid);
-                fetched.load((first + u) * 32);
+                next = after;
+                next.unit = uniform(next.unit);
+                st.load(xh, yh, (first + next.unit * ST::SUBS) * 32, tid);
+                fetched.load((first + next.unit * ST::SUBS) * 32);
+                after = look_up(i + 2);
             }
             body(row0, word, buf, parity);
         }
@@ -116,14 +141,14 @@ __device__ __forceinline__ void store_strip(const f32x16 (&acc)[D / 32], float f
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(256, 2) void bias_forward_dense_kernel(BiasCall a) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_dense_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     typedef BiasStage<T, D> ST;
     constexpr int SUBS = ST::SUBS;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_stages_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
-    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
     fill_bias<T>(a, it.h, tab, tid);
     const int q0 = it.strip * 128 + w * 32;
@@ -132,17 +157,22 @@ __global__ __launch_bounds__(256, 2) void bias_forward_dense_kernel(BiasCall a) 
     const typename TL::At at = TL::at(l);
     const float c2 = a.scale * LOG2E;
     const int qpos = q0 + a.off, far = 2 * (a.R + BIAS_PAD);
+    q.settled();
 
     f32x16 o[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) o[c] = splat16(0.f);
     float m = -__builtin_inff(), z = 0.f;
-    walk_stages<T, D, true>(a, sc, it.b, a.Lk, a.k.head(it.b, it.h), a.k.row, a.v.head(it.b, it.h), a.v.row, lds, tid, NothingElse(),
+    walk_stages<T, D, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, NothingElse(),
         [&](int k0, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
             if (!some) return;
             f32x16 s[SUBS];
+            typename TL::Row kr[SUBS];
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u) s[u] = TL::feat(TL::rows(buf + u * TL::BYTES, at), q);
+            for (int u = 0; u < SUBS; ++u) kr[u] = TL::rows(buf + u * TL::BYTES, at);
+            issue_order();
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) s[u] = TL::feat(kr[u], q);
             const int rel0 = k0 - qpos;
             bool whole = true;
 #pragma unroll
@@ -163,7 +193,8 @@ __global__ __launch_bounds__(256, 2) void bias_forward_dense_kernel(BiasCall a) 
             } else {
 #pragma unroll
                 for (int u = 0; u < SUBS; ++u) {
-                    logits_of<true>(s[u], c2, tab, a.R, rel0 + 32 * u, li, h, word[u], t[u]);
+                    if (whole) logits_of<false>(s[u], c2, tab, a.R, rel0 + 32 * u, li, h, word[u], t[u]);
+                    else logits_of<true>(s[u], c2, tab, a.R, rel0 + 32 * u, li, h, word[u], t[u]);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) mt = fmaxf(mt, t[u][r]);
                 }
@@ -188,12 +219,24 @@ __global__ __launch_bounds__(256, 2) void bias_forward_dense_kernel(BiasCall a) 
                     p[r] = __builtin_amdgcn_exp2f(fmaf(t[u][r], mul, add));
                     z += p[r];
                 }
-                TL::add_t(buf + (SUBS + u) * TL::BYTES, at, p, o);
+                TL::add_t(TL::columns(buf + (SUBS + u) * TL::BYTES, at), p, o);
             }
         });
     z = half_swap_sum(z);
     __syncthreads();  // the stages are done with
     if (!some) return;
+    if (a.splits > 1) {
+        float* slot = a.part + it.slot(a, w) * bias_slot<D>();
+        if (h == 0) {
+            slot[32 * D + li] = m;
+            slot[32 * D + 32 + li] = z;
+            slot[32 * D + 64 + li] = 0.f;
+        }
+        store_strip<D>(o, 1.f, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
+            store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
+        });
+        return;
+    }
     if (h == 0 && q0 + li < a.Lq)
         a.lse[(size_t)it.bh * a.Lq + q0 + li] = z > 0.f ? m + __builtin_amdgcn_logf(z) : __builtin_inff();
     store_strip<D>(o, z > 0.f ? 1.f / z : 0.f, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
@@ -201,15 +244,30 @@ __global__ __launch_bounds__(256, 2) void bias_forward_dense_kernel(BiasCall a) 
     });
 }
 
+// Sums of the same eight features (D = 64; four for 32) of `pieces` slots, in their order.
+template <int D>
+__device__ __forceinline__ void add_pieces(const float* p, int pieces, int stride, float (&x)[D / 8]) {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < pieces; ++k)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p + (size_t)k * stride + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e];
+        }
+}
+
 template <class T, int D>
-__global__ __launch_bounds__(256, 2) void bias_backward_row_dense_kernel(BiasCall a) {
+__global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_dense_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     typedef BiasStage<T, D> ST;
     constexpr int SUBS = ST::SUBS;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_stages_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
-    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
     fill_bias<T>(a, it.h, tab, tid);
     const int q0 = it.strip * 128 + w * 32, qi = min(q0 + li, a.Lq - 1);
@@ -223,19 +281,25 @@ __global__ __launch_bounds__(256, 2) void bias_backward_row_dense_kernel(BiasCal
     const float c2 = a.scale * LOG2E;
     const int qpos = q0 + a.off;
     const f32x16 minus = splat16(-delta);
+    q.settled();
+    go.settled();
     f32x16 dq[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
     float sum = 0.f;
-    walk_stages<T, D, true>(a, sc, it.b, a.Lk, a.k.head(it.b, it.h), a.k.row, a.v.head(it.b, it.h), a.v.row, lds, tid, NothingElse(),
+    walk_stages<T, D, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, NothingElse(),
         [&](int k0, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
             if (!some) return;
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) {
                 if (word[u] == 0) continue;
                 const char *tk = buf + u * TL::BYTES, *tv = buf + (SUBS + u) * TL::BYTES;
-                const f32x16 s = TL::feat(TL::rows(tk, at), q);
-                const f32x16 dp = TL::feat(TL::rows(tv, at), go, minus);  // dP - D
+                const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
+                typename TL::Columns kt;
+                if (TL::EARLY) kt = TL::columns(tk, at);
+                issue_order();
+                const f32x16 s = TL::feat(kr, q);
+                const f32x16 dp = TL::feat(vr, go, minus);  // dP - D
                 const int rel0 = k0 + 32 * u - qpos;
                 float ds[16];
                 if (word[u] == ~0u && (rel0 - 31 >= a.R || rel0 + 31 <= -a.R)) {
@@ -244,22 +308,52 @@ __global__ __launch_bounds__(256, 2) void bias_backward_row_dense_kernel(BiasCal
                     for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, add)) * dp[r];
                 } else {
                     float t[16];
-                    logits_of<true>(s, c2, tab, a.R, rel0, li, h, word[u], t);
+                    if (word[u] == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word[u], t);
+                    else logits_of<true>(s, c2, tab, a.R, rel0, li, h, word[u], t);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(t[r] - lse) * dp[r];
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sum += ds[r];
-                TL::add_t(tk, at, ds, dq);
+                if (!TL::EARLY) kt = TL::columns(tk, at);
+                TL::add_t(kt, ds, dq);
             }
         });
     sum = half_swap_sum(sum);
-    if (h == 0 && there) a.delta[stat] = delta + sum;
     __syncthreads();  // the stages are done with
-    if (some)
+    if (!some) return;
+    if (a.splits > 1) {
+        float* slot = a.part + it.slot(a, w) * bias_slot<D>();
+        if (h == 0) {
+            slot[32 * D + li] = sum;
+            slot[32 * D + 32 + li] = delta;
+        }
+        store_strip<D>(dq, a.scale, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
+            store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
+        });
+    } else {
+        if (h == 0 && there) a.delta[stat] = delta + sum;
         store_strip<D>(dq, a.scale, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
             if (q0 + row < a.Lq) store_eighth<T, D>(a.dq, it.b, it.h, q0 + row, j, x);
         });
+    }
+}
+
+// The pieces of 32 rows of dQ and D.
+template <class T, int D>
+__global__ __launch_bounds__(256) void bias_merge_row_kernel(BiasCall a) {
+    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7;
+    const int strips = (a.Lq + 31) / 32, strip = blockIdx.x % strips, bh = blockIdx.x / strips, q = strip * 32 + row;
+    if (q >= a.Lq) return;
+    const float* slot = a.part + (size_t)blockIdx.x * a.splits * bias_slot<D>();
+    float x[D / 8];
+    add_pieces<D>(slot + row * D + j * (D / 8), a.splits, bias_slot<D>(), x);
+    store_eighth<T, D>(a.dq, bh / a.H, bh % a.H, q, j, x);
+    if (j == 0) {
+        float s = slot[32 * D + row];
+        for (int k = 1; k < a.splits; ++k) s += slot[k * bias_slot<D>() + 32 * D + row];
+        a.delta[(size_t)bh * a.Lq + q] = slot[32 * D + 32 + row] + s;
+    }
 }
 
 // The stage's queries' lse, -D and, for tiles far behind and far ahead, what the outermost buckets' bias leaves of lse.
@@ -288,7 +382,7 @@ struct QueryStats {
 };
 
 template <class T, int D>
-__global__ __launch_bounds__(256, 2) void bias_backward_col_dense_kernel(BiasCall a) {
+__global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_dense_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     typedef BiasStage<T, D> ST;
     constexpr int SUBS = ST::SUBS;
@@ -297,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void bias_backward_col_dense_kernel(BiasCal
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
     HistLds hl(sc, a.R);
     float* stats = reinterpret_cast<float*>(lds + bias_stages_bytes<T, D>() + bias_floats(a.R) * 4 + sizeof(ScanLds) + HistLds::bytes(a.R));
-    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
     fill_bias<T>(a, it.h, tab, tid, hl.bucket);
     hl.clear(a.R, tid);
@@ -313,8 +407,10 @@ __global__ __launch_bounds__(256, 2) void bias_backward_col_dense_kernel(BiasCal
     for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = splat16(0.f);
     QueryStats qs{a.lse + (size_t)it.bh * a.Lq, a.delta + (size_t)it.bh * a.Lq, stats,
                   bias_weight<T>(a, bucket_at(a, -a.R), it.h), bias_weight<T>(a, bucket_at(a, a.R), it.h), a.Lq, tid};
+    k.settled();
+    v.settled();
     if (__syncthreads_or(some))
-        walk_stages<T, D, false>(a, sc, it.b, a.Lq, a.q.head(it.b, it.h), a.q.row, a.dout.head(it.b, it.h), a.dout.row, lds, tid, qs,
+        walk_stages<T, D, false>(a, sc, it, a.Lq, HeadBuf::of<T, D>(a.q, it.b, it.h, a.Lq), HeadBuf::of<T, D>(a.dout, it.b, it.h, a.Lq), lds, tid, qs,
             [&](int r0, const unsigned (&)[SUBS], const char* buf, int parity) __attribute__((always_inline)) {
                 if (!some) return;
 #pragma unroll
@@ -329,8 +425,12 @@ __global__ __launch_bounds__(256, 2) void bias_backward_col_dense_kernel(BiasCal
 #pragma unroll
                         for (int j = 0; j < 4; ++j) dp[4 * g + j] = d[j];
                     }
-                    const f32x16 s = TL::feat(TL::rows(tq, at), k);
-                    dp = TL::feat(TL::rows(tg, at), v, dp);  // dP - D
+                    const typename TL::Row qr = TL::rows(tq, at), gr = TL::rows(tg, at);
+                    typename TL::Columns qt, gt;
+                    if (TL::EARLY) qt = TL::columns(tq, at), gt = TL::columns(tg, at);
+                    issue_order();
+                    const f32x16 s = TL::feat(qr, k);
+                    dp = TL::feat(gr, v, dp);  // dP - D
                     const int rel0 = k0 - r0 - 32 * u - a.off;  // of the tile's corner: lane li, row r has rel0 + li - r
                     const bool near = sums.touches(rel0);
                     float p[16], ds[16];
@@ -358,28 +458,174 @@ __global__ __launch_bounds__(256, 2) void bias_backward_col_dense_kernel(BiasCal
                     }
                     if (near) sums.near(rel0, ds, li, h);
                     else sums.far(rel0, ds);
-                    TL::add_t(tg, at, p, dv);
-                    TL::add_t(tq, at, ds, dk);
+                    if (!TL::EARLY) gt = TL::columns(tg, at);
+                    TL::add_t(gt, p, dv);
+                    if (!TL::EARLY) qt = TL::columns(tq, at);
+                    TL::add_t(qt, ds, dk);
                 }
             });
     sums.finish(l);
     __syncthreads();  // the stages are done with, the histograms whole
     float* red = reinterpret_cast<float*>(lds);
     const unsigned keys = (unsigned)__ballot(key);
-    // (a key that is left out: what it holds has reached its own lane, and nothing else)
-    store_strip<D>(dv, 1.f, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
-        if (k0 + row >= a.Lk) return;
+    if (a.splits > 1) {
+        if (k0 < a.Lk) {
+            float* slot = a.part + it.slot(a, w) * (2 * 32 * D);
+            store_strip<D>(dv, 1.f, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
+                store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
+            });
+            store_strip<D>(dk, a.scale, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
+                store_values<float, D / 8>(reinterpret_cast<char*>(slot + 32 * D + row * D + j * (D / 8)), x);
+            });
+        }
+    } else {
+        // (a key that is left out: what it holds has reached its own lane, and nothing else)
+        store_strip<D>(dv, 1.f, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
+            if (k0 + row >= a.Lk) return;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) x[i] = key_bit(keys, row) ? x[i] : 0.f;
-        store_eighth<T, D>(a.dv, it.b, it.h, k0 + row, j, x);
-    });
-    store_strip<D>(dk, a.scale, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
-        if (k0 + row >= a.Lk) return;
+            for (int i = 0; i < D / 8; ++i) x[i] = key_bit(keys, row) ? x[i] : 0.f;
+            store_eighth<T, D>(a.dv, it.b, it.h, k0 + row, j, x);
+        });
+        store_strip<D>(dk, a.scale, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
+            if (k0 + row >= a.Lk) return;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) x[i] = key_bit(keys, row) ? x[i] : 0.f;
-        store_eighth<T, D>(a.dk, it.b, it.h, k0 + row, j, x);
-    });
-    fold_hists(hl.hist, hl.bucket, bias_entries(a.R), a.buckets, tid, a.part + ((size_t)it.bh * a.strips + it.strip) * a.buckets);
+            for (int i = 0; i < D / 8; ++i) x[i] = key_bit(keys, row) ? x[i] : 0.f;
+            store_eighth<T, D>(a.dk, it.b, it.h, k0 + row, j, x);
+        });
+    }
+    fold_hists(hl.hist, hl.bucket, bias_entries(a.R), a.buckets, tid,
+               a.tables + (((size_t)it.bh * a.strips + it.strip) * a.splits + it.split) * a.buckets);
+}
+
+// The pieces of 32 rows of dV and dK.
+template <class T, int D>
+__global__ __launch_bounds__(256) void bias_merge_col_kernel(BiasCall a) {
+    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7;
+    const int strips = (a.Lk + 31) / 32, strip = blockIdx.x % strips, bh = blockIdx.x / strips, b = bh / a.H, h = bh % a.H;
+    const int key = strip * 32 + row;
+    if (key >= a.Lk) return;
+    const float* slot = a.part + (size_t)blockIdx.x * a.splits * (2 * 32 * D) + row * D + j * (D / 8);
+    const bool keep = key_there(a, b, key);
+    float x[D / 8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        add_pieces<D>(slot + t * 32 * D, a.splits, 2 * 32 * D, x);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) x[i] = keep ? x[i] : 0.f;
+        store_eighth<T, D>(t ? a.dk : a.dv, b, h, key, j, x);
+    }
+}
+
+// -------------------------------------------------------------------------------------------------
+// Mean probability map of all samples and heads
+// -------------------------------------------------------------------------------------------------
+// A work-group has 64 x 64 pairs of the map and goes through the samples of the heads, one head after the other; its wavefronts
+// have a quarter of the pairs each.  Q and K of a pair of tiles are staged (and fp32 ones split) once for all four,
+// probabilities are formed from the forward's lse, added up in registers and never written.  Where the tiles alone do not fill
+// the machine the (head, sample) pairs are cut into pieces whose sums a second launch adds up.  (A tile of 32 x 32 a wavefront,
+// operands straight from memory, bias and lse gathered for each pair: 275 us against NEW, fp32, 128 heads of 1024.)
+template <class T, int D>
+constexpr int bias_mean_bytes() {
+    const int tiles = 4 * BiasTile<T, D>::BYTES, map = 64 * 65 * 4;
+    return tiles > map ? tiles : map;
+}
+template <class T, int D>
+__global__ __launch_bounds__(256) void bias_mean_kernel(BiasCall a) {
+    typedef BiasTile<T, D> TL;
+    constexpr int N = 64 * TL::CPR / 256;  // pieces of each tensor a thread moves
+    __shared__ __attribute__((aligned(16))) char lds[bias_mean_bytes<T, D>()];
+    __shared__ float tab[128];  // the head's bias of differences -63 .. 63 from the tile's corner
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
+    const int kt = (a.Lk + 63) / 64, all = a.B * a.H;
+    int tile = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = tile % a.splits;
+    tile /= a.splits;
+    const int q0 = tile / kt * 64, k0 = tile % kt * 64, qw = 32 * (w >> 1), kw = 32 * (w & 1);
+    const int corner = k0 - q0 - a.off;
+    const bool far = corner - 63 >= a.R || corner + 63 <= -a.R;  // one bucket
+    const int bucket = bucket_at(a, corner + min(tid, 126) - 63);
+    const float c2 = a.scale * LOG2E;
+    const typename TL::At at = TL::at(l);
+    const int q = q0 + qw + li;
+    float sum[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[r] = 0.f;
+
+    PieceInFlight<T> x[N], y[N];
+    float lse = 0.f, bias = 0.f;
+    bool key = false;
+    const int end = (int)((long long)all * (split + 1) / a.splits);
+    int i = (int)((long long)all * split / a.splits);
+    auto fetch = [&](int i) __attribute__((always_inline)) {  // pair i: sample i % B of head i / B
+        const int ih = uniform(i / a.B), b = uniform(i - ih * a.B);
+        const HeadBuf qh = HeadBuf::of<T, D>(a.q, b, ih, a.Lq), kh = HeadBuf::of<T, D>(a.k, b, ih, a.Lk);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int r = (256 * n + tid) / TL::CPR, c = (256 * n + tid) % TL::CPR;
+            x[n].load(qh.r, qh.at(q0, qh.at(r, 8 * c * (int)sizeof(T))));
+            y[n].load(kh.r, kh.at(k0, kh.at(r, 8 * c * (int)sizeof(T))));
+        }
+        key = key_there(a, b, k0 + l);
+        lse = q < a.Lq ? a.lse[((size_t)b * a.H + ih) * a.Lq + q] : __builtin_inff();
+        bias = bias_weight<T>(a, bucket, ih);
+    };
+    if (i < end) fetch(i);
+    for (; i < end; ++i) {
+        const unsigned long long there = __ballot(key);
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int r = (256 * n + tid) / TL::CPR, c = (256 * n + tid) % TL::CPR, s = r >> 5;
+            x[n].template store<D, true>(lds + s * TL::BYTES, r & 31, c, true);
+            if (there == ~0ull) y[n].template store<D, true>(lds + (2 + s) * TL::BYTES, r & 31, c, true);
+            else y[n].template store<D, false>(lds + (2 + s) * TL::BYTES, r & 31, c, (there >> r) & 1u);
+        }
+        if (tid < 127) tab[tid] = bias;
+        const float row = lse;
+        __syncthreads();
+        if (i + 1 < end) fetch(i + 1);
+        const unsigned word = (unsigned)(there >> kw);
+        if (word == 0) continue;
+        const typename TL::Row kr = TL::rows(lds + (2 + (w & 1)) * TL::BYTES, at), qr = TL::rows(lds + (w >> 1) * TL::BYTES, at);
+        const f32x16 s = TL::feat(kr, qr);  // rows: keys, lanes: queries
+        float t[16];
+        if (far) {
+            const float add = tab[0] - row;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t[r] = fmaf(s[r], c2, add);
+        } else {
+            const float* bias_at = tab + 63 + kw - qw - li + 4 * h;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t[r] = fmaf(s[r], c2, bias_at[8 * (r >> 2) + (r & 3)] - row);
+        }
+        if (word == ~0u) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[r] += __builtin_amdgcn_exp2f(t[r]);
+        } else {
+            const unsigned mine = word >> (4 * h);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[r] += (mine >> (8 * (r >> 2) + (r & 3))) & 1u ? __builtin_amdgcn_exp2f(t[r]) : 0.f;
+        }
+    }
+    // queries to the rows
+    __syncthreads();
+    float* map = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) map[(qw + li) * 65 + kw + acc_row(r, h)] = sum[r];
+    __syncthreads();
+    const float inv = a.splits > 1 ? 1.f : 1.f / all;
+    float* out = a.splits > 1 ? a.part + (size_t)split * a.Lq * a.Lk : a.mean;
+    if (k0 + l < a.Lk)
+        for (int r = w; r < min(64, a.Lq - q0); r += 4) out[(size_t)(q0 + r) * a.Lk + k0 + l] = map[r * 65 + l] * inv;
+}
+// The pieces' maps, in their order.
+__global__ __launch_bounds__(256) void bias_mean_merge_kernel(const float* __restrict__ part, float* __restrict__ mean, long long n,
+                                                              int splits, float inv) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        float s = part[i];
+        for (int k = 1; k < splits; ++k) s += part[k * n + i];
+        mean[i] = s * inv;
+    }
 }
 
 }  // namespace spion

@@ -66,6 +66,10 @@ struct BiasItem {
         b = bh / a.H;
         h = bh - b * a.H;
     }
+    // wavefront w's slot in a launch with strips of 128: the pieces of 32 rows lie next to each other
+    __device__ __forceinline__ size_t slot(const BiasCall& a, int w) const {
+        return ((size_t)bh * a.strips32 + strip * 4 + w) * a.splits + split;
+    }
 };
 
 // Wavefronts a SIMD that the registers are for.  fp32 heads of 64 features have one work-group's tiles in a CU's LDS.
@@ -93,17 +97,18 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
-    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
     fill_bias<T>(a, it.h, tab, tid);
     const int q0 = it.strip * 32;
     const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + min(q0 + li, a.Lq - 1) * a.q.row, h, q0 + li < a.Lq);
-    const char *kh = a.k.head(it.b, it.h), *vh = a.v.head(it.b, it.h);
+    const HeadBuf kh = HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), vh = HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk);
     const typename TL::At at = TL::at(l);
     char* tk = lds + w * 2 * TL::BYTES;
     char* tv = tk + TL::BYTES;
     const float c2 = a.scale * LOG2E;
     const int qpos = q0 + a.off;
+    q.settled();
 
     f32x16 o[D / 32];
 #pragma unroll
@@ -116,9 +121,9 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
         const int n = scan_chunk<true>(a, sc, it.b, it.strip, first, min(CHUNK, t1 - first), tid, in_pattern);
         TileInFlight<T, D> fk, fv;
         auto fetch = [&](int i) __attribute__((always_inline)) {
-            const int j = (first + sc.list[i]) * 32;
-            fk.load(kh, a.k.row, j, a.Lk, l);
-            fv.load(vh, a.v.row, j, a.Lk, l);
+            const int j = (first + uniform(sc.list[i])) * 32;
+            fk.load(kh, j, l);
+            fv.load(vh, j, l);
         };
         if (w < n) fetch(w);
         for (int i = w; i < n; i += 4) {
@@ -129,7 +134,11 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
             fv.store(tv, word, l);
             wave_lds_order();
             if (i + 4 < n) fetch(i + 4);
-            const f32x16 s = TL::feat(TL::rows(tk, at), q);
+            const typename TL::Row kr = TL::rows(tk, at);
+            typename TL::Columns vt;
+            if (TL::EARLY) vt = TL::columns(tv, at);
+            issue_order();
+            const f32x16 s = TL::feat(kr, q);
             float t[16];
             const int rel0 = (first + tile) * 32 - qpos;
             if (word == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word, t);
@@ -155,7 +164,8 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
                 p[r] = __builtin_amdgcn_exp2f(t[r] - base);
                 z += p[r];
             }
-            TL::add_t(tv, at, p, o);
+            if (!TL::EARLY) vt = TL::columns(tv, at);
+            TL::add_t(vt, p, o);
         }
     }
     // the four wavefronts' parts
@@ -215,7 +225,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
 template <class T, int D>
 __global__ __launch_bounds__(256) void bias_merge_kernel(BiasCall a) {
     const int tid = threadIdx.x, row = tid >> 3, j = tid & 7;
-    const int strip = blockIdx.x % a.strips, bh = blockIdx.x / a.strips, b = bh / a.H, ih = bh - b * a.H;
+    const int strip = blockIdx.x % a.strips32, bh = blockIdx.x / a.strips32, b = bh / a.H, ih = bh - b * a.H;
     const float* slot = a.part + (size_t)blockIdx.x * a.splits * bias_slot<D>();
     float M = -__builtin_inff();
     int in_pattern = 0;
@@ -266,7 +276,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_k
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
-    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
     fill_bias<T>(a, it.h, tab, tid);
     const int q0 = it.strip * 32, qi = min(q0 + li, a.Lq - 1);
@@ -276,7 +286,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_k
     const size_t stat = (size_t)it.bh * a.Lq + qi;
     const float lse = there ? a.lse[stat] : __builtin_inff();
     const float delta = half_swap_sum(TL::dot(go, TL::load(a.o.head(it.b, it.h) + qi * a.o.row, h, there)));
-    const char *kh = a.k.head(it.b, it.h), *vh = a.v.head(it.b, it.h);
+    const HeadBuf kh = HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), vh = HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk);
     const typename TL::At at = TL::at(l);
     char* tk = lds + w * 2 * TL::BYTES;
     char* tv = tk + TL::BYTES;
@@ -284,6 +294,8 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_k
     const int qpos = q0 + a.off;
 
     const f32x16 minus = splat16(-delta);
+    q.settled();
+    go.settled();
     f32x16 dq[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
@@ -294,9 +306,9 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_k
         const int n = scan_chunk<true>(a, sc, it.b, it.strip, first, min(CHUNK, tiles - first), tid, in_pattern);
         TileInFlight<T, D> fk, fv;
         auto fetch = [&](int i) __attribute__((always_inline)) {
-            const int j = (first + sc.list[i]) * 32;
-            fk.load(kh, a.k.row, j, a.Lk, l);
-            fv.load(vh, a.v.row, j, a.Lk, l);
+            const int j = (first + uniform(sc.list[i])) * 32;
+            fk.load(kh, j, l);
+            fv.load(vh, j, l);
         };
         if (w < n) fetch(w);
         for (int i = w; i < n; i += 4) {
@@ -307,8 +319,12 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_k
             fv.store(tv, word, l);
             wave_lds_order();
             if (i + 4 < n) fetch(i + 4);
-            const f32x16 s = TL::feat(TL::rows(tk, at), q);
-            const f32x16 dp = TL::feat(TL::rows(tv, at), go, minus);  // dP - D
+            const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
+            typename TL::Columns kt;
+            if (TL::EARLY) kt = TL::columns(tk, at);
+            issue_order();
+            const f32x16 s = TL::feat(kr, q);
+            const f32x16 dp = TL::feat(vr, go, minus);  // dP - D
             float t[16];
             const int rel0 = (first + tile) * 32 - qpos;
             if (word == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word, t);
@@ -319,7 +335,8 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_k
                 ds[r] = __builtin_amdgcn_exp2f(t[r] - lse) * dp[r];
                 sum += ds[r];
             }
-            TL::add_t(tk, at, ds, dq);
+            if (!TL::EARLY) kt = TL::columns(tk, at);
+            TL::add_t(kt, ds, dq);
         }
     }
     sum = half_swap_sum(sum);
@@ -356,23 +373,21 @@ constexpr int BIAS_HISTS = 4, DIAG_COLS = 48, DIAG_FLOATS = 4 * DIAG_COLS * 4;
 // are never written are zeros
 __device__ __forceinline__ void add_diagonals(float* buf, float* hist, const float (&ds)[16], int li, int h) {
     const int l = li + 32 * h;
+    float* mine = buf + (h * DIAG_COLS + li - 4 * h + 15) * 4;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         wave_lds_order();
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                buf[((2 * g + h) * DIAG_COLS + li - (8 * g + 4 * h + e) + 15) * 4 + e] = ds[8 * half + 4 * g + e];
+            for (int e = 0; e < 4; ++e) mine[(2 * g * DIAG_COLS - 8 * g - e) * 4 + e] = ds[8 * half + 4 * g + e];
         wave_lds_order();
         if (l < DIAG_COLS - 1) {
-            float s = 0.f;
+            f32x4 v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(buf + (k * DIAG_COLS + l) * 4);
-                s += (v[0] + v[1]) + (v[2] + v[3]);
-            }
-            __hip_atomic_fetch_add(hist - 16 * half - 15 + l, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const f32x4*>(buf + (k * DIAG_COLS + l) * 4);
+            const f32x4 s = (v[0] + v[1]) + (v[2] + v[3]);
+            __hip_atomic_fetch_add(hist - 16 * half - 15 + l, (s[0] + s[1]) + (s[2] + s[3]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
     }
 }
@@ -445,7 +460,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_k
     float* tab = reinterpret_cast<float*>(lds + bias_tiles_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
     HistLds hl(sc, a.R);
-    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
     fill_bias<T>(a, it.h, tab, tid, hl.bucket);
     hl.clear(a.R, tid);
@@ -455,13 +470,15 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_k
     const bool key = key_there(a, it.b, k0 + li);
     const unsigned keys = (unsigned)__ballot(key);
     DifferenceSums sums(hl, w, a.R, key);
-    const char *qh = a.q.head(it.b, it.h), *gh = a.dout.head(it.b, it.h);
+    const HeadBuf qh = HeadBuf::of<T, D>(a.q, it.b, it.h, a.Lq), gh = HeadBuf::of<T, D>(a.dout, it.b, it.h, a.Lq);
     const float *lseh = a.lse + (size_t)it.bh * a.Lq, *deltah = a.delta + (size_t)it.bh * a.Lq;
     const typename TL::At at = TL::at(l);
     char* tq = lds + w * 2 * TL::BYTES;
     char* tg = tq + TL::BYTES;
     float* stats = sc.ml[w][0];  // lse of the tile's 32 queries, then their -D
     const float c2 = a.scale * LOG2E;
+    k.settled();
+    v.settled();
 
     f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
@@ -473,9 +490,9 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_k
         TileInFlight<T, D> fq, fg;
         float st = 0.f;
         auto fetch = [&](int i) __attribute__((always_inline)) {
-            const int r = (first + sc.list[i]) * 32;
-            fq.load(qh, a.q.row, r, a.Lq, l);
-            fg.load(gh, a.dout.row, r, a.Lq, l);
+            const int r = (first + uniform(sc.list[i])) * 32;
+            fq.load(qh, r, l);
+            fg.load(gh, r, l);
             st = r + li < a.Lq ? (h ? -deltah[r + li] : lseh[r + li]) : (h ? 0.f : __builtin_inff());
         };
         if (w < n) fetch(w);
@@ -496,8 +513,12 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_k
 #pragma unroll
                 for (int j = 0; j < 4; ++j) dp[4 * g + j] = d[j];
             }
-            const f32x16 s = TL::feat(TL::rows(tq, at), k);
-            dp = TL::feat(TL::rows(tg, at), v, dp);  // dP - D
+            const typename TL::Row qr = TL::rows(tq, at), gr = TL::rows(tg, at);
+            typename TL::Columns qt, gt;
+            if (TL::EARLY) qt = TL::columns(tq, at), gt = TL::columns(tg, at);
+            issue_order();
+            const f32x16 s = TL::feat(qr, k);
+            dp = TL::feat(gr, v, dp);  // dP - D
             const int rel0 = k0 - r0 - a.off;  // of the tile's corner: lane li, row r has rel0 + li - r
             const bool near = sums.touches(rel0);
             float p[16];
@@ -522,8 +543,10 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_k
             }
             if (near) sums.near(rel0, ds, li, h);
             else sums.far(rel0, ds);
-            TL::add_t(tg, at, p, dv);
-            TL::add_t(tq, at, ds, dk);
+            if (!TL::EARLY) gt = TL::columns(tg, at);
+            TL::add_t(gt, p, dv);
+            if (!TL::EARLY) qt = TL::columns(tq, at);
+            TL::add_t(qt, ds, dk);
         }
     }
     if (keys == 0) __syncthreads();  // the tables are there (a scan has seen to it otherwise)
@@ -545,72 +568,25 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_k
         for (int i = 0; i < D / 8; ++i) x[i] = keep ? x[i] * a.scale : 0.f;
         store_eighth<T, D>(a.dk, it.b, it.h, k0 + row, j, x);
     }
-    fold_hists(hl.hist, hl.bucket, bias_entries(a.R), a.buckets, tid, a.part + ((size_t)it.bh * a.strips + it.strip) * a.buckets);
+    fold_hists(hl.hist, hl.bucket, bias_entries(a.R), a.buckets, tid, a.tables + ((size_t)it.bh * a.strips + it.strip) * a.buckets);
 }
 
-// dw[k][h]: the strips of all samples, 256 partial sums in a fixed order.
+// dw[k][h]: the strips' pieces of all samples, 256 partial sums in a fixed order.
 template <class T>
 __global__ __launch_bounds__(256) void bias_table_kernel(BiasCall a, T* __restrict__ dw) {
     __shared__ float red[4];
     const int k = blockIdx.x % a.buckets, h = blockIdx.x / a.buckets, tid = threadIdx.x;
-    const int n = a.B * a.strips;
+    const int each = a.strips * a.splits, n = a.B * each;
     float s = 0.f;
 #pragma unroll 4
     for (int i = tid; i < n; i += 256) {
-        const int b = i / a.strips, strip = i - b * a.strips;
-        s += a.part[(((size_t)b * a.H + h) * a.strips + strip) * a.buckets + k];
+        const int b = i / each, piece = i - b * each;
+        s += a.tables[(((size_t)b * a.H + h) * each + piece) * a.buckets + k];
     }
     s = wave_sum(s);
     if ((tid & 63) == 0) red[tid >> 6] = s;
     __syncthreads();
     if (tid == 0) dw[(size_t)k * a.H + h] = (T)(red[0] + red[1] + red[2] + red[3]);
-}
-
-// -------------------------------------------------------------------------------------------------
-// Mean probability map of all samples and heads
-// -------------------------------------------------------------------------------------------------
-// A work-group has one 32 x 32 tile of the map and its wavefronts every fourth (sample, head); probabilities are formed from the
-// forward's lse, added up in registers and never written.
-template <class T, int D>
-__global__ __launch_bounds__(256) void bias_mean_kernel(BiasCall a) {
-    typedef BiasTile<T, D> TL;
-    __shared__ float red[4][16][64];
-    const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
-    const int kt = (a.Lk + 31) / 32, tile = xcd_remap(blockIdx.x, gridDim.x);
-    const int q0 = tile / kt * 32, k0 = tile % kt * 32;
-    const int qi = min(q0 + li, a.Lq - 1), ki = min(k0 + li, a.Lk - 1);
-    const float c2 = a.scale * LOG2E;
-    int bucket[16];  // of (query row r, key li)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) bucket[r] = bucket_at(a, k0 + li - (q0 + acc_row(r, h)) - a.off) * a.H;
-    float sum[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sum[r] = 0.f;
-    for (int bh = w; bh < a.B * a.H; bh += 4) {
-        const int b = bh / a.H, ih = bh - b * a.H;
-        const bool key = key_there(a, b, k0 + li);
-        if (!__any(key)) continue;
-        const typename TL::Row q = TL::load(a.q.head(b, ih) + qi * a.q.row, h, q0 + li < a.Lq);
-        const typename TL::Row k = TL::load(a.k.head(b, ih) + ki * a.k.row, h, key);
-        const f32x16 s = TL::feat(q, k);
-        const float* lse = a.lse + (size_t)bh * a.Lq;
-        const T* wh = reinterpret_cast<const T*>(a.w) + ih;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float t = fmaf(s[r], c2, (float)wh[bucket[r]] * LOG2E - lse[min(q0 + acc_row(r, h), a.Lq - 1)]);
-            sum[r] += key ? __builtin_amdgcn_exp2f(t) : 0.f;
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) red[w][r][l] = sum[r];
-    __syncthreads();
-    const float inv = 1.f / (a.B * a.H);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = 4 * w + i, qr = q0 + acc_row(r, h);
-        const float v = (red[0][r][l] + red[1][r][l]) + (red[2][r][l] + red[3][r][l]);
-        if (qr < a.Lq && k0 + li < a.Lk) a.mean[(size_t)qr * a.Lk + k0 + li] = v * inv;
-    }
 }
 
 }  // namespace spion

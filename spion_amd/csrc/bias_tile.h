@@ -11,6 +11,20 @@ struct HeadsAt {
     long long b, h, row;
     __device__ __forceinline__ const char* head(int ib, int ih) const { return p + ib * b + ih * h; }
 };
+// One head: its buffer, the bytes from row to row.  A head lies within 2^31 bytes and its rows 2^24 apart at most, so the offsets
+// of rows up to 64 behind its end still count; what lies behind the buffer reads as zeros.
+struct HeadBuf {
+    rsrc_t r;
+    int ld;
+    template <class T, int D>
+    __device__ static __forceinline__ HeadBuf of(const HeadsAt& t, int b, int h, int rows) {
+        // (the same in every lane, which the compiler does not see through the divisions that b and h come from)
+        const unsigned long long p = reinterpret_cast<unsigned long long>(t.head(b, h));
+        const unsigned long long q = (unsigned)uniform((int)(unsigned)p) | (unsigned long long)(unsigned)uniform((int)(p >> 32)) << 32;
+        return HeadBuf{make_rsrc(reinterpret_cast<const void*>(q), (unsigned)((rows - 1) * t.row + D * (int)sizeof(T))), (int)t.row};
+    }
+    __device__ __forceinline__ int at(int row, int byte) const { return (int)((unsigned)row * (unsigned)ld + (unsigned)byte); }
+};
 
 struct BiasCall {
     HeadsAt q, k, v, o, dout, dq, dk, dv;
@@ -20,11 +34,13 @@ struct BiasCall {
     const float* mat;   // [nb][nb] pattern of bs x bs blocks, or null
     float* lse;         // [B*H][Lq]: log2 of the softmax denominator, +inf for rows that nothing enters
     float* delta;       // [B*H][Lq]: sum over the keys of P dP
-    float* part;        // workspace
+    float* part;        // workspace: the pieces' slots
+    float* tables;      // workspace: the table's gradient by strips, [B*H][strips][splits][buckets]
     float* mean;        // [Lq][Lk]
     int B, H, Lq, Lk, R, buckets, off, bs, nb;
     int mask_bytes;     // 4 or 1
     int strips, splits, per_split;  // strips of 32 (or 128) rows, pieces of the other side, tiles of 32 to a piece
+    int strips32;                   // strips of 32 rows
     float scale;
 };
 
@@ -37,15 +53,25 @@ struct BiasCall {
 // eight values, piece c of row r at c ^ swz(r): sixteen rows' reads of one piece, and the transposing reads of four rows, meet every
 // bank once.
 //   rows()   lane (li, h) has features h*D/2 .. of row li, the operand of a product over the head dimension
-//   add_t()  out[c] += X^T . W, W given as the accumulator values of a 32 x 32 product whose rows are the tile's rows; the
+//   columns(), add_t()  out[c] += X^T . W, W given as the accumulator values of a 32 x 32 product whose rows are the tile's rows; the
 //            accumulator layout is then the other operand's, register for register after conversion.  With bf16 heads W's rounding
 //            is off by up to 2^-8 of each weight, as the outputs' own is; sums are fp32.
 template <class T, int D>
 struct BiasTile {
     static constexpr int IM = sizeof(T) == 4 ? 3 : 1;
+    // Whether the transposed operands are read ahead of the arithmetic that they come after: three images of them are too many registers.
+    static constexpr bool EARLY = IM == 1;
     static constexpr int ROW = D * 2, IMAGE = 32 * ROW, BYTES = IM * IMAGE, CPR = D / 8;
     struct Row {
         bf16x8 x[IM][D / 16];
+        // its loads waited for: else the compiler waits at the first use inside the walk, for the tiles just asked for as well
+        __device__ __forceinline__ void settled() const {
+#pragma unroll
+            for (int m = 0; m < IM; ++m) settle(x[m]);
+        }
+    };
+    struct Columns {
+        bf16x8 x[IM][D / 32][2];
     };
     struct At {
         int row[D / 16], col[D / 32][2];
@@ -132,7 +158,8 @@ struct BiasTile {
         return acc;
     }
     // the tile feature-major, with the transposing LDS read
-    __device__ static __forceinline__ void columns(const char* t, const At& a, bf16x8 (&xt)[IM][D / 32][2]) {
+    __device__ static __forceinline__ Columns columns(const char* t, const At& a) {
+        Columns xt;
         typedef s16x4 __attribute__((address_space(3))) * lds_ptr;
 #pragma unroll
         for (int m = 0; m < IM; ++m)
@@ -142,21 +169,20 @@ struct BiasTile {
                 for (int i = 0; i < 2; ++i) {
                     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + m * IMAGE + a.col[c][0] + 16 * i * ROW));
                     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + m * IMAGE + a.col[c][1] + 16 * i * ROW));
-                    xt[m][c][i] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+                    xt.x[m][c][i] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
                 }
+        return xt;
     }
-    __device__ static __forceinline__ void add_t(const char* t, const At& a, const float (&p)[16], f32x16 (&out)[D / 32]) {
-        bf16x8 xt[IM][D / 32][2];
-        columns(t, a, xt);
+    __device__ static __forceinline__ void add_t(const Columns& xt, const float (&p)[16], f32x16 (&out)[D / 32]) {
         if constexpr (IM == 1) {
             bf16x8 wb[2];
             pack16(p, wb);
-            mma_tile_bf16<D>(xt[0], wb, out);
+            mma_tile_bf16<D>(xt.x[0], wb, out);
         } else {
             const Split3<16> w = split3(p);
             constexpr int PAIRS[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
 #pragma unroll
-            for (int k = 0; k < 6; ++k) mma_tile_bf16<D>(xt[PAIRS[k][0]], w.p[PAIRS[k][1]], out);
+            for (int k = 0; k < 6; ++k) mma_tile_bf16<D>(xt.x[PAIRS[k][0]], w.p[PAIRS[k][1]], out);
         }
     }
 };
@@ -165,12 +191,12 @@ struct BiasTile {
 template <class T>
 struct PieceInFlight {
     u32x4 x[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const char* p) {
+    __device__ __forceinline__ void load(rsrc_t r, int at) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) x[i] = *reinterpret_cast<const u32x4*>(p + 16 * i);
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) x[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at + 16 * i, 0, 0));
     }
     // piece c of row r of tile t; a row that is left out becomes zeros (whatever lies in it: 0 times it is 0)
-    template <int D>
+    template <int D, bool ALL>
     __device__ __forceinline__ void store(char* t, int r, int c, bool there) const {
         typedef BiasTile<T, D> TL;
         u32x4 v[TL::IM];
@@ -178,7 +204,7 @@ struct PieceInFlight {
         else TL::split_values(__builtin_bit_cast(f32x4, x[0]), __builtin_bit_cast(f32x4, x[1]), v);
 #pragma unroll
         for (int m = 0; m < TL::IM; ++m) {
-            if (!there) v[m] = u32x4{0, 0, 0, 0};
+            if (!ALL && !there) v[m] = u32x4{0, 0, 0, 0};
             *reinterpret_cast<u32x4*>(t + m * TL::IMAGE + r * TL::ROW + 16 * (c ^ TL::swz(r))) = v[m];
         }
     }
@@ -190,23 +216,32 @@ struct TileInFlight {
     typedef BiasTile<T, D> TL;
     static constexpr int N = TL::CPR / 2;
     PieceInFlight<T> x[N];
-    // rows first .. first + 31 of a head of `rows` rows; behind its end the last one again, which store() leaves out
-    __device__ __forceinline__ void load(const char* head, long long ld, int first, int rows, int l) {
+    // rows first .. first + 31
+    __device__ __forceinline__ void load(const HeadBuf& head, int first, int l) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int n = 64 * i + l, r = n / TL::CPR, c = n % TL::CPR;
-            x[i].load(head + min(first + r, rows - 1) * ld + 8 * c * sizeof(T));
+            x[i].load(head.r, head.at(first, head.at(r, 8 * c * (int)sizeof(T))));
         }
     }
     // to LDS; rows whose bit of `word` is not set are left out
     __device__ __forceinline__ void store(char* t, unsigned word, int l) const {
+        if (word == ~0u) put<true>(t, word, l);
+        else put<false>(t, word, l);
+    }
+    template <bool ALL>
+    __device__ __forceinline__ void put(char* t, unsigned word, int l) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int n = 64 * i + l, r = n / TL::CPR, c = n % TL::CPR;
-            x[i].template store<D>(t, r, c, (word >> r) & 1u);
+            x[i].template store<D, ALL>(t, r, c, (word >> r) & 1u);
         }
     }
 };
+
+// What stands before is issued before what follows: LDS reads ahead of the arithmetic whose operands they are not, which the
+// compiler would move to their use, one register set and one full latency at a time.
+__device__ __forceinline__ void issue_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // Orders a wavefront's own LDS accesses (they complete in order; this is for the compiler).
 __device__ __forceinline__ void wave_lds_order() {
@@ -275,7 +310,7 @@ __device__ __forceinline__ unsigned tail_word(int left) { return left >= 32 ? ~0
 template <bool KEYS, int SUBS = 1>
 __device__ __forceinline__ int scan_chunk(const BiasCall& a, ScanLds& s, int b, int own, int first, int count, int tid,
                                           int& in_pattern) {
-    const int w = tid >> 6, l = tid & 63;
+    const int w = uniform(tid >> 6), l = tid & 63;
     __syncthreads();
     if (KEYS) {
         if (a.mask) {
@@ -339,7 +374,7 @@ template <int D>
 constexpr int merge_floats() { return 4 * 32 * (D + 4); }
 template <int D>
 __device__ __forceinline__ void merge_waves(const f32x16 (&acc)[D / 32], float* red, int tid, float (&x)[D / 8]) {
-    const int w = tid >> 6, l = tid & 63, li = l & 31, h = l >> 5;
+    const int w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     float* mine = red + (w * 32 + li) * (D + 4);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)

@@ -65,9 +65,10 @@ void fp32_or_bf16(const Tensor& t, const char* what) {
 // Heads as the kernels read them: themselves, or a copy where their strides or address are not theirs.
 Tensor readable_heads(const Tensor& t) {
     spion_head_layout lay{};
-    if (head_layout(t, lay)) return t;
+    const auto fits = [&](const Tensor& x) { return head_layout(x, lay) && x.stride(2) * x.element_size() <= 1 << 24; };
+    if (fits(t)) return t;
     const Tensor c = t.contiguous();
-    return head_layout(c, lay) ? c : t.clone(at::MemoryFormat::Contiguous);
+    return fits(c) ? c : t.clone(at::MemoryFormat::Contiguous);
 }
 Tensor empty_like_heads(const Tensor& t) { return empty_heads(t.sizes(), t.stride(1) < t.stride(2), t.options()); }
 spion_heads heads_of(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }

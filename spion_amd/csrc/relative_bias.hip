@@ -11,21 +11,66 @@ namespace spion {
 
 typedef spion_bias_attention Call;
 
-static long long strips_of(int rows) { return (rows + 31) / 32; }
+static long long strips_of(int rows, int strip = 32) { return (rows + strip - 1) / strip; }
+static int slot_floats(const Call& c) { return 32 * c.head_dim + 96; }  // bias_slot
 
-// Pieces of the keys a forward strip is walked in.  Launches with fewer work-groups than twice the machine's CUs are split
-// until they have that many, each wavefront keeping at least two tiles.
-static int forward_splits(const Call& c) {
-    const long long groups = (long long)c.batch * c.heads * strips_of(c.q_len), tiles = strips_of(c.k_len);
-    const long long want = (2LL * device_cus() + groups - 1) / groups, most = tiles / 8;
-    return (int)std::max(1LL, std::min({want, most, 64LL}));
+// How one side of a call is walked: in strips of 128 rows over shared stages, or of 32 with the tiles dealt to the wavefronts, and
+// the other side in `splits` pieces.
+struct Walk {
+    bool dense;
+    int strips, splits, per_split;  // tiles of 32 to a piece
+    void cut(long long tiles, long long pieces, int unit) {
+        const long long units = (tiles + unit - 1) / unit, each = (units + pieces - 1) / pieces;
+        per_split = (int)(each * unit);
+        splits = (int)((units + each - 1) / each);  // none of them empty
+    }
+};
+// Work-groups wanted: two for each CU.  Sides of more than two tiles without a pattern go in strips of 128; fewer strips than wanted
+// are cut into pieces of at least four stages of 64 rows (256 rows of the other side).  A launch that does not reach a work-group
+// for each CU even so goes in strips of 32.
+static Walk walk_of(const Call& c, int rows, int others, bool can_split) {
+    const long long heads = (long long)c.batch * c.heads, want = 2LL * device_cus(), tiles = strips_of(others);
+    Walk w{};
+    const long long wide = heads * strips_of(rows, 128);
+    long long pieces = std::max(1LL, std::min({(want + wide - 1) / wide, tiles / 8, 16LL}));
+    if (!can_split) pieces = 1;
+    if (!c.mat && rows > 64 && wide * pieces >= device_cus()) {
+        w.dense = true;
+        w.strips = (int)strips_of(rows, 128);
+        w.cut(tiles, pieces, 2);
+        return w;
+    }
+    w.strips = (int)strips_of(rows);
+    w.cut(tiles, 1, 1);
+    return w;
+}
+// The forward's strips of 32 rows go in pieces as well, each wavefront keeping at least two tiles.
+static Walk forward_walk(const Call& c, bool can_split) {
+    Walk w = walk_of(c, c.q_len, c.k_len, can_split);
+    if (w.dense || !can_split) return w;
+    const long long groups = (long long)c.batch * c.heads * w.strips, tiles = strips_of(c.k_len);
+    w.cut(tiles, std::max(1LL, std::min({(2LL * device_cus() + groups - 1) / groups, tiles / 8, 64LL})), 1);
+    return w;
+}
+// Pieces of the (head, sample) pairs that the mean map is added up in.
+static int mean_splits(const Call& c) {
+    const long long tiles = strips_of(c.q_len, 64) * strips_of(c.k_len, 64), pairs = (long long)c.batch * c.heads;
+    return (int)std::max(1LL, std::min({4LL * device_cus() / tiles, pairs / 4, 16LL}));
 }
 
 static long long workspace_floats(const Call& c, bool backward) {
     const long long nb = (long long)c.batch * c.heads;
-    if (backward) return nb * c.q_len + nb * strips_of(c.k_len) * c.num_buckets;
-    const int s = forward_splits(c);
-    return s > 1 ? nb * strips_of(c.q_len) * s * (32 * c.head_dim + 96) : 0;
+    if (backward) {
+        const Walk row = walk_of(c, c.q_len, c.k_len, true), col = walk_of(c, c.k_len, c.q_len, true);
+        const long long a = row.splits > 1 ? nb * strips_of(c.q_len) * row.splits * slot_floats(c) : 0;
+        const long long b = col.splits > 1 ? nb * strips_of(c.k_len) * col.splits * 64 * c.head_dim : 0;
+        // D, rounded up to whole pieces of 16 bytes, the table's gradient by strips, alike, the pieces
+        return ((nb * c.q_len + 3) & ~3LL) + ((nb * col.strips * col.splits * c.num_buckets + 3) & ~3LL) + std::max(a, b);
+    }
+    const Walk w = forward_walk(c, true);
+    const int m = mean_splits(c);
+    return std::max(w.splits > 1 ? nb * strips_of(c.q_len) * w.splits * slot_floats(c) : 0,
+                    c.Mean && m > 1 ? (long long)m * c.q_len * c.k_len : 0);
 }
 
 static bool sizes_ok(const char* who, const Call& c) {
@@ -66,7 +111,7 @@ static bool sizes_ok(const char* who, const Call& c) {
     return true;
 }
 
-static bool heads_ok(const char* who, const char* name, const Call& c, const spion_heads& t, bool written) {
+static bool heads_ok(const char* who, const char* name, const Call& c, const spion_heads& t, int rows, bool written) {
     if (!t.p) {
         set_error("%s: null pointer (%s)", who, name);
         return false;
@@ -75,6 +120,11 @@ static bool heads_ok(const char* who, const char* name, const Call& c, const spi
     if (reinterpret_cast<uintptr_t>(t.p) % 16 || t.batch_stride % unit || t.head_stride % unit || t.row_stride % unit ||
         t.batch_stride < 0 || t.head_stride < 0 || t.row_stride < 0 || (written && t.row_stride < c.head_dim)) {
         set_error("%s: %s: 16-byte aligned heads with strides in multiples of 16 bytes expected", who, name);
+        return false;
+    }
+    const int e = c.bf16 ? 2 : 4;
+    if (t.row_stride * e > (1 << 24) || (rows - 1) * t.row_stride * e + c.head_dim * e > INT_MAX) {
+        set_error("%s: %s: rows up to 2^24 bytes apart and heads within 2^31 bytes expected", who, name);
         return false;
     }
     return true;
@@ -112,60 +162,65 @@ static bool launch(const char* name, K kernel, long long groups, size_t lds, hip
     return check_launch(name);
 }
 
-// Whether a side of `rows` rows is walked in strips of 128: without a pattern, and with strips enough for the machine.
-static bool dense_strips(const Call& c, int rows) {
-    return !c.mat && (long long)c.batch * c.heads * ((rows + 127) / 128) >= 2 * device_cus();
-}
 template <class T, int D>
 static size_t stages_lds(const BiasCall& a) {
     return bias_stages_bytes<T, D>() + bias_floats(a.R) * 4 + sizeof(ScanLds);
 }
-
 template <class T, int D>
 static size_t walk_lds(const BiasCall& a) {
     return bias_tiles_bytes<T, D>() + bias_floats(a.R) * 4 + sizeof(ScanLds);
 }
-
-template <class T, int D>
-static bool mean_map(const Call& c, const BiasCall& a, hipStream_t stream) {
-    return !c.Mean || launch("bias_mean_kernel", bias_mean_kernel<T, D>, strips_of(a.Lq) * strips_of(a.Lk), 0, stream, a);
+static void take(BiasCall& a, const Walk& w, int rows) {
+    a.strips = w.strips;
+    a.splits = w.splits;
+    a.per_split = w.per_split;
+    a.strips32 = (int)strips_of(rows);
 }
 
 template <class T, int D>
 static bool forward(const Call& c, hipStream_t stream) {
     BiasCall a = device_call(c);
-    const long long nb = (long long)a.B * a.H, tiles = strips_of(a.Lk);
-    if (dense_strips(c, a.Lq)) {
-        a.strips = (a.Lq + 127) / 128;
-        return launch("bias_forward_dense_kernel", bias_forward_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a), stream, a) && mean_map<T, D>(c, a, stream);
-    }
-    a.strips = (int)strips_of(a.Lq);
-    a.splits = forward_splits(c);
-    if (a.splits > 1 && (!c.workspace || c.workspace_floats < workspace_floats(c, false))) a.splits = 1;
-    a.per_split = (int)((tiles + a.splits - 1) / a.splits);
-    a.splits = (int)((tiles + a.per_split - 1) / a.per_split);  // none of them empty
+    const long long nb = (long long)a.B * a.H;
+    const bool room = c.workspace && c.workspace_floats >= workspace_floats(c, false);
+    const Walk w = forward_walk(c, room);
+    take(a, w, a.Lq);
     a.part = c.workspace;
-    if (!launch("bias_forward_kernel", bias_forward_kernel<T, D>, nb * a.strips * a.splits, walk_lds<T, D>(a), stream, a)) return false;
-    if (a.splits > 1 && !launch("bias_merge_kernel", bias_merge_kernel<T, D>, nb * a.strips, 0, stream, a)) return false;
-    return mean_map<T, D>(c, a, stream);
+    const long long groups = nb * w.strips * w.splits;
+    if (!(w.dense ? launch("bias_forward_dense_kernel", bias_forward_dense_kernel<T, D>, groups, stages_lds<T, D>(a), stream, a)
+                  : launch("bias_forward_kernel", bias_forward_kernel<T, D>, groups, walk_lds<T, D>(a), stream, a)))
+        return false;
+    if (w.splits > 1 && !launch("bias_merge_kernel", bias_merge_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
+    if (!c.Mean) return true;
+    a.splits = room ? mean_splits(c) : 1;
+    if (!launch("bias_mean_kernel", bias_mean_kernel<T, D>, strips_of(a.Lq, 64) * strips_of(a.Lk, 64) * a.splits, 0, stream, a)) return false;
+    if (a.splits == 1) return true;
+    const long long n = (long long)a.Lq * a.Lk;
+    hipLaunchKernelGGL(bias_mean_merge_kernel, dim3((unsigned)std::min((n + 255) / 256, 4096LL)), dim3(256), 0, stream, a.part, a.mean, n, a.splits,
+                       1.f / nb);
+    return check_launch("bias_mean_merge_kernel");
 }
 
 template <class T, int D>
 static bool backward(const Call& c, hipStream_t stream) {
     BiasCall a = device_call(c);
     const long long nb = (long long)a.B * a.H;
+    const Walk row = walk_of(c, a.Lq, a.Lk, true), col = walk_of(c, a.Lk, a.Lq, true);
     a.delta = c.workspace;
-    a.part = c.workspace + nb * a.Lq;
-    const bool rows = dense_strips(c, a.Lq), cols = dense_strips(c, a.Lk);
-    a.strips = rows ? (a.Lq + 127) / 128 : (int)strips_of(a.Lq);
-    if (!(rows ? launch("bias_backward_row_dense_kernel", bias_backward_row_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a), stream, a)
-               : launch("bias_backward_row_kernel", bias_backward_row_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a), stream, a)))
+    a.tables = a.delta + ((nb * a.Lq + 3) & ~3LL);
+    a.part = a.tables + ((nb * col.strips * col.splits * a.buckets + 3) & ~3LL);
+    take(a, row, a.Lq);
+    if (!(row.dense ? launch("bias_backward_row_dense_kernel", bias_backward_row_dense_kernel<T, D>, nb * row.strips * row.splits,
+                             stages_lds<T, D>(a), stream, a)
+                    : launch("bias_backward_row_kernel", bias_backward_row_kernel<T, D>, nb * row.strips, walk_lds<T, D>(a), stream, a)))
         return false;
-    a.strips = cols ? (a.Lk + 127) / 128 : (int)strips_of(a.Lk);
+    if (row.splits > 1 && !launch("bias_merge_row_kernel", bias_merge_row_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
+    take(a, col, a.Lk);
     const size_t hist = HistLds::bytes(a.R);
-    if (!(cols ? launch("bias_backward_col_dense_kernel", bias_backward_col_dense_kernel<T, D>, nb * a.strips, stages_lds<T, D>(a) + hist + 2048, stream, a)
-               : launch("bias_backward_col_kernel", bias_backward_col_kernel<T, D>, nb * a.strips, walk_lds<T, D>(a) + hist, stream, a)))
+    if (!(col.dense ? launch("bias_backward_col_dense_kernel", bias_backward_col_dense_kernel<T, D>, nb * col.strips * col.splits,
+                             stages_lds<T, D>(a) + hist + 2048, stream, a)
+                    : launch("bias_backward_col_kernel", bias_backward_col_kernel<T, D>, nb * col.strips, walk_lds<T, D>(a) + hist, stream, a)))
         return false;
+    if (col.splits > 1 && !launch("bias_merge_col_kernel", bias_merge_col_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
     hipLaunchKernelGGL((bias_table_kernel<T>), dim3((unsigned)(a.buckets * a.H)), dim3(256), 0, stream, a, reinterpret_cast<T*>(c.dweight));
     return check_launch("bias_table_kernel");
 }
@@ -185,14 +240,18 @@ int bias_forward(const Call* c, hipStream_t stream) {
         set_error("%s: null pointer", who);
         return 1;
     }
-    if (!sizes_ok(who, *c) || !heads_ok(who, "Q", *c, c->Q, false) || !heads_ok(who, "K", *c, c->K, false) ||
-        !heads_ok(who, "V", *c, c->V, false) || !heads_ok(who, "Out", *c, c->Out, true))
+    if (!sizes_ok(who, *c) || !heads_ok(who, "Q", *c, c->Q, c->q_len, false) || !heads_ok(who, "K", *c, c->K, c->k_len, false) ||
+        !heads_ok(who, "V", *c, c->V, c->k_len, false) || !heads_ok(who, "Out", *c, c->Out, c->q_len, true))
         return 1;
     if (c->Mean && c->mat) {
         set_error("%s: the mean map is of the dense phase, without a pattern", who);
         return 1;
     }
-    if (c->Mean && strips_of(c->q_len) * strips_of(c->k_len) > INT_MAX) {
+    if (reinterpret_cast<uintptr_t>(c->workspace) % 16) {
+        set_error("%s: the workspace is not 16-byte aligned", who);
+        return 1;
+    }
+    if (c->Mean && strips_of(c->q_len) * strips_of(c->k_len) > INT_MAX / 16) {
         set_error("%s: mean map too large", who);
         return 1;
     }
@@ -207,10 +266,14 @@ int bias_backward(const Call* c, hipStream_t stream) {
         set_error("%s: null pointer", who);
         return 1;
     }
-    if (!sizes_ok(who, *c) || !heads_ok(who, "Q", *c, c->Q, false) || !heads_ok(who, "K", *c, c->K, false) ||
-        !heads_ok(who, "V", *c, c->V, false) || !heads_ok(who, "Out", *c, c->Out, false) || !heads_ok(who, "dO", *c, c->dO, false) ||
-        !heads_ok(who, "dQ", *c, c->dQ, true) || !heads_ok(who, "dK", *c, c->dK, true) || !heads_ok(who, "dV", *c, c->dV, true))
+    if (!sizes_ok(who, *c) || !heads_ok(who, "Q", *c, c->Q, c->q_len, false) || !heads_ok(who, "K", *c, c->K, c->k_len, false) ||
+        !heads_ok(who, "V", *c, c->V, c->k_len, false) || !heads_ok(who, "Out", *c, c->Out, c->q_len, false) || !heads_ok(who, "dO", *c, c->dO, c->q_len, false) ||
+        !heads_ok(who, "dQ", *c, c->dQ, c->q_len, true) || !heads_ok(who, "dK", *c, c->dK, c->k_len, true) || !heads_ok(who, "dV", *c, c->dV, c->k_len, true))
         return 1;
+    if (reinterpret_cast<uintptr_t>(c->workspace) % 16) {
+        set_error("%s: the workspace is not 16-byte aligned", who);
+        return 1;
+    }
     if (c->workspace_floats < workspace_floats(*c, true)) {
         set_error("%s: workspace of %lld floats, %lld expected", who, c->workspace_floats, workspace_floats(*c, true));
         return 1;

@@ -85,10 +85,10 @@ def _heads(t):
 
 def _readable(t):
     """``t`` as the kernels read it: itself, or a contiguous copy where its strides or address are not theirs."""
-    if _lib.head_layout(t) is not None:
-        return t
-    t = t.contiguous()
-    return t if _lib.head_layout(t) is not None else t.clone(memory_format=torch.contiguous_format)
+    for t in (t, t.contiguous()):
+        if _lib.head_layout(t) is not None and t.stride(2) * t.element_size() <= 1 << 24:
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _empty_like_heads(t):

@@ -101,13 +101,14 @@ def test_c_entry_points_refuse_before_any_gpu_work():
            dict(mat=at, block_size=16), dict(mat=at, block_size=32, offset=1), dict(mat=at, block_size=32, k_len=65),
            dict(key_mask=at, mask_bytes=2), dict(weight=None), dict(Lse=None), dict(buckets=None),
            dict(Q=rb._Heads(None, 0, 0, 32)), dict(K=rb._Heads(at + 4, 0, 0, 32)), dict(V=rb._Heads(at, 2, 0, 32)),
-           dict(Out=rb._Heads(at, 0, -32, 32))]
+           dict(Out=rb._Heads(at, 0, -32, 32)),
+           dict(Q=rb._Heads(at, 0, 0, 1 << 23)), dict(V=rb._Heads(at, 0, 0, 1 << 20), k_len=4096)]
     for kw in bad + [dict(Out=rb._Heads(at, 0, 0, 0)), dict(Mean=at, mat=at, block_size=32)]:
         assert lib.spion_bias_attention_forward(ctypes.addressof(call(**kw)), None) != 0, kw
         with pytest.raises(_lib.SpionLibraryError, match="spion_bias_attention_forward"):
             _lib.check_error()
     for kw in bad + [dict(dQ=rb._Heads(at, 0, 0, 28)), dict(dO=rb._Heads(None, 0, 0, 32)), dict(workspace=None), dict(dweight=None),
-                     dict(workspace_floats=63)]:
+                     dict(workspace_floats=63), dict(workspace=at + 4)]:
         assert lib.spion_bias_attention_backward(ctypes.addressof(call(**kw)), None) != 0, kw
         with pytest.raises(_lib.SpionLibraryError, match="spion_bias_attention_backward"):
             _lib.check_error()
