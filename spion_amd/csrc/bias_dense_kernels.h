@@ -1,5 +1,5 @@
-// The kernels of bias_kernels.h for calls without a pattern that have queries (column pass: keys) enough to fill the machine with
-// strips of 128 rows: each of a work-group's four wavefronts has 32 rows of its own, and the tiles of the other side are staged once
+// The kernels of bias_kernels.h for calls with queries (column pass: keys) enough to fill the machine with strips of 128 rows, without a
+// pattern or with one whose blocks hold whole stages: each of a work-group's four wavefronts has 32 rows of its own, and the tiles of the other side are staged once
 // for all four, in two buffers taken in turn (one barrier a stage).  That is a quarter of the reads from L2 and of the splitting of
 // fp32 values, and of the work-groups whose tables are set up and folded.  Where the strips alone do not fill the machine the
 // other side is cut into pieces; each leaves its sums in a slot of the workspace for every 32 rows, and a second launch adds the
@@ -50,30 +50,96 @@ constexpr int bias_stages_bytes() {
     return stages > merge ? stages : merge;
 }
 
-// The stages of a piece of the other side, one after the other: the list's with a key mask, all of them without.
-// body(stage's first row, words, buffer, its parity).
+// The list of a chunk's stages, for a strip of 128 rows: those that have a key which takes part and lie in the pattern of one of the
+// wavefronts' rows (a block holds whole stages, and a wavefront's 32 rows lie in one block).  in_pattern grows by the keys of
+// the pattern of this wavefront's rows.
+template <bool KEYS, int SUBS>
+__device__ __forceinline__ int scan_stages(const BiasCall& a, ScanLds& s, const BiasItem& it, int first, int count, int tid, int& in_pattern) {
+    const int w = uniform(tid >> 6), l = tid & 63;
+    __syncthreads();
+    if (KEYS) scan_words(a, s, it.b, first, count, tid);
+    constexpr int ROUNDS = CHUNK / SUBS / 256;
+    bool act[ROUNDS];
+    unsigned long long votes[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int i = tid + 256 * r, tile = first + i * SUBS;
+        const bool in = i * SUBS < count;
+        unsigned who = in ? 15u : 0u;
+        if (in && a.mat) {
+            const int t = tile * 32 / a.bs, last = (KEYS ? a.Lq : a.Lk) - 1;
+            who = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int o = min(it.strip * 128 + 32 * k, last) / a.bs;
+                who |= a.mat[KEYS ? (size_t)o * a.nb + t : (size_t)t * a.nb + o] != 0.f ? 1u << k : 0u;
+            }
+        }
+        act[r] = who != 0;
+        if (KEYS && act[r]) {
+            unsigned any = s.words[i * SUBS];
+            if (SUBS == 2 && i * SUBS + 1 < count) any |= s.words[i * SUBS + 1];
+            act[r] = any != 0;
+        }
+        votes[r] = __ballot(act[r]);
+        if (in) s.who[i] = (unsigned char)who;
+        if (KEYS && a.mat) {
+            const int beyond = max(0, tile * 32 + 32 * SUBS - a.Lk);  // of the last stage
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool have = (who >> k) & 1u;
+                const int cut = __any(have && beyond > 0) ? (32 * SUBS - 1 - (a.Lk - 1) % (32 * SUBS)) : 0;
+                const int n = 32 * SUBS * __popcll(__ballot(have)) - cut;
+                if (l == 0) s.pats[k][4 * r + w] = n;
+            }
+        }
+        if (l == 0) s.seg[4 * r + w] = __popcll(votes[r]);
+    }
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        int before = 0;
+#pragma unroll
+        for (int k = 0; k < 4 * ROUNDS; ++k) before += k < 4 * r + w ? s.seg[k] : 0;
+        if (act[r]) s.list[before + __popcll(votes[r] & ((1ull << l) - 1))] = (unsigned short)(tid + 256 * r);
+    }
+#pragma unroll
+    for (int k = 0; k < 4 * ROUNDS; ++k) {
+        total += s.seg[k];
+        if (KEYS && a.mat) in_pattern += s.pats[w][k];
+    }
+    __syncthreads();
+    return total;
+}
+
+// The stages of a piece of the other side, one after the other: the list's with a key mask or a pattern, all of them without.
+// body(stage's first row, words, buffer, its parity): for the wavefronts whose rows have the stage.
 template <class T, int D, bool KEYS, class Store, class Body>
 __device__ __forceinline__ void walk_stages(const BiasCall& a, ScanLds& sc, const BiasItem& it, int rows, const HeadBuf& xh,
-                                            const HeadBuf& yh, char* lds, int tid, Store&& fetched, Body&& body) {
+                                            const HeadBuf& yh, char* lds, int tid, int& in_pattern, Store&& fetched, Body&& body) {
     typedef BiasStage<T, D> ST;
-    const bool listed = KEYS && a.mask;
+    const bool listed = (KEYS && a.mask) || a.mat;
+    const int w = uniform(tid >> 6);
     const int from = it.split * a.per_split, to = min((rows + 31) / 32, from + a.per_split), chunk = listed ? CHUNK : a.per_split;
-    int parity = 0, none = 0;
+    int parity = 0;
     if (!listed) __syncthreads();  // the tables are there
     for (int first = from; first < to; first += chunk) {
         const int count = min(chunk, to - first);
-        const int n = listed ? scan_chunk<true, ST::SUBS>(a, sc, it.b, 0, first, count, tid, none) : (count + ST::SUBS - 1) / ST::SUBS;
+        const int n = listed ? scan_stages<KEYS, ST::SUBS>(a, sc, it, first, count, tid, in_pattern) : (count + ST::SUBS - 1) / ST::SUBS;
         // Which stage comes after next, and its words, are read from LDS while a stage is worked on.
         struct Next {
             int unit;
-            unsigned word[ST::SUBS];
+            unsigned who, word[ST::SUBS];
         };
         auto look_up = [&](int i) __attribute__((always_inline)) {
             Next x;
             x.unit = listed ? (int)sc.list[min(i, n - 1)] : i;
+            x.who = 15u;
             if (listed) {
+                x.who = sc.who[x.unit];
 #pragma unroll
-                for (int s = 0; s < ST::SUBS; ++s) x.word[s] = sc.words[x.unit * ST::SUBS + s];
+                for (int s = 0; s < ST::SUBS; ++s) x.word[s] = KEYS ? sc.words[x.unit * ST::SUBS + s] : 0u;
             }
             return x;
         };
@@ -91,7 +157,8 @@ __device__ __forceinline__ void walk_stages(const BiasCall& a, ScanLds& sc, cons
             unsigned word[ST::SUBS];
 #pragma unroll
             for (int s = 0; s < ST::SUBS; ++s)
-                word[s] = listed ? (u + s < count ? (unsigned)uniform((int)next.word[s]) : 0u) : tail_word(rows - row0 - 32 * s);
+                word[s] = listed && KEYS ? (u + s < count ? (unsigned)uniform((int)next.word[s]) : 0u) : tail_word(rows - row0 - 32 * s);
+            const bool mine = (uniform((int)next.who) >> w) & 1;
             char* buf = lds + parity * ST::BYTES;
             st.store(buf, word, tid);
             fetched.store(parity);
@@ -103,7 +170,7 @@ __device__ __forceinline__ void walk_stages(const BiasCall& a, ScanLds& sc, cons
                 fetched.load((first + next.unit * ST::SUBS) * 32);
                 after = look_up(i + 2);
             }
-            body(row0, word, buf, parity);
+            if (mine) body(row0, word, buf, parity);
         }
     }
 }
@@ -163,7 +230,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_de
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) o[c] = splat16(0.f);
     float m = -__builtin_inff(), z = 0.f;
-    walk_stages<T, D, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, NothingElse(),
+    int in_pattern = 0;
+    walk_stages<T, D, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, in_pattern, NothingElse(),
         [&](int k0, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
             if (!some) return;
             f32x16 s[SUBS];
@@ -230,16 +298,24 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_de
         if (h == 0) {
             slot[32 * D + li] = m;
             slot[32 * D + 32 + li] = z;
-            slot[32 * D + 64 + li] = 0.f;
+            slot[32 * D + 64 + li] = __builtin_bit_cast(float, in_pattern);
         }
         store_strip<D>(o, 1.f, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
             store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
         });
         return;
     }
+    const int off = a.mat ? a.Lk - in_pattern : 0;  // keys off the pattern: a logit of 0 each
+    float scale = 1.f;
+    if (off > 0) {
+        const float up = fmaxf(m, 0.f);
+        scale = __builtin_amdgcn_exp2f(m - up);
+        z = z * scale + off * __builtin_amdgcn_exp2f(-up);
+        m = up;
+    }
     if (h == 0 && q0 + li < a.Lq)
         a.lse[(size_t)it.bh * a.Lq + q0 + li] = z > 0.f ? m + __builtin_amdgcn_logf(z) : __builtin_inff();
-    store_strip<D>(o, z > 0.f ? 1.f / z : 0.f, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
+    store_strip<D>(o, z > 0.f ? scale / z : 0.f, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
         if (q0 + row < a.Lq) store_eighth<T, D>(a.o, it.b, it.h, q0 + row, j, x);
     });
 }
@@ -287,7 +363,8 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_d
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
     float sum = 0.f;
-    walk_stages<T, D, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, NothingElse(),
+    int in_pattern = 0;
+    walk_stages<T, D, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, in_pattern, NothingElse(),
         [&](int k0, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
             if (!some) return;
 #pragma unroll
@@ -327,12 +404,13 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_d
         if (h == 0) {
             slot[32 * D + li] = sum;
             slot[32 * D + 32 + li] = delta;
+            slot[32 * D + 64 + li] = __builtin_bit_cast(float, in_pattern);
         }
         store_strip<D>(dq, a.scale, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
             store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
         });
     } else {
-        if (h == 0 && there) a.delta[stat] = delta + sum;
+        if (h == 0 && there) a.delta[stat] = fmaf(delta, probabilities_of(lse, a.mat ? a.Lk - in_pattern : 0), sum);
         store_strip<D>(dq, a.scale, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
             if (q0 + row < a.Lq) store_eighth<T, D>(a.dq, it.b, it.h, q0 + row, j, x);
         });
@@ -350,9 +428,14 @@ __global__ __launch_bounds__(256) void bias_merge_row_kernel(BiasCall a) {
     add_pieces<D>(slot + row * D + j * (D / 8), a.splits, bias_slot<D>(), x);
     store_eighth<T, D>(a.dq, bh / a.H, bh % a.H, q, j, x);
     if (j == 0) {
-        float s = slot[32 * D + row];
-        for (int k = 1; k < a.splits; ++k) s += slot[k * bias_slot<D>() + 32 * D + row];
-        a.delta[(size_t)bh * a.Lq + q] = slot[32 * D + 32 + row] + s;
+        float s = 0.f;
+        int in_pattern = 0;
+        for (int k = 0; k < a.splits; ++k) {
+            s += slot[k * bias_slot<D>() + 32 * D + row];
+            in_pattern += __builtin_bit_cast(int, slot[k * bias_slot<D>() + 32 * D + 64 + row]);
+        }
+        const size_t stat = (size_t)bh * a.Lq + q;
+        a.delta[stat] = fmaf(slot[32 * D + 32 + row], probabilities_of(a.lse[stat], a.mat ? a.Lk - in_pattern : 0), s);
     }
 }
 
@@ -409,8 +492,9 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_d
                   bias_weight<T>(a, bucket_at(a, -a.R), it.h), bias_weight<T>(a, bucket_at(a, a.R), it.h), a.Lq, tid};
     k.settled();
     v.settled();
+    int none = 0;
     if (__syncthreads_or(some))
-        walk_stages<T, D, false>(a, sc, it, a.Lq, HeadBuf::of<T, D>(a.q, it.b, it.h, a.Lq), HeadBuf::of<T, D>(a.dout, it.b, it.h, a.Lq), lds, tid, qs,
+        walk_stages<T, D, false>(a, sc, it, a.Lq, HeadBuf::of<T, D>(a.q, it.b, it.h, a.Lq), HeadBuf::of<T, D>(a.dout, it.b, it.h, a.Lq), lds, tid, none, qs,
             [&](int r0, const unsigned (&)[SUBS], const char* buf, int parity) __attribute__((always_inline)) {
                 if (!some) return;
 #pragma unroll

@@ -289,6 +289,8 @@ struct ScanLds {
     unsigned words[CHUNK];
     unsigned short list[CHUNK];
     int seg[8], pat[8];
+    unsigned char who[CHUNK];  // of stages: which wavefronts' rows have them in their pattern
+    int pats[4][8];
     float ml[4][2][32];
     float row[32];
 };
@@ -304,46 +306,45 @@ __device__ __forceinline__ bool key_there(const BiasCall& a, int b, int key) {
 // Which of the 32 keys of a tile there are, without a mask.
 __device__ __forceinline__ unsigned tail_word(int left) { return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u; }
 
-// Units of SUBS tiles, from tile `first` on, `count` (<= CHUNK) tiles of the other side, for strip `own` of 32 rows (patterns: SUBS is
-// 1).  KEYS: the other side is the keys, else the queries.  Returns how many units are listed; in_pattern grows by the keys of
-// the pattern's tiles.  All threads of the work-group call it; LDS that they still read must be done with.
-template <bool KEYS, int SUBS = 1>
+// Which keys of tiles first .. first + count - 1 there are.
+__device__ __forceinline__ void scan_words(const BiasCall& a, ScanLds& s, int b, int first, int count, int tid) {
+    const int w = uniform(tid >> 6), l = tid & 63;
+    if (a.mask) {
+        for (int g = w; g < (count + 1) / 2; g += 4) {
+            const unsigned long long there = __ballot(key_there(a, b, (first + 2 * g) * 32 + l));
+            if (l == 0) {
+                s.words[2 * g] = (unsigned)there;
+                if (2 * g + 1 < CHUNK) s.words[2 * g + 1] = (unsigned)(there >> 32);
+            }
+        }
+    } else {
+        for (int i = tid; i < CHUNK; i += 256) s.words[i] = i < count ? tail_word(a.Lk - (first + i) * 32) : 0;
+    }
+    __syncthreads();
+}
+
+// Tiles first .. first + count - 1 (count <= CHUNK) of the other side, for strip `own` of 32 rows.  KEYS: the other side is the
+// keys, else the queries.  Returns how many are listed; in_pattern grows by the keys of the pattern's tiles.  All threads of
+// the work-group call it; LDS that they still read must be done with.
+template <bool KEYS>
 __device__ __forceinline__ int scan_chunk(const BiasCall& a, ScanLds& s, int b, int own, int first, int count, int tid,
                                           int& in_pattern) {
     const int w = uniform(tid >> 6), l = tid & 63;
     __syncthreads();
-    if (KEYS) {
-        if (a.mask) {
-            for (int g = w; g < (count + 1) / 2; g += 4) {
-                const unsigned long long there = __ballot(key_there(a, b, (first + 2 * g) * 32 + l));
-                if (l == 0) {
-                    s.words[2 * g] = (unsigned)there;
-                    if (2 * g + 1 < CHUNK) s.words[2 * g + 1] = (unsigned)(there >> 32);
-                }
-            }
-        } else {
-            for (int i = tid; i < CHUNK; i += 256) s.words[i] = i < count ? tail_word(a.Lk - (first + i) * 32) : 0;
-        }
-        __syncthreads();
-    }
+    if (KEYS) scan_words(a, s, b, first, count, tid);
     bool act[2];
     unsigned long long votes[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        const int i = (tid + 256 * r) * SUBS, tile = first + i;
+        const int i = tid + 256 * r, tile = first + i;
         bool in = i < count;
-        if (SUBS == 1 && in && a.mat) {
+        if (in && a.mat) {
             const int o = own * 32 / a.bs, t = tile * 32 / a.bs;
             in = a.mat[KEYS ? (size_t)o * a.nb + t : (size_t)t * a.nb + o] != 0.f;
         }
         const unsigned long long pat = __ballot(in);
         const unsigned long long tail = KEYS ? __ballot(in && tile * 32 + 32 > a.Lk) : 0;
-        act[r] = in;
-        if (KEYS && in) {
-            unsigned any = s.words[i];
-            if (SUBS == 2 && i + 1 < count) any |= s.words[i + 1];
-            act[r] = any != 0;
-        }
+        act[r] = in && (!KEYS || s.words[i] != 0);
         votes[r] = __ballot(act[r]);
         if (l == 0) {
             s.seg[4 * r + w] = __popcll(votes[r]);

@@ -25,8 +25,8 @@ struct Walk {
         splits = (int)((units + each - 1) / each);  // none of them empty
     }
 };
-// Work-groups wanted: two for each CU.  Sides of more than two tiles without a pattern go in strips of 128; fewer strips than wanted
-// are cut into pieces of at least four stages of 64 rows (256 rows of the other side).  A launch that does not reach a work-group
+// Work-groups wanted: two for each CU.  Sides of more than two tiles go in strips of 128, without a pattern or with blocks that hold
+// whole stages (64 x 64 and more; of smaller blocks the rows of a strip would have few in common); fewer strips than wanted are cut into pieces of at least four stages of 64 rows (256 rows of the other side).  A launch that does not reach a work-group
 // for each CU even so goes in strips of 32.
 static Walk walk_of(const Call& c, int rows, int others, bool can_split) {
     const long long heads = (long long)c.batch * c.heads, want = 2LL * device_cus(), tiles = strips_of(others);
@@ -34,7 +34,7 @@ static Walk walk_of(const Call& c, int rows, int others, bool can_split) {
     const long long wide = heads * strips_of(rows, 128);
     long long pieces = std::max(1LL, std::min({(want + wide - 1) / wide, tiles / 8, 16LL}));
     if (!can_split) pieces = 1;
-    if (!c.mat && rows > 64 && wide * pieces >= device_cus()) {
+    if ((!c.mat || c.block_size % 64 == 0) && rows > 64 && wide * pieces >= device_cus()) {
         w.dense = true;
         w.strips = (int)strips_of(rows, 128);
         w.cut(tiles, pieces, 2);

@@ -141,6 +141,34 @@ def test_block_patterns(L, block, masked, dtype):
     _compare(got, bias_reference(q, k, v, w, buckets, mask, mat, block, do=do))
 
 
+# strips of 128 rows over patterns of 64 x 64 blocks and more, in pieces (B = 32: 384 strips) and whole
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,block,d", [(32, 700, 64, 32), (32, 700, 64, 64), (44, 650, 192, 32), (64, 300, 64, 64)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_block_patterns_that_fill_the_machine(B, L, block, d, masked, dtype):
+    q, k, v, w, buckets, do = _inputs(dtype, B, 2, L, L, d, seed=L)
+    nb = -(-L // block)
+    mat = torch.from_numpy(workloads.band_random_block_mask(nb, 0, extra_frac=0.3, seed=L)).to(DEV)
+    mat[-1] = 0.0
+    mat[0] = 1.0
+    mat[:, nb // 2] = 1.0
+    mask = _lengths_mask(B, L, 9, "holes") if masked else None
+    if masked:
+        k = torch.where(mask[:, None, :, None], k, torch.tensor(math.nan, dtype=dtype, device=DEV))
+    got = _run(q, k, v, w, buckets, do, key_mask=mask, mat=mat, block_size=block)
+    _compare(got, bias_reference(q, k, v, w, buckets, mask, mat, block, do=do))
+
+
+# fewer strips than work-groups wanted: the other side in pieces
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,Lq,Lk,d", [(4, 4, 1000, 1100, 64), (2, 3, 1500, 3000, 32), (8, 8, 90, 2000, 64), (8, 8, 2000, 70, 32), (1, 2, 3000, 3100, 64)])
+@pytest.mark.parametrize("kind", [None, "holes"])
+def test_calls_in_pieces(B, H, Lq, Lk, d, kind, dtype):
+    q, k, v, w, buckets, do = _inputs(dtype, B, H, Lq, Lk, d, 12, 100)
+    mask = None if kind is None else _lengths_mask(B, Lk, 7, kind)
+    _compare(_run(q, k, v, w, buckets, do, key_mask=mask, offset=7), bias_reference(q, k, v, w, buckets, mask, offset=7, do=do))
+
+
 def test_an_empty_pattern():
     q, k, v, w, buckets, do = _inputs(torch.float32, 1, 1, 64, 64, 32)
     got = _run(q, k, v, w, buckets, do, mat=torch.zeros(2, 2, device=DEV), block_size=32)
