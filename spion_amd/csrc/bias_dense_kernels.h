@@ -373,10 +373,13 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_d
                 const char *tk = buf + u * TL::BYTES, *tv = buf + (SUBS + u) * TL::BYTES;
                 const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
                 typename TL::Columns kt;
-                if (TL::EARLY) kt = TL::columns(tk, at);
                 issue_order();
                 const f32x16 s = TL::feat(kr, q);
                 const f32x16 dp = TL::feat(vr, go, minus);  // dP - D
+                if (TL::EARLY) {
+                    kt = TL::columns(tk, at);
+                    read_behind_products<D / 8, D / 8>();
+                }
                 const int rel0 = k0 + 32 * u - qpos;
                 float ds[16];
                 if (word[u] == ~0u && (rel0 - 31 >= a.R || rel0 + 31 <= -a.R)) {
@@ -511,10 +514,13 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_d
                     }
                     const typename TL::Row qr = TL::rows(tq, at), gr = TL::rows(tg, at);
                     typename TL::Columns qt, gt;
-                    if (TL::EARLY) qt = TL::columns(tq, at), gt = TL::columns(tg, at);
                     issue_order();
                     const f32x16 s = TL::feat(qr, k);
                     dp = TL::feat(gr, v, dp);  // dP - D
+                    if (TL::EARLY) {
+                        gt = TL::columns(tg, at), qt = TL::columns(tq, at);
+                        read_behind_products<D / 8, 2 * D / 8>();
+                    }
                     const int rel0 = k0 - r0 - 32 * u - a.off;  // of the tile's corner: lane li, row r has rel0 + li - r
                     const bool near = sums.touches(rel0);
                     float p[16], ds[16];
@@ -540,12 +546,12 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_d
                         p[r] = __builtin_amdgcn_exp2f(p[r]);
                         ds[r] = p[r] * dp[r];
                     }
-                    if (near) sums.near(rel0, ds, li, h);
-                    else sums.far(rel0, ds);
                     if (!TL::EARLY) gt = TL::columns(tg, at);
                     TL::add_t(gt, p, dv);
                     if (!TL::EARLY) qt = TL::columns(tq, at);
                     TL::add_t(qt, ds, dk);
+                    if (near) sums.near(rel0, ds, li, h);
+                    else sums.far(rel0, ds);
                 }
             });
     sums.finish(l);

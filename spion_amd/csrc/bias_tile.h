@@ -243,6 +243,16 @@ struct TileInFlight {
 // compiler would move to their use, one register set and one full latency at a time.
 __device__ __forceinline__ void issue_order() { __builtin_amdgcn_sched_barrier(0); }
 
+// READS LDS reads issued between PRODUCTS matrix instructions that stand in the same block.
+template <int PRODUCTS, int READS>
+__device__ __forceinline__ void read_behind_products() {
+#pragma unroll
+    for (int i = 0; i < PRODUCTS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS / PRODUCTS, 0);
+    }
+}
+
 // Orders a wavefront's own LDS accesses (they complete in order; this is for the compiler).
 __device__ __forceinline__ void wave_lds_order() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -82,7 +82,8 @@ def test_long_sides(Lq, Lk, dtype):
 # ranges of differences that tiles lie within, across and outside of
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,H,Lq,Lk,d,distance,offset", [(32, 16, 60, 60, 32, 40, 0), (64, 4, 200, 130, 64, 9, -50), (32, 4, 500, 700, 32, 100, 200),
-                                                         (128, 4, 33, 1, 64, 40, 0), (16, 8, 512, 520, 64, 200, 0), (43, 12, 128, 96, 32, 4, 5)])
+                                                         (128, 4, 33, 1, 64, 40, 0), (16, 8, 512, 520, 64, 200, 0), (43, 12, 128, 96, 32, 4, 5),
+                                                         (128, 4, 300, 310, 64, 30, 0), (64, 8, 520, 260, 32, 64, -100)])
 @pytest.mark.parametrize("kind", [None, "lengths", "holes"])
 def test_calls_that_fill_the_machine(B, H, Lq, Lk, d, distance, offset, kind, dtype):
     q, k, v, w, buckets, do = _inputs(dtype, B, H, Lq, Lk, d, 12, distance)
@@ -143,7 +144,7 @@ def test_block_patterns(L, block, masked, dtype):
 
 # strips of 128 rows over patterns of 64 x 64 blocks and more, in pieces (B = 32: 384 strips) and whole
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("B,L,block,d", [(32, 700, 64, 32), (32, 700, 64, 64), (44, 650, 192, 32), (64, 300, 64, 64)])
+@pytest.mark.parametrize("B,L,block,d", [(32, 700, 64, 32), (32, 700, 64, 64), (44, 650, 192, 32), (64, 300, 64, 64), (256, 300, 64, 64), (256, 290, 128, 32)])
 @pytest.mark.parametrize("masked", [False, True])
 def test_block_patterns_that_fill_the_machine(B, L, block, d, masked, dtype):
     q, k, v, w, buckets, do = _inputs(dtype, B, 2, L, L, d, seed=L)
