@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_de
     z = half_swap_sum(z);
     __syncthreads();  // the stages are done with
     if (!some) return;
-    if (a.splits > 1) {
+    if (sizeof(T) == 4 && a.splits > 1) {  // (bf16 strips are never cut)
         float* slot = a.part + it.slot(a, w) * bias_slot<D>();
         if (h == 0) {
             slot[32 * D + li] = m;
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_d
     sum = half_swap_sum(sum);
     __syncthreads();  // the stages are done with
     if (!some) return;
-    if (a.splits > 1) {
+    if (sizeof(T) == 4 && a.splits > 1) {
         float* slot = a.part + it.slot(a, w) * bias_slot<D>();
         if (h == 0) {
             slot[32 * D + li] = sum;
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_d
     __syncthreads();  // the stages are done with, the histograms whole
     float* red = reinterpret_cast<float*>(lds);
     const unsigned keys = (unsigned)__ballot(key);
-    if (a.splits > 1) {
+    if (sizeof(T) == 4 && a.splits > 1) {
         if (k0 < a.Lk) {
             float* slot = a.part + it.slot(a, w) * (2 * 32 * D);
             store_strip<D>(dv, 1.f, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
@@ -613,7 +613,7 @@ __global__ __launch_bounds__(256) void bias_merge_col_kernel(BiasCall a) {
 // have a quarter of the pairs each.  Q and K of a pair of tiles are staged (and fp32 ones split) once for all four,
 // probabilities are formed from the forward's lse, added up in registers and never written.  Where the tiles alone do not fill
 // the machine the (head, sample) pairs are cut into pieces whose sums a second launch adds up.  (A tile of 32 x 32 a wavefront,
-// operands straight from memory, bias and lse gathered for each pair: 275 us against NEW, fp32, 128 heads of 1024.)
+// operands straight from memory, bias and lse gathered for each pair: 275 us against 91, fp32, 128 heads of 1024.)
 template <class T, int D>
 constexpr int bias_mean_bytes() {
     const int tiles = 4 * BiasTile<T, D>::BYTES, map = 64 * 65 * 4;

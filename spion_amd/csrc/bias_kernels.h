@@ -47,7 +47,7 @@ __device__ __forceinline__ void logits_of(const f32x16& s, float c2, const float
 // Work-group -> (sample, head, strip, piece).  The hardware deals work-groups round-robin over the XCDs; the strips of a head follow
 // each other on one of them, whose L2 then holds its K and V, and the heads go round-robin, so that every XCD has heads of
 // every sample: with key masks samples differ in length (consecutive heads on an XCD instead: 8 heads each of 16 samples of
-// 1024 to 2048 tokens take 803 us a step against NEW).  What is left of eight heads is spread evenly.
+// 1024 to 2048 tokens take 803 us a step against 753).  What is left of eight heads is spread evenly.
 struct BiasItem {
     int b, h, bh, strip, split;
     __device__ __forceinline__ BiasItem(const BiasCall& a, int total) {

@@ -25,28 +25,44 @@ struct Walk {
         splits = (int)((units + each - 1) / each);  // none of them empty
     }
 };
-// Work-groups wanted: two for each CU.  Sides of more than two tiles go in strips of 128, without a pattern or with blocks that hold
-// whole stages (64 x 64 and more; of smaller blocks the rows of a strip would have few in common); fewer strips than wanted are cut into pieces of at least four stages of 64 rows (256 rows of the other side).  A launch that does not reach a work-group
-// for each CU even so goes in strips of 32.
-static Walk walk_of(const Call& c, int rows, int others, bool can_split) {
-    const long long heads = (long long)c.batch * c.heads, want = 2LL * device_cus(), tiles = strips_of(others);
-    Walk w{};
-    const long long wide = heads * strips_of(rows, 128);
-    long long pieces = std::max(1LL, std::min({(want + wide - 1) / wide, tiles / 8, 16LL}));
-    if (!can_split) pieces = 1;
-    if ((!c.mat || c.block_size % 64 == 0) && rows > 64 && wide * pieces >= device_cus()) {
-        w.dense = true;
-        w.strips = (int)strips_of(rows, 128);
-        w.cut(tiles, pieces, 2);
-        return w;
+// Which of the two, by what fills the machine.  A pattern goes in strips of 128 only with blocks that hold whole stages (64 x 64 and
+// more; of smaller blocks the rows of a strip would have few in common), and so does a side of more than two tiles only.  (us below:
+// strips of 32 against strips of 128; forward of L = 1024 unless said otherwise.)
+//   bf16: strips of 128, uncut, once there is one for each CU (d = 64: 256 strips 28.4 / 24.4, 128 strips 16.1 / 24.0); the forward
+//     and the row pass at d = 32, with half the arithmetic to a stage, from two for each CU (384: 24.2 / 25.6, 512: 29.4 / 25.7).
+//     Cut in two to fill the machine, 128 strips take 22.8: the pieces' merge costs what they gain.
+//   fp32, six products for one: fewer strips than the CUs hold are cut into pieces of at least 256 rows of the other side, and
+//     strips of 32 stay for launches that leave a quarter of the CUs idle even so (d = 64, 192 strips of L = 320: 39.8 / 24.5), and
+//     at d = 32 for the short ones among those that would have to be cut (128 strips: 24.7 / 27.3, of L = 4096 77.9 / 63.0).
+// The number of pieces is the one with the least rounds of work-groups times tiles to a piece.  A CU holds one work-group of the
+// fp32 backward at d = 64 (its LDS) and else two, which take 1.75 times as long together as one alone; a merge (5 us) counts as so
+// many tiles.  (backward, d = 64: 96 strips of L = 1000 in 2 / 4 pieces 128 / 137, 384 of 2048 in 1 / 2 pieces 614 / 563.)
+enum class Pass { FORWARD, ROW, COL };
+static Walk walk_of(const Call& c, int rows, int others, bool can_split, Pass pass) {
+    const long long cus = device_cus(), wide = (long long)c.batch * c.heads * strips_of(rows, 128), tiles = strips_of(others);
+    long long pieces = 1;
+    bool dense = (!c.mat || c.block_size % 64 == 0) && rows > 64;
+    if (c.bf16) {
+        dense = dense && wide >= (c.head_dim == 32 && pass != Pass::COL ? 2 * cus : cus);
+    } else {
+        const bool alone = c.head_dim == 64 && pass != Pass::FORWARD;
+        double least = 0;
+        for (long long n = 1; n == 1 || (can_split && n <= std::min(tiles / 8, 16LL)); ++n) {
+            const long long rounds = (wide * n + cus - 1) / cus, each = (tiles + n - 1) / n;
+            const double cost = (alone ? (double)rounds : 1.75 * (rounds / 2) + rounds % 2) * each + (n == 1 ? 0 : alone ? 2 : 6);
+            if (n == 1 || cost < least) least = cost, pieces = n;
+        }
+        dense = dense && 4 * wide * pieces >= 3 * cus && (c.head_dim == 64 || tiles > 32 || 4 * wide >= 3 * cus);
     }
-    w.strips = (int)strips_of(rows);
-    w.cut(tiles, 1, 1);
+    Walk w{};
+    w.dense = dense;
+    w.strips = (int)strips_of(rows, dense ? 128 : 32);
+    w.cut(tiles, dense ? pieces : 1, dense ? 2 : 1);
     return w;
 }
 // The forward's strips of 32 rows go in pieces as well, each wavefront keeping at least two tiles.
 static Walk forward_walk(const Call& c, bool can_split) {
-    Walk w = walk_of(c, c.q_len, c.k_len, can_split);
+    Walk w = walk_of(c, c.q_len, c.k_len, can_split, Pass::FORWARD);
     if (w.dense || !can_split) return w;
     const long long groups = (long long)c.batch * c.heads * w.strips, tiles = strips_of(c.k_len);
     w.cut(tiles, std::max(1LL, std::min({(2LL * device_cus() + groups - 1) / groups, tiles / 8, 64LL})), 1);
@@ -61,7 +77,7 @@ static int mean_splits(const Call& c) {
 static long long workspace_floats(const Call& c, bool backward) {
     const long long nb = (long long)c.batch * c.heads;
     if (backward) {
-        const Walk row = walk_of(c, c.q_len, c.k_len, true), col = walk_of(c, c.k_len, c.q_len, true);
+        const Walk row = walk_of(c, c.q_len, c.k_len, true, Pass::ROW), col = walk_of(c, c.k_len, c.q_len, true, Pass::COL);
         const long long a = row.splits > 1 ? nb * strips_of(c.q_len) * row.splits * slot_floats(c) : 0;
         const long long b = col.splits > 1 ? nb * strips_of(c.k_len) * col.splits * 64 * c.head_dim : 0;
         // D, rounded up to whole pieces of 16 bytes, the table's gradient by strips, alike, the pieces
@@ -204,7 +220,7 @@ template <class T, int D>
 static bool backward(const Call& c, hipStream_t stream) {
     BiasCall a = device_call(c);
     const long long nb = (long long)a.B * a.H;
-    const Walk row = walk_of(c, a.Lq, a.Lk, true), col = walk_of(c, a.Lk, a.Lq, true);
+    const Walk row = walk_of(c, a.Lq, a.Lk, true, Pass::ROW), col = walk_of(c, a.Lk, a.Lq, true, Pass::COL);
     a.delta = c.workspace;
     a.tables = a.delta + ((nb * a.Lq + 3) & ~3LL);
     a.part = a.tables + ((nb * col.strips * col.splits * a.buckets + 3) & ~3LL);
@@ -213,14 +229,18 @@ static bool backward(const Call& c, hipStream_t stream) {
                              stages_lds<T, D>(a), stream, a)
                     : launch("bias_backward_row_kernel", bias_backward_row_kernel<T, D>, nb * row.strips, walk_lds<T, D>(a), stream, a)))
         return false;
-    if (row.splits > 1 && !launch("bias_merge_row_kernel", bias_merge_row_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
+    if constexpr (sizeof(T) == 4) {  // (bf16 strips are never cut)
+        if (row.splits > 1 && !launch("bias_merge_row_kernel", bias_merge_row_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
+    }
     take(a, col, a.Lk);
     const size_t hist = HistLds::bytes(a.R);
     if (!(col.dense ? launch("bias_backward_col_dense_kernel", bias_backward_col_dense_kernel<T, D>, nb * col.strips * col.splits,
                              stages_lds<T, D>(a) + hist + 2048, stream, a)
                     : launch("bias_backward_col_kernel", bias_backward_col_kernel<T, D>, nb * col.strips, walk_lds<T, D>(a) + hist, stream, a)))
         return false;
-    if (col.splits > 1 && !launch("bias_merge_col_kernel", bias_merge_col_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
+    if constexpr (sizeof(T) == 4) {
+        if (col.splits > 1 && !launch("bias_merge_col_kernel", bias_merge_col_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
+    }
     hipLaunchKernelGGL((bias_table_kernel<T>), dim3((unsigned)(a.buckets * a.H)), dim3(256), 0, stream, a, reinterpret_cast<T*>(c.dweight));
     return check_launch("bias_table_kernel");
 }
