@@ -4,6 +4,10 @@ Mirrors the reference wrapper (models/attention.py:40-191): same constructor ``(
 ``forward(X, mask, mat=None) -> (out, attn)``, ``reconstruct_for_blocksparse(config)`` and the four
 static library loaders.  ``config`` keys read: transformer_dim, head_dim, num_head, max_seq_len,
 block_size, batch_size, attention_dropout, task.
+
+Two keys the reference does not have: ``relative_buckets`` (with ``relative_max_distance``) gives the layer a learned bias by
+relative position: ``attn`` is then a ``RelativeBiasAttention`` and the core of both phases; ``rms_norm`` (True, or the eps) lets it
+normalise its input first, ``norm`` (spion_amd/norm.py).
 """
 from __future__ import annotations
 
@@ -112,7 +116,18 @@ class Attention(nn.Module):
         self.W_k = nn.Linear(self.dim, self.num_head * self.head_dim)
         self.W_v = nn.Linear(self.dim, self.num_head * self.head_dim)
 
-        if not inference:
+        # one core for both phases and for inference: its table keeps its name in a state dict
+        self.relative = bool(config.get("relative_buckets"))
+        if self.relative:
+            from .relative_bias import RelativeBiasAttention
+            self.attn = RelativeBiasAttention(config, key_mask=config["task"] in mask_task)
+        self.norm = None
+        if config.get("rms_norm"):
+            from .norm import RMSNorm
+            eps = config["rms_norm"]
+            self.norm = RMSNorm(self.dim) if eps is True else RMSNorm(self.dim, eps)
+
+        if not inference and not self.relative:
             if config["task"] == "lra-pathfinder32-curv_contour_length_14":
                 self.attn = SoftmaxAttention(config, inference)
             else:
@@ -137,8 +152,10 @@ class Attention(nn.Module):
         torch's usual rule for capturing a backward: warm up on a side stream and keep no autograd graph of a step
         that ran on the default stream alive (its AccumulateGrad nodes belong to the legacy stream, which a capture
         must not touch; breaking this rule ends in a crash inside capture_end on ROCm, not in an error message)."""
+        if self.norm is not None:
+            X = self.norm(X)
         node, weights = self._compiled_node(X, mask)
-        if node is not None and mat is not None:
+        if node is not None and mat is not None and not self.relative:
             done = self._sparse_layer(node, weights, X, mask, mat)
             if done is not None:
                 return done
@@ -153,7 +170,9 @@ class Attention(nn.Module):
             V = self.split_heads(self.W_v(X))
         # the kernels are fp32: leave autocast for the attention core (models/attention.py:88-92)
         with torch.autocast(device_type=X.device.type, enabled=False):
-            if mat is None:
+            if self.relative:
+                attn_out, attn = self.attn(Q.float(), K.float(), V.float(), mask, mat)
+            elif mat is None:
                 attn_out, attn = self.attn(Q.float(), K.float(), V.float(), mask.float())
             else:
                 attn_out, attn = self.block_attn(Q.float(), K.float(), V.float(), mask.float(), mat)
@@ -212,7 +231,10 @@ class Attention(nn.Module):
 
     def reconstruct_for_blocksparse(self, config):
         """Switch the layer to the sparse path: load the block library, create its handle and the
-        block module (models/attention.py:105-129)."""
+        block module (models/attention.py:105-129).  A layer with a relative position bias has one core for both phases."""
+        if self.relative:
+            self.attn.block_size = config["block_size"]
+            return
         num_batches = int(config["num_head"] * config["batch_size"])
         if config["task"] in mask_task:
             from .attention_blockcuda_mask import CUDABlockMaskAttention

@@ -22,13 +22,18 @@ from .masks import load_mask_list
 
 def attach_mask_sidecars(attention_layers, mat_lst: torch.Tensor, config) -> list:
     """``attention_layers[l]`` (``spion_amd.Attention``) gets its block module (if it has none yet) and the prebuilt,
-    registered index of ``mat_lst[0][l]``.  Returns the indices (one ``CsrIndex`` per layer)."""
+    registered index of ``mat_lst[0][l]``.  Returns the indices (one ``CsrIndex`` per layer; None for a layer with a relative
+    position bias, whose kernels read the mask itself)."""
     if mat_lst.dim() != 4 or mat_lst.shape[1] != len(attention_layers):
         raise ValueError(f"mask tensor {tuple(mat_lst.shape)} does not match {len(attention_layers)} layers")
     bs = int(config["block_size"])
     host = mat_lst[0].detach().cpu().numpy()
     out = []
     for l, layer in enumerate(attention_layers):
+        if getattr(layer, "relative", False):
+            layer.reconstruct_for_blocksparse(config)
+            out.append(None)
+            continue
         if not hasattr(layer, "block_attn"):
             layer.reconstruct_for_blocksparse(config)
         mod = layer.block_attn

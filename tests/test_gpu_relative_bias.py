@@ -414,3 +414,25 @@ def test_c_entry_points_keep_to_their_buffers():
     assert lib.spion_bias_attention_backward(ctypes.addressof(call), stream) != 0
     with pytest.raises(_lib.SpionLibraryError, match="workspace"):
         _lib.check_error()
+
+
+# the widest range of differences: the bias, the tiles of heads of 64 and the histograms together take nearly all of a CU's LDS
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,block", [(1, 1100, 0), (1, 1100, 32), (33, 1100, 64), (44, 700, 0)])
+def test_the_widest_range(B, L, block, dtype):
+    q, k, v, w, buckets, do = _inputs(dtype, B, 2, L, L, 64, 64, 1024)
+    mat = None
+    if block:
+        nb = -(-L // block)
+        mat = torch.from_numpy(workloads.band_random_block_mask(nb, 1, extra_frac=0.2, seed=L)).to(DEV)
+    kw = dict(mat=mat, block_size=block) if block else {}
+    _compare(_run(q, k, v, w, buckets, do, **kw), bias_reference(q, k, v, w, buckets, mat=mat, block=block, do=do))
+
+
+# sides of more than two tiles that leave fewer than a work-group for each CU, of either type: strips of 32 and of 128 next to each other
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,Lq,Lk,d", [(8, 8, 320, 320, 64), (8, 8, 320, 320, 32), (4, 4, 1500, 1030, 32), (6, 8, 1030, 1000, 64), (1, 4, 2100, 4200, 64)])
+def test_between_strips_of_32_and_of_128(B, H, Lq, Lk, d, dtype):
+    q, k, v, w, buckets, do = _inputs(dtype, B, H, Lq, Lk, d)
+    mask = _lengths_mask(B, Lk, 4, "lengths")
+    _compare(_run(q, k, v, w, buckets, do, key_mask=mask, offset=-3), bias_reference(q, k, v, w, buckets, mask, offset=-3, do=do))
