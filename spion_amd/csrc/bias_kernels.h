@@ -192,7 +192,8 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
     const int row = tid >> 3, j = tid & 7;
     if (a.splits > 1) {
         float* slot = a.part + (size_t)((it.bh * (size_t)a.strips + it.strip) * a.splits + it.split) * bias_slot<D>();
-        store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
+        // (rows behind the last query are not read again: of a single query's pieces 0.3 KB are written, not 8.6)
+        if (q0 + row < a.Lq) store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
         if (w == 0 && h == 0) {
             slot[32 * D + li] = M;
             slot[32 * D + 32 + li] = Z;
@@ -221,14 +222,18 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
     }
 }
 
-// The pieces of a strip, in their order.
+// The pieces of a strip, in their order; eight pieces' loads are in flight together (there is little else in this launch than the
+// two waits for them).
 template <class T, int D>
 __global__ __launch_bounds__(256) void bias_merge_kernel(BiasCall a) {
     const int tid = threadIdx.x, row = tid >> 3, j = tid & 7;
     const int strip = blockIdx.x % a.strips32, bh = blockIdx.x / a.strips32, b = bh / a.H, ih = bh - b * a.H;
+    const int q = strip * 32 + row;
+    if (q >= a.Lq) return;
     const float* slot = a.part + (size_t)blockIdx.x * a.splits * bias_slot<D>();
     float M = -__builtin_inff();
     int in_pattern = 0;
+#pragma unroll 8
     for (int k = 0; k < a.splits; ++k) {
         M = fmaxf(M, slot[k * bias_slot<D>() + 32 * D + row]);
         in_pattern += __builtin_bit_cast(int, slot[k * bias_slot<D>() + 32 * D + 64 + row]);
@@ -239,6 +244,7 @@ __global__ __launch_bounds__(256) void bias_merge_kernel(BiasCall a) {
     float Z = off > 0 ? off * __builtin_amdgcn_exp2f(-base) : 0.f, x[D / 8];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
+#pragma unroll 8
     for (int k = 0; k < a.splits; ++k) {
         const float* s = slot + k * bias_slot<D>();
         const float f = __builtin_amdgcn_exp2f(s[32 * D + row] - base);
@@ -250,8 +256,6 @@ __global__ __launch_bounds__(256) void bias_merge_kernel(BiasCall a) {
             for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e] * f;
         }
     }
-    const int q = strip * 32 + row;
-    if (q >= a.Lq) return;
     const float inv = Z > 0.f ? 1.f / Z : 0.f;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) x[i] *= inv;
