@@ -50,10 +50,40 @@ constexpr int bias_stages_bytes() {
     return stages > merge ? stages : merge;
 }
 
-// The list of a chunk's stages, for a strip of 128 rows: those that have a key which takes part and lie in the pattern of one of the
+// The rows of a work-group and which of them a wavefront has.  WIDE: 128, each wavefront 32 of its own and all tiles of a stage.  Else
+// 64, which lie in one block of a pattern of 64 x 64 blocks: two wavefronts have the same 32 rows and each one tile of the
+// stage's two, and their sums are added in LDS at the end.
+template <bool WIDE>
+struct StripRows {
+    static constexpr int ROWS = WIDE ? 128 : 64;
+    static __device__ __forceinline__ int first(int strip, int w) { return strip * ROWS + 32 * (WIDE ? w : w & 1); }
+};
+// acc of wavefronts w and w + 2, in the first; red: 64 x D floats.  A barrier for all wavefronts.
+template <int D>
+__device__ __forceinline__ void join_halves(f32x16 (&acc)[D / 32], float* red, int w, int l) {
+    float* at = red + (w & 1) * 32 * D + 4 * l;
+    if (w >= 2)
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(at + 256 * (4 * c + g)) = f32x4{acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]};
+    __syncthreads();
+    if (w < 2)
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(at + 256 * (4 * c + g));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[c][4 * g + j] += x[j];
+            }
+}
+
+// The list of a chunk's stages, for a strip of 128 or 64 rows: those that have a key which takes part and lie in the pattern of one of the
 // wavefronts' rows (a block holds whole stages, and a wavefront's 32 rows lie in one block).  in_pattern grows by the keys of
 // the pattern of this wavefront's rows.
-template <bool KEYS, int SUBS>
+template <bool KEYS, int SUBS, bool WIDE>
 __device__ __forceinline__ int scan_stages(const BiasCall& a, ScanLds& s, const BiasItem& it, int first, int count, int tid, int& in_pattern) {
     const int w = uniform(tid >> 6), l = tid & 63;
     __syncthreads();
@@ -71,7 +101,7 @@ __device__ __forceinline__ int scan_stages(const BiasCall& a, ScanLds& s, const 
             who = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int o = min(it.strip * 128 + 32 * k, last) / a.bs;
+                const int o = min(StripRows<WIDE>::first(it.strip, k), last) / a.bs;
                 who |= a.mat[KEYS ? (size_t)o * a.nb + t : (size_t)t * a.nb + o] != 0.f ? 1u << k : 0u;
             }
         }
@@ -115,7 +145,7 @@ __device__ __forceinline__ int scan_stages(const BiasCall& a, ScanLds& s, const 
 
 // The stages of a piece of the other side, one after the other: the list's with a key mask or a pattern, all of them without.
 // body(stage's first row, words, buffer, its parity): for the wavefronts whose rows have the stage.
-template <class T, int D, bool KEYS, class Store, class Body>
+template <class T, int D, bool WIDE, bool KEYS, class Store, class Body>
 __device__ __forceinline__ void walk_stages(const BiasCall& a, ScanLds& sc, const BiasItem& it, int rows, const HeadBuf& xh,
                                             const HeadBuf& yh, char* lds, int tid, int& in_pattern, Store&& fetched, Body&& body) {
     typedef BiasStage<T, D> ST;
@@ -126,7 +156,7 @@ __device__ __forceinline__ void walk_stages(const BiasCall& a, ScanLds& sc, cons
     if (!listed) __syncthreads();  // the tables are there
     for (int first = from; first < to; first += chunk) {
         const int count = min(chunk, to - first);
-        const int n = listed ? scan_stages<KEYS, ST::SUBS>(a, sc, it, first, count, tid, in_pattern) : (count + ST::SUBS - 1) / ST::SUBS;
+        const int n = listed ? scan_stages<KEYS, ST::SUBS, WIDE>(a, sc, it, first, count, tid, in_pattern) : (count + ST::SUBS - 1) / ST::SUBS;
         // Which stage comes after next, and its words, are read from LDS while a stage is worked on.
         struct Next {
             int unit;
@@ -207,18 +237,19 @@ __device__ __forceinline__ void store_strip(const f32x16 (&acc)[D / 32], float f
     }
 }
 
-template <class T, int D>
+template <class T, int D, bool WIDE>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_dense_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     typedef BiasStage<T, D> ST;
-    constexpr int SUBS = ST::SUBS;
+    constexpr int SUBS = ST::SUBS, MINE = WIDE ? SUBS : 1;  // tiles of a stage, and a wavefront's among them
+    static_assert(WIDE || SUBS == 2, "a tile for each half");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_stages_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
     const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
     fill_bias<T>(a, it.h, tab, tid);
-    const int q0 = it.strip * 128 + w * 32;
+    const int q0 = StripRows<WIDE>::first(it.strip, w), half = WIDE ? 0 : w >> 1;
     const bool some = q0 < a.Lq;
     const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + min(q0 + li, a.Lq - 1) * a.q.row, h, q0 + li < a.Lq);
     const typename TL::At at = TL::at(l);
@@ -231,27 +262,31 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_de
     for (int c = 0; c < D / 32; ++c) o[c] = splat16(0.f);
     float m = -__builtin_inff(), z = 0.f;
     int in_pattern = 0;
-    walk_stages<T, D, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, in_pattern, NothingElse(),
-        [&](int k0, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
+    walk_stages<T, D, WIDE, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, in_pattern, NothingElse(),
+        [&](int k0, const unsigned (&words)[SUBS], const char* stage, int) __attribute__((always_inline)) {
             if (!some) return;
-            f32x16 s[SUBS];
-            typename TL::Row kr[SUBS];
+            const char* buf = stage + half * TL::BYTES;
+            unsigned word[MINE];
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u) kr[u] = TL::rows(buf + u * TL::BYTES, at);
+            for (int u = 0; u < MINE; ++u) word[u] = WIDE ? words[u] : half ? words[SUBS - 1] : words[0];
+            f32x16 s[MINE];
+            typename TL::Row kr[MINE];
+#pragma unroll
+            for (int u = 0; u < MINE; ++u) kr[u] = TL::rows(buf + u * TL::BYTES, at);
             issue_order();
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u) s[u] = TL::feat(kr[u], q);
-            const int rel0 = k0 - qpos;
+            for (int u = 0; u < MINE; ++u) s[u] = TL::feat(kr[u], q);
+            const int rel0 = k0 + 32 * half - qpos;
             bool whole = true;
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u) whole = whole && word[u] == ~0u;
-            float t[SUBS][16], mul = 1.f, add = 0.f, mt = -__builtin_inff();
-            if (whole && (rel0 - 31 >= a.R || rel0 + 32 * SUBS - 1 <= -a.R)) {
+            for (int u = 0; u < MINE; ++u) whole = whole && word[u] == ~0u;
+            float t[MINE][16], mul = 1.f, add = 0.f, mt = -__builtin_inff();
+            if (whole && (rel0 - 31 >= a.R || rel0 + 32 * MINE - 1 <= -a.R)) {
                 // one number for the bias of all pairs: the products as they are, scaled where they enter the exponential
                 mul = c2;
                 add = tab[rel0 > 0 ? far : 0];
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u)
+                for (int u = 0; u < MINE; ++u)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         t[u][r] = s[u][r];
@@ -260,7 +295,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_de
                 mt = fmaf(mt, c2, add);
             } else {
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u) {
+                for (int u = 0; u < MINE; ++u) {
                     if (whole) logits_of<false>(s[u], c2, tab, a.R, rel0 + 32 * u, li, h, word[u], t[u]);
                     else logits_of<true>(s[u], c2, tab, a.R, rel0 + 32 * u, li, h, word[u], t[u]);
 #pragma unroll
@@ -280,7 +315,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_de
             }
             add -= m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u) {
+            for (int u = 0; u < MINE; ++u) {
                 float p[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -291,9 +326,21 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_de
             }
         });
     z = half_swap_sum(z);
+    if (!WIDE) {
+        if (h == 0) sc.ml[w][0][li] = m, sc.ml[w][1][li] = z;
+        __syncthreads();
+        const float mo = sc.ml[w ^ 2][0][li], M = fmaxf(m, mo), base = M == -__builtin_inff() ? 0.f : M, f = __builtin_amdgcn_exp2f(m - base);
+        z = z * f + sc.ml[w ^ 2][1][li] * __builtin_amdgcn_exp2f(mo - base);
+        m = M;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[c][r] *= f;
+        join_halves<D>(o, reinterpret_cast<float*>(lds), w, l);
+    }
     __syncthreads();  // the stages are done with
-    if (!some) return;
-    if (sizeof(T) == 4 && a.splits > 1) {  // (bf16 strips are never cut)
+    if (!some || half) return;
+    if (sizeof(T) == 4 && WIDE && a.splits > 1) {  // (bf16 strips and strips of 64 are never cut)
         float* slot = a.part + it.slot(a, w) * bias_slot<D>();
         if (h == 0) {
             slot[32 * D + li] = m;
@@ -335,18 +382,19 @@ __device__ __forceinline__ void add_pieces(const float* p, int pieces, int strid
         }
 }
 
-template <class T, int D>
+template <class T, int D, bool WIDE>
 __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_dense_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     typedef BiasStage<T, D> ST;
-    constexpr int SUBS = ST::SUBS;
+    constexpr int SUBS = ST::SUBS, MINE = WIDE ? SUBS : 1;  // tiles of a stage, and a wavefront's among them
+    static_assert(WIDE || SUBS == 2, "a tile for each half");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_stages_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
     const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const BiasItem it(a, gridDim.x);
     fill_bias<T>(a, it.h, tab, tid);
-    const int q0 = it.strip * 128 + w * 32, qi = min(q0 + li, a.Lq - 1);
+    const int q0 = StripRows<WIDE>::first(it.strip, w), half = WIDE ? 0 : w >> 1, qi = min(q0 + li, a.Lq - 1);
     const bool some = q0 < a.Lq, there = q0 + li < a.Lq;
     const typename TL::Row q = TL::load(a.q.head(it.b, it.h) + qi * a.q.row, h, there);
     const typename TL::Row go = TL::load(a.dout.head(it.b, it.h) + qi * a.dout.row, h, there);
@@ -364,12 +412,14 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_d
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
     float sum = 0.f;
     int in_pattern = 0;
-    walk_stages<T, D, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, in_pattern, NothingElse(),
-        [&](int k0, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
+    walk_stages<T, D, WIDE, true>(a, sc, it, a.Lk, HeadBuf::of<T, D>(a.k, it.b, it.h, a.Lk), HeadBuf::of<T, D>(a.v, it.b, it.h, a.Lk), lds, tid, in_pattern, NothingElse(),
+        [&](int k0, const unsigned (&words)[SUBS], const char* buf, int) __attribute__((always_inline)) {
             if (!some) return;
 #pragma unroll
-            for (int u = 0; u < SUBS; ++u) {
-                if (word[u] == 0) continue;
+            for (int n = 0; n < MINE; ++n) {
+                const int u = WIDE ? n : half;
+                const unsigned word = WIDE ? words[n] : half ? words[SUBS - 1] : words[0];
+                if (word == 0) continue;
                 const char *tk = buf + u * TL::BYTES, *tv = buf + (SUBS + u) * TL::BYTES;
                 const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
                 typename TL::Columns kt;
@@ -382,14 +432,14 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_d
                 }
                 const int rel0 = k0 + 32 * u - qpos;
                 float ds[16];
-                if (word[u] == ~0u && (rel0 - 31 >= a.R || rel0 + 31 <= -a.R)) {
+                if (word == ~0u && (rel0 - 31 >= a.R || rel0 + 31 <= -a.R)) {
                     const float add = tab[rel0 > 0 ? 2 * (a.R + BIAS_PAD) : 0] - lse;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, add)) * dp[r];
                 } else {
                     float t[16];
-                    if (word[u] == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word[u], t);
-                    else logits_of<true>(s, c2, tab, a.R, rel0, li, h, word[u], t);
+                    if (word == ~0u) logits_of<false>(s, c2, tab, a.R, rel0, li, h, word, t);
+                    else logits_of<true>(s, c2, tab, a.R, rel0, li, h, word, t);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(t[r] - lse) * dp[r];
                 }
@@ -401,8 +451,14 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_d
         });
     sum = half_swap_sum(sum);
     __syncthreads();  // the stages are done with
-    if (!some) return;
-    if (sizeof(T) == 4 && a.splits > 1) {
+    if (!WIDE) {
+        if (h == 0) sc.ml[w][0][li] = sum;
+        join_halves<D>(dq, reinterpret_cast<float*>(lds), w, l);
+        sum += sc.ml[w ^ 2][0][li];
+        __syncthreads();
+    }
+    if (!some || half) return;
+    if (sizeof(T) == 4 && WIDE && a.splits > 1) {
         float* slot = a.part + it.slot(a, w) * bias_slot<D>();
         if (h == 0) {
             slot[32 * D + li] = sum;
@@ -467,11 +523,12 @@ struct QueryStats {
     }
 };
 
-template <class T, int D>
+template <class T, int D, bool WIDE>
 __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_dense_kernel(BiasCall a) {
     typedef BiasTile<T, D> TL;
     typedef BiasStage<T, D> ST;
-    constexpr int SUBS = ST::SUBS;
+    constexpr int SUBS = ST::SUBS, MINE = WIDE ? SUBS : 1;  // tiles of a stage, and a wavefront's among them
+    static_assert(WIDE || SUBS == 2, "a tile for each half");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* tab = reinterpret_cast<float*>(lds + bias_stages_bytes<T, D>());
     ScanLds& sc = *reinterpret_cast<ScanLds*>(tab + bias_floats(a.R));
@@ -481,7 +538,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_d
     const BiasItem it(a, gridDim.x);
     fill_bias<T>(a, it.h, tab, tid, hl.bucket);
     hl.clear(a.R, tid);
-    const int k0 = it.strip * 128 + w * 32, ki = min(k0 + li, a.Lk - 1);
+    const int k0 = StripRows<WIDE>::first(it.strip, w), half = WIDE ? 0 : w >> 1, ki = min(k0 + li, a.Lk - 1);
     const bool key = key_there(a, it.b, k0 + li), some = __any(key);  // false behind the last key
     const typename TL::Row k = TL::load(a.k.head(it.b, it.h) + ki * a.k.row, h, k0 + li < a.Lk);
     const typename TL::Row v = TL::load(a.v.head(it.b, it.h) + ki * a.v.row, h, k0 + li < a.Lk);
@@ -497,11 +554,12 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_d
     v.settled();
     int none = 0;
     if (__syncthreads_or(some))
-        walk_stages<T, D, false>(a, sc, it, a.Lq, HeadBuf::of<T, D>(a.q, it.b, it.h, a.Lq), HeadBuf::of<T, D>(a.dout, it.b, it.h, a.Lq), lds, tid, none, qs,
+        walk_stages<T, D, WIDE, false>(a, sc, it, a.Lq, HeadBuf::of<T, D>(a.q, it.b, it.h, a.Lq), HeadBuf::of<T, D>(a.dout, it.b, it.h, a.Lq), lds, tid, none, qs,
             [&](int r0, const unsigned (&)[SUBS], const char* buf, int parity) __attribute__((always_inline)) {
                 if (!some) return;
 #pragma unroll
-                for (int u = 0; u < SUBS; ++u) {
+                for (int n = 0; n < MINE; ++n) {
+                    const int u = WIDE ? n : half;
                     if (SUBS == 2 && r0 + 32 * u >= a.Lq) continue;
                     const char *tq = buf + u * TL::BYTES, *tg = buf + (SUBS + u) * TL::BYTES;
                     const float* st = stats + 256 * parity + 32 * u + 4 * h;
@@ -557,8 +615,14 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_d
     sums.finish(l);
     __syncthreads();  // the stages are done with, the histograms whole
     float* red = reinterpret_cast<float*>(lds);
+    if (!WIDE) {
+        join_halves<D>(dv, red, w, l);
+        join_halves<D>(dk, red + 64 * D, w, l);
+        __syncthreads();
+    }
     const unsigned keys = (unsigned)__ballot(key);
-    if (sizeof(T) == 4 && a.splits > 1) {
+    if (half) {  // (the other wavefront has both halves' sums)
+    } else if (sizeof(T) == 4 && WIDE && a.splits > 1) {
         if (k0 < a.Lk) {
             float* slot = a.part + it.slot(a, w) * (2 * 32 * D);
             store_strip<D>(dv, 1.f, red, w, l, [&](int row, int j, float (&x)[D / 8]) {

@@ -14,10 +14,10 @@ typedef spion_bias_attention Call;
 static long long strips_of(int rows, int strip = 32) { return (rows + strip - 1) / strip; }
 static int slot_floats(const Call& c) { return 32 * c.head_dim + 96; }  // bias_slot
 
-// How one side of a call is walked: in strips of 128 rows over shared stages, or of 32 with the tiles dealt to the wavefronts, and
-// the other side in `splits` pieces.
+// How one side of a call is walked: in strips of 128 or 64 rows over shared stages, or of 32 with the tiles dealt to the wavefronts,
+// and the other side in `splits` pieces.
 struct Walk {
-    bool dense;
+    int rows;
     int strips, splits, per_split;  // tiles of 32 to a piece
     void cut(long long tiles, long long pieces, int unit) {
         const long long units = (tiles + unit - 1) / unit, each = (units + pieces - 1) / pieces;
@@ -55,15 +55,22 @@ static Walk walk_of(const Call& c, int rows, int others, bool can_split, Pass pa
         dense = dense && 4 * wide * pieces >= 3 * cus && (c.head_dim == 64 || tiles > 32 || 4 * wide >= 3 * cus);
     }
     Walk w{};
-    w.dense = dense;
-    w.strips = (int)strips_of(rows, dense ? 128 : 32);
+    w.rows = dense ? 128 : 32;
+    // (fp32 heads of 64 features have no second tile in a stage)
+    const bool halves = (c.bf16 || c.head_dim == 32) && rows > 32;
+    if (halves && c.mat && c.block_size % 64 == 0 && c.block_size % 128 != 0 && (long long)c.batch * c.heads * strips_of(rows, 64) >= cus) {
+        w.rows = 64;
+        pieces = 1;
+        dense = true;
+    }
+    w.strips = (int)strips_of(rows, w.rows);
     w.cut(tiles, dense ? pieces : 1, dense ? 2 : 1);
     return w;
 }
 // The forward's strips of 32 rows go in pieces as well, each wavefront keeping at least two tiles.
 static Walk forward_walk(const Call& c, bool can_split) {
     Walk w = walk_of(c, c.q_len, c.k_len, can_split, Pass::FORWARD);
-    if (w.dense || !can_split) return w;
+    if (w.rows > 32 || !can_split) return w;
     const long long groups = (long long)c.batch * c.heads * w.strips, tiles = strips_of(c.k_len);
     w.cut(tiles, std::max(1LL, std::min({(2LL * device_cus() + groups - 1) / groups, tiles / 8, 64LL})), 1);
     return w;
@@ -202,9 +209,12 @@ static bool forward(const Call& c, hipStream_t stream) {
     take(a, w, a.Lq);
     a.part = c.workspace;
     const long long groups = nb * w.strips * w.splits;
-    if (!(w.dense ? launch("bias_forward_dense_kernel", bias_forward_dense_kernel<T, D>, groups, stages_lds<T, D>(a), stream, a)
-                  : launch("bias_forward_kernel", bias_forward_kernel<T, D>, groups, walk_lds<T, D>(a), stream, a)))
-        return false;
+    bool ok = true;
+    if (w.rows == 128) ok = launch("bias_forward_dense_kernel", bias_forward_dense_kernel<T, D, true>, groups, stages_lds<T, D>(a), stream, a);
+    if (w.rows == 32) ok = launch("bias_forward_kernel", bias_forward_kernel<T, D>, groups, walk_lds<T, D>(a), stream, a);
+    if constexpr (BiasStage<T, D>::SUBS == 2)
+        if (w.rows == 64) ok = launch("bias_forward_dense_kernel", bias_forward_dense_kernel<T, D, false>, groups, stages_lds<T, D>(a), stream, a);
+    if (!ok) return false;
     if (w.splits > 1 && !launch("bias_merge_kernel", bias_merge_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
     if (!c.Mean) return true;
     a.splits = room ? mean_splits(c) : 1;
@@ -225,19 +235,27 @@ static bool backward(const Call& c, hipStream_t stream) {
     a.tables = a.delta + ((nb * a.Lq + 3) & ~3LL);
     a.part = a.tables + ((nb * col.strips * col.splits * a.buckets + 3) & ~3LL);
     take(a, row, a.Lq);
-    if (!(row.dense ? launch("bias_backward_row_dense_kernel", bias_backward_row_dense_kernel<T, D>, nb * row.strips * row.splits,
-                             stages_lds<T, D>(a), stream, a)
-                    : launch("bias_backward_row_kernel", bias_backward_row_kernel<T, D>, nb * row.strips, walk_lds<T, D>(a), stream, a)))
-        return false;
+    const char* name = row.rows > 32 ? "bias_backward_row_dense_kernel" : "bias_backward_row_kernel";
+    long long groups = nb * row.strips * row.splits;
+    bool ok = true;
+    if (row.rows == 128) ok = launch(name, bias_backward_row_dense_kernel<T, D, true>, groups, stages_lds<T, D>(a), stream, a);
+    if (row.rows == 32) ok = launch(name, bias_backward_row_kernel<T, D>, groups, walk_lds<T, D>(a), stream, a);
+    if constexpr (BiasStage<T, D>::SUBS == 2)
+        if (row.rows == 64) ok = launch(name, bias_backward_row_dense_kernel<T, D, false>, groups, stages_lds<T, D>(a), stream, a);
+    if (!ok) return false;
     if constexpr (sizeof(T) == 4) {  // (bf16 strips are never cut)
         if (row.splits > 1 && !launch("bias_merge_row_kernel", bias_merge_row_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
     }
     take(a, col, a.Lk);
     const size_t hist = HistLds::bytes(a.R);
-    if (!(col.dense ? launch("bias_backward_col_dense_kernel", bias_backward_col_dense_kernel<T, D>, nb * col.strips * col.splits,
-                             stages_lds<T, D>(a) + hist + 2048, stream, a)
-                    : launch("bias_backward_col_kernel", bias_backward_col_kernel<T, D>, nb * col.strips, walk_lds<T, D>(a) + hist, stream, a)))
-        return false;
+    name = col.rows > 32 ? "bias_backward_col_dense_kernel" : "bias_backward_col_kernel";
+    groups = nb * col.strips * col.splits;
+    const size_t staged = stages_lds<T, D>(a) + hist + 2048;
+    if (col.rows == 128) ok = launch(name, bias_backward_col_dense_kernel<T, D, true>, groups, staged, stream, a);
+    if (col.rows == 32) ok = launch(name, bias_backward_col_kernel<T, D>, groups, walk_lds<T, D>(a) + hist, stream, a);
+    if constexpr (BiasStage<T, D>::SUBS == 2)
+        if (col.rows == 64) ok = launch(name, bias_backward_col_dense_kernel<T, D, false>, groups, staged, stream, a);
+    if (!ok) return false;
     if constexpr (sizeof(T) == 4) {
         if (col.splits > 1 && !launch("bias_merge_col_kernel", bias_merge_col_kernel<T, D>, nb * a.strips32, 0, stream, a)) return false;
     }
