@@ -647,7 +647,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_col_d
             store_eighth<T, D>(a.dk, it.b, it.h, k0 + row, j, x);
         });
     }
-    fold_hists(hl.hist, hl.bucket, bias_entries(a.R), a.buckets, tid,
+    fold_hists(hl.hist, hl.bucket, reinterpret_cast<int*>(hl.diag), bias_entries(a.R), a.buckets, tid,
                a.tables + (((size_t)it.bh * a.strips + it.strip) * a.splits + it.split) * a.buckets);
 }
 
