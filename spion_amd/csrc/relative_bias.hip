@@ -56,9 +56,14 @@ static Walk walk_of(const Call& c, int rows, int others, bool can_split, Pass pa
     }
     Walk w{};
     w.rows = dense ? 128 : 32;
-    // (fp32 heads of 64 features have no second tile in a stage)
-    const bool halves = (c.bf16 || c.head_dim == 32) && rows > 32;
-    if (halves && c.mat && c.block_size % 64 == 0 && c.block_size % 128 != 0 && (long long)c.batch * c.heads * strips_of(rows, 64) >= cus) {
+    // Strips of 64 rows, uncut, two wavefronts to the same rows (fp32 heads of 64 features have no second tile in a stage for that): in
+    // patterns of odd multiples of 64, where the rows of a strip of 128 lie in two block rows (16 heads of 8192, bf16, a tenth
+    // of the blocks: 326 / 312), and in the column pass at d = 32, whose strips of 128 come in less than two rounds (bf16,
+    // 384 strips of L = 1024 and 2048 75 / 67 and 113 / 99, 512 of 1024 79 / 89; fp32 184 / 165, 512 186 / 194).
+    const bool halves = (c.bf16 || c.head_dim == 32) && rows > 64 && (!c.mat || c.block_size % 64 == 0);
+    const bool odd = c.mat && c.block_size % 128 != 0 && (long long)c.batch * c.heads * strips_of(rows, 64) >= cus;
+    const bool few = !c.mat && pass == Pass::COL && c.head_dim == 32 && 4 * wide >= 3 * cus && wide < 2 * cus;
+    if (halves && (odd || few)) {
         w.rows = 64;
         pieces = 1;
         dense = true;

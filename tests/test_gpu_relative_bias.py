@@ -436,3 +436,28 @@ def test_between_strips_of_32_and_of_128(B, H, Lq, Lk, d, dtype):
     q, k, v, w, buckets, do = _inputs(dtype, B, H, Lq, Lk, d)
     mask = _lengths_mask(B, Lk, 4, "lengths")
     _compare(_run(q, k, v, w, buckets, do, key_mask=mask, offset=-3), bias_reference(q, k, v, w, buckets, mask, offset=-3, do=do))
+
+
+# the column pass in strips of 64 rows, two wavefronts to the same rows: strips, halves and stages that end anywhere, keys left out
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,Lq,Lk,offset", [(64, 4, 100, 127, 0), (64, 4, 31, 97, 5), (32, 4, 300, 161, -70), (40, 8, 64, 66, 0)])
+@pytest.mark.parametrize("kind", [None, "holes"])
+def test_columns_in_strips_of_64(B, H, Lq, Lk, offset, kind, dtype):
+    q, k, v, w, buckets, do = _inputs(dtype, B, H, Lq, Lk, 32, 16, 90)
+    mask = None if kind is None else _lengths_mask(B, Lk, 8, kind)
+    _compare(_run(q, k, v, w, buckets, do, key_mask=mask, offset=offset), bias_reference(q, k, v, w, buckets, mask, offset=offset, do=do))
+
+
+# maps that no division into ranges makes: buckets that come back, neighbours that all differ, one bucket for everything
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L", [(2, 150), (128, 150)])
+@pytest.mark.parametrize("how", ["random", "cyclic", "pairs", "one"])
+def test_any_map_of_buckets(how, B, L, dtype):
+    q, k, v, w, _, do = _inputs(dtype, B, 4, L, L, 32, 12)
+    n = torch.arange(2 * 75 + 1)
+    buckets = {"random": torch.randint(0, 12, n.shape, generator=torch.Generator().manual_seed(0)), "cyclic": n % 12,
+               "pairs": (n // 2) % 5, "one": torch.full_like(n, 7)}[how].to(torch.int32).to(DEV)
+    got = _run(q, k, v, w, buckets, do)
+    _compare(got, bias_reference(q, k, v, w, buckets, do=do))
+    again = _run(q, k, v, w, buckets, do)
+    assert all(torch.equal(got[x], again[x]) for x in got)
