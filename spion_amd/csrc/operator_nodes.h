@@ -338,6 +338,7 @@ void check_norm(const Tensor& x, const Tensor& weight, const c10::optional<Tenso
     TORCH_CHECK_VALUE(!res.has_value() || res->sizes() == x.sizes(), "residual shape ", res.has_value() ? res->sizes() : x.sizes(),
                       " does not match ", x.sizes());
     fp32_or_bf16(x, "rows");
+    TORCH_CHECK_VALUE(x.size(-1) <= int64_t(1) << 29, "width out of range");
     TORCH_CHECK_VALUE(eps >= 0, "eps is not negative");
     on_one_gpu(x, x);
     on_one_gpu(weight, x);

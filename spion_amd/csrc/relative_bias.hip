@@ -101,6 +101,9 @@ static long long workspace_floats(const Call& c, bool backward) {
                     c.Mean && m > 1 ? (long long)m * c.q_len * c.k_len : 0);
 }
 
+// Work-groups of 256 threads that a launch holds (2^32 threads and more are refused by the runtime, in the middle of a call).
+constexpr long long MOST_GROUPS = (1 << 24) - 1;
+
 static bool sizes_ok(const char* who, const Call& c) {
     if (c.batch < 1 || c.heads < 1 || c.q_len < 1 || c.k_len < 1 || c.num_buckets < 1) {
         set_error("%s: sizes are positive", who);
@@ -123,11 +126,12 @@ static bool sizes_ok(const char* who, const Call& c) {
         return false;
     }
     const long long longest = std::max(c.q_len, c.k_len);
-    if ((long long)c.batch * c.heads > INT_MAX / 64 || (long long)c.batch * c.heads * strips_of((int)longest) > INT_MAX / 64) {
-        set_error("%s: too many heads and rows for one launch", who);
+    if ((long long)c.batch * c.heads > MOST_GROUPS || (long long)c.batch * c.heads * strips_of((int)longest) > MOST_GROUPS ||
+        (long long)c.num_buckets * c.heads > MOST_GROUPS) {
+        set_error("%s: too many heads and rows, or heads and buckets, for one launch", who);
         return false;
     }
-    if (c.mat && (c.block_size < 32 || c.block_size % 32 || c.q_len != c.k_len || c.offset != 0)) {
+    if (c.mat && (c.block_size < 32 || c.block_size % 32 || c.block_size > (1 << 29) || c.q_len != c.k_len || c.offset != 0)) {
         set_error("%s: a pattern has blocks of a multiple of 32 (%d) and as many queries as keys, without an offset", who,
                   c.block_size);
         return false;
@@ -151,7 +155,7 @@ static bool heads_ok(const char* who, const char* name, const Call& c, const spi
         return false;
     }
     const int e = c.bf16 ? 2 : 4;
-    if (t.row_stride * e > (1 << 24) || (rows - 1) * t.row_stride * e + c.head_dim * e > INT_MAX) {
+    if (t.row_stride > (1 << 24) / e || (rows - 1) * t.row_stride * e + c.head_dim * e > INT_MAX) {
         set_error("%s: %s: rows up to 2^24 bytes apart and heads within 2^31 bytes expected", who, name);
         return false;
     }
@@ -294,7 +298,7 @@ int bias_forward(const Call* c, hipStream_t stream) {
         set_error("%s: the workspace is not 16-byte aligned", who);
         return 1;
     }
-    if (c->Mean && strips_of(c->q_len) * strips_of(c->k_len) > INT_MAX / 16) {
+    if (c->Mean && strips_of(c->q_len, 64) * strips_of(c->k_len, 64) > MOST_GROUPS) {
         set_error("%s: mean map too large", who);
         return 1;
     }
@@ -319,10 +323,6 @@ int bias_backward(const Call* c, hipStream_t stream) {
     }
     if (c->workspace_floats < workspace_floats(*c, true)) {
         set_error("%s: workspace of %lld floats, %lld expected", who, c->workspace_floats, workspace_floats(*c, true));
-        return 1;
-    }
-    if ((long long)c->num_buckets * c->heads > INT_MAX) {
-        set_error("%s: table too large", who);
         return 1;
     }
     const bool ok = c->bf16 ? (c->head_dim == 32 ? backward<__bf16, 32>(*c, stream) : backward<__bf16, 64>(*c, stream))

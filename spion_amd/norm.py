@@ -64,6 +64,8 @@ def _check(x, weight, residual, eps):
         raise ValueError(f"residual shape {tuple(residual.shape)} does not match {tuple(x.shape)}")
     if x.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"fp32 or bf16 rows expected, got {x.dtype}")
+    if x.shape[-1] > 1 << 29:  # (the library takes it in 32 bits)
+        raise ValueError("width out of range")
     if not eps >= 0:
         raise ValueError("eps is not negative")
     for t in (x, weight, residual):

@@ -208,7 +208,7 @@ def _check(query, key, value, weight, buckets, key_mask, mat, block_size, offset
     if key_mask is not None and tuple(key_mask.shape) != (B, Lk):
         raise ValueError(f"key mask shape {tuple(key_mask.shape)}: [{B}, {Lk}] expected")
     if mat is not None:
-        if block_size is None or block_size < 32 or block_size % 32:
+        if block_size is None or not 32 <= block_size <= 1 << 29 or block_size % 32:
             raise ValueError(f"block_size {block_size}: a multiple of 32 expected with a pattern")
         nb = -(-Lk // block_size)
         if tuple(mat.shape) != (nb, nb):
@@ -217,6 +217,8 @@ def _check(query, key, value, weight, buckets, key_mask, mat, block_size, offset
             raise ValueError("a pattern has as many queries as keys and no offset")
         if score_map:
             raise ValueError("the mean map is of the dense phase, without a pattern")
+    if max(B, H, weight.shape[0]) >= 1 << 31 or max(Lq, Lk) > 1 << 29:  # (the library takes them in 32 bits)
+        raise ValueError("sizes out of range")
     for t in (query, key, value, weight, buckets, key_mask, mat):
         if t is not None and (not t.is_cuda or t.device != query.device):
             raise RuntimeError("tensors on one GPU expected")

@@ -116,3 +116,48 @@ def test_c_entry_points_refuse_before_any_gpu_work():
     assert lib.spion_bias_workspace(ctypes.addressof(call(head_dim=16)), 0) == -1
     _lib.core().spion_clear_error()
     assert lib.spion_bias_workspace(ctypes.addressof(call()), 1) == 64 + 2 * 8
+
+
+def _huge(*shape):
+    return torch.zeros(()).expand(*shape)  # no memory behind it
+
+
+@pytest.mark.parametrize("change", [
+    dict(mat=torch.ones(1, 1), block_size=(1 << 32) + 32),  # 32 in 32 bits, and the pattern would be read past its end
+    dict(key=_huge(2, 3, (1 << 32) + 40, 32), value=_huge(2, 3, (1 << 32) + 40, 32)),
+    dict(query=_huge(2, 3, (1 << 32) + 40, 32)),
+    dict(weight=_huge((1 << 32) + 8, 3)),
+])
+def test_sizes_past_32_bits_are_refused(change):
+    with pytest.raises(ValueError):
+        spion_amd.relative_bias_attention(**{**_ok(), **change})
+
+
+def _c_call(**sizes):
+    c = rb._Call(batch=1, heads=1, q_len=40, k_len=40, head_dim=32, num_buckets=8, max_distance=20)
+    for n, x in sizes.items():
+        setattr(c, n, x)
+    return rb._lib_typed().spion_bias_workspace(ctypes.addressof(c), 1)
+
+
+@pytest.mark.parametrize("sizes", [dict(mat=16, block_size=(1 << 31) - 32), dict(batch=1 << 20, q_len=1000, k_len=1000),
+                                   dict(num_buckets=32767, heads=1 << 10)])
+def test_c_entry_points_refuse_what_no_launch_holds(sizes):
+    assert _c_call() > 0
+    assert _c_call(**sizes) == -1
+    with pytest.raises(_lib.SpionLibraryError, match="spion_bias_workspace"):
+        _lib.check_error()
+
+
+def test_strides_past_64_bits_of_bytes_are_refused():
+    """A row stride whose bytes come out as 0 in 64 bits."""
+    lib = rb._lib_typed()
+    buf = (ctypes.c_char * 4096)()
+    at = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 16  # never read
+    c = rb._Call(weight=at, buckets=at, Lse=at, batch=1, heads=1, q_len=1, k_len=1, head_dim=32, num_buckets=8, max_distance=20)
+    for n in ("K", "V", "Out"):
+        setattr(c, n, rb._Heads(at, 32, 32, 32))
+    c.Q = rb._Heads(at, 32, 32, 1 << 62)
+    assert lib.spion_bias_attention_forward(ctypes.addressof(c), None) != 0
+    with pytest.raises(_lib.SpionLibraryError, match="Q: rows up to"):
+        _lib.check_error()

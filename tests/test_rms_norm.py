@@ -53,3 +53,11 @@ def test_c_entry_points_refuse_before_any_gpu_work():
     assert lib.spion_rms_norm_forward(None, None) != 0 and lib.spion_rms_norm_backward(None, None) != 0
     assert lib.spion_rms_norm_workspace(ctypes.addressof(call(rows=0))) == -1
     _lib.core().spion_clear_error()
+
+
+@pytest.mark.parametrize("op", ["rms_norm", "rms_norm_fp8"])
+def test_rows_past_32_bits_are_refused(op):
+    n = (1 << 32) + 64  # 64 in 32 bits
+    x = torch.zeros(()).expand(2, n)
+    with pytest.raises(ValueError, match="width"):
+        getattr(spion_amd, op)(x, x[0])
