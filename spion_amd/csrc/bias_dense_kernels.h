@@ -1,9 +1,16 @@
-// The kernels of bias_kernels.h for calls with queries (column pass: keys) enough to fill the machine with strips of 128 rows, without a
-// pattern or with one whose blocks hold whole stages: each of a work-group's four wavefronts has 32 rows of its own, and the tiles of the other side are staged once
-// for all four, in two buffers taken in turn (one barrier a stage).  That is a quarter of the reads from L2 and of the splitting of
-// fp32 values, and of the work-groups whose tables are set up and folded.  Where the strips alone do not fill the machine the
-// other side is cut into pieces; each leaves its sums in a slot of the workspace for every 32 rows, and a second launch adds the
-// pieces of a strip up in their order.
+// The kernels of bias_kernels.h for calls with queries (column pass: keys) enough to fill the machine, without a pattern or with one
+// whose blocks hold whole stages.  A work-group has 128 rows, 32 to each of its four wavefronts, and the tiles of the other side
+// are staged once for all four, in two buffers taken in turn (one barrier a stage).  That is a quarter of the reads from L2 and
+// of the splitting of fp32 values, and of the work-groups whose tables are set up and folded.  Where the strips alone do not
+// fill the machine the other side of an fp32 call is cut into pieces; each leaves its sums in a slot of the workspace for every 32
+// rows, and a second launch adds the pieces of a strip up in their order.  (Which calls: walk_of in relative_bias.hip.)
+//
+// What bounds them, 128 padded heads of 2048, bf16, d = 64: forward 169 us (610 TFLOP/s), row pass 224 (690), column pass 337 (610).  The
+// matrix units are busy for 31 to 33 % of it, the vector units for about half (exponentials, bias, conversions, sums), LDS has 0.3
+// to 4 % conflicts, and memory moves 0.1 to 0.2 GB: two wavefronts a SIMD (three in the forward) take turns, and what one waits
+// for the others do not fill.  64 rows to a wavefront halve the LDS reads, and were slower for the registers they take (column
+// pass 337 -> 449).  16 heads of 8192 with a tenth of their 64 x 64 blocks: 79, 106 and 148 us, of which 19, 30 and 45 are there
+// without any block.  128 fp32 heads of 1024, d = 32: forward 121 to 127 us, matrix units 42 % busy.
 #pragma once
 #include "bias_kernels.h"
 
@@ -469,7 +476,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_d
             store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
         });
     } else {
-        if (h == 0 && there) a.delta[stat] = fmaf(delta, probabilities_of(lse, a.mat ? a.Lk - in_pattern : 0), sum);
+        if (h == 0 && there) a.delta[stat] = exact_d<T>(delta, sum, lse, a.mat ? a.Lk - in_pattern : 0);
         store_strip<D>(dq, a.scale, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
             if (q0 + row < a.Lq) store_eighth<T, D>(a.dq, it.b, it.h, q0 + row, j, x);
         });
@@ -494,7 +501,7 @@ __global__ __launch_bounds__(256) void bias_merge_row_kernel(BiasCall a) {
             in_pattern += __builtin_bit_cast(int, slot[k * bias_slot<D>() + 32 * D + 64 + row]);
         }
         const size_t stat = (size_t)bh * a.Lq + q;
-        a.delta[stat] = fmaf(slot[32 * D + 32 + row], probabilities_of(a.lse[stat], a.mat ? a.Lk - in_pattern : 0), s);
+        a.delta[stat] = exact_d<T>(slot[32 * D + 32 + row], s, a.lse[stat], a.mat ? a.Lk - in_pattern : 0);
     }
 }
 

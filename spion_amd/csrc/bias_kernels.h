@@ -10,6 +10,8 @@
 // every fourth tile of the strip's list; each stages its tiles in its own part of LDS, so nothing waits for a barrier inside
 // the walk, and long strips (a global block row, a single query over a long sample) are shared by four wavefronts and, in the
 // forward, by several work-groups.
+// Small calls are bound by the latency of a strip's steps (table, list, tiles, the wavefronts' merge): 64 heads, one query over 2048
+// padded keys, bf16: 9.6 us and 3.8 for the merge, 33 MB that a copy moves in 6.6; 16 fp32 heads of 1024, d = 32: 27, 33 and 43 us.
 #pragma once
 #include "bias_tile.h"
 
@@ -271,8 +273,19 @@ __global__ __launch_bounds__(256) void bias_merge_kernel(BiasCall a) {
 // and the column pass has that.  (The table's gradient adds up P (dP - D) over thousands of rows whose terms nearly cancel:
 // with dO.O for D the buckets of far keys come out wrong by 0.8 %, 28 heads of 2923 tokens in bf16, 8 buckets, against 0.16 % of
 // rounding at the end.)
-// What the strip's probabilities add up to: keys off the pattern have the rest.
-__device__ __forceinline__ float probabilities_of(float lse, int off) { return 1.f - (off > 0 ? off * __builtin_amdgcn_exp2f(-lse) : 0.f); }
+//
+// With rest = off * exp2(-lse), what keys off the pattern have of the row's probabilities, and S = 1 - rest: the strip's `sum` is
+// sum_j P (dP - dO.O), and D = S dO.O + sum.  In fp32 that is not all.  The matrix units' products come out low by some b (2.8e-8 in
+// the mean at d = 32), while dO.O, added up by the vector units, has none of it: sum = rest dO.O + S b, and D = dO.O + S b.  But
+// every dP of the column pass has the whole b, so D is to have it as well: D = dO.O + (sum - rest dO.O) / S.  (S b left the far
+// buckets off by b S (1 - S) a row, all of one sign: 2.7e-6 of the table's gradient, 6 heads of 2994, a quarter of the blocks.)
+// bf16 outputs, and dO.O with them, are rounded by far more than b.
+template <class T>
+__device__ __forceinline__ float exact_d(float delta, float sum, float lse, int off) {
+    const float rest = off > 0 ? off * __builtin_amdgcn_exp2f(-lse) : 0.f, S = 1.f - rest;
+    if (sizeof(T) == 4 && rest > 0.f && S > 0.f) return delta + fmaf(-delta, rest, sum) / S;
+    return fmaf(delta, S, sum);
+}
 
 template <class T, int D>
 __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_kernel(BiasCall a) {
@@ -348,7 +361,7 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_backward_row_k
     __syncthreads();  // the tiles are done with
     if (w == 0 && h == 0 && there) {
         const float all = (sc.ml[0][0][li] + sc.ml[1][0][li]) + (sc.ml[2][0][li] + sc.ml[3][0][li]);
-        a.delta[stat] = fmaf(delta, probabilities_of(lse, a.mat ? a.Lk - in_pattern : 0), all);
+        a.delta[stat] = exact_d<T>(delta, all, lse, a.mat ? a.Lk - in_pattern : 0);
     }
     float x[D / 8];
     merge_waves<D>(dq, reinterpret_cast<float*>(lds), tid, x);

@@ -461,3 +461,19 @@ def test_any_map_of_buckets(how, B, L, dtype):
     _compare(got, bias_reference(q, k, v, w, buckets, do=do))
     again = _run(q, k, v, w, buckets, do)
     assert all(torch.equal(got[x], again[x]) for x in got)
+
+
+def test_far_buckets_of_a_pattern_have_no_bias():
+    """fp32, rows whose probabilities lie on the pattern by half: the table's gradient adds up P (dP - D) over 3 x 1500 rows a head, where
+    an error of one sign in dP grows with their number n and roundings with its root.  A row's dP and D are off by a few
+    2^-24 of |dO| |v| ~ d, of which its sum keeps at most a quarter (S (1 - S)): 4 * 2^-24 * 32 / 4 * sqrt(n) / 4 for rounding
+    (n = 4500: 3.2e-5 where every row has the same buckets), against 2.8e-8 / 4 * n = 3.1e-5 an error of 2^-25 in every dP leaves.
+    Their mean over 24 tables tells them apart: rounding leaves 3.2e-5 / sqrt(24) = 6.5e-6, so 1e-5 is between them."""
+    total = 0.0
+    for seed in range(6):
+        q, k, v, w, buckets, do = _inputs(torch.float32, 3, 4, 1500, 1500, 32, 8, 16, seed=seed)
+        mat = (torch.rand(47, 47, generator=torch.Generator().manual_seed(seed)) < 0.5).float().to(DEV)
+        got = _run(q, k, v, w, buckets, do, mat=mat, block_size=32)["dw"].double()
+        ref = bias_reference(q, k, v, w, buckets, mat=mat, block=32, do=do)["dw"][0]
+        total += float((got - ref)[3].sum())  # everything far behind
+    assert abs(total / 24) <= 1e-5, total / 24
