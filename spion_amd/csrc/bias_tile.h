@@ -316,17 +316,33 @@ __device__ __forceinline__ bool key_there(const BiasCall& a, int b, int key) {
 // Which of the 32 keys of a tile there are, without a mask.
 __device__ __forceinline__ unsigned tail_word(int left) { return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u; }
 
+// Words of groups of 64 keys, w, w + 4, ... of n, from a mask: eight groups' loads are on their way together.
+template <class M>
+__device__ __forceinline__ void mask_words(const M* mask, unsigned* words, int first, int n, int keys, int w, int l) {
+    constexpr int AHEAD = 8;
+    for (int g0 = w; g0 < n; g0 += 4 * AHEAD) {
+        M x[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) x[u] = mask[min((first + 2 * (g0 + 4 * u)) * 32 + l, keys - 1)];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int g = g0 + 4 * u;
+            const unsigned long long there = __ballot(x[u] != (M)0 && (first + 2 * g) * 32 + l < keys);
+            if (l == 0 && g < n) {
+                words[2 * g] = (unsigned)there;
+                if (2 * g + 1 < CHUNK) words[2 * g + 1] = (unsigned)(there >> 32);
+            }
+        }
+    }
+}
+
 // Which keys of tiles first .. first + count - 1 there are.
 __device__ __forceinline__ void scan_words(const BiasCall& a, ScanLds& s, int b, int first, int count, int tid) {
     const int w = uniform(tid >> 6), l = tid & 63;
     if (a.mask) {
-        for (int g = w; g < (count + 1) / 2; g += 4) {
-            const unsigned long long there = __ballot(key_there(a, b, (first + 2 * g) * 32 + l));
-            if (l == 0) {
-                s.words[2 * g] = (unsigned)there;
-                if (2 * g + 1 < CHUNK) s.words[2 * g + 1] = (unsigned)(there >> 32);
-            }
-        }
+        const size_t row = (size_t)b * a.Lk;
+        if (a.mask_bytes == 4) mask_words(reinterpret_cast<const float*>(a.mask) + row, s.words, first, (count + 1) / 2, a.Lk, w, l);
+        else mask_words(reinterpret_cast<const unsigned char*>(a.mask) + row, s.words, first, (count + 1) / 2, a.Lk, w, l);
     } else {
         for (int i = tid; i < CHUNK; i += 256) s.words[i] = i < count ? tail_word(a.Lk - (first + i) * 32) : 0;
     }
