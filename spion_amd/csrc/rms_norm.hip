@@ -63,16 +63,22 @@ struct Piece {
             *reinterpret_cast<u32x4*>(p) = u;
         }
     }
-    // codes of x * inv
-    __device__ __forceinline__ void store_codes(unsigned char* p, float inv) const {
+    // x / scale, by = 1 / scale: the product corrected by what it leaves, which makes it the quotient rounded once (a rounded 1 / scale
+    // alone puts one code in a million on the wrong side of a midpoint).  Infinite scales have a by of 0 and nothing to correct.
+    __device__ static __forceinline__ float over(float x, float scale, float by) {
+        const float q = x * by;
+        return by != 0.f ? fmaf(fmaf(-q, scale, x), by, q) : q;
+    }
+    // codes of x / scale
+    __device__ __forceinline__ void store_codes(unsigned char* p, float scale, float by) const {
         if constexpr (V == 1) {
-            *p = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, 0.f, 0, false);
+            *p = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(over(x[0], scale, by), 0.f, 0, false);
         } else {
             unsigned u[V / 4];
 #pragma unroll
             for (int i = 0; i < V / 4; ++i) {
-                int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
-                u[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, c, true);
+                int c = __builtin_amdgcn_cvt_pk_fp8_f32(over(x[4 * i], scale, by), over(x[4 * i + 1], scale, by), 0, false);
+                u[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(over(x[4 * i + 2], scale, by), over(x[4 * i + 3], scale, by), c, true);
             }
             if constexpr (V == 4) *reinterpret_cast<unsigned*>(p) = u[0];
             else *reinterpret_cast<unsigned long long*>(p) = u[0] | (unsigned long long)u[V / 4 - 1] << 32;
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(norm_threads<LANES>()) void norm_forward_kernel(Nor
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int i = (c * LANES + lane) * V;
-                if (there && i < a.n) h[c].store_codes(a.codes + row * a.n + i, by);
+                if (there && i < a.n) h[c].store_codes(a.codes + row * a.n + i, scale, by);
             }
             if (there && lane == 0) a.scales[row] = scale;
         } else {
@@ -313,7 +319,7 @@ __global__ __launch_bounds__(1024) void norm_forward_long_kernel(NormCall a) {
         for (int i = threadIdx.x; i < a.n; i += 1024) {
             Piece<T, 1> p;
             p.x[0] = y(i);
-            if (F8) p.store_codes(a.codes + row * a.n + i, by);
+            if (F8) p.store_codes(a.codes + row * a.n + i, scale, by);
             else p.store(reinterpret_cast<T*>(a.y) + row * a.n + i);
         }
     }

@@ -262,3 +262,16 @@ def test_module():
     with torch.no_grad():
         codes, scales = mod.quantized(x)
     assert codes.shape == x.shape and scales.shape == (2, 7)
+
+
+def test_fp8_rounds_the_quotient_once():
+    """A code is that of y / scale, rounded to fp32 once, for the y (the norm's own in fp32, before any rounding to a smaller type) and the
+    scale of the call.  By way of a rounded 1 / scale four of these 3.1 million lie on the other side of a midpoint."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(4096, 768, generator=g).to(DEV)
+    w = (1.0 + 0.2 * torch.randn(768, generator=g)).to(DEV)
+    codes, scales = spion_amd.rms_norm_fp8(x, w)
+    y = spion_amd.rms_norm(x, w)  # the same y, unrounded in fp32
+    best = (y.double() / scales.double()[:, None])
+    want = best.float().to(torch.float8_e4m3fn)
+    assert int((codes.float() != want.float()).sum()) == 0
