@@ -1,7 +1,7 @@
 // Root-mean-square norm of rows with the residual's addition ahead of it (the pre-norm encoder's other pass over the stream; the
 // reference's layer has nn.LayerNorm there, models/model_transformer.py:55-102), its 8-bit form and its backward:
 //   h = x + residual, rounded to the tensors' type: the stream as it goes on;   inv = 1 / sqrt(mean(h^2) + eps);   y = h inv w
-//   8 bits: scale = max|y| / 448 of the unrounded row, codes = e4m3(y / scale)
+//   8 bits: scale = max|y| / 448 of the unrounded row, codes = e4m3(y / scale), where 1 / rms cancels
 //   dh = inv (dy w - h inv mean(dy w h inv)) + (gradient of the stream);   dw = sum over the rows of dy h inv
 // Bound by memory: every tensor is read or written once.  A row lies in the registers of 16, 64, 256 or 1024 lanes in pieces of
 // 16 bytes, so the statistics need no second pass over it; rows that are not 16-byte aligned go an element a lane, and rows longer
@@ -63,22 +63,16 @@ struct Piece {
             *reinterpret_cast<u32x4*>(p) = u;
         }
     }
-    // x / scale, by = 1 / scale: the product corrected by what it leaves, which makes it the quotient rounded once (a rounded 1 / scale
-    // alone puts one code in a million on the wrong side of a midpoint).  Infinite scales have a by of 0 and nothing to correct.
-    __device__ static __forceinline__ float over(float x, float scale, float by) {
-        const float q = x * by;
-        return by != 0.f ? fmaf(fmaf(-q, scale, x), by, q) : q;
-    }
-    // codes of x / scale
-    __device__ __forceinline__ void store_codes(unsigned char* p, float scale, float by) const {
+    template <class Codes>
+    __device__ __forceinline__ void store_codes(unsigned char* p, const Codes& of) const {
         if constexpr (V == 1) {
-            *p = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(over(x[0], scale, by), 0.f, 0, false);
+            *p = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(of(x[0]), 0.f, 0, false);
         } else {
             unsigned u[V / 4];
 #pragma unroll
             for (int i = 0; i < V / 4; ++i) {
-                int c = __builtin_amdgcn_cvt_pk_fp8_f32(over(x[4 * i], scale, by), over(x[4 * i + 1], scale, by), 0, false);
-                u[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(over(x[4 * i + 2], scale, by), over(x[4 * i + 3], scale, by), c, true);
+                int c = __builtin_amdgcn_cvt_pk_fp8_f32(of(x[4 * i]), of(x[4 * i + 1]), 0, false);
+                u[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(of(x[4 * i + 2]), of(x[4 * i + 3]), c, true);
             }
             if constexpr (V == 4) *reinterpret_cast<unsigned*>(p) = u[0];
             else *reinterpret_cast<unsigned long long*>(p) = u[0] | (unsigned long long)u[V / 4 - 1] << 32;
@@ -116,12 +110,38 @@ struct RowReduce {
 };
 
 constexpr float NORM_LEAST_SCALE = 0x1p-126f;
-// max|y| by its bits, which order magnitudes and put NaN above infinity -> scale: 448 is e4m3's largest; a row of zeros and rows
-// below 448 * 2^-126 get the least normal scale, and their codes are exact or as fine as e4m3 is there
-__device__ __forceinline__ float scale_of(unsigned bits) {
-    const float s = __builtin_bit_cast(float, bits) / 448.f;
-    return s < NORM_LEAST_SCALE ? NORM_LEAST_SCALE : s;
-}
+// 1 / rms as a power of two and what is left of it, in [1, 2).  The 8-bit form takes t = h 2^e w for the elements, which is exact for bf16
+// (16 bits), and the rest for the scale alone: it cancels in the codes.
+struct PowerAndRest {
+    float power, rest;
+    __device__ __forceinline__ explicit PowerAndRest(float inv) {
+        power = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, inv) & 0x7f800000u);
+        rest = power == 0.f ? 1.f : inv / power;  // (0: the squares' sum is infinite)
+    }
+};
+// A row's scale and codes from max|t| by its bits, which order magnitudes and put NaN above infinity.  448 is e4m3's largest:
+//   scale = max|t| rest / 448,   code = e4m3(448 t / max|t|) = e4m3((7/8 t) / (max|t| / 512))
+// the quotient corrected by what it leaves, so that it is rounded once and ties of bf16 rows are ties (a rounded y over a rounded scale has
+// 16 to 1000 codes of 2048 rows on their other side).  A row of zeros and rows whose scale would be below the least normal number have
+// that for a scale, and their codes are exact or as fine as e4m3 is there.  An infinite max|t| has a reciprocal of 0 and nothing to
+// correct.
+struct RowCodes {
+    float scale, num, den, by;
+    bool correct;
+    __device__ __forceinline__ RowCodes(unsigned bits, float rest) {
+        const float most = __builtin_bit_cast(float, bits), s = most * rest / 448.f;
+        const bool least = s < NORM_LEAST_SCALE;
+        scale = least ? NORM_LEAST_SCALE : s;
+        num = least ? rest : 0.875f;
+        den = most * 0x1p-9f;
+        by = least ? 0x1p126f : 1.f / den;
+        correct = !least && by != 0.f;
+    }
+    __device__ __forceinline__ float operator()(float t) const {
+        const float n = t * num, q = n * by;
+        return correct ? fmaf(fmaf(-q, den, n), by, q) : q;
+    }
+};
 
 // LANES lanes to a row of up to LANES * C * V elements; LANES <= 256: work-groups of 256 threads with 256 / LANES rows at a time.
 template <int LANES>
@@ -170,10 +190,12 @@ __global__ __launch_bounds__(norm_threads<LANES>()) void norm_forward_kernel(Nor
 #pragma unroll
             for (int e = 0; e < V; ++e) s = fmaf(h[c].x[e], h[c].x[e], s);
         const float inv = rsqrtf(red.sum(s) * rn + a.eps);
+        const PowerAndRest parts(inv);
+        const float by = F8 ? parts.power : inv;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int e = 0; e < V; ++e) h[c].x[e] *= inv * w[c].x[e];
+            for (int e = 0; e < V; ++e) h[c].x[e] *= by * w[c].x[e];
         if constexpr (F8) {
             unsigned m = 0;
 #pragma unroll
@@ -181,13 +203,13 @@ __global__ __launch_bounds__(norm_threads<LANES>()) void norm_forward_kernel(Nor
                 if ((c * LANES + lane) * V < a.n)  // lanes without elements have 0 * inv, which may be NaN
 #pragma unroll
                     for (int e = 0; e < V; ++e) m = max(m, __builtin_bit_cast(unsigned, h[c].x[e]) & 0x7fffffffu);
-            const float scale = scale_of(red.max_bits(m)), by = 1.f / scale;
+            const RowCodes codes(red.max_bits(m), parts.rest);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int i = (c * LANES + lane) * V;
-                if (there && i < a.n) h[c].store_codes(a.codes + row * a.n + i, scale, by);
+                if (there && i < a.n) h[c].store_codes(a.codes + row * a.n + i, codes);
             }
-            if (there && lane == 0) a.scales[row] = scale;
+            if (there && lane == 0) a.scales[row] = codes.scale;
         } else {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
@@ -305,22 +327,27 @@ __global__ __launch_bounds__(1024) void norm_forward_long_kernel(NormCall a) {
             s = fmaf(v, v, s);
         }
         const float inv = rsqrtf(red.sum(s) / a.n + a.eps);
+        const PowerAndRest parts(inv);
+        const float by = F8 ? parts.power : inv;
         auto y = [&](int i) {  // of this thread's own elements of h: they are its own writes
-            return (float)(r ? h[i] : x[i]) * (inv * (float)w[i]);
+            return (float)(r ? h[i] : x[i]) * (by * (float)w[i]);
         };
-        float scale = 1.f;
-        if (F8) {
+        if constexpr (F8) {
             unsigned m = 0;
             for (int i = threadIdx.x; i < a.n; i += 1024) m = max(m, __builtin_bit_cast(unsigned, y(i)) & 0x7fffffffu);
-            scale = scale_of(red.max_bits(m));
-            if (threadIdx.x == 0) a.scales[row] = scale;
-        }
-        const float by = 1.f / scale;
-        for (int i = threadIdx.x; i < a.n; i += 1024) {
-            Piece<T, 1> p;
-            p.x[0] = y(i);
-            if (F8) p.store_codes(a.codes + row * a.n + i, scale, by);
-            else p.store(reinterpret_cast<T*>(a.y) + row * a.n + i);
+            const RowCodes codes(red.max_bits(m), parts.rest);
+            if (threadIdx.x == 0) a.scales[row] = codes.scale;
+            for (int i = threadIdx.x; i < a.n; i += 1024) {
+                Piece<T, 1> p;
+                p.x[0] = y(i);
+                p.store_codes(a.codes + row * a.n + i, codes);
+            }
+        } else {
+            for (int i = threadIdx.x; i < a.n; i += 1024) {
+                Piece<T, 1> p;
+                p.x[0] = y(i);
+                p.store(reinterpret_cast<T*>(a.y) + row * a.n + i);
+            }
         }
     }
 }

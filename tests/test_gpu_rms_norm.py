@@ -264,14 +264,24 @@ def test_module():
     assert codes.shape == x.shape and scales.shape == (2, 7)
 
 
-def test_fp8_rounds_the_quotient_once():
-    """A code is that of y / scale, rounded to fp32 once, for the y (the norm's own in fp32, before any rounding to a smaller type) and the
-    scale of the call.  By way of a rounded 1 / scale four of these 3.1 million lie on the other side of a midpoint."""
-    g = torch.Generator().manual_seed(3)
-    x = torch.randn(4096, 768, generator=g).to(DEV)
-    w = (1.0 + 0.2 * torch.randn(768, generator=g)).to(DEV)
-    codes, scales = spion_amd.rms_norm_fp8(x, w)
-    y = spion_amd.rms_norm(x, w)  # the same y, unrounded in fp32
-    best = (y.double() / scales.double()[:, None])
-    want = best.float().to(torch.float8_e4m3fn)
-    assert int((codes.float() != want.float()).sum()) == 0
+@pytest.mark.parametrize("width", [84, 768, 1000, 5415])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_codes_are_those_of_the_exact_quotient(dtype, residual, width):
+    """1 / rms cancels in y / scale: a code is that of 448 h w / max|h w|.  bf16: the products are exact (16 bits), and a quotient that is not a
+    midpoint of e4m3 is at least 2^-20 of itself away from one, further than its rounding to fp32: every code is the 64-bit
+    quotient's, ties to even.  fp32: the product, 7 / 8 of it, the largest product and the quotient are rounded, 2^-24 each: a code
+    may differ where the quotient lies within 4 * 2^-24 of a midpoint."""
+    g = torch.Generator().manual_seed(width)
+    x = torch.randn(2048, width, generator=g).to(dtype).to(DEV)
+    res = (2.0 * torch.randn(2048, width, generator=g)).to(dtype).to(DEV) if residual else None
+    w = (1.0 + 0.2 * torch.randn(width, generator=g)).to(dtype).to(DEV)
+    codes = spion_amd.rms_norm_fp8(x, w, res)[0].double()
+    hw = (x if res is None else x + res).double() * w.double()
+    q = 448.0 * hw / hw.abs().amax(1, keepdim=True)
+    want, step = _e4m3(q)  # (torch.round: ties to even)
+    off = codes != want
+    if dtype == torch.float32:
+        to_midpoint = ((q / step).abs() % 1.0 - 0.5).abs() * step
+        off &= to_midpoint > 4 * U * q.abs()
+    assert int(off.sum()) == 0
