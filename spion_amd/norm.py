@@ -136,6 +136,17 @@ class _RMSNormFunction(torch.autograd.Function):
         return dx, dw, dx if ctx.residual else None, None
 
 
+class _RMSNormFp8Function(torch.autograd.Function):
+    """Without a gradient.  A function all the same: torch.jit.trace records it as one operation (of the calls inside it, only the
+    allocations), and forward-mode tangents and functorch transforms meet torch's refusal."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        out = tuple(t for t in _forward(x, weight, residual, eps, True) if t is not None)
+        ctx.mark_non_differentiable(*out)
+        return out
+
+
 def _in_node(name, *args):
     """The compiled form (csrc/operator_nodes.h: the same steps), or None where Python's is asked for."""
     node = _lib.autograd_node()
@@ -169,8 +180,7 @@ def rms_norm_fp8(x, weight, residual=None, eps: float = 1e-6):
     _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
-    codes, scales, h = _forward(x.detach(), weight.detach(), None if residual is None else residual.detach(), float(eps), True)
-    return (codes, scales) if h is None else (codes, scales, h)
+    return _RMSNormFp8Function.apply(x, weight, residual, float(eps))
 
 
 class RMSNorm(nn.Module):

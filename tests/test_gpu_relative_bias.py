@@ -477,3 +477,20 @@ def test_far_buckets_of_a_pattern_have_no_bias():
         ref = bias_reference(q, k, v, w, buckets, mat=mat, block=32, do=do)["dw"][0]
         total += float((got - ref)[3].sum())  # everything far behind
     assert abs(total / 24) <= 1e-5, total / 24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_traced_call_computes(grad, dtype):
+    """A traced call gives on other inputs what the function gives, with gradients and with the mean map."""
+    first, other = (_inputs(dtype, 2, 2, 70, 70, 32, seed=s) for s in (1, 2))
+    buckets, mask = first[4], _lengths_mask(2, 70, 3, "lengths")
+    call = lambda *x: spion_amd.relative_bias_attention(*x, buckets, key_mask=mask, score_map=not grad)  # noqa: E731
+    leaves = [t.detach().requires_grad_(grad) for t in other[:4]]
+    with torch.set_grad_enabled(grad):
+        traced = torch.jit.trace(call, tuple(t.detach().requires_grad_(grad) for t in first[:4]), check_trace=False)
+        got, want = traced(*leaves), call(*leaves)
+    if grad:
+        got, want = ([y, *torch.autograd.grad(y, leaves, other[5])] for y in (got, want))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

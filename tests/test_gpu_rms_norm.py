@@ -285,3 +285,21 @@ def test_codes_are_those_of_the_exact_quotient(dtype, residual, width):
         to_midpoint = ((q / step).abs() % 1.0 - 0.5).abs() * step
         off &= to_midpoint > 4 * U * q.abs()
     assert int(off.sum()) == 0
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_traced_norms_compute(dtype, residual):
+    """A traced norm, of either output, gives on other inputs what the function gives."""
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        return tuple(torch.randn(37, 200, generator=g).to(dtype).to(DEV) for _ in range(2))
+
+    w = torch.linspace(0.5, 1.5, 200, device=DEV).to(dtype)
+    for op in (spion_amd.rms_norm, spion_amd.rms_norm_fp8):
+        call = lambda x, r: op(x, w, r if residual else None)  # noqa: E731, B023
+        with torch.no_grad():
+            traced = torch.jit.trace(call, inputs(1), check_trace=False)
+            got, want = traced(*inputs(2)), call(*inputs(2))
+        for a, b in zip(*(y if isinstance(y, tuple) else (y,) for y in (got, want))):
+            assert torch.equal(a.float(), b.float())

@@ -61,3 +61,39 @@ def test_rows_past_32_bits_are_refused(op):
     x = torch.zeros(()).expand(2, n)
     with pytest.raises(ValueError, match="width"):
         getattr(spion_amd, op)(x, x[0])
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_a_traced_call_in_8_bits_runs_again(residual, monkeypatch):
+    """torch.jit.trace records the call, not the allocations inside it: every call of the traced function makes it anew."""
+    made = []
+
+    def forward(x, weight, residual, eps, fp8):
+        made.append(x.shape[0])
+        return (x * weight).to(torch.float8_e4m3fn), x.abs().amax(-1), None if residual is None else x + residual
+
+    monkeypatch.setattr(rn, "_check", lambda *_: None)  # (the tensors here are not on a GPU)
+    monkeypatch.setattr(rn, "_forward", forward)
+    w = torch.arange(1.0, 9.0)
+    x, y = torch.ones(3, 8), torch.full((3, 8), 2.0)
+    traced = torch.jit.trace(lambda x, r: spion_amd.rms_norm_fp8(x, w, r if residual else None), (x, x), check_trace=False)
+    got = traced(y, x)
+    assert len(made) == 2 and len(got) == 2 + residual
+    assert torch.equal(got[0].float(), (y * w).to(torch.float8_e4m3fn).float()) and torch.equal(got[1], y[:, 0])
+    assert not residual or torch.equal(got[2], y + x)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused_in_8_bits(grad, monkeypatch):
+    """Forward-mode derivatives do not depend on grad mode: they are refused, not dropped."""
+    import torch.autograd.forward_ad as fwd
+
+    monkeypatch.setattr(rn, "_check", lambda *_: None)
+    monkeypatch.setattr(rn, "_forward", lambda x, *_: (x.to(torch.float8_e4m3fn), x[:, 0], None))
+    x = torch.ones(3, 8)
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        assert spion_amd.rms_norm_fp8(x, x[0])[0].shape == x.shape
+        with pytest.raises(NotImplementedError):
+            spion_amd.rms_norm_fp8(fwd.make_dual(x, x), x[0])
+        with pytest.raises(NotImplementedError):
+            spion_amd.rms_norm_fp8(x, fwd.make_dual(x[0], x[0]))
