@@ -206,9 +206,13 @@ int spion_transition_update(const float* Cur, float* Prev, int layers, long long
  * Additions with no counterpart in the reference (which reports no errors at all).
  * ---------------------------------------------------------------------------------------------- */
 
-/* Message of the most recent failure in this process, or "" if none since spion_clear_error(). */
+/* Message of the most recent failure in this process, or "" if none since spion_clear_error().  The entry points of the relative
+ * position bias and of the norm have no handle, return a status and may run in several threads at once: their failures are kept for
+ * the calling thread, which alone finds and clears them. */
 const char* spion_last_error(void);
 void spion_clear_error(void);
+/* Message of the calling thread's most recent failure of such an entry point, or "": it is taken out, and nothing else is. */
+const char* spion_take_call_error(void);
 /* 1 if spion_last_error() would return a message, else 0: the cheap check for a caller that polls after every
  * call. */
 int spion_error_pending(void);
@@ -499,7 +503,7 @@ int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, i
  *                not with mat.
  *   workspace    spion_bias_workspace(call, backward) floats, 16-byte aligned, contents unspecified; a forward without it walks
  *                long rows in one piece.  The backward's gradients come out the same in every call with the same inputs.
- * Each returns 0 on success (spion_bias_workspace: -1 on failure).
+ * Each returns 0 on success (spion_bias_workspace: -1 on failure); spion_take_call_error has the message.
  * ---------------------------------------------------------------------------------------------- */
 #define SPION_BIAS_MAX_DISTANCE 1024
 typedef struct spion_heads {
@@ -538,7 +542,8 @@ int spion_bias_attention_backward(const spion_bias_attention* call, void* stream
  *   backward   x: the stream h of the forward; dy, and dh (may be null), the gradients of y and of the stream; out: dx [rows][width],
  *              the gradient of x and of the residual, and dweight [width].  workspace: spion_rms_norm_workspace(call)
  *              floats, contents unspecified.  The same inputs give the same bits.
- * Row strides in elements for what is read; what is written is contiguous and overlaps nothing that is read.  Each returns 0 on success (the workspace: -1 on failure).
+ * Row strides in elements for what is read; what is written is contiguous and overlaps nothing that is read.  Each returns 0 on
+ * success (the workspace: -1 on failure); spion_take_call_error has the message.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct spion_rms_norm {
     const void *x, *residual, *weight;

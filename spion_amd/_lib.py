@@ -78,6 +78,8 @@ def core() -> ctypes.CDLL:
     lib.spion_last_error.argtypes = []
     lib.spion_clear_error.argtypes = []
     lib.spion_clear_error.restype = None
+    lib.spion_take_call_error.restype = c_char_p
+    lib.spion_take_call_error.argtypes = []
     lib.spion_error_pending.argtypes = []
     lib.spion_error_pending.restype = c_int
     lib.spion_set_stream.argtypes = [_P, _P]
@@ -347,6 +349,14 @@ def check_error(where: str = "") -> None:
     text = lib.spion_last_error().decode("utf-8", "replace")
     lib.spion_clear_error()
     raise SpionLibraryError(f"{where}: {text}" if where else text)
+
+
+def check_call(ok: bool, where: str) -> None:
+    """Raise unless a call without a handle succeeded, by its status: the message is the calling thread's, and what other calls
+    and threads have left in the process-wide slot stays there."""
+    if not ok:
+        text = core().spion_take_call_error().decode("utf-8", "replace")
+        raise SpionLibraryError(f"{where}: {text}" if text else f"{where} failed")
 
 
 def load_dropin(name: str, n_init: int, n_fwd: int, n_bwd: int, trailing_int: bool) -> ctypes.CDLL:

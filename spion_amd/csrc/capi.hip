@@ -1,6 +1,7 @@
 // extern "C" surface of libspion_hip.so (declared in include/spion_hip.h) and the error slot.
 #include "common.h"
 
+#include <atomic>
 #include <cstdlib>
 #include <set>
 #include "../../include/spion_hip.h"
@@ -13,6 +14,22 @@ static std::string g_err;
 static thread_local HandleHeader* t_handle = nullptr;
 
 void note_current_handle(HandleHeader* h) { t_handle = h; }
+
+// Failures of the entry points that have no handle and return a status, which may run in several threads at once: kept for the
+// calling thread, where no other thread's check finds or clears them.  Counted along with the process-wide slot's, so that
+// spion_last_error knows the later one.
+static std::atomic<unsigned long long> g_failures{0};
+static unsigned long long g_err_at = 0;
+static thread_local std::string t_err;
+static thread_local unsigned long long t_err_at = 0;
+static thread_local bool t_own_errors = false;
+struct CallWithoutHandle {
+    CallWithoutHandle() {
+        note_current_handle(nullptr);
+        t_own_errors = true;
+    }
+    ~CallWithoutHandle() { t_own_errors = false; }
+};
 
 // Every handle that has not been freed; also what its holds are counted under.  (Never destroyed itself: a handle may be
 // let go as late as the end of the process.)
@@ -39,9 +56,14 @@ void set_error(const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    {
+    const unsigned long long at = ++g_failures;
+    if (t_own_errors) {
+        t_err = buf;
+        t_err_at = at;
+    } else {
         std::lock_guard<std::mutex> lock(g_err_mutex);
         g_err = buf;
+        g_err_at = at;
     }
     {
         std::lock_guard<std::mutex> lock(g_handle_mutex);
@@ -54,10 +76,6 @@ void set_error(const char* fmt, ...) {
     if (!quiet || quiet[0] != '1') fprintf(stderr, "spion_hip: error: %s\n", buf);
     const char* fatal = getenv("SPION_ABORT_ON_ERROR");
     if (fatal && fatal[0] == '1') abort();
-}
-bool error_pending() {
-    std::lock_guard<std::mutex> lock(g_err_mutex);
-    return !g_err.empty();
 }
 
 // implemented in sparse_attn.hip / dense_attn.hip / pattern.hip
@@ -312,29 +330,29 @@ int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, i
 
 // ---- attention with a bias by relative position ---------------------------------------------------
 long long spion_bias_workspace(const spion_bias_attention* call, int backward) {
-    note_current_handle(nullptr);
+    const CallWithoutHandle own;
     return bias_workspace(call, backward);
 }
 int spion_bias_attention_forward(const spion_bias_attention* call, void* stream) {
-    note_current_handle(nullptr);
+    const CallWithoutHandle own;
     return bias_forward(call, static_cast<hipStream_t>(stream));
 }
 int spion_bias_attention_backward(const spion_bias_attention* call, void* stream) {
-    note_current_handle(nullptr);
+    const CallWithoutHandle own;
     return bias_backward(call, static_cast<hipStream_t>(stream));
 }
 
 // ---- root-mean-square norm -------------------------------------------------------------------------
 long long spion_rms_norm_workspace(const spion_rms_norm* call) {
-    note_current_handle(nullptr);
+    const CallWithoutHandle own;
     return norm_workspace(call);
 }
 int spion_rms_norm_forward(const spion_rms_norm* call, void* stream) {
-    note_current_handle(nullptr);
+    const CallWithoutHandle own;
     return norm_forward(call, static_cast<hipStream_t>(stream));
 }
 int spion_rms_norm_backward(const spion_rms_norm* call, void* stream) {
-    note_current_handle(nullptr);
+    const CallWithoutHandle own;
     return norm_backward(call, static_cast<hipStream_t>(stream));
 }
 
@@ -371,16 +389,23 @@ int spion_transition_update(const float* Cur, float* Prev, int layers, long long
 const char* spion_last_error(void) {
     static thread_local std::string copy;
     std::lock_guard<std::mutex> lock(g_err_mutex);
-    copy = g_err;
+    copy = t_err.empty() || (!g_err.empty() && g_err_at > t_err_at) ? g_err : t_err;
     return copy.c_str();
 }
 void spion_clear_error(void) {
     std::lock_guard<std::mutex> lock(g_err_mutex);
     g_err.clear();
+    t_err.clear();
 }
 int spion_error_pending(void) {
     std::lock_guard<std::mutex> lock(g_err_mutex);
-    return g_err.empty() ? 0 : 1;
+    return g_err.empty() && t_err.empty() ? 0 : 1;
+}
+const char* spion_take_call_error(void) {
+    static thread_local std::string taken;
+    taken = std::move(t_err);
+    t_err.clear();
+    return taken.c_str();
 }
 const char* spion_handle_error(void* h) {
     HandleHeader* hd = static_cast<HandleHeader*>(h);

@@ -13,9 +13,9 @@
 
 namespace spion {
 
-// ---- process-wide error slot (read through spion_last_error) ---------------------------------
+// ---- error slots (read through spion_last_error) -----------------------------------------------
+// The process-wide one; within an entry point that keeps its failures for the calling thread, that thread's (capi.hip).
 void set_error(const char* fmt, ...);
-bool error_pending();
 
 #define SPION_HIP_OK(expr)                                                                  \
     ([&]() -> bool {                                                                        \

@@ -37,6 +37,13 @@ variable_list saved_as_is(AutogradContext* ctx) {
     return saved;
 }
 
+// A call of the library by its status: its message is this thread's, whatever other calls have left behind.
+void check_call(bool ok, const char* where) {
+    if (ok) return;
+    const std::string text = spion_take_call_error();
+    throw std::runtime_error(std::string(where) + (text.empty() ? " failed" : ": " + text));
+}
+
 // Gradients that a second derivative would have to go through: it is refused, not left out.
 void once_differentiable(variable_list& grads, size_t used) {
     if (!torch::GradMode::is_enabled()) return;
@@ -102,8 +109,8 @@ spion_bias_attention bias_call(const Tensor& q, const Tensor& k, const Tensor& v
 }
 Tensor bias_workspace(spion_bias_attention& c, bool backward, const Tensor& q) {
     const int64_t n = spion_bias_workspace(&c, backward);
-    if (n < 0) check_library("spion_bias_workspace");
-    if (n <= 0) return Tensor();
+    check_call(n >= 0, "spion_bias_workspace");
+    if (n == 0) return Tensor();
     Tensor ws = torch::empty({n}, q.options().dtype(torch::kFloat32));
     c.workspace = fpm(ws);
     c.workspace_floats = n;
@@ -128,8 +135,8 @@ BiasForward bias_forward(const Tensor& query, const Tensor& key, const Tensor& v
     spion_bias_attention c = bias_call(r.q, r.k, r.v, r.out, r.w, r.buckets, mask, mat, r.lse, block, offset);
     if (score_map) c.Mean = fpm(r.mean);
     const Tensor ws = bias_workspace(c, false, query);
-    spion_bias_attention_forward(&c, reinterpret_cast<void*>(current_stream(query.device().index())));
-    check_library("spion_bias_attention_forward");
+    void* const stream = reinterpret_cast<void*>(current_stream(query.device().index()));
+    check_call(spion_bias_attention_forward(&c, stream) == 0, "spion_bias_attention_forward");
     return r;
 }
 
@@ -172,8 +179,8 @@ struct BiasNode : public torch::autograd::Function<BiasNode> {
         c.dV = heads_of(g[2]);
         c.dweight = g[3].data_ptr();
         const Tensor ws = bias_workspace(c, true, q);
-        spion_bias_attention_backward(&c, reinterpret_cast<void*>(current_stream(q.device().index())));
-        check_library("spion_bias_attention_backward");
+        void* const stream = reinterpret_cast<void*>(current_stream(q.device().index()));
+        check_call(spion_bias_attention_backward(&c, stream) == 0, "spion_bias_attention_backward");
         once_differentiable(g, 4);
         return g;
     }
@@ -280,8 +287,8 @@ variable_list norm_forward(const Tensor& x, const Tensor& weight, const Tensor& 
     } else {
         c.y = r[0].data_ptr();
     }
-    spion_rms_norm_forward(&c, reinterpret_cast<void*>(current_stream(x.device().index())));
-    check_library("spion_rms_norm_forward");
+    void* const stream = reinterpret_cast<void*>(current_stream(x.device().index()));
+    check_call(spion_rms_norm_forward(&c, stream) == 0, "spion_rms_norm_forward");
     return r;
 }
 
@@ -321,11 +328,11 @@ struct NormNode : public torch::autograd::Function<NormNode> {
         c.dx = g[0].data_ptr();
         c.dweight = g[1].data_ptr();
         c.workspace_floats = spion_rms_norm_workspace(&c);
-        if (c.workspace_floats < 0) check_library("spion_rms_norm_workspace");
+        check_call(c.workspace_floats >= 0, "spion_rms_norm_workspace");
         Tensor ws = torch::empty({(int64_t)c.workspace_floats}, h.options().dtype(torch::kFloat32));
         c.workspace = fpm(ws);
-        spion_rms_norm_backward(&c, reinterpret_cast<void*>(current_stream(h.device().index())));
-        check_library("spion_rms_norm_backward");
+        void* const stream = reinterpret_cast<void*>(current_stream(h.device().index()));
+        check_call(spion_rms_norm_backward(&c, stream) == 0, "spion_rms_norm_backward");
         once_differentiable(g, 2);
         if (residual) g[2] = g[0];
         return g;

@@ -52,9 +52,7 @@ def _rows(t):
 
 def _run(name, call, device):
     with torch.cuda.device(device):
-        if getattr(_lib_typed(), name)(ctypes.addressof(call), _lib._raw_stream(device.index)) != 0:
-            _lib.check_error(name)
-            raise _lib.SpionLibraryError(f"{name} failed")
+        _lib.check_call(getattr(_lib_typed(), name)(ctypes.addressof(call), _lib._raw_stream(device.index)) == 0, name)
 
 
 def _check(x, weight, residual, eps):
@@ -128,8 +126,7 @@ class _RMSNormFunction(torch.autograd.Function):
             d = _rows(dh.to(h.dtype))
             call.dh, call.dh_stride = d.data_ptr(), d.stride(0)
         floats = _lib_typed().spion_rms_norm_workspace(ctypes.addressof(call))
-        if floats < 0:
-            _lib.check_error("spion_rms_norm_workspace")
+        _lib.check_call(floats >= 0, "spion_rms_norm_workspace")
         ws = torch.empty(floats, dtype=torch.float32, device=h.device)
         call.workspace, call.workspace_floats = ws.data_ptr(), floats
         _run("spion_rms_norm_backward", call, h.device)

@@ -100,12 +100,6 @@ def _empty_like_heads(t):
     return torch.empty((B, H, L, d), dtype=t.dtype, device=t.device)
 
 
-def _raise(status, where):
-    if status != 0:
-        _lib.check_error(where)
-        raise _lib.SpionLibraryError(f"{where} failed")
-
-
 def _call_of(q, k, weight, buckets, key_mask, mat, block_size, offset):
     B, H, Lq, d = q.shape
     c = _Call(weight=weight.data_ptr(), buckets=buckets.data_ptr(), batch=B, heads=H, q_len=Lq, k_len=k.shape[2], head_dim=d,
@@ -120,8 +114,7 @@ def _call_of(q, k, weight, buckets, key_mask, mat, block_size, offset):
 
 def _workspace(lib, call, backward, device):
     n = lib.spion_bias_workspace(ctypes.addressof(call), int(backward))
-    if n < 0:
-        _raise(1, "spion_bias_workspace")
+    _lib.check_call(n >= 0, "spion_bias_workspace")
     ws = torch.empty(n, dtype=torch.float32, device=device)
     call.workspace, call.workspace_floats = ws.data_ptr() if n else None, n
     return ws
@@ -143,8 +136,8 @@ class _RelativeBiasFunction(torch.autograd.Function):
             if mean is not None:
                 call.Mean = mean.data_ptr()
             ws = _workspace(lib, call, False, dev)
-            _raise(lib.spion_bias_attention_forward(ctypes.addressof(call), _lib._raw_stream(dev.index)),
-                   "spion_bias_attention_forward")
+            _lib.check_call(lib.spion_bias_attention_forward(ctypes.addressof(call), _lib._raw_stream(dev.index)) == 0,
+                            "spion_bias_attention_forward")
             del ws
         optional = {"key_mask": key_mask, "mat": mat}
         ctx.given = [n for n, t in optional.items() if t is not None]
@@ -178,8 +171,8 @@ class _RelativeBiasFunction(torch.autograd.Function):
             call.dO, call.dQ, call.dK, call.dV = (_heads(t) for t in (go, dq, dk, dv))
             call.Lse, call.dweight = lse.data_ptr(), dw.data_ptr()
             ws = _workspace(lib, call, True, dev)
-            _raise(lib.spion_bias_attention_backward(ctypes.addressof(call), _lib._raw_stream(dev.index)),
-                   "spion_bias_attention_backward")
+            _lib.check_call(lib.spion_bias_attention_backward(ctypes.addressof(call), _lib._raw_stream(dev.index)) == 0,
+                            "spion_bias_attention_backward")
             del ws
         return dq, dk, dv, dw, None, None, None, None, None, None
 

@@ -494,3 +494,19 @@ def test_a_traced_call_computes(grad, dtype):
         got, want = ([y, *torch.autograd.grad(y, leaves, other[5])] for y in (got, want))
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_calls_go_by_their_own_status():
+    """A call that the library refuses raises; what another call has left in the process-wide error slot neither fails a call nor is
+    taken by it."""
+    lib = _lib.core()
+    q, k, v, w, buckets, do = _inputs(torch.float32, 1, 2, 40, 40, 32)
+    lib.spion_set_stream(None, None)  # a failure: no handle
+    try:
+        got = _run(q, k, v, w, buckets, do)
+        with pytest.raises(_lib.SpionLibraryError, match="32767 buckets"):
+            _run(q, k, v, torch.zeros(32768, 2, device=DEV), buckets, do)
+        assert lib.spion_last_error().startswith(b"spion_set_stream")
+    finally:
+        lib.spion_clear_error()
+    _compare(got, bias_reference(q, k, v, w, buckets, do=do))

@@ -303,3 +303,19 @@ def test_traced_norms_compute(dtype, residual):
             got, want = traced(*inputs(2)), call(*inputs(2))
         for a, b in zip(*(y if isinstance(y, tuple) else (y,) for y in (got, want))):
             assert torch.equal(a.float(), b.float())
+
+
+def test_calls_go_by_their_own_status():
+    """What another call has left in the process-wide error slot neither fails a call nor is taken by it."""
+    lib = _lib.core()
+    x, dy = torch.randn(5, 64, device=DEV), torch.ones(5, 64, device=DEV)
+    w = torch.ones(64, device=DEV)
+    lib.spion_set_stream(None, None)  # a failure: no handle
+    try:
+        got = _train(x, w, None, dy, None)
+        with torch.no_grad():
+            spion_amd.rms_norm_fp8(x, w)
+        assert lib.spion_error_pending() == 1
+    finally:
+        lib.spion_clear_error()
+    _check(x, w, None, dy, None, *got)
