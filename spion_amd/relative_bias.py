@@ -83,12 +83,16 @@ def _heads(t):
     return _Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
 
 
+def _fits(t):
+    return _lib.head_layout(t) is not None and t.stride(2) * t.element_size() <= 1 << 24
+
+
 def _readable(t):
     """``t`` as the kernels read it: itself, or a contiguous copy where its strides or address are not theirs."""
-    for t in (t, t.contiguous()):
-        if _lib.head_layout(t) is not None and t.stride(2) * t.element_size() <= 1 << 24:
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
+    if _fits(t):
+        return t
+    c = t.contiguous()
+    return c if _fits(c) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _empty_like_heads(t):

@@ -161,3 +161,25 @@ def test_strides_past_64_bits_of_bytes_are_refused():
     assert lib.spion_bias_attention_forward(ctypes.addressof(c), None) != 0
     with pytest.raises(_lib.SpionLibraryError, match="Q: rows up to"):
         _lib.check_error()
+
+
+def _aligned(*shape):
+    x = torch.zeros(math.prod(shape) + 4)
+    return x[(-x.data_ptr() % 16) // 4:][: math.prod(shape)].view(shape)
+
+
+def test_heads_are_copied_only_where_they_have_to_be(monkeypatch):
+    views = _aligned(2, 40, 3, 32).transpose(1, 2), _aligned(2, 3, 40, 32), _aligned(2, 40, 3, 3, 32)[:, :, 1].transpose(1, 2)
+    off = _aligned(2 * 3 * 40 * 32 + 1)[1:].view(2, 3, 40, 32)  # contiguous, 4 bytes off
+    turned = _aligned(2, 3, 32, 40).transpose(2, 3)
+    copies = []
+    contiguous, clone = torch.Tensor.contiguous, torch.Tensor.clone
+    monkeypatch.setattr(torch.Tensor, "contiguous", lambda t, *a, **k: (copies.append("contiguous"), contiguous(t, *a, **k))[1])
+    monkeypatch.setattr(torch.Tensor, "clone", lambda t, *a, **k: (copies.append("clone"), clone(t, *a, **k))[1])
+    for t in views:
+        assert rb._readable(t) is t
+    assert copies == []
+    for t, how in ((off, ["contiguous", "clone"]), (turned, ["contiguous"])):
+        copies.clear()
+        got = rb._readable(t)
+        assert copies == how and rb._fits(got) and torch.equal(got, t)
