@@ -77,7 +77,12 @@ Tensor readable_heads(const Tensor& t) {
     const Tensor c = t.contiguous();
     return fits(c) ? c : t.clone(at::MemoryFormat::Contiguous);
 }
-Tensor empty_like_heads(const Tensor& t) { return empty_heads(t.sizes(), t.stride(1) < t.stride(2), t.options()); }
+// In the memory order of t, [B, L, H, d] where the heads of a row lie next to each other and the kernels take that.
+Tensor empty_like_heads(const Tensor& t) {
+    const int64_t row = t.size(1) * t.size(3);
+    const bool interleaved = t.stride(1) < t.stride(2) && row * t.element_size() <= 1 << 24 && t.size(2) * row < int64_t(1) << 29;
+    return empty_heads(t.sizes(), interleaved, t.options());
+}
 spion_heads heads_of(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 
 spion_bias_attention bias_call(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& w, const Tensor& buckets,

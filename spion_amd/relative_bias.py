@@ -97,9 +97,10 @@ def _readable(t):
 
 def _empty_like_heads(t):
     """Uninitialised heads in the memory order of ``t``: [B, L, H, d] where the heads of a row lie next to each other, as a
-    projection leaves them."""
+    projection leaves them.  [B, H, L, d] where the kernels would not take that (rows 2^24 bytes apart, heads of 2^29 elements and
+    more from their first row to their last): such a ``t`` is itself read from a copy."""
     B, H, L, d = t.shape
-    if t.stride(1) < t.stride(2):
+    if t.stride(1) < t.stride(2) and H * d * t.element_size() <= 1 << 24 and L * H * d < 1 << 29:
         return torch.empty((B, L, H, d), dtype=t.dtype, device=t.device).transpose(1, 2)
     return torch.empty((B, H, L, d), dtype=t.dtype, device=t.device)
 

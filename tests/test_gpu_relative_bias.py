@@ -510,3 +510,15 @@ def test_calls_go_by_their_own_status():
     finally:
         lib.spion_clear_error()
     _compare(got, bias_reference(q, k, v, w, buckets, do=do))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("how", ["interleaved", "shared"])
+def test_more_heads_than_rows_of_them_may_lie_apart(how, dtype):
+    """Heads next to each other in rows of more than 2^24 bytes: the operands are read from copies, and outputs and gradients lie
+    as the copies do.  One head shared by all is read in place, and its output would have such rows."""
+    H = (1 << 24) // (32 * (4 if dtype == torch.float32 else 2)) + 1
+    q, k, v, w, buckets, do = _inputs(dtype, 1, H, 2, 2, 32)
+    if how == "shared":
+        q, k, v = (t[:, :1].expand(1, H, 2, 32) for t in (q, k, v))
+    _compare(_run(q, k, v, w, buckets, do), bias_reference(q, k, v, w, buckets, do=do))

@@ -183,3 +183,24 @@ def test_heads_are_copied_only_where_they_have_to_be(monkeypatch):
         copies.clear()
         got = rb._readable(t)
         assert copies == how and rb._fits(got) and torch.equal(got, t)
+
+
+@pytest.mark.parametrize("dtype,H,L,d,interleaved", [
+    (torch.float32, 64, (1 << 17) - 1, 64, True), (torch.float32, 64, 1 << 17, 64, False),  # 2^29 elements to a head's rows
+    (torch.float32, 1 << 17, 2, 32, True), (torch.float32, (1 << 17) + 1, 2, 32, False),  # 2^24 bytes from row to row
+    (torch.bfloat16, 1 << 18, 2, 32, True), (torch.bfloat16, (1 << 18) + 1, 2, 32, False)])
+def test_outputs_lie_as_the_kernels_take_them(dtype, H, L, d, interleaved):
+    """Outputs follow the operands' memory order, but not where the library would refuse it: the operands are copied then."""
+    shared = torch.empty(1, 1, L, d, dtype=dtype, device="meta").expand(1, H, L, d)  # fits, its heads' stride is 0
+    for t in (torch.empty(1, L, H, d, dtype=dtype, device="meta").transpose(1, 2), shared):
+        out = rb._empty_like_heads(t)
+        assert out.shape == t.shape and out.stride()[1:] == ((d, H * d, 1) if interleaved else (L * d, d, 1))
+        call = rb._Call(weight=16, buckets=16, Lse=16, batch=1, heads=H, q_len=L, k_len=L, head_dim=d, bf16=int(dtype == torch.bfloat16),
+                        num_buckets=8, max_distance=20, Mean=16, mat=16, block_size=1 << 29)
+        for n in ("Q", "K", "V"):
+            setattr(call, n, rb._Heads(16, 0, 0, d))
+        call.Out = rb._Heads(16, *out.stride()[:3])
+        # refused for the map with a pattern, which is looked at after the heads: these are in order
+        assert rb._lib_typed().spion_bias_attention_forward(ctypes.addressof(call), None) != 0
+        with pytest.raises(_lib.SpionLibraryError, match="mean map"):
+            _lib.check_error()
