@@ -34,9 +34,14 @@ struct Walk {
 //   fp32, six products for one: fewer strips than the CUs hold are cut into pieces of at least 256 rows of the other side, and
 //     strips of 32 stay for launches that leave a quarter of the CUs idle even so (d = 64, 192 strips of L = 320: 39.8 / 24.5), and
 //     at d = 32 for the short ones among those that would have to be cut (128 strips: 24.7 / 27.3, of L = 4096 77.9 / 63.0).
-// The number of pieces is the one with the least rounds of work-groups times tiles to a piece.  A CU holds one work-group of the
-// fp32 backward at d = 64 (its LDS) and else two, which take 1.75 times as long together as one alone; a merge (5 us) counts as so
-// many tiles.  (backward, d = 64: 96 strips of L = 1000 in 2 / 4 pieces 128 / 137, 384 of 2048 in 1 / 2 pieces 614 / 563.)
+// The number of pieces is the one with the least rounds of work-groups times tiles to a piece, and the cost of the pieces.  A CU holds one
+// work-group of the fp32 backward at d = 64 (its LDS) and else two, which take 1.75 times as long together as one alone.  A merge
+// (5 us) counts as 2 tiles and 6, and every round of work-groups past the first that the machine holds as 4 and 2.5: their sums are
+// written and read again, and their tables set up.  (us, 12 heads of 1000, d = 64, backward: 1 / 2 / 4 pieces 163 / 129 / 142.  24
+// heads of 2048 in 1 / 2 / 8 pieces: forward 167 / 157 / 173, backward 663 / 563 / 755, at d = 32 102 / 95 / 104 and 297 / 288 / 302; 34 heads
+// 273 / 238 / 240, 994 / 901 / 1074, 166 / 142 / 142, 490 / 435 / 451; 257 heads 1467 / 1512 / 1855, 5744 / 6067 / 8130, 838 / 867 / 1048,
+// 2641 / 2743 / 3482.)  No more than eight work-groups to a CU: what pieces leave in the workspace stays below 71 MB forward and 135
+// backward at d = 64, half of it at 32; launches that fill the machine four times over are not cut, and could gain a tenth at most.
 enum class Pass { FORWARD, ROW, COL };
 static Walk walk_of(const Call& c, int rows, int others, bool can_split, Pass pass) {
     const long long cus = device_cus(), wide = (long long)c.batch * c.heads * strips_of(rows, 128), tiles = strips_of(others);
@@ -47,9 +52,11 @@ static Walk walk_of(const Call& c, int rows, int others, bool can_split, Pass pa
     } else {
         const bool alone = c.head_dim == 64 && pass != Pass::FORWARD;
         double least = 0;
-        for (long long n = 1; n == 1 || (can_split && n <= std::min(tiles / 8, 16LL)); ++n) {
+        for (long long n = 1; n == 1 || (can_split && n <= std::min(tiles / 8, 16LL) && n * wide <= 8 * cus); ++n) {
             const long long rounds = (wide * n + cus - 1) / cus, each = (tiles + n - 1) / n;
-            const double cost = (alone ? (double)rounds : 1.75 * (rounds / 2) + rounds % 2) * each + (n == 1 ? 0 : alone ? 2 : 6);
+            const double all = (double)(wide * n) / cus;
+            const double extra = n == 1 ? 0 : alone ? 2 + 4 * std::max(0., all - 1) : 6 + 2.5 * std::max(0., all - 2);
+            const double cost = (alone ? (double)rounds : 1.75 * (rounds / 2) + rounds % 2) * each + extra;
             if (n == 1 || cost < least) least = cost, pieces = n;
         }
         dense = dense && 4 * wide * pieces >= 3 * cus && (c.head_dim == 64 || tiles > 32 || 4 * wide >= 3 * cus);

@@ -522,3 +522,21 @@ def test_more_heads_than_rows_of_them_may_lie_apart(how, dtype):
     if how == "shared":
         q, k, v = (t[:, :1].expand(1, H, 2, 32) for t in (q, k, v))
     _compare(_run(q, k, v, w, buckets, do), bias_reference(q, k, v, w, buckets, do=do))
+
+
+# fewer strips of 128 rows than work-groups wanted, over a pattern: pieces of its stages in both passes
+@pytest.mark.parametrize("H,L,block,d", [(9, 2000, 128, 32), (12, 1000, 64, 64), (12, 1000, 128, 64)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_block_patterns_in_pieces(H, L, block, d, masked):
+    q, k, v, w, buckets, do = _inputs(torch.float32, 1, H, L, L, d, seed=L)
+    nb = -(-L // block)
+    mat = torch.from_numpy(workloads.band_random_block_mask(nb, 0, extra_frac=0.3, seed=L)).to(DEV)
+    mat[-1] = 0.0
+    mat[0] = 1.0
+    mask = _lengths_mask(1, L, 9, "lengths") if masked else None
+    call = rb._call_of(q, k, w, buckets, mask, mat, block, 0)
+    lib = rb._lib_typed()
+    assert lib.spion_bias_workspace(ctypes.addressof(call), 0) >= 2 * H * -(-L // 32) * 32 * d  # sums of two pieces at least
+    assert lib.spion_bias_workspace(ctypes.addressof(call), 1) >= 2 * H * -(-L // 32) * 64 * d
+    got = _run(q, k, v, w, buckets, do, key_mask=mask, mat=mat, block_size=block)
+    _compare(got, bias_reference(q, k, v, w, buckets, mask, mat, block, do=do))

@@ -204,3 +204,31 @@ def test_outputs_lie_as_the_kernels_take_them(dtype, H, L, d, interleaved):
         assert rb._lib_typed().spion_bias_attention_forward(ctypes.addressof(call), None) != 0
         with pytest.raises(_lib.SpionLibraryError, match="mean map"):
             _lib.check_error()
+
+
+def _floats(nb, Lq, Lk, d, backward, **more):
+    c = rb._Call(batch=nb, heads=1, q_len=Lq, k_len=Lk, head_dim=d, num_buckets=32, max_distance=128, **more)
+    return rb._lib_typed().spion_bias_workspace(ctypes.addressof(c), backward)
+
+
+@pytest.mark.parametrize("d", [32, 64])
+@pytest.mark.parametrize("nb,L", [(257, 2048), (130, 4096), (1030, 4096), (131000, 4096)])
+def test_calls_that_fill_the_machine_many_times_over_are_not_cut(nb, L, d):
+    """(A machine of 256 CUs.)  Only D and the table's gradient by strips of 128 rows are left in the workspace; the pieces of 257 heads
+    of 2048 took 1.1 GB forward and 2.2 GB backward, and of 131000 heads of 4096 more work-groups than a launch holds."""
+    assert _floats(nb, L, L, d, 0) == 0
+    assert _floats(nb, L, L, d, 1) == nb * L + nb * (L // 128) * 32
+
+
+@pytest.mark.parametrize("d", [32, 64])
+def test_pieces_leave_a_bounded_workspace(d):
+    """Eight work-groups of 128 rows for each of 256 CUs at most, whatever the sizes; strips of 32 rows in the forward come in pieces of
+    fewer."""
+    groups, slot = 8 * 256, 4 * (32 * d + 96)
+    for nb in (1, 3, 12, 40, 100, 128, 200, 257, 300, 512, 700, 1000):
+        for Lq in (65, 200, 700, 1030, 2048, 5000):
+            for Lk in (90, Lq, 3000, 40000):
+                for more in ({},) if Lq != Lk else ({}, dict(mat=16, block_size=64), dict(mat=16, block_size=32)):
+                    assert _floats(nb, Lq, Lk, d, 0, **more) <= groups * slot, (nb, Lq, Lk)
+                    base = nb * Lq + 3 + 32 * max(groups, nb * -(-Lk // 32)) + 3
+                    assert _floats(nb, Lq, Lk, d, 1, **more) <= base + groups * max(slot, 4 * 64 * d), (nb, Lq, Lk)
