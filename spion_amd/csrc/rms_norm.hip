@@ -376,29 +376,33 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormCall a) {
     }
 }
 
-// dw = sum of the work-groups' parts, 16 columns (one line of 64 bytes) a work-group, so that narrow rows still spread over CUs: 64
-// threads to a column take every 64th part, four loads in flight, and add up in a fixed order.
+// dw = sum of the work-groups' parts, 16 columns (one line of 64 bytes) at a time, so that narrow rows still spread over CUs: 64
+// threads to a column take every 64th part, four loads in flight, and add up in a fixed order.  (2^18 work-groups at most: a launch holds fewer
+// than 2^32 threads, and rows are up to 2^29 wide.)
 template <class T>
 __global__ __launch_bounds__(1024) void norm_weight_kernel(const float* __restrict__ part, T* __restrict__ dw, int groups, int n) {
     __shared__ float s[64][17];
-    const int l = threadIdx.x & 15, w = threadIdx.x >> 4, i = blockIdx.x * 16 + l;
-    float v = 0.f;
-    if (i < n) {
-        const float* p = part + i;
-        int g = w;
-        for (; g + 192 < groups; g += 256) {
-            const float x0 = p[(size_t)g * n], x1 = p[(size_t)(g + 64) * n], x2 = p[(size_t)(g + 128) * n], x3 = p[(size_t)(g + 192) * n];
-            v += (x0 + x1) + (x2 + x3);
+    const int l = threadIdx.x & 15, w = threadIdx.x >> 4;
+    for (int first = blockIdx.x * 16; first < n; first += gridDim.x * 16) {
+        float v = 0.f;
+        if (first + l < n) {
+            const float* p = part + first + l;
+            int g = w;
+            for (; g + 192 < groups; g += 256) {
+                const float x0 = p[(size_t)g * n], x1 = p[(size_t)(g + 64) * n], x2 = p[(size_t)(g + 128) * n], x3 = p[(size_t)(g + 192) * n];
+                v += (x0 + x1) + (x2 + x3);
+            }
+            for (; g < groups; g += 64) v += p[(size_t)g * n];
         }
-        for (; g < groups; g += 64) v += p[(size_t)g * n];
-    }
-    s[w][l] = v;
-    __syncthreads();
-    if (w < 16) {  // thread (w, l): column w, parts l, l + 16, ...
-        v = (s[l][w] + s[l + 16][w]) + (s[l + 32][w] + s[l + 48][w]);
+        s[w][l] = v;
+        __syncthreads();
+        if (w < 16) {  // thread (w, l): column w, parts l, l + 16, ...
+            v = (s[l][w] + s[l + 16][w]) + (s[l + 32][w] + s[l + 48][w]);
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
-        if (l == 0 && blockIdx.x * 16 + w < n) dw[blockIdx.x * 16 + w] = (T)v;
+            for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
+            if (l == 0 && first + w < n) dw[first + w] = (T)v;
+        }
+        __syncthreads();
     }
 }
 
@@ -483,7 +487,7 @@ static bool run_norm(const Call& c, bool backward, hipStream_t stream) {
     const bool ok = norm_piece(c, backward) == 1 ? run_piece<T, 1>(c, a, backward, stream, groups)
                                                  : run_piece<T, 16 / sizeof(T)>(c, a, backward, stream, groups);
     if (!ok || !backward) return ok;
-    hipLaunchKernelGGL((norm_weight_kernel<T>), dim3((c.width + 15) / 16), dim3(1024), 0, stream, c.workspace, reinterpret_cast<T*>(c.dweight),
+    hipLaunchKernelGGL((norm_weight_kernel<T>), dim3(std::min((c.width + 15) / 16, 1 << 18)), dim3(1024), 0, stream, c.workspace, reinterpret_cast<T*>(c.dweight),
                        (int)groups, c.width);
     return check_launch("norm_weight_kernel");
 }

@@ -319,3 +319,19 @@ def test_calls_go_by_their_own_status():
     finally:
         lib.spion_clear_error()
     _check(x, w, None, dy, None, *got)
+
+
+def test_rows_wider_than_a_launch_has_threads_for():
+    """2^26 columns and more: at 64 threads to a column the weight's gradient would take 2^32 threads.  Elements of 1 and -1 make every sum
+    exact up to 2^24 and rounded by a few u beyond: 16 u of the magnitudes in each result."""
+    n = (1 << 26) + 5
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, dy = ((torch.randint(0, 2, (2, n), generator=g, device=DEV) * 2 - 1).float() for _ in range(2))
+    w = torch.ones(n, device=DEV)
+    y, _, dx, dw = _train(x, w, None, dy, None)
+    inv = 1.0 / (1.0 + EPS) ** 0.5
+    m = inv * (x.double() * dy.double()).sum(1, keepdim=True) / n  # mean of dy w h inv
+    assert float((y.detach().double() - x.double() * inv).abs().max()) <= 16 * U
+    assert float((dx.double() - inv * (dy.double() - x.double() * inv * m)).abs().max()) <= 16 * U * (1 + float(m.abs().max()))
+    want = (x.double() * dy.double()).sum(0) * inv
+    assert float((dw.double() - want).abs().max()) <= 16 * U * 2
