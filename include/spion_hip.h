@@ -498,7 +498,8 @@ int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, i
  *   mat          null: Z_i is the sum over all keys that take part.  Else [nb][nb] floats, nb = ceil(k_len / block_size): pairs
  *                in blocks that are 0 have P = 0 but count in Z_i with a logit of 0, masked or not, as in the other sparse
  *                families; block_size a multiple of 32, q_len = k_len, offset 0.
- *   Lse          [batch * heads][q_len] fp32, out of the forward and into the backward: log2 Z_i, +infinity for empty rows.
+ *   Lse          [batch * heads][q_len] fp32, out of the forward and into the backward: log2 Z_i, +infinity for empty rows, NaN
+ *                where a logit that takes part is one (all of the row's P are NaN then).
  *   Mean         null, or [q_len][k_len] fp32, out: the mean of P over batch and heads (spion_pattern_generate's Score input);
  *                not with mat.
  *   workspace    spion_bias_workspace(call, backward) floats, 16-byte aligned, contents unspecified; a forward without it walks

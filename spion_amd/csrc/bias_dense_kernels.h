@@ -368,8 +368,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 2)) void bias_forward_de
         m = up;
     }
     if (h == 0 && q0 + li < a.Lq)
-        a.lse[(size_t)it.bh * a.Lq + q0 + li] = z > 0.f ? m + __builtin_amdgcn_logf(z) : __builtin_inff();
-    store_strip<D>(o, z > 0.f ? scale / z : 0.f, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
+        a.lse[(size_t)it.bh * a.Lq + q0 + li] = z == 0.f ? __builtin_inff() : m + __builtin_amdgcn_logf(z);
+    store_strip<D>(o, z == 0.f ? 0.f : scale / z, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&x)[D / 8]) {
         if (q0 + row < a.Lq) store_eighth<T, D>(a.o, it.b, it.h, q0 + row, j, x);
     });
 }

@@ -212,9 +212,9 @@ __global__ __launch_bounds__(256, (bias_waves<T, D>())) void bias_forward_kernel
             Z = Z * scale + off * __builtin_amdgcn_exp2f(-up);
             M = up;
         }
-        sc.row[li] = Z > 0.f ? scale / Z : 0.f;
+        sc.row[li] = Z == 0.f ? 0.f : scale / Z;
         if (q0 + li < a.Lq)
-            a.lse[(size_t)it.bh * a.Lq + q0 + li] = Z > 0.f ? M + __builtin_amdgcn_logf(Z) : __builtin_inff();
+            a.lse[(size_t)it.bh * a.Lq + q0 + li] = Z == 0.f ? __builtin_inff() : M + __builtin_amdgcn_logf(Z);
     }
     __syncthreads();
     if (q0 + row < a.Lq) {
@@ -258,11 +258,11 @@ __global__ __launch_bounds__(256) void bias_merge_kernel(BiasCall a) {
             for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e] * f;
         }
     }
-    const float inv = Z > 0.f ? 1.f / Z : 0.f;
+    const float inv = Z == 0.f ? 0.f : 1.f / Z;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) x[i] *= inv;
     store_eighth<T, D>(a.o, b, ih, q, j, x);
-    if (j == 0) a.lse[(size_t)bh * a.Lq + q] = Z > 0.f ? M + __builtin_amdgcn_logf(Z) : __builtin_inff();
+    if (j == 0) a.lse[(size_t)bh * a.Lq + q] = Z == 0.f ? __builtin_inff() : M + __builtin_amdgcn_logf(Z);
 }
 
 // -------------------------------------------------------------------------------------------------

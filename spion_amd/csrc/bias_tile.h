@@ -32,7 +32,7 @@ struct BiasCall {
     const int* map;     // [2 R + 1]: bucket of every difference -R .. R
     const void* mask;   // [B][Lk]: null, float (0 = left out) or bytes
     const float* mat;   // [nb][nb] pattern of bs x bs blocks, or null
-    float* lse;         // [B*H][Lq]: log2 of the softmax denominator, +inf for rows that nothing enters
+    float* lse;         // [B*H][Lq]: log2 of the softmax denominator, +inf for rows that nothing enters (NaN stays NaN)
     float* delta;       // [B*H][Lq]: sum over the keys of P dP
     float* part;        // workspace: the pieces' slots
     float* tables;      // workspace: the table's gradient by strips, [B*H][strips][splits][buckets]

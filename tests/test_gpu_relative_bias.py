@@ -540,3 +540,36 @@ def test_block_patterns_in_pieces(H, L, block, d, masked):
     assert lib.spion_bias_workspace(ctypes.addressof(call), 1) >= 2 * H * -(-L // 32) * 64 * d
     got = _run(q, k, v, w, buckets, do, key_mask=mask, mat=mat, block_size=block)
     _compare(got, bias_reference(q, k, v, w, buckets, mask, mat, block, do=do))
+
+
+# every walk: strips of 32, whole and in pieces, of 128, of 64 over a pattern; the NaN in a key that takes part, in one head of one sample
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,Lq,Lk,d,block", [(2, 2, 70, 90, 32, 0), (1, 2, 3, 3000, 64, 0), (64, 4, 200, 200, 64, 0), (2, 2, 160, 160, 32, 32),
+                                               (40, 2, 300, 300, 64, 64)])
+def test_a_nan_is_not_hidden(B, H, Lq, Lk, d, block, dtype):
+    """A NaN among a row's logits makes all of its probabilities NaN: the output, the map and dV show it, for the rows (with a pattern:
+    of the blocks) that see the key, and nowhere else."""
+    q, k, v, w, buckets, do = _inputs(dtype, B, H, Lq, Lk, d)
+    mask = torch.ones(B, Lk, dtype=torch.bool, device=DEV)
+    mask[:, -5:] = False
+    k[1 if B > 1 else 0, 1, 17, 3] = math.nan
+    mat = None
+    rows, keys = torch.ones(Lq, dtype=torch.bool, device=DEV), mask[0]
+    if block:
+        nb = -(-Lk // block)
+        mat = torch.eye(nb, device=DEV)
+        mat[2, 0] = mat[2, 1] = 1.0
+        at = torch.arange(Lk, device=DEV) // block
+        rows = mat[at, 0] != 0
+        keys = keys & (at <= 2)  # blocks that rows of the first block or of the third see
+    kw = dict(key_mask=mask, mat=mat, block_size=block) if block else dict(key_mask=mask)
+    got = _run(q, k, v, w, buckets, do, **kw)
+    for n, t, seen in (("out", got["out"], rows), ("dq", got["dq"], rows), ("dv", got["dv"], keys)):
+        bad = torch.isnan(t)
+        hit = bad[1 if B > 1 else 0, 1]
+        assert bool(hit[seen].all()) and not bool(hit[~seen].any()), n
+        assert int(bad.sum()) == int(hit.sum()), n
+    if not block:
+        with torch.no_grad():
+            mean = spion_amd.relative_bias_attention(q, k, v, w, buckets, score_map=True, **kw)[1]
+        assert bool(torch.isnan(mean[:, mask[0]]).all()) and not bool(mean[:, ~mask[0]].any())
