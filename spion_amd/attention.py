@@ -152,8 +152,8 @@ class Attention(nn.Module):
         torch's usual rule for capturing a backward: warm up on a side stream and keep no autograd graph of a step
         that ran on the default stream alive (its AccumulateGrad nodes belong to the legacy stream, which a capture
         must not touch; breaking this rule ends in a crash inside capture_end on ROCm, not in an error message)."""
-        if self.norm is not None:
-            X = self.norm(X)
+        if self.norm is not None:  # (fp16 rows, as autocast leaves them, in fp32: what follows casts for itself)
+            X = self.norm(X.float() if X.dtype == torch.float16 else X)
         node, weights = self._compiled_node(X, mask)
         if node is not None and mat is not None and not self.relative:
             done = self._sparse_layer(node, weights, X, mask, mat)

@@ -160,3 +160,18 @@ def test_two_streams_at_once():
     for i in range(2):
         for run in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
+
+
+@pytest.mark.parametrize("mat", [False, True])
+def test_half_rows_under_autocast(mat):
+    """Autocast leaves rows in fp16, which a layer without the norm takes as well: they are normalised in fp32."""
+    layer = _layer("lra-listops")
+    mask, pattern = torch.ones(B, L, device=DEV), torch.ones(L // BS, L // BS, device=DEV) if mat else None
+    X = torch.randn(B, L, 64, generator=torch.Generator().manual_seed(5)).half().to(DEV)
+    got = []
+    for x in (X.detach().requires_grad_(), X.float().requires_grad_()):
+        with torch.autocast("cuda", torch.float16):
+            y, _ = layer(x, mask, pattern)
+        got.append((y, *torch.autograd.grad(y.float().sum(), (x, layer.norm.weight))))
+    (a, da, wa), (b, db, wb) = got
+    assert torch.equal(a, b) and torch.equal(da, db.half()) and torch.equal(wa, wb)
