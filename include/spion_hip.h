@@ -490,7 +490,8 @@ int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, i
  *   heads        [B][H][L][d] tensors or views, strides in elements, multiples of 16 bytes; pointers 16-byte aligned; d = 32 or 64.
  *                The strides of tensors that are only read may be 0 (a head shared by others).  Rows lie up to 2^24 bytes apart,
  *                a head within 2^31 bytes.
- *   weight       [num_buckets][heads], of the heads' type, up to 32767 buckets; dweight alike.
+ *   weight       [num_buckets][heads], of the heads' type, up to 32767 buckets; dweight alike.  -infinity (and below -2.3e38) takes a
+ *                bucket's pairs out.
  *   buckets      [2 R + 1] ints in 0 .. num_buckets - 1 (anything else is read as the nearest of them); 1 <= R <= 1024.
  *   offset       query i stands at position i + offset of the keys' count.
  *   key_mask     null, or [batch][k_len] floats (mask_bytes 4) or bytes (1): keys with a 0 are left out, and nothing of their K and V
@@ -499,7 +500,8 @@ int spion_key_penalty(const float* mask, float* penalty, int batch, int heads, i
  *                in blocks that are 0 have P = 0 but count in Z_i with a logit of 0, masked or not, as in the other sparse
  *                families; block_size a multiple of 32, q_len = k_len, offset 0.
  *   Lse          [batch * heads][q_len] fp32, out of the forward and into the backward: log2 Z_i, +infinity for empty rows, NaN
- *                where a logit that takes part is one (all of the row's P are NaN then).
+ *                where a logit that takes part is one (all of the row's P are NaN then).  One number: logits of size m leave the
+ *                P of the backward and of Mean off by m 2^-24 of themselves.
  *   Mean         null, or [q_len][k_len] fp32, out: the mean of P over batch and heads (spion_pattern_generate's Score input);
  *                not with mat.
  *   workspace    spion_bias_workspace(call, backward) floats, 16-byte aligned, contents unspecified; a forward without it walks

@@ -5,12 +5,14 @@
 // fill the machine the other side of an fp32 call is cut into pieces; each leaves its sums in a slot of the workspace for every 32
 // rows, and a second launch adds the pieces of a strip up in their order.  (Which calls: walk_of in relative_bias.hip.)
 //
-// What bounds them, 128 padded heads of 2048, bf16, d = 64: forward 169 us (610 TFLOP/s), row pass 224 (690), column pass 337 (610).  The
-// matrix units are busy for 31 to 33 % of it, the vector units for about half (exponentials, bias, conversions, sums), LDS has 0.3
-// to 4 % conflicts, and memory moves 0.1 to 0.2 GB: two wavefronts a SIMD (three in the forward) take turns, and what one waits
-// for the others do not fill.  64 rows to a wavefront halve the LDS reads, and were slower for the registers they take (column
-// pass 337 -> 449).  16 heads of 8192 with a tenth of their 64 x 64 blocks: 79, 106 and 148 us, of which 19, 30 and 45 are there
-// without any block.  128 fp32 heads of 1024, d = 32: forward 121 to 127 us, matrix units 42 % busy.
+// What bounds them, 128 padded heads of 2048, bf16, d = 64: forward 169 us (610 TFLOP/s), row pass 226 (680), column pass 337 to 345 (600).
+// The matrix units are busy for 31 to 33 % of it, the vector units for about half (exponentials, bias, conversions, sums), LDS has 0.3
+// to 4 % conflicts, and memory moves 0.1 to 0.2 GB: two wavefronts a SIMD (three in the forward, for which it spills 20 bytes a
+// lane) take turns, and what one waits for the others do not fill.  64 rows to a wavefront halve the LDS reads, and were slower
+// for the registers they take (column pass 337 -> 449).  16 heads of 8192 with a tenth of their 64 x 64 blocks: 79, 106 and 145 us,
+// of which 19, 30 and 45 are there without any block.  128 fp32 heads of 1024, d = 32: forward 121 to 127 us, matrix units 42 % busy.
+// (Times of kernels by themselves, under the profiler; in a call they follow each other more closely: these steps take 657 to 699 us and
+// 305, table included.)
 #pragma once
 #include "bias_kernels.h"
 

@@ -74,7 +74,9 @@ struct BiasItem {
     }
 };
 
-// Wavefronts a SIMD that the registers are for.  fp32 heads of 64 features have one work-group's tiles in a CU's LDS.
+// Wavefronts a SIMD that the registers are for.  fp32 heads of 64 features: one.  Strips of 32 have one work-group's tiles in a CU's
+// LDS (98 KB); the backward passes over shared stages take 56 to 93 KB, which mostly leaves room for two, but 320 and 350 registers.
+// (The bf16 column pass of strips of 32 at d = 64 has all of its 256 registers in use and spills 44 bytes a lane.)
 template <class T, int D>
 constexpr int bias_waves() { return sizeof(T) == 4 && D == 64 ? 1 : 2; }
 

@@ -3,13 +3,16 @@
 //   h = x + residual, rounded to the tensors' type: the stream as it goes on;   inv = 1 / sqrt(mean(h^2) + eps);   y = h inv w
 //   8 bits: scale = max|y| / 448 of the unrounded row, codes = e4m3(y / scale), where 1 / rms cancels
 //   dh = inv (dy w - h inv mean(dy w h inv)) + (gradient of the stream);   dw = sum over the rows of dy h inv
-// Bound by memory: every tensor is read or written once.  A row lies in the registers of 16, 64, 256 or 1024 lanes in pieces of
-// 16 bytes, so the statistics need no second pass over it; rows that are not 16-byte aligned go an element a lane, and rows longer
-// than the registers of a work-group are read again for each step (from L2).  Statistics and sums are fp32.  Work-groups
-// walk several rows each: the weight is read once, and the backward leaves one partial dw a work-group, which a second launch
-// adds up in a fixed order.
+// Bound by memory: every tensor is read or written once where rows start on 16 bytes.  A row lies in the registers of 16, 64, 256 or
+// 1024 lanes in pieces of 16 bytes (up to 16384 fp32 or 32768 bf16 elements), so the statistics need no second pass over it.  Where a
+// width or stride is no multiple of 16 bytes a piece is one element, which holds rows of up to 4096; longer rows are read again
+// for each step (from L2).  Statistics and sums are fp32.  Work-groups walk several rows each: the weight is read once, and the
+// backward leaves one partial dw a work-group, which a second launch adds up in a fixed order.
 // 262144 x 64 fp32: forward 45 us, backward 42 + 4; 8192 x 4096 bf16: 45 and 51 + 6; 16384 x 1000 bf16 to 8 bits: 20.  As many bytes at the
-// 5062 GB/s of a copy of 1 GB: 53, 53 and 53, 53 and 23.
+// 5062 GB/s of a copy of 1 GB: 53, 53 and 53, 53 and 23.  Off 16 bytes, bf16, calls: 16384 x 1001 25 us forward and 74 a step (1000: 21 and
+// 73), 262144 x 65 39 and 114 (64: 23 and 74), 8192 x 4100 94 and 289 (4096: 41 and 105), 8192 x 5415 165 and 383 (5416: 73 and 170); fp32
+// 262144 x 65 60 and 148 (64: 40 and 90), 8192 x 5415 201 and 452 (5416: 135 and 284).  The backward of bf16 rows past 16384 spills
+// (424 bytes a lane): 1024 x 32768 312 us a step (2048 x 16384: 115).
 #include "common.h"
 #include "tile_ops.h"
 #include "../../include/spion_hip.h"

@@ -234,7 +234,11 @@ def relative_bias_attention(query, key, value, weight, buckets, key_mask=None, m
     key_mask [B, Lk]: keys with a 0 are left out (bool, or any type, compared with 0); a row without keys gives zeros.
     mat [nb, nb] with block_size: pairs in blocks that are 0 have probability 0 and count in the softmax with a logit of 0, as in
     the other sparse modules.  offset: query i stands at position i + offset (the last queries of a sequence: Lk - Lq).
-    score_map: also return the mean of the probability maps over batch and heads, fp32 [Lq, Lk], without a gradient."""
+    score_map: also return the mean of the probability maps over batch and heads, fp32 [Lq, Lk], without a gradient.
+
+    An entry of weight that is -infinity (or the type's lowest value) takes its pairs out; a row that loses all of them gives zeros.
+    Large finite entries do not serve for that: log2 Z is one fp32 number, and where all of a row's logits are near -1e9 it has no
+    room for the sum: the row's gradients come out too large."""
     node = _lib.autograd_node()
     if node is not None and _lib.plain_autograd():  # csrc/operator_nodes.h: the same steps
         try:

@@ -573,3 +573,14 @@ def test_a_nan_is_not_hidden(B, H, Lq, Lk, d, block, dtype):
         with torch.no_grad():
             mean = spion_amd.relative_bias_attention(q, k, v, w, buckets, score_map=True, **kw)[1]
         assert bool(torch.isnan(mean[:, mask[0]]).all()) and not bool(mean[:, ~mask[0]].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_buckets_of_the_lowest_value_are_left_out_too(dtype):
+    """The type's lowest value times log2(e) is -infinity: the same bits as with -infinity, rows that lose everything among them."""
+    q, k, v, w, buckets, do = _inputs(dtype, 1, 2, 200, 120, 32, buckets=8, distance=20)
+    got = []
+    for x in (-math.inf, torch.finfo(dtype).min):
+        w[3] = w[7] = x
+        got.append(_run(q, k, v, w, buckets, do))
+    assert all(torch.equal(got[0][n], got[1][n]) for n in got[0])
