@@ -584,3 +584,36 @@ def test_buckets_of_the_lowest_value_are_left_out_too(dtype):
         w[3] = w[7] = x
         got.append(_run(q, k, v, w, buckets, do))
     assert all(torch.equal(got[0][n], got[1][n]) for n in got[0])
+
+
+def test_refused_calls_in_another_thread(monkeypatch):
+    """One thread's calls are all refused by the library while another's steps run: each raises for its own, and no step is disturbed."""
+    import threading
+
+    monkeypatch.setenv("SPION_QUIET", "1")
+    q, k, v, w, buckets, do = _inputs(torch.float32, 1, 2, 40, 40, 32)
+    many = torch.zeros(32768, 2, device=DEV)
+    first = _run(q, k, v, w, buckets, do)
+    torch.cuda.synchronize()
+    refused, began, stop = [0, 0], threading.Event(), threading.Event()
+
+    def refuse():
+        while not stop.is_set():
+            try:
+                spion_amd.relative_bias_attention(q, k, v, many, buckets)
+            except _lib.SpionLibraryError as e:
+                refused["32767 buckets" not in str(e)] += 1
+            began.set()
+
+    other = threading.Thread(target=refuse)
+    other.start()
+    try:
+        assert began.wait(60)
+        steps = [_run(q, k, v, w, buckets, do) for _ in range(200)]
+    finally:
+        stop.set()
+        other.join()
+    assert refused[0] > 0 and refused[1] == 0
+    assert _lib.core().spion_error_pending() == 0
+    for got in steps:
+        assert all(torch.equal(got[n], first[n]) for n in first)
