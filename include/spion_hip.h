@@ -565,6 +565,68 @@ long long spion_rms_norm_workspace(const spion_rms_norm* call);
 int spion_rms_norm_forward(const spion_rms_norm* call, void* stream);
 int spion_rms_norm_backward(const spion_rms_norm* call, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Attention of queries to keys of another length (no counterpart in the reference, whose attention is an encoder's own):
+ * cross attention to an encoder's states.  Forward and backward of
+ *
+ *   P_ij = exp((q_i . k_j) / sqrt(d)) / Z_i,   Out_i = sum_j P_ij v_j        over the keys j that take part
+ *
+ * where heads / key_heads heads of queries, one behind the other, share a head of keys and values; their dK and dV are summed.
+ * fp32 or bf16 tensors, sums and softmax in fp32; the probabilities are never written.  Sizes come with every call; there is no
+ * handle, nothing is kept between calls, and the workspace is the caller's: calls with workspaces of their own may overlap.
+ *   heads        Q, Out, dO, dQ [B][heads][q_len][d], K, V, dK, dV [B][key_heads][k_len][d]: tensors or views, strides in elements,
+ *                multiples of 16 bytes; pointers 16-byte aligned; d = 32, 64 or 128.  The strides of tensors that are only read may
+ *                be 0.  Rows lie up to 2^24 bytes apart, a head of keys and the heads of queries that share it within 2^31 bytes.
+ *   key_mask     null, or [batch][k_len] floats (mask_bytes 4) or bytes (1): keys with a 0 are left out, and nothing of their K and V
+ *                is used.  A row without any key has an Out of 0 and no gradients.
+ *   Lse          [batch * heads][q_len] fp32, out of the forward and into the backward: log2 Z_i, +infinity for empty rows, NaN
+ *                where a logit that takes part is one.
+ *   workspace    spion_cross_workspace(call, backward) floats, 16-byte aligned, contents unspecified; a forward without it walks
+ *                the keys in one piece.  The same inputs give the same bits.
+ * Each returns 0 on success (spion_cross_workspace: -1 on failure); spion_take_call_error has the message.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct spion_cross_attention {
+    spion_heads Q, K, V, Out;      /* Out: written by the forward, read by the backward */
+    spion_heads dO, dQ, dK, dV;    /* backward only */
+    const void* key_mask;
+    float* Lse;
+    float* workspace;
+    long long workspace_floats;
+    int batch, heads, key_heads, q_len, k_len, head_dim, bf16, mask_bytes;
+} spion_cross_attention;
+long long spion_cross_workspace(const spion_cross_attention* call, int backward);
+int spion_cross_attention_forward(const spion_cross_attention* call, void* stream);
+int spion_cross_attention_backward(const spion_cross_attention* call, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Layer norm of rows with the residual's addition (the reference's layer adds in one operation and normalises with nn.LayerNorm in
+ * the next, models/model_transformer.py:55-102):
+ *
+ *   h = x + residual (rounded to the tensors' type),  y = (h - mean(h)) / sqrt(mean((h - mean(h))^2) + eps) * weight + bias
+ *
+ * fp32 or bf16 rows of any width; statistics and sums in fp32.  No handle; the workspace is the caller's.
+ *   forward    x, residual (may be null: h is x and not written), weight [width], bias [width] (may be null); out: h and y [rows][width].
+ *   backward   x: the stream h of the forward; dy, and dh (may be null), the gradients of y and of the stream; out: dx [rows][width],
+ *              the gradient of x and of the residual, dweight [width] and dbias [width] (may be null).  workspace:
+ *              spion_layer_norm_workspace(call) floats, contents unspecified.  The same inputs give the same bits.
+ * Row strides in elements for what is read; what is written is contiguous and overlaps nothing that is read.  Each returns 0 on
+ * success (the workspace: -1 on failure); spion_take_call_error has the message.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct spion_layer_norm {
+    const void *x, *residual, *weight, *bias;
+    void *y, *h;
+    const void *dy, *dh;
+    void *dx, *dweight, *dbias;
+    float* workspace;
+    long long workspace_floats;
+    long long rows, x_stride, residual_stride, dy_stride, dh_stride;
+    int width, bf16;
+    float eps;
+} spion_layer_norm;
+long long spion_layer_norm_workspace(const spion_layer_norm* call);
+int spion_layer_norm_forward(const spion_layer_norm* call, void* stream);
+int spion_layer_norm_backward(const spion_layer_norm* call, void* stream);
+
 const char* spion_version(void);
 
 #ifdef __cplusplus

@@ -20,7 +20,8 @@ from .pattern import (
     mean_score_map,
 )
 from .relative_bias import RelativeBiasAttention, relative_bias_attention, relative_position_buckets
-from .norm import RMSNorm, rms_norm, rms_norm_fp8
+from .attention_cross import CrossAttention, cross_attention
+from .norm import LayerNorm, RMSNorm, layer_norm, rms_norm, rms_norm_fp8
 
 __all__ = [
     "Attention",
@@ -50,4 +51,8 @@ __all__ = [
     "RMSNorm",
     "rms_norm",
     "rms_norm_fp8",
+    "CrossAttention",
+    "cross_attention",
+    "LayerNorm",
+    "layer_norm",
 ]

@@ -7,7 +7,7 @@ block_size, batch_size, attention_dropout, task.
 
 Two keys the reference does not have: ``relative_buckets`` (with ``relative_max_distance``) gives the layer a learned bias by
 relative position: ``attn`` is then a ``RelativeBiasAttention`` and the core of both phases; ``rms_norm`` (True, or the eps) lets it
-normalise its input first, ``norm`` (spion_amd/norm.py).
+normalise its input first, ``norm`` (spion_amd/norm.py); so does ``layer_norm`` with the layer norm.
 """
 from __future__ import annotations
 
@@ -126,6 +126,12 @@ class Attention(nn.Module):
             from .norm import RMSNorm
             eps = config["rms_norm"]
             self.norm = RMSNorm(self.dim) if eps is True else RMSNorm(self.dim, eps)
+        if config.get("layer_norm"):
+            from .norm import LayerNorm
+            if self.norm is not None:
+                raise ValueError("rms_norm or layer_norm expected, not both")
+            eps = config["layer_norm"]
+            self.norm = LayerNorm(self.dim) if eps is True else LayerNorm(self.dim, eps)
 
         if not inference and not self.relative:
             if config["task"] == "lra-pathfinder32-curv_contour_length_14":

@@ -17,7 +17,7 @@ LIB = os.path.join(HERE, "lib")
 OBJ = os.path.join(LIB, "obj")
 
 HIP_SOURCES = ["sparse_attn.hip", "dense_attn.hip", "capi.hip", "pattern.hip", "project.hip", "relative_bias.hip",
-               "rms_norm.hip"]
+               "rms_norm.hip", "cross_attention.hip", "layer_norm.hip"]
 DROPINS = {1: "attn.so", 2: "attn_mask.so", 3: "block_attn.so", 4: "block_attn_mask.so"}
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -835,5 +835,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("relative_bias_attention", &relative_bias_attention, "attention with a relative position bias; returns [out] or [out, mean map]");
     m.def("rms_norm", &rms_norm, "norm of rows; returns [y] or [y, h]");
     m.def("rms_norm_fp8", &rms_norm_fp8, "norm of rows in 8 bits; returns [codes, scales] or [codes, scales, h]");
+    m.def("layer_norm", &layer_norm, "layer norm of rows; returns [y] or [y, h]");
+    m.def("cross_attention", &cross_attention, "attention to keys of another length");
     m.def("merge_heads", &merge_heads, "the output projection of [B, H, L, d] heads");
 }

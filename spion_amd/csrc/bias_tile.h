@@ -78,6 +78,7 @@ struct BiasTile {
     };
     __device__ static __forceinline__ int swz(int r) {
         if constexpr (D == 64) return ((r << 1) & 4) | ((r >> 1) & 2) | ((r >> 3) & 1);  // even (odd) rows of 16: all eight, r and r + 2 differ in 4
+        else if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);  // sixteen rows: all sixteen, four rows differ in 4 and 8
         else return (r >> 2) & 3;
     }
     __device__ static __forceinline__ At at(int l) {

@@ -150,6 +150,12 @@ int bias_backward(const spion_bias_attention*, hipStream_t);
 long long norm_workspace(const spion_rms_norm*);
 int norm_forward(const spion_rms_norm*, hipStream_t);
 int norm_backward(const spion_rms_norm*, hipStream_t);
+long long cross_workspace(const spion_cross_attention*, int);
+int cross_forward(const spion_cross_attention*, hipStream_t);
+int cross_backward(const spion_cross_attention*, hipStream_t);
+long long layer_norm_workspace(const spion_layer_norm*);
+int layer_norm_forward(const spion_layer_norm*, hipStream_t);
+int layer_norm_backward(const spion_layer_norm*, hipStream_t);
 int key_penalty(const float*, float*, int, int, int, hipStream_t);
 int pattern_generate_maps(const float* const*, int, int, int, int, int, double, float*, int, float*, float*, hipStream_t);
 int score_map_mean(const float*, int, int, int, int, float*, hipStream_t, float post = 1.0f);
@@ -354,6 +360,34 @@ int spion_rms_norm_forward(const spion_rms_norm* call, void* stream) {
 int spion_rms_norm_backward(const spion_rms_norm* call, void* stream) {
     const CallWithoutHandle own;
     return norm_backward(call, static_cast<hipStream_t>(stream));
+}
+
+// ---- attention of queries to keys of another length -------------------------------------------------
+long long spion_cross_workspace(const spion_cross_attention* call, int backward) {
+    const CallWithoutHandle own;
+    return cross_workspace(call, backward);
+}
+int spion_cross_attention_forward(const spion_cross_attention* call, void* stream) {
+    const CallWithoutHandle own;
+    return cross_forward(call, static_cast<hipStream_t>(stream));
+}
+int spion_cross_attention_backward(const spion_cross_attention* call, void* stream) {
+    const CallWithoutHandle own;
+    return cross_backward(call, static_cast<hipStream_t>(stream));
+}
+
+// ---- layer norm --------------------------------------------------------------------------------------
+long long spion_layer_norm_workspace(const spion_layer_norm* call) {
+    const CallWithoutHandle own;
+    return layer_norm_workspace(call);
+}
+int spion_layer_norm_forward(const spion_layer_norm* call, void* stream) {
+    const CallWithoutHandle own;
+    return layer_norm_forward(call, static_cast<hipStream_t>(stream));
+}
+int spion_layer_norm_backward(const spion_layer_norm* call, void* stream) {
+    const CallWithoutHandle own;
+    return layer_norm_backward(call, static_cast<hipStream_t>(stream));
 }
 
 // ---- pattern discovery ---------------------------------------------------------------------------

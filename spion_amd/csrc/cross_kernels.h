@@ -1,0 +1,798 @@
+// Attention of queries to keys of another length (no counterpart in the reference, whose attention is an encoder's own,
+// models/attention.py:79-103): cross attention, with heads of keys that several heads of queries share.
+// With t_ij = (q_i . k_j) log2(e) / sqrt(d) over the keys that take part
+//   forward   P_ij = exp2(t_ij - lse_i),  O = P V
+//   backward  dP = dO V^T,  D_i = dO_i . O_i,  dS = P (dP - D),  dQ = dS K / sqrt(d),  dK = dS^T Q / sqrt(d),  dV = P^T dO
+// No position enters, so the queries of the heads that share a head of keys are rows of one problem: row r of such a group is query
+// r % Lq of its head r / Lq.  K and V of a group are then read once for all of them, a single token of four heads is four rows of
+// one strip, and dK and dV are summed over the group by the products themselves.
+// P is never written: the forward leaves lse, and the backward, in a pass over rows (dQ) and one over keys (dK, dV), forms P again.
+#pragma once
+#include "bias_tile.h"
+
+namespace spion {
+
+struct CrossCall {
+    HeadsAt q, k, v, o, dout, dq, dk, dv;
+    const void* mask;  // [B][Lk]: null, float (0 = left out) or bytes
+    float* lse;        // [B * G][rows]: log2 of the softmax denominator, +inf for rows that nothing enters (NaN stays NaN)
+    float* delta;      // [B * G][rows]: dO . O
+    float* part;       // workspace: the pieces' slots
+    int B, G, each, Lq, Lk, rows;  // G heads of keys, each for `each` heads of queries; rows = each * Lq
+    unsigned magic;                // r / Lq = r * magic >> shift, for r < 2^31
+    int shift;
+    int mask_bytes;                  // 4 or 1
+    int strips, splits, per_split;   // strips of a head's rows or keys, pieces of the other side, tiles of 32 to a piece
+    float scale;
+    __device__ __forceinline__ int head_of(int r) const { return each == 1 ? 0 : (int)((unsigned long long)(unsigned)r * magic >> shift); }
+    // row r of group g of sample b
+    __device__ __forceinline__ const char* row(const HeadsAt& t, int b, int g, int r) const {
+        const int n = head_of(r);
+        return t.p + b * t.b + (g * (long long)each + n) * t.h + (r - n * Lq) * t.row;
+    }
+};
+
+// The running maximum is raised only when a tile exceeds it by 2^8: sums stay below 2^8 times the keys, and most tiles have nothing
+// to rescale.
+constexpr float CROSS_LAZY = 8.f;
+
+// Rows that are staged: a head of keys, or a group of queries.  A head, or a group, lies within 2^31 bytes and its rows 2^24 apart at
+// most; rows up to 64 behind the last are asked for (and left out when they are stored to LDS): they read as the last row or as zeros.
+template <class T, int D, bool KEYS>
+struct CrossSource {
+    rsrc_t r;
+    int ld, head;
+    const CrossCall& a;
+    __device__ __forceinline__ CrossSource(const CrossCall& a, const HeadsAt& t, int b, int g) : ld((int)t.row), head((int)t.h), a(a) {
+        const unsigned long long p = reinterpret_cast<unsigned long long>(t.p + b * t.b + (KEYS ? g : g * (long long)a.each) * t.h);
+        // (the same in every lane, which the compiler does not see through the divisions that b and g come from)
+        const unsigned long long u = (unsigned)uniform((int)(unsigned)p) | (unsigned long long)(unsigned)uniform((int)(p >> 32)) << 32;
+        const long long bytes = KEYS ? (a.Lk - 1) * t.row : (a.each - 1) * t.h + (a.Lq - 1) * t.row;
+        r = make_rsrc(reinterpret_cast<const void*>(u), (unsigned)(bytes + D * (int)sizeof(T)));
+    }
+    __device__ __forceinline__ int at(int first, int row, int byte) const {
+        if (KEYS || a.each == 1) return (int)((unsigned)first * (unsigned)ld + ((unsigned)row * (unsigned)ld + (unsigned)byte));
+        const int x = min(first + row, a.rows - 1), n = a.head_of(x);
+        return (int)((unsigned)n * (unsigned)head + (unsigned)(x - n * a.Lq) * (unsigned)ld + (unsigned)byte);
+    }
+};
+
+// Work-group -> (group, strip, piece): the strips of a group follow each other on one XCD, whose L2 then holds what they share, and
+// the groups go round-robin, so that every XCD has groups of every sample (padded ones differ in length).
+struct CrossItem {
+    int b, g, bg, strip, split;
+    __device__ __forceinline__ CrossItem(const CrossCall& a, int total) {
+        const int each = a.strips * a.splits, whole = a.B * a.G / 8 * 8 * each;  // work-groups of a group, of the whole rounds
+        int i = blockIdx.x;
+        if (i < whole) {
+            const int n = i / 8;
+            i = (n / each * 8 + i % 8) * each + n % each;
+        } else {
+            i = whole + xcd_remap(i - whole, total - whole);
+        }
+        split = i % a.splits;
+        i /= a.splits;
+        strip = i % a.strips;
+        bg = i / a.strips;
+        b = bg / a.G;
+        g = bg - b * a.G;
+    }
+    // the piece's slot for 32 rows (or keys), of which the head has `all`
+    __device__ __forceinline__ size_t slot(const CrossCall& a, int all, int first) const {
+        return ((size_t)bg * ((all + 31) / 32) + first / 32) * a.splits + split;
+    }
+};
+
+// floats a piece leaves: of the forward the unscaled sums, maxima and denominators, of the row pass dQ, of the column pass dV and dK
+template <int D>
+constexpr int cross_slot() { return 32 * D + 64; }
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Which keys take part
+// ---------------------------------------------------------------------------------------------------------------------
+// Keys are walked in chunks of CHUNK tiles of 32; with a mask the work-group makes, in LDS, the words of a chunk (which keys of each
+// tile take part) and the list of its stages that have any.  The mask is read as it is at the call.
+struct CrossLds {
+    unsigned words[CHUNK];
+    unsigned short list[CHUNK];
+    int seg[8];
+    float ml[4][2][32];
+    float row[32];
+};
+static_assert(sizeof(CrossLds) % 16 == 0, "what follows it is aligned");
+
+__device__ __forceinline__ bool cross_key(const CrossCall& a, int b, int key) {
+    if (key >= a.Lk) return false;
+    if (a.mask == nullptr) return true;
+    const size_t i = (size_t)b * a.Lk + key;
+    return a.mask_bytes == 4 ? reinterpret_cast<const float*>(a.mask)[i] != 0.f : reinterpret_cast<const unsigned char*>(a.mask)[i] != 0;
+}
+
+// The stages of SUBS tiles among tiles first .. first + count - 1 that have a key: how many; which, in s.list.  All 256 threads; LDS that
+// they still read must be done with.
+template <int SUBS>
+__device__ __forceinline__ int cross_scan(const CrossCall& a, CrossLds& s, int b, int first, int count, int tid) {
+    const int w = uniform(tid >> 6), l = tid & 63;
+    __syncthreads();
+    const size_t row = (size_t)b * a.Lk;
+    if (a.mask_bytes == 4) mask_words(reinterpret_cast<const float*>(a.mask) + row, s.words, first, (count + 1) / 2, a.Lk, w, l);
+    else mask_words(reinterpret_cast<const unsigned char*>(a.mask) + row, s.words, first, (count + 1) / 2, a.Lk, w, l);
+    __syncthreads();
+    constexpr int ROUNDS = CHUNK / SUBS / 256;
+    bool act[ROUNDS];
+    unsigned long long votes[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int i = tid + 256 * r;
+        unsigned any = i * SUBS < count ? s.words[i * SUBS] : 0u;
+        if (SUBS == 2 && i * SUBS + 1 < count) any |= s.words[i * SUBS + 1];
+        act[r] = any != 0;
+        votes[r] = __ballot(act[r]);
+        if (l == 0) s.seg[4 * r + w] = __popcll(votes[r]);
+    }
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        int before = 0;
+#pragma unroll
+        for (int k = 0; k < 4 * ROUNDS; ++k) before += k < 4 * r + w ? s.seg[k] : 0;
+        if (act[r]) s.list[before + __popcll(votes[r] & ((1ull << l) - 1))] = (unsigned short)(tid + 256 * r);
+    }
+#pragma unroll
+    for (int k = 0; k < 4 * ROUNDS; ++k) total += s.seg[k];
+    __syncthreads();
+    return total;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Stages: what a work-group's four wavefronts share
+// ---------------------------------------------------------------------------------------------------------------------
+// SUBS tiles of 32 rows of two tensors (K and V; Q and dO).  fp32 heads of 64 features and more have one tile a stage: their images take
+// three times the LDS.
+template <class T, int D>
+struct CrossStage {
+    typedef BiasTile<T, D> TL;
+    static constexpr int SUBS = sizeof(T) == 4 && D >= 64 ? 1 : 2, ROWS = 32 * SUBS;
+    static constexpr int BYTES = 2 * SUBS * TL::BYTES;  // the first tensor's tiles, then the second's
+    static constexpr int N = ROWS * TL::CPR / 256;      // pieces of each tensor a thread moves
+    static_assert(N * 256 == ROWS * TL::CPR, "whole pieces");
+    PieceInFlight<T> x[N], y[N];
+    template <class S>
+    __device__ __forceinline__ void load(const S& xs, const S& ys, int first, int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int n = 256 * i + tid, r = n / TL::CPR, c = n % TL::CPR;
+            x[i].load(xs.r, xs.at(first, r, 8 * c * (int)sizeof(T)));
+            y[i].load(ys.r, ys.at(first, r, 8 * c * (int)sizeof(T)));
+        }
+    }
+    // word[s]: which rows of tile s take part; the others become zeros
+    __device__ __forceinline__ void store(char* buf, const unsigned (&word)[SUBS], int tid) const {
+        if ((word[0] & word[SUBS - 1]) == ~0u) put<true>(buf, word, tid);
+        else put<false>(buf, word, tid);
+    }
+    template <bool ALL>
+    __device__ __forceinline__ void put(char* buf, const unsigned (&word)[SUBS], int tid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int n = 256 * i + tid, r = n / TL::CPR, c = n % TL::CPR, s = r >> 5;
+            const bool there = ((SUBS == 2 && s ? word[SUBS - 1] : word[0]) >> (r & 31)) & 1u;
+            x[i].template store<D, ALL>(buf + s * TL::BYTES, r & 31, c, there);
+            y[i].template store<D, ALL>(buf + (SUBS + s) * TL::BYTES, r & 31, c, there);
+        }
+    }
+};
+
+template <class T, int D>
+constexpr int cross_stages_bytes() {
+    const int stages = 2 * CrossStage<T, D>::BYTES, merge = merge_floats<D>() * 4;
+    return stages > merge ? stages : merge;
+}
+
+struct NothingElseToFetch {
+    __device__ __forceinline__ void load(int) {}
+    __device__ __forceinline__ void store(int) {}
+};
+
+// The stages of a piece of the other side, one after the other, in two buffers taken in turn (one barrier a stage).
+// body(stage's first row, words, buffer, its parity).
+template <class T, int D, bool KEYS, class S, class Fetched, class Body>
+__device__ __forceinline__ void cross_walk(const CrossCall& a, CrossLds& sc, const CrossItem& it, const S& xs, const S& ys, char* lds, int tid,
+                                           Fetched&& fetched, Body&& body) {
+    typedef CrossStage<T, D> ST;
+    const bool listed = KEYS && a.mask;
+    const int rows = KEYS ? a.Lk : a.rows;
+    const int from = it.split * a.per_split, to = min((rows + 31) / 32, from + a.per_split), chunk = listed ? CHUNK : a.per_split;
+    int parity = 0;
+    for (int first = from; first < to; first += chunk) {
+        const int count = min(chunk, to - first);
+        const int n = listed ? cross_scan<ST::SUBS>(a, sc, it.b, first, count, tid) : (count + ST::SUBS - 1) / ST::SUBS;
+        auto unit_of = [&](int i) __attribute__((always_inline)) { return listed ? uniform((int)sc.list[i]) : i; };
+        ST st;
+        int unit = 0;
+        if (n > 0) {
+            unit = unit_of(0);
+            st.load(xs, ys, (first + unit * ST::SUBS) * 32, tid);
+            fetched.load((first + unit * ST::SUBS) * 32);
+        }
+        for (int i = 0; i < n; ++i, parity ^= 1) {
+            const int u = unit * ST::SUBS, row0 = (first + u) * 32;
+            unsigned word[ST::SUBS];
+#pragma unroll
+            for (int s = 0; s < ST::SUBS; ++s)
+                word[s] = listed ? (u + s < count ? (unsigned)uniform((int)sc.words[u + s]) : 0u) : u + s < count ? tail_word(rows - row0 - 32 * s) : 0u;
+            char* buf = lds + parity * ST::BYTES;
+            st.store(buf, word, tid);
+            fetched.store(parity);
+            __syncthreads();
+            if (i + 1 < n) {
+                unit = unit_of(i + 1);
+                st.load(xs, ys, (first + unit * ST::SUBS) * 32, tid);
+                fetched.load((first + unit * ST::SUBS) * 32);
+            }
+            body(row0, word, buf, parity);
+        }
+    }
+}
+
+// A wavefront's 32 x D result acc[c][r] (lane (li, h): row li, feature 32 c + acc_row(r, h)), scaled by the lane's f, through its part of
+// red; out(row, eighth, values).
+template <int D, class Out>
+__device__ __forceinline__ void cross_store(const f32x16 (&acc)[D / 32], float f, float* red, int w, int l, Out&& out) {
+    const int li = l & 31, h = l >> 5;
+    float* mine = red + w * 32 * (D + 4);
+    wave_lds_order();
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(mine + li * (D + 4) + 32 * c + 8 * g + 4 * h) =
+                f32x4{acc[c][4 * g] * f, acc[c][4 * g + 1] * f, acc[c][4 * g + 2] * f, acc[c][4 * g + 3] * f};
+    wave_lds_order();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 8 * i + (l >> 3), j = l & 7;
+        float x[D / 8];
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(mine + row * (D + 4) + j * (D / 8) + 4 * k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * k + e] = v[e];
+        }
+        out(row, j, x);
+    }
+}
+// eighth j of a row of a tensor
+template <class T, int D>
+__device__ __forceinline__ void cross_put(const char* row, int j, const float (&x)[D / 8]) {
+    store_values<T, D / 8>(const_cast<char*>(row) + j * (D / 8) * sizeof(T), x);
+}
+template <int D>
+__device__ __forceinline__ void cross_leave(float* slot, int row, int j, const float (&x)[D / 8]) {
+    store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
+}
+// The same eighth of `pieces` slots, added up in their order.
+template <int D>
+__device__ __forceinline__ void cross_add_pieces(const float* p, int pieces, int stride, float (&x)[D / 8]) {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < pieces; ++k)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p + (size_t)k * stride + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e];
+        }
+}
+
+// -------------------------------------------------------------------------------------------------
+// Forward
+// -------------------------------------------------------------------------------------------------
+// The softmax of one wavefront's rows, a lane each (twice: half-wave h has the keys of its accumulator rows).
+template <class T, int D>
+struct CrossSoftmax {
+    typedef BiasTile<T, D> TL;
+    f32x16 o[D / 32];
+    float m = -__builtin_inff(), z = 0.f;
+    __device__ __forceinline__ CrossSoftmax() {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) o[c] = splat16(0.f);
+    }
+    // the maximum of N tiles' products s, keys that are left out at -infinity
+    template <int N>
+    __device__ __forceinline__ void raise(f32x16 (&s)[N], const unsigned (&word)[N], float c2, int h) {
+        float mt = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            if (word[u] != ~0u) {
+                const unsigned mine = word[u] >> (4 * h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = (mine >> (8 * (r >> 2) + (r & 3))) & 1u ? s[u][r] : -__builtin_inff();
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[u][r]);
+        }
+        mt = half_swap_max(mt) * c2;
+        if (__any(mt > m + CROSS_LAZY)) {
+            const float up = fmaxf(m, mt);
+            const float f = up == m ? 1.f : __builtin_amdgcn_exp2f(m - up);  // equal: also -infinity twice
+            m = up;
+            z *= f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[c][r] *= f;
+        }
+    }
+    __device__ __forceinline__ float base() const { return m == -__builtin_inff() ? 0.f : m; }
+    __device__ __forceinline__ void weights(const f32x16& s, float c2, float minus, float (&p)[16]) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, minus));
+            z += p[r];
+        }
+    }
+};
+
+// Wavefronts a SIMD that the registers are for.
+template <class T, int D>
+constexpr int cross_forward_waves() { return D == 128 ? (sizeof(T) == 2 ? 2 : 1) : sizeof(T) == 2 ? 3 : 2; }
+template <class T, int D>
+constexpr int cross_backward_waves() { return sizeof(T) == 2 ? (D == 128 ? 1 : 2) : D == 32 ? 2 : 1; }
+
+// 128 rows to a work-group, 32 to each of its wavefronts.
+template <class T, int D>
+__global__ __launch_bounds__(256, (cross_forward_waves<T, D>())) void cross_forward_kernel(CrossCall a) {
+    typedef BiasTile<T, D> TL;
+    typedef CrossStage<T, D> ST;
+    constexpr int SUBS = ST::SUBS;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    CrossLds& sc = *reinterpret_cast<CrossLds*>(lds + cross_stages_bytes<T, D>());
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
+    const CrossItem it(a, gridDim.x);
+    const int q0 = it.strip * 128 + 32 * w;
+    const bool some = q0 < a.rows;
+    const typename TL::Row q = TL::load(a.row(a.q, it.b, it.g, min(q0 + li, a.rows - 1)), h, q0 + li < a.rows);
+    const typename TL::At at = TL::at(l);
+    const float c2 = a.scale * LOG2E;
+    q.settled();
+    CrossSoftmax<T, D> x;
+    typedef CrossSource<T, D, true> S;
+    cross_walk<T, D, true>(a, sc, it, S(a, a.k, it.b, it.g), S(a, a.v, it.b, it.g), lds, tid, NothingElseToFetch(),
+        [&](int, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
+            if (!some) return;
+            f32x16 s[SUBS];
+            typename TL::Row kr[SUBS];
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) kr[u] = TL::rows(buf + u * TL::BYTES, at);
+            issue_order();
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) s[u] = TL::feat(kr[u], q);
+            x.raise(s, word, c2, h);
+            const float minus = -x.base();
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) {
+                float p[16];
+                x.weights(s[u], c2, minus, p);
+                TL::add_t(TL::columns(buf + (SUBS + u) * TL::BYTES, at), p, x.o);
+            }
+        });
+    const float z = half_swap_sum(x.z);
+    __syncthreads();  // the stages are done with
+    if (!some) return;
+    if (a.splits > 1) {
+        float* slot = a.part + it.slot(a, a.rows, q0) * cross_slot<D>();
+        if (h == 0) {
+            slot[32 * D + li] = x.m;
+            slot[32 * D + 32 + li] = z;
+        }
+        cross_store<D>(x.o, 1.f, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&v)[D / 8]) {
+            if (q0 + row < a.rows) cross_leave<D>(slot, row, j, v);
+        });
+        return;
+    }
+    if (h == 0 && q0 + li < a.rows)
+        a.lse[(size_t)it.bg * a.rows + q0 + li] = z == 0.f ? __builtin_inff() : x.m + __builtin_amdgcn_logf(z);
+    cross_store<D>(x.o, z == 0.f ? 0.f : 1.f / z, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&v)[D / 8]) {
+        if (q0 + row < a.rows) cross_put<T, D>(a.row(a.o, it.b, it.g, q0 + row), j, v);
+    });
+}
+
+// Few rows: 32 of them to a work-group, and its wavefronts take every fourth tile of the keys, each through its own part of LDS, so that
+// nothing waits for a barrier inside the walk.
+template <class T, int D>
+constexpr int cross_tiles_bytes() {
+    const int tiles = 4 * 2 * BiasTile<T, D>::BYTES, merge = merge_floats<D>() * 4;
+    return tiles > merge ? tiles : merge;
+}
+template <class T, int D, class Body>
+__device__ __forceinline__ void cross_few_walk(const CrossCall& a, CrossLds& sc, const CrossItem& it, char* tk, char* tv, int tid, Body&& body) {
+    const int w = uniform(tid >> 6), l = tid & 63;
+    const HeadBuf kh = HeadBuf::of<T, D>(a.k, it.b, it.g, a.Lk), vh = HeadBuf::of<T, D>(a.v, it.b, it.g, a.Lk);
+    const int t0 = it.split * a.per_split, t1 = min((a.Lk + 31) / 32, t0 + a.per_split);
+    const bool listed = a.mask != nullptr;
+    const int chunk = listed ? CHUNK : a.per_split;
+    for (int first = t0; first < t1; first += chunk) {
+        const int count = min(chunk, t1 - first), n = listed ? cross_scan<1>(a, sc, it.b, first, count, tid) : count;
+        auto tile_of = [&](int i) __attribute__((always_inline)) { return listed ? uniform((int)sc.list[i]) : i; };
+        TileInFlight<T, D> fk, fv;
+        int tile = 0;
+        if (w < n) {
+            tile = tile_of(w);
+            fk.load(kh, (first + tile) * 32, l);
+            fv.load(vh, (first + tile) * 32, l);
+        }
+        for (int i = w; i < n; i += 4) {
+            const unsigned word = listed ? (unsigned)uniform((int)sc.words[tile]) : tail_word(a.Lk - (first + tile) * 32);
+            wave_lds_order();
+            fk.store(tk, word, l);
+            fv.store(tv, word, l);
+            wave_lds_order();
+            if (i + 4 < n) {
+                tile = tile_of(i + 4);
+                fk.load(kh, (first + tile) * 32, l);
+                fv.load(vh, (first + tile) * 32, l);
+            }
+            body(word);
+        }
+    }
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_forward_few_kernel(CrossCall a) {
+    typedef BiasTile<T, D> TL;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    CrossLds& sc = *reinterpret_cast<CrossLds*>(lds + cross_tiles_bytes<T, D>());
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
+    const CrossItem it(a, gridDim.x);
+    const int q0 = it.strip * 32;
+    const typename TL::Row q = TL::load(a.row(a.q, it.b, it.g, min(q0 + li, a.rows - 1)), h, q0 + li < a.rows);
+    const typename TL::At at = TL::at(l);
+    char* tk = lds + w * 2 * TL::BYTES;
+    char* tv = tk + TL::BYTES;
+    const float c2 = a.scale * LOG2E;
+    q.settled();
+    CrossSoftmax<T, D> x;
+    cross_few_walk<T, D>(a, sc, it, tk, tv, tid, [&](unsigned word) __attribute__((always_inline)) {
+        const typename TL::Row kr = TL::rows(tk, at);
+        typename TL::Columns vt;
+        if (TL::EARLY) vt = TL::columns(tv, at);
+        issue_order();
+        f32x16 s[1] = {TL::feat(kr, q)};
+        const unsigned words[1] = {word};
+        x.raise(s, words, c2, h);
+        float p[16];
+        x.weights(s[0], c2, -x.base(), p);
+        if (!TL::EARLY) vt = TL::columns(tv, at);
+        TL::add_t(vt, p, x.o);
+    });
+    // the four wavefronts' parts
+    const float z = half_swap_sum(x.z);
+    if (h == 0) {
+        sc.ml[w][0][li] = x.m;
+        sc.ml[w][1][li] = z;
+    }
+    __syncthreads();
+    float M = sc.ml[0][0][li];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) M = fmaxf(M, sc.ml[k][0][li]);
+    const float base = M == -__builtin_inff() ? 0.f : M;
+    float Z = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) Z += sc.ml[k][1][li] * __builtin_amdgcn_exp2f(sc.ml[k][0][li] - base);
+    const float f = __builtin_amdgcn_exp2f(x.m - base);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x.o[c][r] *= f;
+    float v[D / 8];
+    merge_waves<D>(x.o, reinterpret_cast<float*>(lds), tid, v);
+    const int row = tid >> 3, j = tid & 7;
+    if (a.splits > 1) {
+        float* slot = a.part + it.slot(a, a.rows, q0) * cross_slot<D>();
+        if (q0 + row < a.rows) cross_leave<D>(slot, row, j, v);
+        if (w == 0 && h == 0) {
+            slot[32 * D + li] = M;
+            slot[32 * D + 32 + li] = Z;
+        }
+        return;
+    }
+    if (w == 0 && h == 0) {
+        sc.row[li] = Z == 0.f ? 0.f : 1.f / Z;
+        if (q0 + li < a.rows) a.lse[(size_t)it.bg * a.rows + q0 + li] = Z == 0.f ? __builtin_inff() : M + __builtin_amdgcn_logf(Z);
+    }
+    __syncthreads();
+    if (q0 + row < a.rows) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) v[i] *= sc.row[row];
+        cross_put<T, D>(a.row(a.o, it.b, it.g, q0 + row), j, v);
+    }
+}
+
+// The pieces of 32 rows, in their order; eight pieces' loads are in flight together.
+template <class T, int D>
+__global__ __launch_bounds__(256) void cross_merge_kernel(CrossCall a) {
+    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7, strips = (a.rows + 31) / 32;
+    const int strip = blockIdx.x % strips, bg = blockIdx.x / strips, r = strip * 32 + row;
+    if (r >= a.rows) return;
+    const float* slot = a.part + (size_t)blockIdx.x * a.splits * cross_slot<D>();
+    float M = -__builtin_inff();
+#pragma unroll 8
+    for (int k = 0; k < a.splits; ++k) M = fmaxf(M, slot[(size_t)k * cross_slot<D>() + 32 * D + row]);
+    const float base = M == -__builtin_inff() ? 0.f : M;
+    float Z = 0.f, x[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < a.splits; ++k) {
+        const float* s = slot + (size_t)k * cross_slot<D>();
+        const float f = __builtin_amdgcn_exp2f(s[32 * D + row] - base);
+        Z += s[32 * D + 32 + row] * f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(s + row * D + j * (D / 8) + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e] * f;
+        }
+    }
+    const float inv = Z == 0.f ? 0.f : 1.f / Z;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) x[i] *= inv;
+    cross_put<T, D>(a.row(a.o, bg / a.G, bg % a.G, r), j, x);
+    if (j == 0) a.lse[(size_t)bg * a.rows + r] = Z == 0.f ? __builtin_inff() : M + __builtin_amdgcn_logf(Z);
+}
+
+// -------------------------------------------------------------------------------------------------
+// Backward, rows: dQ and D
+// -------------------------------------------------------------------------------------------------
+// dS of a tile: rows keys, lanes queries.  minus_lse of the lane's row; dp: dP - D.
+__device__ __forceinline__ void cross_ds(const f32x16& s, const f32x16& dp, float c2, float minus_lse, unsigned word, int h, float (&ds)[16]) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, minus_lse)) * dp[r];
+    if (word != ~0u) {
+        const unsigned mine = word >> (4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = (mine >> (8 * (r >> 2) + (r & 3))) & 1u ? ds[r] : 0.f;
+    }
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_row_kernel(CrossCall a) {
+    typedef BiasTile<T, D> TL;
+    typedef CrossStage<T, D> ST;
+    constexpr int SUBS = ST::SUBS;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    CrossLds& sc = *reinterpret_cast<CrossLds*>(lds + cross_stages_bytes<T, D>());
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
+    const CrossItem it(a, gridDim.x);
+    const int q0 = it.strip * 128 + 32 * w, qi = min(q0 + li, a.rows - 1);
+    const bool some = q0 < a.rows, there = q0 + li < a.rows;
+    const typename TL::Row q = TL::load(a.row(a.q, it.b, it.g, qi), h, there);
+    const typename TL::Row go = TL::load(a.row(a.dout, it.b, it.g, qi), h, there);
+    const size_t stat = (size_t)it.bg * a.rows + qi;
+    const float minus_lse = there ? -a.lse[stat] : -__builtin_inff();
+    const float delta = half_swap_sum(TL::dot(go, TL::load(a.row(a.o, it.b, it.g, qi), h, there)));
+    if (it.split == 0 && h == 0 && there) a.delta[stat] = delta;
+    const typename TL::At at = TL::at(l);
+    const float c2 = a.scale * LOG2E;
+    const f32x16 minus = splat16(-delta);
+    q.settled();
+    go.settled();
+    f32x16 dq[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
+    typedef CrossSource<T, D, true> S;
+    cross_walk<T, D, true>(a, sc, it, S(a, a.k, it.b, it.g), S(a, a.v, it.b, it.g), lds, tid, NothingElseToFetch(),
+        [&](int, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
+            if (!some) return;
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) {
+                if (word[u] == 0) continue;
+                const char *tk = buf + u * TL::BYTES, *tv = buf + (SUBS + u) * TL::BYTES;
+                const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
+                typename TL::Columns kt;
+                issue_order();
+                const f32x16 s = TL::feat(kr, q);
+                const f32x16 dp = TL::feat(vr, go, minus);
+                if (TL::EARLY) {
+                    kt = TL::columns(tk, at);
+                    read_behind_products<D / 8, D / 8>();
+                }
+                float ds[16];
+                cross_ds(s, dp, c2, minus_lse, word[u], h, ds);
+                if (!TL::EARLY) kt = TL::columns(tk, at);
+                TL::add_t(kt, ds, dq);
+            }
+        });
+    __syncthreads();  // the stages are done with
+    if (!some) return;
+    float* slot = a.part + it.slot(a, a.rows, q0) * (32 * D);
+    cross_store<D>(dq, a.scale, reinterpret_cast<float*>(lds), w, l, [&](int row, int j, float (&v)[D / 8]) {
+        if (q0 + row >= a.rows) return;
+        if (a.splits > 1) cross_leave<D>(slot, row, j, v);
+        else cross_put<T, D>(a.row(a.dq, it.b, it.g, q0 + row), j, v);
+    });
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_row_few_kernel(CrossCall a) {
+    typedef BiasTile<T, D> TL;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    CrossLds& sc = *reinterpret_cast<CrossLds*>(lds + cross_tiles_bytes<T, D>());
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
+    const CrossItem it(a, gridDim.x);
+    const int q0 = it.strip * 32, qi = min(q0 + li, a.rows - 1);
+    const bool there = q0 + li < a.rows;
+    const typename TL::Row q = TL::load(a.row(a.q, it.b, it.g, qi), h, there);
+    const typename TL::Row go = TL::load(a.row(a.dout, it.b, it.g, qi), h, there);
+    const size_t stat = (size_t)it.bg * a.rows + qi;
+    const float minus_lse = there ? -a.lse[stat] : -__builtin_inff();
+    const float delta = half_swap_sum(TL::dot(go, TL::load(a.row(a.o, it.b, it.g, qi), h, there)));
+    if (it.split == 0 && w == 0 && h == 0 && there) a.delta[stat] = delta;
+    const typename TL::At at = TL::at(l);
+    char* tk = lds + w * 2 * TL::BYTES;
+    char* tv = tk + TL::BYTES;
+    const float c2 = a.scale * LOG2E;
+    const f32x16 minus = splat16(-delta);
+    q.settled();
+    go.settled();
+    f32x16 dq[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
+    cross_few_walk<T, D>(a, sc, it, tk, tv, tid, [&](unsigned word) __attribute__((always_inline)) {
+        const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
+        typename TL::Columns kt;
+        if (TL::EARLY) kt = TL::columns(tk, at);
+        issue_order();
+        const f32x16 s = TL::feat(kr, q);
+        const f32x16 dp = TL::feat(vr, go, minus);
+        float ds[16];
+        cross_ds(s, dp, c2, minus_lse, word, h, ds);
+        if (!TL::EARLY) kt = TL::columns(tk, at);
+        TL::add_t(kt, ds, dq);
+    });
+    __syncthreads();  // the tiles are done with
+    float v[D / 8];
+    merge_waves<D>(dq, reinterpret_cast<float*>(lds), tid, v);
+    const int row = tid >> 3, j = tid & 7;
+    if (q0 + row >= a.rows) return;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) v[i] *= a.scale;
+    if (a.splits > 1) cross_leave<D>(a.part + it.slot(a, a.rows, q0) * (32 * D), row, j, v);
+    else cross_put<T, D>(a.row(a.dq, it.b, it.g, q0 + row), j, v);
+}
+
+// The pieces of 32 rows of dQ.
+template <class T, int D>
+__global__ __launch_bounds__(256) void cross_merge_row_kernel(CrossCall a) {
+    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7, strips = (a.rows + 31) / 32;
+    const int strip = blockIdx.x % strips, bg = blockIdx.x / strips, r = strip * 32 + row;
+    if (r >= a.rows) return;
+    float x[D / 8];
+    cross_add_pieces<D>(a.part + (size_t)blockIdx.x * a.splits * (32 * D) + row * D + j * (D / 8), a.splits, 32 * D, x);
+    cross_put<T, D>(a.row(a.dq, bg / a.G, bg % a.G, r), j, x);
+}
+
+// -------------------------------------------------------------------------------------------------
+// Backward, keys: dK and dV
+// -------------------------------------------------------------------------------------------------
+// The strip's keys are the lanes: what a key that is left out holds reaches its own lane only, whose results are zeros.
+// The stage's rows' -lse and -D; rows behind the last have P = 0.
+template <int ROWS>
+struct CrossRowStats {
+    const float *lse, *delta;
+    float* lds;  // [2][2][64]
+    int rows, tid;
+    float e = 0.f, d = 0.f;
+    __device__ __forceinline__ void load(int first) {
+        if (tid < ROWS) {
+            const bool there = first + tid < rows;
+            e = there ? -lse[first + tid] : -__builtin_inff();
+            d = there ? -delta[first + tid] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void store(int parity) {
+        if (tid < ROWS) {
+            lds[128 * parity + tid] = e;
+            lds[128 * parity + 64 + tid] = d;
+        }
+    }
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_col_kernel(CrossCall a) {
+    typedef BiasTile<T, D> TL;
+    typedef CrossStage<T, D> ST;
+    constexpr int SUBS = ST::SUBS;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    CrossLds& sc = *reinterpret_cast<CrossLds*>(lds + cross_stages_bytes<T, D>());
+    float* stats = reinterpret_cast<float*>(lds + cross_stages_bytes<T, D>() + sizeof(CrossLds));
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
+    const CrossItem it(a, gridDim.x);
+    const int k0 = it.strip * 128 + 32 * w, ki = min(k0 + li, a.Lk - 1);
+    const bool key = cross_key(a, it.b, k0 + li), some = __any(key);  // false behind the last key
+    const typename TL::Row k = TL::load(a.k.head(it.b, it.g) + ki * a.k.row, h, k0 + li < a.Lk);
+    const typename TL::Row v = TL::load(a.v.head(it.b, it.g) + ki * a.v.row, h, k0 + li < a.Lk);
+    const typename TL::At at = TL::at(l);
+    const float c2 = a.scale * LOG2E;
+    f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = splat16(0.f);
+    CrossRowStats<ST::ROWS> rs{a.lse + (size_t)it.bg * a.rows, a.delta + (size_t)it.bg * a.rows, stats, a.rows, tid};
+    k.settled();
+    v.settled();
+    typedef CrossSource<T, D, false> S;
+    if (__syncthreads_or(some))
+        cross_walk<T, D, false>(a, sc, it, S(a, a.q, it.b, it.g), S(a, a.dout, it.b, it.g), lds, tid, rs,
+            [&](int, const unsigned (&word)[SUBS], const char* buf, int parity) __attribute__((always_inline)) {
+                if (!some) return;
+#pragma unroll
+                for (int u = 0; u < SUBS; ++u) {
+                    if (word[u] == 0) continue;
+                    const char *tq = buf + u * TL::BYTES, *tg = buf + (SUBS + u) * TL::BYTES;
+                    const float* st = stats + 128 * parity + 32 * u + 4 * h;
+                    f32x16 dp;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 d = *reinterpret_cast<const f32x4*>(st + 64 + 8 * g);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) dp[4 * g + j] = d[j];
+                    }
+                    const typename TL::Row qr = TL::rows(tq, at), gr = TL::rows(tg, at);
+                    typename TL::Columns qt, gt;
+                    issue_order();
+                    const f32x16 s = TL::feat(qr, k);
+                    dp = TL::feat(gr, v, dp);  // dP - D
+                    if (TL::EARLY) {
+                        gt = TL::columns(tg, at), qt = TL::columns(tq, at);
+                        read_behind_products<D / 8, 2 * D / 8>();
+                    }
+                    float p[16], ds[16];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 e = *reinterpret_cast<const f32x4*>(st + 8 * g);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) p[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], c2, e[j]));
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r] = p[r] * dp[r];
+                    if (!TL::EARLY) gt = TL::columns(tg, at);
+                    TL::add_t(gt, p, dv);
+                    if (!TL::EARLY) qt = TL::columns(tq, at);
+                    TL::add_t(qt, ds, dk);
+                }
+            });
+    __syncthreads();  // the stages are done with
+    if (k0 >= a.Lk) return;
+    const unsigned keys = (unsigned)__ballot(key);
+    float* red = reinterpret_cast<float*>(lds);
+    float* slot = a.part + it.slot(a, a.Lk, k0) * (2 * 32 * D);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+        cross_store<D>(t ? dk : dv, t ? a.scale : 1.f, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
+            if (k0 + row >= a.Lk) return;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) x[i] = (keys >> row) & 1u ? x[i] : 0.f;
+            if (a.splits > 1) cross_leave<D>(slot + t * 32 * D, row, j, x);
+            else cross_put<T, D>((t ? a.dk : a.dv).head(it.b, it.g) + (k0 + row) * (t ? a.dk : a.dv).row, j, x);
+        });
+}
+
+// The pieces of 32 keys of dV and dK.
+template <class T, int D>
+__global__ __launch_bounds__(256) void cross_merge_col_kernel(CrossCall a) {
+    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7, strips = (a.Lk + 31) / 32;
+    const int strip = blockIdx.x % strips, bg = blockIdx.x / strips, key = strip * 32 + row;
+    if (key >= a.Lk) return;
+    const float* slot = a.part + (size_t)blockIdx.x * a.splits * (2 * 32 * D) + row * D + j * (D / 8);
+    float x[D / 8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        cross_add_pieces<D>(slot + t * 32 * D, a.splits, 2 * 32 * D, x);
+        cross_put<T, D>((t ? a.dk : a.dv).head(bg / a.G, bg % a.G) + key * (t ? a.dk : a.dv).row, j, x);
+    }
+}
+
+}  // namespace spion

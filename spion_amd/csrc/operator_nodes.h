@@ -1,7 +1,7 @@
 // Autograd nodes of the operators without handles (part of autograd_node.cpp): attention with a relative position bias
-// (relative_bias.py) and the root-mean-square norm (norm.py).  They do what the Python functions there do, checks of arguments
-// included, with the node, the saved tensors and the allocations on the C++ side: a training step of 16 heads of 1024 and one of
-// a few rows are bound by the host.
+// (relative_bias.py), attention to keys of another length (attention_cross.py), the root-mean-square norm and the layer norm (norm.py).
+// They do what the Python functions there do, checks of arguments included, with the node, the saved tensors and the allocations on
+// the C++ side: a training step of 16 heads of 1024 and one of a few rows are bound by the host.
 #pragma once
 
 // A tensor as it was saved, which hooks may have brought back as something else: the kernels take types and sizes as they
@@ -378,4 +378,232 @@ std::vector<Tensor> rms_norm_fp8(const Tensor& x, const Tensor& weight, const c1
     variable_list r = norm_forward(x, weight, res.value_or(Tensor()), eps, true);
     if (!r[1].defined()) return {r[0], r[2]};
     return {r[0], r[2], r[1]};
+}
+
+// ---- the layer norm ---------------------------------------------------------------------------------------------------
+spion_layer_norm layer_norm_call(const Tensor& rows, const Tensor& w, double eps) {
+    spion_layer_norm c{};
+    c.x = rows.data_ptr();
+    c.weight = w.data_ptr();
+    c.rows = rows.size(0);
+    c.width = (int)rows.size(1);
+    c.bf16 = rows.scalar_type() == torch::kBFloat16;
+    c.x_stride = rows.stride(0);
+    c.eps = (float)eps;
+    return c;
+}
+// {y, h or nothing}
+variable_list layer_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& res, double eps) {
+    variable_list r{torch::empty(x.sizes(), x.options())};
+    if (res.defined()) r.push_back(torch::empty(x.sizes(), x.options()));
+    if (x.numel() == 0) return r;
+    const Tensor xr = rows_of(x), w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : Tensor(), rr = res.defined() ? rows_of(res) : Tensor();
+    spion_layer_norm c = layer_norm_call(xr, w, eps);
+    if (b.defined()) c.bias = b.data_ptr();
+    if (res.defined()) {
+        c.residual = rr.data_ptr();
+        c.residual_stride = rr.stride(0);
+        c.h = r[1].data_ptr();
+    }
+    c.y = r[0].data_ptr();
+    void* const stream = reinterpret_cast<void*>(current_stream(x.device().index()));
+    check_call(spion_layer_norm_forward(&c, stream) == 0, "spion_layer_norm_forward");
+    return r;
+}
+
+struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
+    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor weight, c10::optional<Tensor> bias, c10::optional<Tensor> res, double eps) {
+        variable_list r = layer_norm_forward(x, weight, bias.value_or(Tensor()), res.value_or(Tensor()), eps);
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["bias"] = bias.has_value();
+        ctx->set_materialize_grads(false);
+        save_as_is(ctx, {r.size() > 1 ? r[1] : x, weight});
+        return r;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list s = saved_as_is(ctx);
+        const Tensor &h = s[0], &dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
+        variable_list g(5);
+        if (!dy.defined() && !dh.defined()) return g;
+        const bool residual = grads.size() > 1, bias = ctx->saved_data["bias"].toBool();
+        const c10::DeviceGuard on(h.device());
+        if (!dy.defined() || h.numel() == 0) {  // only the stream was used
+            g[0] = dh.defined() ? dh : torch::zeros_like(h);
+            g[1] = torch::zeros_like(s[1]);
+            if (bias) g[2] = torch::zeros_like(s[1]);
+            if (residual) g[3] = g[0];
+            return g;
+        }
+        const Tensor hr = rows_of(h), w = s[1].contiguous(), dyr = rows_of(dy.to(h.scalar_type()));
+        const Tensor dhr = dh.defined() ? rows_of(dh.to(h.scalar_type())) : Tensor();
+        g[0] = torch::empty(h.sizes(), h.options());
+        g[1] = torch::empty(w.sizes(), w.options());
+        if (bias) g[2] = torch::empty(w.sizes(), w.options());
+        spion_layer_norm c = layer_norm_call(hr, w, ctx->saved_data["eps"].toDouble());
+        c.dy = dyr.data_ptr();
+        c.dy_stride = dyr.stride(0);
+        if (dhr.defined()) {
+            c.dh = dhr.data_ptr();
+            c.dh_stride = dhr.stride(0);
+        }
+        c.dx = g[0].data_ptr();
+        c.dweight = g[1].data_ptr();
+        if (bias) c.dbias = g[2].data_ptr();
+        c.workspace_floats = spion_layer_norm_workspace(&c);
+        check_call(c.workspace_floats >= 0, "spion_layer_norm_workspace");
+        Tensor ws = torch::empty({(int64_t)c.workspace_floats}, h.options().dtype(torch::kFloat32));
+        c.workspace = fpm(ws);
+        void* const stream = reinterpret_cast<void*>(current_stream(h.device().index()));
+        check_call(spion_layer_norm_backward(&c, stream) == 0, "spion_layer_norm_backward");
+        once_differentiable(g, 3);
+        if (residual) g[3] = g[0];
+        return g;
+    }
+};
+
+std::vector<Tensor> layer_norm(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias, const c10::optional<Tensor>& res, double eps) {
+    TORCH_CHECK_VALUE(!bias.has_value() || bias->sizes() == weight.sizes(), "bias shape ", bias.has_value() ? bias->sizes() : weight.sizes(),
+                      " does not match the weight's ", weight.sizes());
+    check_norm(x, weight, res, eps);
+    if (bias.has_value()) {
+        on_one_gpu(*bias, x);
+        TORCH_CHECK_TYPE(bias->scalar_type() == x.scalar_type(), "rows, weight and bias of one type expected");
+    }
+    const c10::DeviceGuard on(x.device());
+    const Tensor b = bias.value_or(Tensor()), r = res.value_or(Tensor());
+    if (without_node({&x, &weight, &b, &r})) return layer_norm_forward(x, weight, b, r, eps);
+    return LayerNormNode::apply(x, weight, bias, res, eps);
+}
+
+// ---- attention to keys of another length ------------------------------------------------------------------------------
+// Heads as the kernels read them: themselves, or a copy where their strides or address are not theirs.  `together` heads are reached
+// from one address.
+Tensor readable_group(const Tensor& t, int64_t together) {
+    spion_head_layout lay{};
+    const auto fits = [&](const Tensor& x) {
+        return head_layout(x, lay) && x.stride(2) * x.element_size() <= 1 << 24 &&
+               ((together - 1) * x.stride(1) + (x.size(2) - 1) * x.stride(2) + x.size(3)) * (int64_t)x.element_size() < int64_t(1) << 31;
+    };
+    if (fits(t)) return t;
+    const Tensor c = t.contiguous();
+    return fits(c) ? c : t.clone(at::MemoryFormat::Contiguous);
+}
+// k, v are the two slices of one [B, L, 2, G, d] buffer, in this order
+bool paired_views(const Tensor& k, const Tensor& v) {
+    const int64_t G = k.size(1), L = k.size(2), d = k.size(3);
+    const int64_t want[4] = {L * 2 * G * d, d, 2 * G * d, 1};
+    for (int i = 0; i < 4; ++i)
+        if (k.stride(i) != want[i] || v.stride(i) != want[i]) return false;
+    return (const char*)v.data_ptr() - (const char*)k.data_ptr() == G * d * (int64_t)k.element_size();
+}
+spion_cross_attention cross_call(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse, const Tensor& mask) {
+    spion_cross_attention c{};
+    c.Q = heads_of(q);
+    c.K = heads_of(k);
+    c.V = heads_of(v);
+    c.Out = heads_of(out);
+    if (mask.defined()) {
+        c.key_mask = mask.data_ptr();
+        c.mask_bytes = (int)mask.element_size();
+    }
+    c.Lse = static_cast<float*>(lse.data_ptr());
+    c.batch = (int)q.size(0);
+    c.heads = (int)q.size(1);
+    c.key_heads = (int)k.size(1);
+    c.q_len = (int)q.size(2);
+    c.k_len = (int)k.size(2);
+    c.head_dim = (int)q.size(3);
+    c.bf16 = q.scalar_type() == torch::kBFloat16;
+    return c;
+}
+Tensor cross_workspace(spion_cross_attention& c, bool backward, const Tensor& q) {
+    const int64_t n = spion_cross_workspace(&c, backward);
+    check_call(n >= 0, "spion_cross_workspace");
+    if (n == 0) return Tensor();
+    Tensor ws = torch::empty({n}, q.options().dtype(torch::kFloat32));
+    c.workspace = fpm(ws);
+    c.workspace_floats = n;
+    return ws;
+}
+struct CrossForward {
+    Tensor q, k, v, out, lse;
+};
+CrossForward cross_forward(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& mask) {
+    CrossForward r;
+    r.q = readable_group(query, query.size(1) / key.size(1));
+    r.k = readable_group(key, 1);
+    r.v = readable_group(value, 1);
+    r.out = empty_like_heads(query);
+    r.lse = torch::empty({query.size(0) * query.size(1), query.size(2)}, query.options().dtype(torch::kFloat32));
+    spion_cross_attention c = cross_call(r.q, r.k, r.v, r.out, r.lse, mask);
+    const Tensor ws = cross_workspace(c, false, query);
+    void* const stream = reinterpret_cast<void*>(current_stream(query.device().index()));
+    check_call(spion_cross_attention_forward(&c, stream) == 0, "spion_cross_attention_forward");
+    return r;
+}
+
+struct CrossNode : public torch::autograd::Function<CrossNode> {
+    static Tensor forward(AutogradContext* ctx, Tensor query, Tensor key, Tensor value, c10::optional<Tensor> mask) {
+        const Tensor m = mask.value_or(Tensor());
+        const CrossForward r = cross_forward(query, key, value, m);
+        save_as_is(ctx, {r.q, r.k, r.v, r.out, r.lse, m});
+        return r.out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list s = saved_as_is(ctx);
+        const c10::DeviceGuard on(s[0].device());
+        const int64_t each = s[0].size(1) / s[1].size(1);
+        const Tensor q = readable_group(s[0], each), k = readable_group(s[1], 1), v = readable_group(s[2], 1), out = readable_group(s[3], each);
+        const Tensor lse = s[4].contiguous(), mask = s[5].defined() ? s[5].contiguous() : Tensor();
+        const Tensor go = readable_group(grads[0].to(q.scalar_type()), each);
+        variable_list g(4);
+        g[0] = empty_like_heads(q);
+        if (paired_views(k, v)) {  // slices of one projection: the gradients likewise
+            const Tensor both = torch::empty({k.size(0), k.size(2), 2, k.size(1), k.size(3)}, k.options());
+            for (int i = 0; i < 2; ++i) g[1 + i] = both.select(2, i).transpose(1, 2);
+        } else {
+            g[1] = empty_like_heads(k);
+            g[2] = empty_like_heads(v);
+        }
+        spion_cross_attention c = cross_call(q, k, v, out, lse, mask);
+        c.dO = heads_of(go);
+        c.dQ = heads_of(g[0]);
+        c.dK = heads_of(g[1]);
+        c.dV = heads_of(g[2]);
+        const Tensor ws = cross_workspace(c, true, q);
+        void* const stream = reinterpret_cast<void*>(current_stream(q.device().index()));
+        check_call(spion_cross_attention_backward(&c, stream) == 0, "spion_cross_attention_backward");
+        once_differentiable(g, 3);
+        return g;
+    }
+};
+
+Tensor cross_attention(const Tensor& query, const Tensor& key, const Tensor& value, const c10::optional<Tensor>& key_mask) {
+    constexpr int64_t far = int64_t(1) << 29;
+    TORCH_CHECK_VALUE(query.dim() == 4 && key.dim() == 4, "heads [B, H, L, d] expected");
+    const int64_t B = query.size(0), H = query.size(1), Lq = query.size(2), d = query.size(3), G = key.size(1), Lk = key.size(2);
+    TORCH_CHECK_VALUE(key.size(0) == B && key.size(3) == d, "key shape ", key.sizes(), " does not match the query's ", query.sizes());
+    TORCH_CHECK_VALUE(value.sizes() == key.sizes(), "value shape ", value.sizes(), " does not match the key's ", key.sizes());
+    TORCH_CHECK_VALUE((G == 0) == (H == 0) && (G == 0 || H % G == 0), H, " heads over ", G, " heads of keys: a multiple expected");
+    fp32_or_bf16(query, "heads");
+    TORCH_CHECK_VALUE(d == 32 || d == 64 || d == 128, "head dimension ", d, ": 32, 64 or 128 expected");
+    Tensor mask = key_mask.value_or(Tensor());
+    TORCH_CHECK_VALUE(!mask.defined() || (mask.dim() == 2 && mask.size(0) == B && mask.size(1) == Lk), "key mask shape ",
+                      mask.defined() ? mask.sizes() : c10::IntArrayRef(), ": [", B, ", ", Lk, "] expected");
+    TORCH_CHECK_VALUE(B <= INT_MAX && H <= INT_MAX && Lk <= far && Lq <= far && (G == 0 || H / G * Lq <= far), "sizes out of range");
+    for (const Tensor* t : {&query, &key, &value, static_cast<const Tensor*>(&mask)}) on_one_gpu(*t, query);
+    TORCH_CHECK_TYPE(key.scalar_type() == query.scalar_type() && value.scalar_type() == query.scalar_type(), "heads of one type expected");
+    const c10::DeviceGuard on(query.device());
+    if (mask.defined()) {
+        const auto type = mask.scalar_type();
+        if (type != torch::kFloat32 && type != torch::kBool && type != torch::kUInt8) mask = mask.ne(0);
+        mask = mask.detach().contiguous();
+    }
+    if (query.numel() == 0 || key.numel() == 0) {  // nothing to attend to, or nobody to
+        const Tensor every = torch::ones({}, query.options().dtype(torch::kBool));
+        const auto nothing = [&](const Tensor& t) { return t.masked_fill(every, 0.0); };
+        return nothing(query) + nothing(key).sum() + nothing(value).sum();
+    }
+    if (without_node({&query, &key, &value})) return cross_forward(query, key, value, mask).out;
+    return CrossNode::apply(query, key, value, mask.defined() ? c10::optional<Tensor>(mask) : c10::nullopt);
 }
