@@ -11,7 +11,7 @@ namespace spion {
 
 typedef spion_cross_attention Cross;
 
-static long long tiles_of(long long rows, int tile = 32) { return (rows + tile - 1) / tile; }
+static long long tiles_of(long long rows, long long tile = 32) { return (rows + tile - 1) / tile; }
 static int each_of(const Cross& c) { return c.heads / c.key_heads; }
 static long long rows_of(const Cross& c) { return (long long)each_of(c) * c.q_len; }
 
@@ -22,24 +22,46 @@ struct CrossWalk {
     int rows;
     int strips, splits, per_split;  // tiles of 32 to a piece
 };
+// All rows of a group in one strip of 32: the backward is one pass over the keys.
+static bool cross_one_strip(const Cross& c) { return rows_of(c) <= 32 && (c.bf16 || c.head_dim < 128); }
+
+// Which, by an estimate of the launch's time, us.  A CU's work-groups share it: it takes as long for them as for one after the other, within a
+// fifth (bf16, d = 64: 0.49 us a tile of 32 keys and 128 rows alone, 0.41 with four of them).  So a launch takes the most work-groups that a CU
+// has, times a piece's tiles, times what a tile (strips of 32: four tiles, one to a wavefront) takes, measured with one work-group to
+// a CU in the forward; the row pass takes 1.3 times, the column pass 1.75 times that.  All rows in one strip: K and V come from memory
+// once, at 20 bytes a ns to a CU.  Pieces cost a second launch, and their sums are written and read at some 4 TB/s.
+//   us, forward, one launch / its best cut in strips of 128, strips of 32:  64 heads of 512 x 512, bf16, d = 64: 14 / 22, 17;  32 of 256 x 256: 9 / 14, 7
+//   16 of 1024 x 4096: 63 / 37, 41;  d = 128 97 / 60, 93;  fp32 199 / 96, 159;  64 of 256 x 1024, fp32, d = 32: 35 / 25, 23
+// At most eight work-groups to a CU where there are pieces, so the workspace is bounded.
+static double cross_tile_us(const Cross& c, CrossPass pass, bool few) {
+    static const double wide_us[2][3] = {{0.85, 1.5, 3.2}, {0.25, 0.45, 0.75}}, few_us[2][3] = {{1.05, 2.4, 0.}, {0.4, 0.6, 1.35}};
+    const int d = c.head_dim == 32 ? 0 : c.head_dim == 64 ? 1 : 2, bf16 = c.bf16 ? 1 : 0;
+    const double us = (few ? few_us : wide_us)[bf16][d] * (pass == CrossPass::FORWARD ? 1. : pass == CrossPass::ROW ? 1.3 : 1.75);
+    return few && pass != CrossPass::COL && cross_one_strip(c) ? std::max(us, 4 * 64 * c.head_dim * (c.bf16 ? 2 : 4) / 20e3) : us;
+}
 static CrossWalk cross_walk_of(const Cross& c, CrossPass pass, bool can_split) {
     const long long own = pass == CrossPass::COL ? c.k_len : rows_of(c), other = pass == CrossPass::COL ? rows_of(c) : c.k_len;
-    const bool few = pass != CrossPass::COL && own <= 32 && (c.bf16 || c.head_dim < 128);
+    const long long groups = (long long)c.batch * c.key_heads, tiles = tiles_of(other), cus = device_cus();
+    const bool fits = c.bf16 || c.head_dim < 128;  // (tiles of 128 fp32 features for four wavefronts do not fit a CU)
+    const bool must = pass == CrossPass::ROW && cross_one_strip(c);
     CrossWalk w{};
-    w.rows = few ? 32 : 128;
-    w.strips = (int)tiles_of(own, w.rows);
-    const long long groups = (long long)c.batch * c.key_heads * w.strips, tiles = tiles_of(other), unit = few ? 1 : 2;
-    const long long at_once = 2LL * device_cus();
-    long long pieces = 1;
     double least = 0;
-    for (long long n = 1; n == 1 || (can_split && n <= std::min(tiles / (few ? 8 : 4), 64LL) && groups * n <= 8LL * device_cus()); ++n) {
-        const long long rounds = (groups * n + at_once - 1) / at_once, each = (tiles + n - 1) / n;
-        const double cost = rounds * ((few ? each / 4. : each) + 4.) + (n > 1 ? 6 : 0);
-        if (n == 1 || cost < least) least = cost, pieces = n;
+    for (int few = must; few <= (int)fits; ++few) {
+        const int rows = few ? 32 : 128, unit = few ? 1 : 2;
+        const long long strips = tiles_of(own, rows), steps = tiles_of(tiles, few ? 4 : unit);
+        const double us = cross_tile_us(c, pass, few) * (few ? 1 : unit);
+        for (long long n = 1; n == 1 || (can_split && n <= std::min(steps / 2, 64LL) && groups * strips * n <= 8 * cus); ++n) {
+            const long long rounds = tiles_of(groups * strips * n, cus), each = tiles_of(steps, n);
+            double cost = 3 + rounds * each * us;
+            if (n > 1) cost += 3 + (pass == CrossPass::COL ? 2 : 1) * groups * own * n * c.head_dim * 8 / 4e6;
+            if (w.rows && cost >= least) continue;
+            least = cost;
+            w.rows = rows;
+            w.strips = (int)strips;
+            w.per_split = (int)(each * (few ? 4 : unit));
+            w.splits = few ? (int)n : (int)tiles_of(steps, each);  // none of them empty
+        }
     }
-    const long long units = (tiles + unit - 1) / unit, each = (units + pieces - 1) / pieces;
-    w.per_split = (int)(each * unit);
-    w.splits = (int)((units + each - 1) / each);  // none of them empty
     return w;
 }
 
@@ -51,7 +73,7 @@ static long long cross_floats(const Cross& c, bool backward) {
     }
     const CrossWalk row = cross_walk_of(c, CrossPass::ROW, true), col = cross_walk_of(c, CrossPass::COL, true);
     const long long a = row.splits > 1 ? groups * tiles_of(rows) * row.splits * 32 * c.head_dim : 0;
-    const long long b = col.splits > 1 ? groups * tiles_of(c.k_len) * col.splits * 64 * c.head_dim : 0;
+    const long long b = !cross_one_strip(c) && col.splits > 1 ? groups * tiles_of(c.k_len) * col.splits * 64 * c.head_dim : 0;
     return ((groups * rows + 3) & ~3LL) + std::max(a, b);  // D, rounded up to whole pieces of 16 bytes, and the pieces
 }
 
@@ -152,10 +174,16 @@ static bool cross_launch(const char* name, K kernel, long long groups, size_t ld
     return check_launch(name);
 }
 
+template <int D, class K>
+static bool cross_join(const char* name, K few, K many, long long groups, long long rows, hipStream_t stream, const CrossCall& a) {
+    if (a.splits > 8) return cross_launch(name, many, groups * rows, 0, stream, a);
+    return cross_launch(name, few, groups * tiles_of(rows, CrossJoin<D, false>::ROWS), 0, stream, a);
+}
+
 template <class T, int D>
 struct CrossRun {
     static constexpr size_t STAGES = cross_stages_bytes<T, D>() + sizeof(CrossLds);
-    static constexpr bool FEW = sizeof(T) == 2 || D < 128;  // (tiles of 128 fp32 features for four wavefronts do not fit a CU)
+    static constexpr bool FEW = sizeof(T) == 2 || D < 128;
     static bool forward(const Cross& c, hipStream_t stream) {
         CrossCall a = cross_device_call(c);
         const long long groups = (long long)a.B * a.G;
@@ -167,8 +195,8 @@ struct CrossRun {
         if (w.rows == 128) ok = cross_launch("cross_forward_kernel", cross_forward_kernel<T, D>, n, STAGES, stream, a);
         if constexpr (FEW)
             if (w.rows == 32)
-                ok = cross_launch("cross_forward_few_kernel", cross_forward_few_kernel<T, D>, n, cross_tiles_bytes<T, D>() + sizeof(CrossLds), stream, a);
-        return ok && (w.splits == 1 || cross_launch("cross_merge_kernel", cross_merge_kernel<T, D>, groups * tiles_of(a.rows), 0, stream, a));
+                ok = cross_launch("cross_forward_few_kernel", cross_forward_few_kernel<T, D>, n, cross_tiles_bytes<T, D>(), stream, a);
+        return ok && (w.splits == 1 || cross_join<D>("cross_merge_kernel", cross_merge_kernel<T, D, false>, cross_merge_kernel<T, D, true>, groups, a.rows, stream, a));
     }
     static bool backward(const Cross& c, hipStream_t stream) {
         CrossCall a = cross_device_call(c);
@@ -180,16 +208,25 @@ struct CrossRun {
         long long n = groups * row.strips * row.splits;
         bool ok = false;
         if (row.rows == 128) ok = cross_launch("cross_backward_row_kernel", cross_backward_row_kernel<T, D>, n, STAGES, stream, a);
-        if constexpr (FEW)
-            if (row.rows == 32)
-                ok = cross_launch("cross_backward_row_few_kernel", cross_backward_row_few_kernel<T, D>, n,
-                                  cross_tiles_bytes<T, D>() + sizeof(CrossLds), stream, a);
+        if constexpr (FEW) {
+            if (cross_one_strip(c)) ok = cross_launch("cross_backward_few_kernel", cross_backward_few_kernel<T, D>, n, cross_few_bytes<T, D>(), stream, a);
+            else if (row.rows == 32)
+                ok = cross_launch("cross_backward_row_few_kernel", cross_backward_row_few_kernel<T, D>, n, cross_tiles_bytes<T, D>(), stream, a);
+        }
         if (!ok) return false;
-        if (row.splits > 1 && !cross_launch("cross_merge_row_kernel", cross_merge_row_kernel<T, D>, groups * tiles_of(a.rows), 0, stream, a)) return false;
+        if (row.splits > 1 &&
+            !cross_join<D>("cross_merge_row_kernel", cross_merge_row_kernel<T, D, false>, cross_merge_row_kernel<T, D, true>, groups, a.rows, stream, a))
+            return false;
+        if (cross_one_strip(c)) return true;  // (with all three gradients)
         cross_take(a, col);
         n = groups * col.strips * col.splits;
-        if (!cross_launch("cross_backward_col_kernel", cross_backward_col_kernel<T, D>, n, STAGES + 1024, stream, a)) return false;
-        return col.splits == 1 || cross_launch("cross_merge_col_kernel", cross_merge_col_kernel<T, D>, groups * tiles_of(a.Lk), 0, stream, a);
+        if (col.rows == 128) ok = cross_launch("cross_backward_col_kernel", cross_backward_col_kernel<T, D>, n, STAGES + 1024, stream, a);
+        if constexpr (FEW)
+            if (col.rows == 32)
+                ok = cross_launch("cross_backward_col_few_kernel", cross_backward_col_few_kernel<T, D>, n, cross_col_few_bytes<T, D>(), stream, a);
+        if (!ok) return false;
+        return col.splits == 1 ||
+               cross_join<D>("cross_merge_col_kernel", cross_merge_col_kernel<T, D, false>, cross_merge_col_kernel<T, D, true>, groups, a.Lk, stream, a);
     }
 };
 

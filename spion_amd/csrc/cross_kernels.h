@@ -96,8 +96,6 @@ struct CrossLds {
     unsigned words[CHUNK];
     unsigned short list[CHUNK];
     int seg[8];
-    float ml[4][2][32];
-    float row[32];
 };
 static_assert(sizeof(CrossLds) % 16 == 0, "what follows it is aligned");
 
@@ -272,20 +270,6 @@ template <int D>
 __device__ __forceinline__ void cross_leave(float* slot, int row, int j, const float (&x)[D / 8]) {
     store_values<float, D / 8>(reinterpret_cast<char*>(slot + row * D + j * (D / 8)), x);
 }
-// The same eighth of `pieces` slots, added up in their order.
-template <int D>
-__device__ __forceinline__ void cross_add_pieces(const float* p, int pieces, int stride, float (&x)[D / 8]) {
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < pieces; ++k)
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(p + (size_t)k * stride + 4 * i);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e];
-        }
-}
 
 // -------------------------------------------------------------------------------------------------
 // Forward
@@ -400,6 +384,24 @@ __global__ __launch_bounds__(256, (cross_forward_waves<T, D>())) void cross_forw
     });
 }
 
+// out += X^T . W of bf16 tiles with W as the sum of two bf16 numbers (fp32: of three, as everywhere).  Calls of few rows wait for memory, so that
+// the second product and its 40 vector instructions cost nothing there (one token over 2048 keys 8.6 us with either), and the
+// rounding of the weights is gone from their results: errors of 0.0017, that of the result's own rounding, against 0.0025.
+template <class TL, class Columns, int N>
+__device__ __forceinline__ void cross_add_fine(const Columns& xt, const float (&p)[16], f32x16 (&out)[N]) {
+    TL::add_t(xt, p, out);
+    if constexpr (TL::IM == 1) {
+        float rest[16];
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const unsigned hi = pack_bf16(p[r], p[r + 1]);
+            rest[r] = p[r] - bf16_lo(hi);
+            rest[r + 1] = p[r + 1] - bf16_hi(hi);
+        }
+        TL::add_t(xt, rest, out);
+    }
+}
+
 // Few rows: 32 of them to a work-group, and its wavefronts take every fourth tile of the keys, each through its own part of LDS, so that
 // nothing waits for a barrier inside the walk.
 template <class T, int D>
@@ -407,36 +409,43 @@ constexpr int cross_tiles_bytes() {
     const int tiles = 4 * 2 * BiasTile<T, D>::BYTES, merge = merge_floats<D>() * 4;
     return tiles > merge ? tiles : merge;
 }
-template <class T, int D, class Body>
-__device__ __forceinline__ void cross_few_walk(const CrossCall& a, CrossLds& sc, const CrossItem& it, char* tk, char* tv, int tid, Body&& body) {
-    const int w = uniform(tid >> 6), l = tid & 63;
+// Wavefront w of piece s has tiles 4 s + w, 4 (s + splits) + w, ...: what padding leaves is dealt evenly (in ranges of tiles, a piece could have
+// none).  It makes the words of its tiles itself, from mask values that were asked for two tiles ahead; K and V are one tile ahead.
+// body(tile's first key, word): for all tiles, those without a key (a word of 0) among them if EVERY.
+template <class T, int D, bool EVERY, class Body>
+__device__ __forceinline__ void cross_few_walk(const CrossCall& a, const CrossItem& it, char* tk, char* tv, int w, int l, Body&& body) {
     const HeadBuf kh = HeadBuf::of<T, D>(a.k, it.b, it.g, a.Lk), vh = HeadBuf::of<T, D>(a.v, it.b, it.g, a.Lk);
-    const int t0 = it.split * a.per_split, t1 = min((a.Lk + 31) / 32, t0 + a.per_split);
-    const bool listed = a.mask != nullptr;
-    const int chunk = listed ? CHUNK : a.per_split;
-    for (int first = t0; first < t1; first += chunk) {
-        const int count = min(chunk, t1 - first), n = listed ? cross_scan<1>(a, sc, it.b, first, count, tid) : count;
-        auto tile_of = [&](int i) __attribute__((always_inline)) { return listed ? uniform((int)sc.list[i]) : i; };
-        TileInFlight<T, D> fk, fv;
-        int tile = 0;
-        if (w < n) {
-            tile = tile_of(w);
-            fk.load(kh, (first + tile) * 32, l);
-            fv.load(vh, (first + tile) * 32, l);
-        }
-        for (int i = w; i < n; i += 4) {
-            const unsigned word = listed ? (unsigned)uniform((int)sc.words[tile]) : tail_word(a.Lk - (first + tile) * 32);
+    const int tiles = (a.Lk + 31) / 32, step = 4 * a.splits;
+    const size_t row = (size_t)it.b * a.Lk;
+    auto ask = [&](int tile) __attribute__((always_inline)) -> unsigned {  // (a float of 0 or -0 and a byte of 0 are left out)
+        const int key = tile * 32 + (l & 31);
+        if (!a.mask || key >= a.Lk) return 0u;
+        return a.mask_bytes == 4 ? reinterpret_cast<const unsigned*>(a.mask)[row + key] << 1 : reinterpret_cast<const unsigned char*>(a.mask)[row + key];
+    };
+    auto word_of = [&](int tile, unsigned asked) __attribute__((always_inline)) -> unsigned {
+        if (tile >= tiles) return 0u;
+        return a.mask ? (unsigned)__ballot(asked != 0) : tail_word(a.Lk - tile * 32);
+    };
+    TileInFlight<T, D> fk, fv;
+    auto fetch = [&](int tile) __attribute__((always_inline)) {
+        fk.load(kh, tile * 32, l);
+        fv.load(vh, tile * 32, l);
+    };
+    int tile = 4 * it.split + w;
+    unsigned asked = ask(tile), next = ask(tile + step), word = word_of(tile, asked);
+    if (word) fetch(tile);
+    for (; tile < tiles; tile += step) {
+        const unsigned now = word;
+        word = word_of(tile + step, next);
+        next = ask(tile + 2 * step);
+        if (now) {
             wave_lds_order();
-            fk.store(tk, word, l);
-            fv.store(tv, word, l);
+            fk.store(tk, now, l);
+            fv.store(tv, now, l);
             wave_lds_order();
-            if (i + 4 < n) {
-                tile = tile_of(i + 4);
-                fk.load(kh, (first + tile) * 32, l);
-                fv.load(vh, (first + tile) * 32, l);
-            }
-            body(word);
         }
+        if (word) fetch(tile + step);
+        if (EVERY || now) body(tile * 32, now);
     }
 }
 
@@ -444,7 +453,7 @@ template <class T, int D>
 __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_forward_few_kernel(CrossCall a) {
     typedef BiasTile<T, D> TL;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    CrossLds& sc = *reinterpret_cast<CrossLds*>(lds + cross_tiles_bytes<T, D>());
+    __shared__ float ml[4][2][32], inv[32];
     const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const CrossItem it(a, gridDim.x);
     const int q0 = it.strip * 32;
@@ -455,7 +464,7 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_for
     const float c2 = a.scale * LOG2E;
     q.settled();
     CrossSoftmax<T, D> x;
-    cross_few_walk<T, D>(a, sc, it, tk, tv, tid, [&](unsigned word) __attribute__((always_inline)) {
+    cross_few_walk<T, D, false>(a, it, tk, tv, w, l, [&](int, unsigned word) __attribute__((always_inline)) {
         const typename TL::Row kr = TL::rows(tk, at);
         typename TL::Columns vt;
         if (TL::EARLY) vt = TL::columns(tv, at);
@@ -466,22 +475,22 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_for
         float p[16];
         x.weights(s[0], c2, -x.base(), p);
         if (!TL::EARLY) vt = TL::columns(tv, at);
-        TL::add_t(vt, p, x.o);
+        cross_add_fine<TL>(vt, p, x.o);
     });
     // the four wavefronts' parts
     const float z = half_swap_sum(x.z);
     if (h == 0) {
-        sc.ml[w][0][li] = x.m;
-        sc.ml[w][1][li] = z;
+        ml[w][0][li] = x.m;
+        ml[w][1][li] = z;
     }
     __syncthreads();
-    float M = sc.ml[0][0][li];
+    float M = ml[0][0][li];
 #pragma unroll
-    for (int k = 1; k < 4; ++k) M = fmaxf(M, sc.ml[k][0][li]);
+    for (int k = 1; k < 4; ++k) M = fmaxf(M, ml[k][0][li]);
     const float base = M == -__builtin_inff() ? 0.f : M;
     float Z = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) Z += sc.ml[k][1][li] * __builtin_amdgcn_exp2f(sc.ml[k][0][li] - base);
+    for (int k = 0; k < 4; ++k) Z += ml[k][1][li] * __builtin_amdgcn_exp2f(ml[k][0][li] - base);
     const float f = __builtin_amdgcn_exp2f(x.m - base);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
@@ -500,48 +509,107 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_for
         return;
     }
     if (w == 0 && h == 0) {
-        sc.row[li] = Z == 0.f ? 0.f : 1.f / Z;
+        inv[li] = Z == 0.f ? 0.f : 1.f / Z;
         if (q0 + li < a.rows) a.lse[(size_t)it.bg * a.rows + q0 + li] = Z == 0.f ? __builtin_inff() : M + __builtin_amdgcn_logf(Z);
     }
     __syncthreads();
     if (q0 + row < a.rows) {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) v[i] *= sc.row[row];
+        for (int i = 0; i < D / 8; ++i) v[i] *= inv[row];
         cross_put<T, D>(a.row(a.o, it.b, it.g, q0 + row), j, v);
     }
 }
 
-// The pieces of 32 rows, in their order; eight pieces' loads are in flight together.
-template <class T, int D>
-__global__ __launch_bounds__(256) void cross_merge_kernel(CrossCall a) {
-    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7, strips = (a.rows + 31) / 32;
-    const int strip = blockIdx.x % strips, bg = blockIdx.x / strips, r = strip * 32 + row;
-    if (r >= a.rows) return;
-    const float* slot = a.part + (size_t)blockIdx.x * a.splits * cross_slot<D>();
-    float M = -__builtin_inff();
+// The pieces of a row, added up in a fixed order; a lane has four features.  MANY (more than eight pieces): a work-group has one row, and its
+// groups of D / 4 lanes every GROUPS-th piece.  Else a group has a row of its own and all of its pieces.  (16 rows in 64 pieces, d = 128: 4.5 us,
+// and 18 with all pieces to a lane; 32768 rows in two pieces, d = 64: a wavefront a row 17.)
+template <int D, bool MANY>
+struct CrossJoin {
+    static constexpr int COLS = D / 4, SETS = 256 / COLS, GROUPS = MANY ? SETS : 1, ROWS = MANY ? 1 : SETS;
+    int row, col, group;  // of the work-group's ROWS, four features, which of the GROUPS
+    __device__ __forceinline__ CrossJoin(int tid) : row(MANY ? 0 : tid / COLS), col(tid % COLS), group(MANY ? tid / COLS : 0) {}
+    // sum over the pieces of f(piece) * the row of slot `piece`; whole in the lanes of group 0
+    template <class F>
+    __device__ __forceinline__ f32x4 sum(const float* rows, int pieces, int stride, f32x4* red, F&& f) const {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int k = 0; k < a.splits; ++k) M = fmaxf(M, slot[(size_t)k * cross_slot<D>() + 32 * D + row]);
-    const float base = M == -__builtin_inff() ? 0.f : M;
-    float Z = 0.f, x[D / 8];
+        for (int k = group; k < pieces; k += GROUPS) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(rows + (size_t)k * stride + 4 * col);
+            const float by = f(k);
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) x[i] = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < a.splits; ++k) {
-        const float* s = slot + (size_t)k * cross_slot<D>();
-        const float f = __builtin_amdgcn_exp2f(s[32 * D + row] - base);
-        Z += s[32 * D + 32 + row] * f;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(s + row * D + j * (D / 8) + 4 * i);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * i + e] += v[e] * f;
+            for (int e = 0; e < 4; ++e) x[e] = fmaf(v[e], by, x[e]);
         }
+        if constexpr (MANY) {
+            red[group * COLS + col] = x;
+            __syncthreads();
+            if (group == 0)
+#pragma unroll
+                for (int g = 1; g < GROUPS; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] += red[g * COLS + col][e];
+        }
+        return x;
     }
+};
+// four values to memory, rounded once
+template <class T>
+__device__ __forceinline__ void cross_put4(const char* row, int col, f32x4 x) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<f32x4*>(const_cast<char*>(row))[col] = x;
+    } else {
+        bf16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (__bf16)x[e];
+        reinterpret_cast<bf16x4*>(const_cast<char*>(row))[col] = v;
+    }
+}
+
+template <class T, int D, bool MANY>
+__global__ __launch_bounds__(256) void cross_merge_kernel(CrossCall a) {
+    typedef CrossJoin<D, MANY> J;
+    __shared__ f32x4 red[MANY ? 256 : 1];
+    __shared__ float by[MANY ? 64 : 1];
+    const int tid = threadIdx.x, l = tid & 63;
+    const J j(tid);
+    const int sets = (a.rows + J::ROWS - 1) / J::ROWS, bg = blockIdx.x / sets, r = min((int)(blockIdx.x - bg * sets) * J::ROWS + j.row, a.rows - 1);
+    const float* slot = a.part + ((size_t)bg * ((a.rows + 31) / 32) + r / 32) * a.splits * cross_slot<D>();
+    const float* stats = slot + 32 * D + r % 32;  // of the first piece
+    float M = -__builtin_inff(), Z = 0.f;
+    f32x4 x;
+    if constexpr (MANY) {  // a piece a lane (there are no more than 64)
+        const bool have = l < a.splits;
+        const float* mine = stats + (size_t)min(l, a.splits - 1) * cross_slot<D>();
+        const float m = have ? mine[0] : -__builtin_inff(), z = have ? mine[32] : 0.f;
+        M = m;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+        const float f = __builtin_amdgcn_exp2f(m - (M == -__builtin_inff() ? 0.f : M));
+        Z = z * f;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) Z += __shfl_xor(Z, o, 64);
+        if (tid < 64) by[l] = f;
+        __syncthreads();
+        x = j.sum(slot + (r % 32) * D, a.splits, cross_slot<D>(), red, [&](int k) { return by[k]; });
+    } else {
+        float m[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            m[k] = k < a.splits ? stats[(size_t)k * cross_slot<D>()] : -__builtin_inff();
+            M = fmaxf(M, m[k]);
+        }
+        const float base = M == -__builtin_inff() ? 0.f : M;
+        x = j.sum(slot + (r % 32) * D, a.splits, cross_slot<D>(), red, [&](int k) {
+            const float f = __builtin_amdgcn_exp2f(stats[(size_t)k * cross_slot<D>()] - base);
+            Z = fmaf(stats[(size_t)k * cross_slot<D>() + 32], f, Z);
+            return f;
+        });
+    }
+    if (j.group != 0) return;
     const float inv = Z == 0.f ? 0.f : 1.f / Z;
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) x[i] *= inv;
-    cross_put<T, D>(a.row(a.o, bg / a.G, bg % a.G, r), j, x);
-    if (j == 0) a.lse[(size_t)bg * a.rows + r] = Z == 0.f ? __builtin_inff() : M + __builtin_amdgcn_logf(Z);
+    for (int e = 0; e < 4; ++e) x[e] *= inv;
+    cross_put4<T>(a.row(a.o, bg / a.G, bg % a.G, r), j.col, x);
+    if (j.col == 0) a.lse[(size_t)bg * a.rows + r] = Z == 0.f ? __builtin_inff() : M + __builtin_amdgcn_logf(Z);
 }
 
 // -------------------------------------------------------------------------------------------------
@@ -616,11 +684,11 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     });
 }
 
+// Strips of 32 rows, as in cross_forward_few_kernel.
 template <class T, int D>
 __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_row_few_kernel(CrossCall a) {
     typedef BiasTile<T, D> TL;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    CrossLds& sc = *reinterpret_cast<CrossLds*>(lds + cross_tiles_bytes<T, D>());
     const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
     const CrossItem it(a, gridDim.x);
     const int q0 = it.strip * 32, qi = min(q0 + li, a.rows - 1);
@@ -630,7 +698,7 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     const size_t stat = (size_t)it.bg * a.rows + qi;
     const float minus_lse = there ? -a.lse[stat] : -__builtin_inff();
     const float delta = half_swap_sum(TL::dot(go, TL::load(a.row(a.o, it.b, it.g, qi), h, there)));
-    if (it.split == 0 && w == 0 && h == 0 && there) a.delta[stat] = delta;
+    if (it.split == 0 && tid < 32 && there) a.delta[stat] = delta;
     const typename TL::At at = TL::at(l);
     char* tk = lds + w * 2 * TL::BYTES;
     char* tv = tk + TL::BYTES;
@@ -641,7 +709,7 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     f32x16 dq[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
-    cross_few_walk<T, D>(a, sc, it, tk, tv, tid, [&](unsigned word) __attribute__((always_inline)) {
+    cross_few_walk<T, D, false>(a, it, tk, tv, w, l, [&](int, unsigned word) __attribute__((always_inline)) {
         const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
         typename TL::Columns kt;
         if (TL::EARLY) kt = TL::columns(tk, at);
@@ -651,7 +719,7 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
         float ds[16];
         cross_ds(s, dp, c2, minus_lse, word, h, ds);
         if (!TL::EARLY) kt = TL::columns(tk, at);
-        TL::add_t(kt, ds, dq);
+        cross_add_fine<TL>(kt, ds, dq);
     });
     __syncthreads();  // the tiles are done with
     float v[D / 8];
@@ -664,15 +732,141 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     else cross_put<T, D>(a.row(a.dq, it.b, it.g, q0 + row), j, v);
 }
 
-// The pieces of 32 rows of dQ.
-template <class T, int D>
+template <class T, int D, bool MANY>
 __global__ __launch_bounds__(256) void cross_merge_row_kernel(CrossCall a) {
-    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7, strips = (a.rows + 31) / 32;
-    const int strip = blockIdx.x % strips, bg = blockIdx.x / strips, r = strip * 32 + row;
-    if (r >= a.rows) return;
-    float x[D / 8];
-    cross_add_pieces<D>(a.part + (size_t)blockIdx.x * a.splits * (32 * D) + row * D + j * (D / 8), a.splits, 32 * D, x);
-    cross_put<T, D>(a.row(a.dq, bg / a.G, bg % a.G, r), j, x);
+    typedef CrossJoin<D, MANY> J;
+    __shared__ f32x4 red[MANY ? 256 : 1];
+    const int tid = threadIdx.x;
+    const J j(tid);
+    const int sets = (a.rows + J::ROWS - 1) / J::ROWS, bg = blockIdx.x / sets, r = min((int)(blockIdx.x - bg * sets) * J::ROWS + j.row, a.rows - 1);
+    const float* slot = a.part + ((size_t)bg * ((a.rows + 31) / 32) + r / 32) * a.splits * (32 * D);
+    const f32x4 x = j.sum(slot + (r % 32) * D, a.splits, 32 * D, red, [](int) { return 1.f; });
+    if (j.group == 0) cross_put4<T>(a.row(a.dq, bg / a.G, bg % a.G, r), j.col, x);
+}
+
+// A wavefront's tile of rows of Q or dO on its way to LDS (TileInFlight, which has the rows of one head).
+template <class T, int D>
+struct RowsInFlight {
+    typedef BiasTile<T, D> TL;
+    PieceInFlight<T> x[TL::CPR / 2];
+    template <class S>
+    __device__ __forceinline__ void load(const S& from, int first, int l) {
+#pragma unroll
+        for (int i = 0; i < TL::CPR / 2; ++i) x[i].load(from.r, from.at(first, (64 * i + l) / TL::CPR, 8 * (l % TL::CPR) * (int)sizeof(T)));
+    }
+    __device__ __forceinline__ void store(char* tile, unsigned word, int l) const {
+#pragma unroll
+        for (int i = 0; i < TL::CPR / 2; ++i) x[i].template store<D, false>(tile, (64 * i + l) / TL::CPR, l % TL::CPR, (word >> ((64 * i + l) / TL::CPR)) & 1u);
+    }
+};
+
+// -------------------------------------------------------------------------------------------------
+// Backward of few rows, in one pass over the keys
+// -------------------------------------------------------------------------------------------------
+// All rows of a group in one strip of 32: a tile's dK and dV are then whole after its own products, and K and V are read once for
+// all three gradients (the two passes read them twice: 64 fp32 heads of 4096 padded keys, 16 rows, d = 32: 61 us, this one 30).  dQ wants the
+// rows as lanes and dK, dV the keys, so both products over the head dimension are formed twice, with their operands exchanged: they
+// lie in registers either way.  Every wavefront takes every fourth tile, leaves its dK and dV and keeps dQ; bound by memory.
+template <class T, int D>
+constexpr int cross_few_region() {  // a wavefront's tiles of K and V, then its results on their way out
+    const int tiles = 2 * BiasTile<T, D>::BYTES, out = 32 * (D + 4) * 4;
+    return tiles > out ? tiles : out;
+}
+template <class T, int D>
+constexpr int cross_few_bytes() { return 4 * cross_few_region<T, D>() + 2 * BiasTile<T, D>::BYTES + 64 * 4; }
+
+template <class T, int D>
+__global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_few_kernel(CrossCall a) {
+    typedef BiasTile<T, D> TL;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* const tq = lds + 4 * cross_few_region<T, D>();
+    char* const tg = tq + TL::BYTES;
+    float* const stats = reinterpret_cast<float*>(tg + TL::BYTES);
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
+    const CrossItem it(a, gridDim.x);
+    const int qi = min(li, a.rows - 1);
+    const bool there = li < a.rows;
+    if (w < 2) {  // the tiles of Q and dO, for the products over the rows
+        typedef CrossSource<T, D, false> S;
+        const S from(a, w ? a.dout : a.q, it.b, it.g);
+        RowsInFlight<T, D> x;
+        x.load(from, 0, l);
+        x.store(w ? tg : tq, tail_word(a.rows), l);
+    }
+    const float minus_lse = there ? -a.lse[(size_t)it.bg * a.rows + qi] : -__builtin_inff();
+    const float delta = half_swap_sum(TL::dot(TL::load(a.row(a.dout, it.b, it.g, qi), h, there), TL::load(a.row(a.o, it.b, it.g, qi), h, there)));
+    if (tid < 32) {
+        stats[li] = minus_lse;
+        stats[32 + li] = -delta;
+    }
+    const typename TL::At at = TL::at(l);
+    char* const tk = lds + w * cross_few_region<T, D>();
+    char* const tv = tk + TL::BYTES;
+    const float c2 = a.scale * LOG2E;
+    f32x16 dq[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
+    const char *const ok = a.dk.head(it.b, it.g), *const ov = a.dv.head(it.b, it.g);
+    __syncthreads();  // the tiles of Q and dO, and the rows' numbers
+    cross_few_walk<T, D, true>(a, it, tk, tv, w, l, [&](int k0, unsigned word) __attribute__((always_inline)) {
+        float p[16], ds[16];
+        // (an offset that is not the same in every turn to the compiler, which would keep what the tiles of Q and dO hold in registers)
+        int same = 0;
+        asm volatile("" : "+v"(same));
+        const float* const st = stats + same + 4 * h;
+        if (word) {
+            cross_ds(TL::feat(TL::rows(tk, at), TL::rows(tq + same, at)), TL::feat(TL::rows(tv, at), TL::rows(tg + same, at), splat16(-delta)), c2,
+                     minus_lse, word, h, ds);
+            cross_add_fine<TL>(TL::columns(tk, at), ds, dq);
+            issue_order();
+            f32x16 dp;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 d = *reinterpret_cast<const f32x4*>(st + 32 + 8 * g);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dp[4 * g + j] = d[j];
+            }
+            const f32x16 s = TL::feat(TL::rows(tq + same, at), TL::rows(tk, at));
+            dp = TL::feat(TL::rows(tg + same, at), TL::rows(tv, at), dp);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 e = *reinterpret_cast<const f32x4*>(st + 8 * g);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], c2, e[j]));
+            }
+            // a key that is left out was stored as zeros, and its P is exp2(-lse)
+            const bool key = (word >> li) & 1u;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                ds[r] = key ? p[r] * dp[r] : 0.f;
+                p[r] = key ? p[r] : 0.f;
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] = ds[r] = 0.f;
+        }
+        issue_order();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 x[D / 32];
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) x[c] = splat16(0.f);
+            if (word) cross_add_fine<TL>(TL::columns((t ? tq : tg) + same, at), t ? ds : p, x);
+            cross_store<D>(x, t ? a.scale : 1.f, reinterpret_cast<float*>(tk), 0, l, [&](int row, int j, float (&v)[D / 8]) {
+                if (k0 + row < a.Lk) cross_put<T, D>((t ? ok : ov) + (k0 + row) * (t ? a.dk : a.dv).row, j, v);
+            });
+            issue_order();
+        }
+    });
+    __syncthreads();  // the tiles are done with
+    float v[D / 8];
+    merge_waves<D>(dq, reinterpret_cast<float*>(lds), tid, v);
+    const int row = tid >> 3, j = tid & 7;
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) v[i] *= a.scale;
+    if (a.splits > 1) cross_leave<D>(a.part + it.slot(a, a.rows, 0) * (32 * D), row, j, v);
+    else cross_put<T, D>(a.row(a.dq, it.b, it.g, row), j, v);
 }
 
 // -------------------------------------------------------------------------------------------------
@@ -780,18 +974,108 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
         });
 }
 
-// The pieces of 32 keys of dV and dK.
+// Strips of 32 keys, and a work-group's wavefronts take every fourth tile of the rows.
 template <class T, int D>
-__global__ __launch_bounds__(256) void cross_merge_col_kernel(CrossCall a) {
-    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7, strips = (a.Lk + 31) / 32;
-    const int strip = blockIdx.x % strips, bg = blockIdx.x / strips, key = strip * 32 + row;
-    if (key >= a.Lk) return;
-    const float* slot = a.part + (size_t)blockIdx.x * a.splits * (2 * 32 * D) + row * D + j * (D / 8);
-    float x[D / 8];
+constexpr int cross_col_few_bytes() { return cross_tiles_bytes<T, D>() + 4 * 64 * 4; }
+template <class T, int D>
+__global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_col_few_kernel(CrossCall a) {
+    typedef BiasTile<T, D> TL;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
+    float* const stats = reinterpret_cast<float*>(lds + cross_tiles_bytes<T, D>()) + 64 * w;
+    const CrossItem it(a, gridDim.x);
+    const int k0 = it.strip * 32, ki = min(k0 + li, a.Lk - 1);
+    const bool key = cross_key(a, it.b, k0 + li);
+    const typename TL::Row k = TL::load(a.k.head(it.b, it.g) + ki * a.k.row, h, k0 + li < a.Lk);
+    const typename TL::Row v = TL::load(a.v.head(it.b, it.g) + ki * a.v.row, h, k0 + li < a.Lk);
+    const typename TL::At at = TL::at(l);
+    char* const tq = lds + w * 2 * TL::BYTES;
+    char* const tg = tq + TL::BYTES;
+    const float c2 = a.scale * LOG2E;
+    f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = splat16(0.f);
+    k.settled();
+    v.settled();
+    typedef CrossSource<T, D, false> S;
+    const S qs(a, a.q, it.b, it.g), gs(a, a.dout, it.b, it.g);
+    const float *lse = a.lse + (size_t)it.bg * a.rows, *delta = a.delta + (size_t)it.bg * a.rows;
+    const int tiles = __any(key) ? (a.rows + 31) / 32 : 0, step = 4 * a.splits;
+    RowsInFlight<T, D> fq, fg;
+    float e = 0.f, d = 0.f;
+    auto fetch = [&](int tile) __attribute__((always_inline)) {
+        fq.load(qs, tile * 32, l);
+        fg.load(gs, tile * 32, l);
+        const int r = min(tile * 32 + li, a.rows - 1);
+        e = lse[r], d = delta[r];
+    };
+    int tile = 4 * it.split + w;
+    if (tile < tiles) fetch(tile);
+    for (; tile < tiles; tile += step) {
+        const unsigned word = tail_word(a.rows - tile * 32);
+        const bool there = (word >> li) & 1u;
+        wave_lds_order();
+        fq.store(tq, word, l);
+        fg.store(tg, word, l);
+        if (l < 32) {
+            stats[li] = there ? -e : -__builtin_inff();  // (rows behind the last have P = 0)
+            stats[32 + li] = there ? -d : 0.f;
+        }
+        wave_lds_order();
+        if (tile + step < tiles) fetch(tile + step);
+        const float* const st = stats + 4 * h;
+        f32x16 dp;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(st + 32 + 8 * g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dp[4 * g + j] = x[j];
+        }
+        const typename TL::Row qr = TL::rows(tq, at), gr = TL::rows(tg, at);
+        issue_order();
+        const f32x16 s = TL::feat(qr, k);
+        dp = TL::feat(gr, v, dp);  // dP - D
+        float p[16], ds[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(st + 8 * g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], c2, x[j]));
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = p[r] * dp[r];
+        cross_add_fine<TL>(TL::columns(tg, at), p, dv);
+        cross_add_fine<TL>(TL::columns(tq, at), ds, dk);
+    }
+    const unsigned keys = (unsigned)__ballot(key);
+    const int row = tid >> 3, j = tid & 7;
+    const bool keep = (keys >> row) & 1u;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        cross_add_pieces<D>(slot + t * 32 * D, a.splits, 2 * 32 * D, x);
-        cross_put<T, D>((t ? a.dk : a.dv).head(bg / a.G, bg % a.G) + key * (t ? a.dk : a.dv).row, j, x);
+        __syncthreads();  // the tiles, and what was there before, are done with
+        float x[D / 8];
+        merge_waves<D>(t ? dk : dv, reinterpret_cast<float*>(lds), tid, x);
+        if (k0 + row >= a.Lk) continue;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) x[i] = keep ? x[i] * (t ? a.scale : 1.f) : 0.f;
+        if (a.splits > 1) cross_leave<D>(a.part + it.slot(a, a.Lk, k0) * (2 * 32 * D) + t * 32 * D, row, j, x);
+        else cross_put<T, D>((t ? a.dk : a.dv).head(it.b, it.g) + (k0 + row) * (t ? a.dk : a.dv).row, j, x);
+    }
+}
+
+template <class T, int D, bool MANY>
+__global__ __launch_bounds__(256) void cross_merge_col_kernel(CrossCall a) {
+    typedef CrossJoin<D, MANY> J;
+    __shared__ f32x4 red[2][MANY ? 256 : 1];
+    const int tid = threadIdx.x;
+    const J j(tid);
+    const int sets = (a.Lk + J::ROWS - 1) / J::ROWS, bg = blockIdx.x / sets, key = min((int)(blockIdx.x - bg * sets) * J::ROWS + j.row, a.Lk - 1);
+    const float* slot = a.part + ((size_t)bg * ((a.Lk + 31) / 32) + key / 32) * a.splits * (2 * 32 * D) + (key % 32) * D;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const f32x4 x = j.sum(slot + t * 32 * D, a.splits, 2 * 32 * D, red[t], [](int) { return 1.f; });
+        const HeadsAt& to = t ? a.dk : a.dv;
+        if (j.group == 0) cross_put4<T>(to.head(bg / a.G, bg % a.G) + key * to.row, j.col, x);
     }
 }
 
