@@ -10,6 +10,8 @@
 #pragma once
 #include "bias_tile.h"
 
+#include <type_traits>
+
 namespace spion {
 
 struct CrossCall {
@@ -41,21 +43,37 @@ constexpr float CROSS_LAZY = 8.f;
 template <class T, int D, bool KEYS>
 struct CrossSource {
     rsrc_t r;
+    unsigned long long first_row;
+    unsigned bytes;
     int ld, head;
     const CrossCall& a;
     __device__ __forceinline__ CrossSource(const CrossCall& a, const HeadsAt& t, int b, int g) : ld((int)t.row), head((int)t.h), a(a) {
         const unsigned long long p = reinterpret_cast<unsigned long long>(t.p + b * t.b + (KEYS ? g : g * (long long)a.each) * t.h);
         // (the same in every lane, which the compiler does not see through the divisions that b and g come from)
-        const unsigned long long u = (unsigned)uniform((int)(unsigned)p) | (unsigned long long)(unsigned)uniform((int)(p >> 32)) << 32;
-        const long long bytes = KEYS ? (a.Lk - 1) * t.row : (a.each - 1) * t.h + (a.Lq - 1) * t.row;
-        r = make_rsrc(reinterpret_cast<const void*>(u), (unsigned)(bytes + D * (int)sizeof(T)));
+        first_row = (unsigned)uniform((int)(unsigned)p) | (unsigned long long)(unsigned)uniform((int)(p >> 32)) << 32;
+        bytes = (unsigned)((KEYS ? (a.Lk - 1) * t.row : (a.each - 1) * t.h + (a.Lq - 1) * t.row) + D * (int)sizeof(T));
+        r = make_rsrc(reinterpret_cast<const void*>(first_row), bytes);
     }
+    // whether the rows lie one behind the other
+    __device__ __forceinline__ bool linear() const { return KEYS || a.each == 1; }
     __device__ __forceinline__ int at(int first, int row, int byte) const {
-        if (KEYS || a.each == 1) return (int)((unsigned)first * (unsigned)ld + ((unsigned)row * (unsigned)ld + (unsigned)byte));
+        if (linear()) return (int)((unsigned)first * (unsigned)ld + ((unsigned)row * (unsigned)ld + (unsigned)byte));
         const int x = min(first + row, a.rows - 1), n = a.head_of(x);
         return (int)((unsigned)n * (unsigned)head + (unsigned)(x - n * a.Lq) * (unsigned)ld + (unsigned)byte);
     }
 };
+
+// The same from row `first` on (an existing one), for loads into LDS: what follows the buffer's end is out of its range, whatever the lane.
+template <class S>
+__device__ __forceinline__ u32x4 cross_words(const S& s, int first) {
+    const unsigned skip = s.linear() ? (unsigned)first * (unsigned)s.ld : 0u;
+    const unsigned long long p = s.first_row + skip;
+    return u32x4{(unsigned)uniform((int)(unsigned)p), (unsigned)uniform((int)(p >> 32)), (unsigned)uniform((int)(s.bytes - skip)), 0x00020000u};
+}
+template <class S>
+__device__ __forceinline__ int cross_lane(const S& s, int first, int row, int byte) {
+    return s.linear() ? row * s.ld + byte : s.at(first, row, byte);
+}
 
 // Work-group -> (group, strip, piece): the strips of a group follow each other on one XCD, whose L2 then holds what they share, and
 // the groups go round-robin, so that every XCD has groups of every sample (padded ones differ in length).
@@ -94,6 +112,7 @@ constexpr int cross_slot() { return 32 * D + 64; }
 // tile take part) and the list of its stages that have any.  The mask is read as it is at the call.
 struct CrossLds {
     unsigned words[CHUNK];
+    unsigned of[CHUNK];  // the same in the order of the list
     unsigned short list[CHUNK];
     int seg[8];
 };
@@ -106,7 +125,7 @@ __device__ __forceinline__ bool cross_key(const CrossCall& a, int b, int key) {
     return a.mask_bytes == 4 ? reinterpret_cast<const float*>(a.mask)[i] != 0.f : reinterpret_cast<const unsigned char*>(a.mask)[i] != 0;
 }
 
-// The stages of SUBS tiles among tiles first .. first + count - 1 that have a key: how many; which, in s.list.  All 256 threads; LDS that
+// The stages of SUBS tiles among tiles first .. first + count - 1 that have a key: how many; which, in s.list, and their words in s.of.  All 256 threads; LDS that
 // they still read must be done with.
 template <int SUBS>
 __device__ __forceinline__ int cross_scan(const CrossCall& a, CrossLds& s, int b, int first, int count, int tid) {
@@ -135,7 +154,11 @@ __device__ __forceinline__ int cross_scan(const CrossCall& a, CrossLds& s, int b
         int before = 0;
 #pragma unroll
         for (int k = 0; k < 4 * ROUNDS; ++k) before += k < 4 * r + w ? s.seg[k] : 0;
-        if (act[r]) s.list[before + __popcll(votes[r] & ((1ull << l) - 1))] = (unsigned short)(tid + 256 * r);
+        if (!act[r]) continue;
+        const int at = before + __popcll(votes[r] & ((1ull << l) - 1)), i = tid + 256 * r;
+        s.list[at] = (unsigned short)i;
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) s.of[at * SUBS + u] = i * SUBS + u < count ? s.words[i * SUBS + u] : 0u;
     }
 #pragma unroll
     for (int k = 0; k < 4 * ROUNDS; ++k) total += s.seg[k];
@@ -182,6 +205,44 @@ struct CrossStage {
     }
 };
 
+// bf16 stages go from global memory straight into LDS (tile_kernels.h: loads in assembly blocks, waited for with wait_vm), which takes no
+// registers and no LDS stores.  Wavefront w has rows 16 w .. 16 w + 15 of both tensors, 1 KB an instruction; a lane asks for the piece that
+// belongs to its place in LDS.  Rows that take no part are overwritten with zeros when they have arrived.
+template <int D>
+struct CrossStage<__bf16, D> {
+    typedef BiasTile<__bf16, D> TL;
+    static constexpr int SUBS = 2, ROWS = 64, BYTES = 2 * SUBS * TL::BYTES;
+    static constexpr int AT_ONCE = 1024 / TL::ROW, N = 16 / AT_ONCE;  // rows an instruction moves, instructions a tensor
+    template <class S>
+    __device__ static __forceinline__ void ask(const S& xs, const S& ys, int first, char* buf, int w, int l) {
+        const u32x4 xr = cross_words(xs, first), yr = cross_words(ys, first);
+        const unsigned at = lds_address(buf) + 16 * w * TL::ROW;
+        if constexpr (D == 128) asm volatile("" : "+v"(l));  // (the lane's places made anew: kept, they are registers that the column pass spills)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = 16 * w + AT_ONCE * i + l / TL::CPR, byte = 16 * ((l % TL::CPR) ^ TL::swz(r & 31));
+            load(xr, at + 1024 * i, cross_lane(xs, first, r, byte));
+            load(yr, at + SUBS * TL::BYTES + 1024 * i, cross_lane(ys, first, r, byte));
+        }
+    }
+    __device__ static __forceinline__ void load(u32x4 r, unsigned lds, int voff) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r) : "memory");
+    }
+    __device__ static __forceinline__ void arrived(char* buf, const unsigned (&word)[SUBS], int w, int l) {
+        wait_vm<0>();
+        if ((word[0] & word[1]) == ~0u) return;
+        const unsigned mine = word[w >> 1] >> (16 * (w & 1));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = AT_ONCE * i + l / TL::CPR;
+            if ((mine >> r) & 1u) continue;
+            char* const at = buf + (16 * w + r) * TL::ROW + 16 * (l % TL::CPR);
+            *reinterpret_cast<u32x4*>(at) = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(at + SUBS * TL::BYTES) = u32x4{0, 0, 0, 0};
+        }
+    }
+};
+
 template <class T, int D>
 constexpr int cross_stages_bytes() {
     const int stages = 2 * CrossStage<T, D>::BYTES, merge = merge_floats<D>() * 4;
@@ -193,44 +254,90 @@ struct NothingElseToFetch {
     __device__ __forceinline__ void store(int) {}
 };
 
-// The stages of a piece of the other side, one after the other, in two buffers taken in turn (one barrier a stage).
-// body(stage's first row, words, buffer, its parity).
+// The stages of a piece of the other side, one after the other, in two buffers taken in turn (one barrier a stage; of bf16 stages the buffer is
+// known at compile time, so that the operands' LDS addresses are constants beside the lane's, and fp32 bodies are too large to stand
+// there twice).  body(words, buffer, which).
 template <class T, int D, bool KEYS, class S, class Fetched, class Body>
 __device__ __forceinline__ void cross_walk(const CrossCall& a, CrossLds& sc, const CrossItem& it, const S& xs, const S& ys, char* lds, int tid,
                                            Fetched&& fetched, Body&& body) {
     typedef CrossStage<T, D> ST;
+    constexpr bool DIRECT = sizeof(T) == 2;
     const bool listed = KEYS && a.mask;
-    const int rows = KEYS ? a.Lk : a.rows;
+    const int rows = KEYS ? a.Lk : a.rows, w = uniform(tid >> 6), l = tid & 63;
     const int from = it.split * a.per_split, to = min((rows + 31) / 32, from + a.per_split), chunk = listed ? CHUNK : a.per_split;
-    int parity = 0;
     for (int first = from; first < to; first += chunk) {
         const int count = min(chunk, to - first);
         const int n = listed ? cross_scan<ST::SUBS>(a, sc, it.b, first, count, tid) : (count + ST::SUBS - 1) / ST::SUBS;
-        auto unit_of = [&](int i) __attribute__((always_inline)) { return listed ? uniform((int)sc.list[i]) : i; };
         ST st;
-        int unit = 0;
-        if (n > 0) {
-            unit = unit_of(0);
-            st.load(xs, ys, (first + unit * ST::SUBS) * 32, tid);
-            fetched.load((first + unit * ST::SUBS) * 32);
-        }
-        for (int i = 0; i < n; ++i, parity ^= 1) {
-            const int u = unit * ST::SUBS, row0 = (first + u) * 32;
+        // A stage's place and words are read from the list while the one two before it is worked on: read where they are needed, they cost a padded
+        // call a third of its time (128 heads of 1024 x 2048, three quarters of the keys: forward 90 us, and 88 of all of them).
+        struct Entry {
+            int unit;
+            unsigned word[ST::SUBS];
+        };
+        auto look_up = [&](int i) __attribute__((always_inline)) {
+            Entry e;
+            e.unit = i;
+            if (listed) {
+                const int at = min(i, n - 1);
+                e.unit = sc.list[at];
+#pragma unroll
+                for (int u = 0; u < ST::SUBS; ++u) e.word[u] = sc.of[at * ST::SUBS + u];
+            }
+            return e;
+        };
+        Entry now, next;
+        auto ask = [&](char* buf) __attribute__((always_inline)) {  // the stage of `now`
+            now.unit = uniform(now.unit);
+            const int row = (first + now.unit * ST::SUBS) * 32;
+#pragma unroll
+            for (int u = 0; u < ST::SUBS; ++u)
+                now.word[u] = listed ? (unsigned)uniform((int)now.word[u]) : now.unit * ST::SUBS + u < count ? tail_word(rows - row - 32 * u) : 0u;
+            if constexpr (DIRECT) ST::ask(xs, ys, row, buf, w, l);
+            else st.load(xs, ys, row, tid);
+            fetched.load(row);
+        };
+        auto step = [&](int i, auto which) __attribute__((always_inline)) {
+            const int P = which;
             unsigned word[ST::SUBS];
 #pragma unroll
-            for (int s = 0; s < ST::SUBS; ++s)
-                word[s] = listed ? (u + s < count ? (unsigned)uniform((int)sc.words[u + s]) : 0u) : u + s < count ? tail_word(rows - row0 - 32 * s) : 0u;
-            char* buf = lds + parity * ST::BYTES;
-            st.store(buf, word, tid);
-            fetched.store(parity);
-            __syncthreads();
+            for (int u = 0; u < ST::SUBS; ++u) word[u] = now.word[u];
+            char* const buf = lds + P * ST::BYTES;
+            if constexpr (DIRECT) ST::arrived(buf, word, w, l);
+            else st.store(buf, word, tid);
+            fetched.store(P);
+            group_barrier();
             if (i + 1 < n) {
-                unit = unit_of(i + 1);
-                st.load(xs, ys, (first + unit * ST::SUBS) * 32, tid);
-                fetched.load((first + unit * ST::SUBS) * 32);
+                now = next;
+                ask(lds + (1 - P) * ST::BYTES);
+                next = look_up(i + 2);
             }
-            body(row0, word, buf, parity);
+            body(word, buf, which);
+        };
+        if (n > 0) {
+            now = look_up(0);
+            next = look_up(1);
+            ask(lds);
         }
+        if constexpr (DIRECT) {
+            for (int i = 0; i < n; i += 2) {
+                step(i, std::integral_constant<int, 0>());
+                if (i + 1 < n) step(i + 1, std::integral_constant<int, 1>());
+            }
+        } else {
+            for (int i = 0; i < n; ++i) step(i, i & 1);
+        }
+    }
+}
+
+// PRODUCTS matrix instructions of a block, and behind each VECTORS vector instructions and READS LDS reads of the same block.
+template <int PRODUCTS, int VECTORS, int READS>
+__device__ __forceinline__ void cross_beside() {
+#pragma unroll
+    for (int i = 0; i < PRODUCTS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, VECTORS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
     }
 }
 
@@ -323,6 +430,10 @@ struct CrossSoftmax {
 // Wavefronts a SIMD that the registers are for.
 template <class T, int D>
 constexpr int cross_forward_waves() { return D == 128 ? (sizeof(T) == 2 ? 2 : 1) : sizeof(T) == 2 ? 3 : 2; }
+// (Row pass, D = 128, bf16, whose operands are read as the products need them: 256 heads of 2048 x 4096 2050 us with one wavefront, 1555 with two.
+// Three at D = 64: 900 and 815.)
+template <class T, int D>
+constexpr int cross_row_waves() { return sizeof(T) == 2 ? (D == 128 ? 2 : 3) : D == 32 ? 2 : 1; }
 template <class T, int D>
 constexpr int cross_backward_waves() { return sizeof(T) == 2 ? (D == 128 ? 1 : 2) : D == 32 ? 2 : 1; }
 
@@ -345,7 +456,7 @@ __global__ __launch_bounds__(256, (cross_forward_waves<T, D>())) void cross_forw
     CrossSoftmax<T, D> x;
     typedef CrossSource<T, D, true> S;
     cross_walk<T, D, true>(a, sc, it, S(a, a.k, it.b, it.g), S(a, a.v, it.b, it.g), lds, tid, NothingElseToFetch(),
-        [&](int, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
+        [&](const unsigned (&word)[SUBS], const char* buf, auto) __attribute__((always_inline)) {
             if (!some) return;
             f32x16 s[SUBS];
             typename TL::Row kr[SUBS];
@@ -627,7 +738,7 @@ __device__ __forceinline__ void cross_ds(const f32x16& s, const f32x16& dp, floa
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_row_kernel(CrossCall a) {
+__global__ __launch_bounds__(256, (cross_row_waves<T, D>())) void cross_backward_row_kernel(CrossCall a) {
     typedef BiasTile<T, D> TL;
     typedef CrossStage<T, D> ST;
     constexpr int SUBS = ST::SUBS;
@@ -653,7 +764,7 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
     typedef CrossSource<T, D, true> S;
     cross_walk<T, D, true>(a, sc, it, S(a, a.k, it.b, it.g), S(a, a.v, it.b, it.g), lds, tid, NothingElseToFetch(),
-        [&](int, const unsigned (&word)[SUBS], const char* buf, int) __attribute__((always_inline)) {
+        [&](const unsigned (&word)[SUBS], const char* buf, auto) __attribute__((always_inline)) {
             if (!some) return;
 #pragma unroll
             for (int u = 0; u < SUBS; ++u) {
@@ -661,16 +772,18 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
                 const char *tk = buf + u * TL::BYTES, *tv = buf + (SUBS + u) * TL::BYTES;
                 const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
                 typename TL::Columns kt;
-                issue_order();
+                if (D < 128) issue_order();
                 const f32x16 s = TL::feat(kr, q);
-                const f32x16 dp = TL::feat(vr, go, minus);
-                if (TL::EARLY) {
+                if (D == 128) issue_order();
+                const f32x16 dp = TL::feat(vr, go, D == 128 ? splat16(-delta) : minus);
+                if (D == 128) issue_order();
+                if (TL::EARLY && D < 128) {
                     kt = TL::columns(tk, at);
                     read_behind_products<D / 8, D / 8>();
                 }
                 float ds[16];
                 cross_ds(s, dp, c2, minus_lse, word[u], h, ds);
-                if (!TL::EARLY) kt = TL::columns(tk, at);
+                if (!TL::EARLY || D == 128) kt = TL::columns(tk, at);
                 TL::add_t(kt, ds, dq);
             }
         });
@@ -895,6 +1008,8 @@ struct CrossRowStats {
     }
 };
 
+// At D = 128 dK and dV are 128 registers beside the 64 of K and V, so one wavefront a SIMD.  (In a pass each, two wavefronts a SIMD, five products for
+// four: 813 us against 767, 32 heads of 2048 x 8192.)
 template <class T, int D>
 __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_col_kernel(CrossCall a) {
     typedef BiasTile<T, D> TL;
@@ -918,43 +1033,79 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     k.settled();
     v.settled();
     typedef CrossSource<T, D, false> S;
-    if (__syncthreads_or(some))
+    // -lse or -D of a tile's rows
+    auto stat = [&](const float* st) __attribute__((always_inline)) {
+        f32x16 x;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 d = *reinterpret_cast<const f32x4*>(st + 8 * g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * g + j] = d[j];
+        }
+        return x;
+    };
+    auto weights = [&](const f32x16& s, const f32x16& dp, const f32x16& e, float (&p)[16], float (&ds)[16]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, e[r]));
+            ds[r] = p[r] * dp[r];
+        }
+    };
+    if (l == 0) sc.seg[w] = some;
+    __syncthreads();
+    if (sc.seg[0] | sc.seg[1] | sc.seg[2] | sc.seg[3])
         cross_walk<T, D, false>(a, sc, it, S(a, a.q, it.b, it.g), S(a, a.dout, it.b, it.g), lds, tid, rs,
-            [&](int, const unsigned (&word)[SUBS], const char* buf, int parity) __attribute__((always_inline)) {
+            [&](const unsigned (&word)[SUBS], const char* buf, auto which) __attribute__((always_inline)) {
                 if (!some) return;
+                if constexpr (sizeof(T) == 2 && D == 128) {
+                    if (word[SUBS - 1] != 0) {
+                        // One wavefront a SIMD: two tiles, the arithmetic of each beside the products of the other.
+                        const float* st = stats + 128 * which + 4 * h;
+                        const typename TL::Row q0 = TL::rows(buf, at), g0 = TL::rows(buf + SUBS * TL::BYTES, at);
+                        const f32x16 d0 = stat(st + 64);
+                        issue_order();
+                        const f32x16 s0 = TL::feat(q0, k), dp0 = TL::feat(g0, v, d0);
+                        const typename TL::Row q1 = TL::rows(buf + TL::BYTES, at), g1 = TL::rows(buf + (SUBS + 1) * TL::BYTES, at);
+                        const f32x16 d1 = stat(st + 96);
+                        read_behind_products<D / 8, 2>();
+                        issue_order();
+                        float p0[16], ds0[16], p1[16], ds1[16];
+                        const f32x16 s1 = TL::feat(q1, k), dp1 = TL::feat(g1, v, d1);
+                        weights(s0, dp0, stat(st), p0, ds0);
+                        const typename TL::Columns gt0 = TL::columns(buf + SUBS * TL::BYTES, at), qt0 = TL::columns(buf, at);
+                        issue_order();
+                        TL::add_t(gt0, p0, dv);
+                        TL::add_t(qt0, ds0, dk);
+                        weights(s1, dp1, stat(st + 32), p1, ds1);
+                        const typename TL::Columns gt1 = TL::columns(buf + (SUBS + 1) * TL::BYTES, at), qt1 = TL::columns(buf + TL::BYTES, at);
+                        issue_order();
+                        TL::add_t(gt1, p1, dv);
+                        TL::add_t(qt1, ds1, dk);
+                        return;
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < SUBS; ++u) {
                     if (word[u] == 0) continue;
                     const char *tq = buf + u * TL::BYTES, *tg = buf + (SUBS + u) * TL::BYTES;
-                    const float* st = stats + 128 * parity + 32 * u + 4 * h;
-                    f32x16 dp;
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f32x4 d = *reinterpret_cast<const f32x4*>(st + 64 + 8 * g);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) dp[4 * g + j] = d[j];
-                    }
+                    const float* st = stats + 128 * which + 32 * u + 4 * h;
+                    const f32x16 d = stat(st + 64);
                     const typename TL::Row qr = TL::rows(tq, at), gr = TL::rows(tg, at);
                     typename TL::Columns qt, gt;
-                    issue_order();
+                    if (D < 128) issue_order();
                     const f32x16 s = TL::feat(qr, k);
-                    dp = TL::feat(gr, v, dp);  // dP - D
-                    if (TL::EARLY) {
+                    if (D == 128) issue_order();
+                    const f32x16 dp = TL::feat(gr, v, d);  // dP - D
+                    if (D == 128) issue_order();
+                    if (TL::EARLY && D < 128) {
                         gt = TL::columns(tg, at), qt = TL::columns(tq, at);
                         read_behind_products<D / 8, 2 * D / 8>();
                     }
                     float p[16], ds[16];
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f32x4 e = *reinterpret_cast<const f32x4*>(st + 8 * g);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) p[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], c2, e[j]));
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) ds[r] = p[r] * dp[r];
-                    if (!TL::EARLY) gt = TL::columns(tg, at);
+                    weights(s, dp, stat(st), p, ds);
+                    if (!TL::EARLY || D == 128) gt = TL::columns(tg, at);
                     TL::add_t(gt, p, dv);
-                    if (!TL::EARLY) qt = TL::columns(tq, at);
+                    if (!TL::EARLY || D == 128) qt = TL::columns(tq, at);
                     TL::add_t(qt, ds, dk);
                 }
             });
@@ -964,7 +1115,7 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     float* red = reinterpret_cast<float*>(lds);
     float* slot = a.part + it.slot(a, a.Lk, k0) * (2 * 32 * D);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
         cross_store<D>(t ? dk : dv, t ? a.scale : 1.f, red, w, l, [&](int row, int j, float (&x)[D / 8]) {
             if (k0 + row >= a.Lk) return;
 #pragma unroll
@@ -972,6 +1123,7 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
             if (a.splits > 1) cross_leave<D>(slot + t * 32 * D, row, j, x);
             else cross_put<T, D>((t ? a.dk : a.dv).head(it.b, it.g) + (k0 + row) * (t ? a.dk : a.dv).row, j, x);
         });
+    }
 }
 
 // Strips of 32 keys, and a work-group's wavefronts take every fourth tile of the rows.
