@@ -3,7 +3,7 @@
 //   h = x + residual, rounded to the tensors' type: the stream as it goes on
 //   mu = mean(h),  s = 1 / sqrt(mean((h - mu)^2) + eps),  xh = (h - mu) s,  y = xh w + b
 //   g = dy w,  dh = s (g - mean(g) - xh mean(g xh)) + (gradient of the stream);   dw, db = sums over the rows of dy xh and dy
-// Bound by memory: every tensor is read or written once.  A row lies in the registers of 16, 64, 256 or 1024 lanes in pieces of 16
+// Bound by memory: every tensor is read or written once.  A row lies in the registers of 8, 16, 64, 256 or 1024 lanes in pieces of 16
 // bytes, so the mean, and the variance as the mean of squares about it (not as a difference of sums, which loses what a large mean leaves),
 // need no second pass over memory.  Rows need not start on 16 bytes: the hardware loads and stores 16 bytes from any element's address, and
 // only what is left of a row behind its last whole piece goes element by element.  The backward forms mu and s again (8 bytes a row
@@ -29,7 +29,11 @@ struct LayerNormCall {
 };
 
 typedef unsigned words4 __attribute__((ext_vector_type(4)));
-typedef words4 words4_anywhere __attribute__((aligned(2)));  // (global memory instructions take any address here)
+typedef unsigned words2 __attribute__((ext_vector_type(2)));
+// (global memory instructions take any address here)
+typedef words4 words4_anywhere __attribute__((aligned(2)));
+typedef words2 words2_anywhere __attribute__((aligned(2)));
+typedef unsigned word_anywhere __attribute__((aligned(2)));
 
 // Elements i .. i + V - 1 of a row of n, those behind its end zeros: the words as they come from memory, so that nothing waits for them
 // before all of a row's pieces are asked for, and then as floats.  (Converted where they are loaded, each piece waited for its own: backward
@@ -42,22 +46,35 @@ struct RowWords {
     __device__ __forceinline__ void again() {
         if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(u));
     }
+    // The row's last V where there are fewer from i on (one load for every lane), which down() then moves to where they belong.  It stands
+    // apart, behind all loads, and rows of fewer than V elements (TINY) have kernels of their own: beside each load, either makes the
+    // compiler wait for one before the next (262144 x 64 fp32, training: 92 and 104 us).
+    template <bool TINY>
     __device__ __forceinline__ void load(const T* row, int i, int n) {
         u = words4{0, 0, 0, 0};
-        if (i + V <= n) {
-            u = *reinterpret_cast<const words4_anywhere*>(row + i);
-        } else if (i < n) {
-            if constexpr (sizeof(T) == 4) {
-                const unsigned* p = reinterpret_cast<const unsigned*>(row);
+        if (i >= n) return;
+        if constexpr (!TINY) {
+            u = *reinterpret_cast<const words4_anywhere*>(row + min(i, n - V));
+        } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (i + e < n) u[e] = p[i + e];
-            } else {
-                const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
+            for (int e = 0; e < V; ++e)
+                if (i + e < n) u[e] = reinterpret_cast<const unsigned*>(row)[i + e];
+        } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (i + e < n) u[e / 2] |= (unsigned)p[i + e] << (16 * (e & 1));
-            }
+            for (int e = 0; e < V; ++e)
+                if (i + e < n) u[e / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(row)[i + e] << (16 * (e & 1));
+        }
+    }
+    __device__ __forceinline__ void down(int i, int n) {
+        const int off = i - min(i, n - V);
+        if (i >= n) return;
+        if constexpr (sizeof(T) == 4) {
+            if (off & 1) u = words4{u[1], u[2], u[3], 0};
+            if (off & 2) u = words4{u[2], u[3], 0, 0};
+        } else {
+            if (off & 1) u = words4{u[0] >> 16 | u[1] << 16, u[1] >> 16 | u[2] << 16, u[2] >> 16 | u[3] << 16, u[3] >> 16};
+            if (off & 2) u = words4{u[1], u[2], u[3], 0};
+            if (off & 4) u = words4{u[2], u[3], 0, 0};
         }
     }
 };
@@ -81,22 +98,42 @@ struct RowPiece {
     }
     __device__ __forceinline__ void load(const T* row, int i, int n) {
         RowWords<T> w;
-        w.load(row, i, n);
+        w.template load<false>(row, i, n);
+        if (n % V) w.down(i, n);
         take(w);
     }
     __device__ __forceinline__ void store(T* row, int i, int n) const {
+        words4 u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (sizeof(T) == 4) u[k] = __builtin_bit_cast(unsigned, x[k]);
+            else u[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+        }
+        T* p = row + i;
         if (i + V <= n) {
-            words4 u;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if constexpr (sizeof(T) == 4) u[k] = __builtin_bit_cast(unsigned, x[k]);
-                else u[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+            *reinterpret_cast<words4_anywhere*>(p) = u;
+        } else if (i < n) {  // four, two and one of what is left
+            const int left = n - i;
+            if constexpr (sizeof(T) == 2) {
+                if (left & 4) {
+                    *reinterpret_cast<words2_anywhere*>(p) = words2{u[0], u[1]};
+                    u = words4{u[2], u[3], 0, 0};
+                    p += 4;
+                }
+                if (left & 2) {
+                    *reinterpret_cast<word_anywhere*>(p) = u[0];
+                    u[0] = u[1];
+                    p += 2;
+                }
+                if (left & 1) *reinterpret_cast<unsigned short*>(p) = (unsigned short)u[0];
+            } else {
+                if (left & 2) {
+                    *reinterpret_cast<words2_anywhere*>(p) = words2{u[0], u[1]};
+                    u[0] = u[2];
+                    p += 2;
+                }
+                if (left & 1) *reinterpret_cast<unsigned*>(p) = u[0];
             }
-            *reinterpret_cast<words4_anywhere*>(row + i) = u;
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (i + e < n) row[i + e] = (T)x[e];
         }
     }
     __device__ __forceinline__ void clear() {
@@ -145,19 +182,25 @@ struct RowSums {
 template <int LANES>
 constexpr int row_threads() { return LANES < 256 ? 256 : LANES; }
 
-template <class T, int LANES, int C>
+template <class T, int LANES, int C, bool TINY>
 __global__ __launch_bounds__(row_threads<LANES>()) void layer_norm_forward_kernel(LayerNormCall a) {
     constexpr int V = RowPiece<T>::V, ROWS = row_threads<LANES>() / LANES;
     __shared__ float slots[2][2][16];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     RowSums<LANES> sums{slots};
-    RowPiece<T> w[C], b[C];
+    RowWords<T> w[C], b[C];  // (words: converted where they are used)
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        w[c].load(reinterpret_cast<const T*>(a.w), (c * LANES + lane) * V, a.n);
-        if (a.b) b[c].load(reinterpret_cast<const T*>(a.b), (c * LANES + lane) * V, a.n);
-        else b[c].clear();
+        w[c].template load<TINY>(reinterpret_cast<const T*>(a.w), (c * LANES + lane) * V, a.n);
+        b[c].template load<TINY>(reinterpret_cast<const T*>(a.b), (c * LANES + lane) * V, a.b ? a.n : 0);
     }
+    const bool whole = TINY || a.n % V == 0;
+    if (!whole)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            w[c].down((c * LANES + lane) * V, a.n);
+            if (a.b) b[c].down((c * LANES + lane) * V, a.n);
+        }
     const float rn = 1.f / a.n;
     for (long long r0 = (long long)blockIdx.x * ROWS; r0 < a.rows; r0 += (long long)gridDim.x * ROWS) {
         const long long row = r0 + sub;
@@ -166,10 +209,16 @@ __global__ __launch_bounds__(row_threads<LANES>()) void layer_norm_forward_kerne
         RowWords<T> x[C], r[C];
         float s = 0.f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) x[c].load(reinterpret_cast<const T*>(a.x) + row * a.xs, (c * LANES + lane) * V, n);
+        for (int c = 0; c < C; ++c) x[c].template load<TINY>(reinterpret_cast<const T*>(a.x) + row * a.xs, (c * LANES + lane) * V, n);
         if (a.res)
 #pragma unroll
-            for (int c = 0; c < C; ++c) r[c].load(reinterpret_cast<const T*>(a.res) + row * a.rs, (c * LANES + lane) * V, n);
+            for (int c = 0; c < C; ++c) r[c].template load<TINY>(reinterpret_cast<const T*>(a.res) + row * a.rs, (c * LANES + lane) * V, n);
+        if (!whole)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                x[c].down((c * LANES + lane) * V, n);
+                if (a.res) r[c].down((c * LANES + lane) * V, n);
+            }
 #pragma unroll
         for (int c = 0; c < C; ++c) h[c].take(x[c]);
         if (a.res) {
@@ -198,15 +247,18 @@ __global__ __launch_bounds__(row_threads<LANES>()) void layer_norm_forward_kerne
         const float inv = rsqrtf(sums.over(q) * rn + a.eps);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
+            w[c].again();
+            b[c].again();
+            const RowPiece<T> by(w[c]), to(b[c]);
 #pragma unroll
-            for (int e = 0; e < V; ++e) h[c].x[e] = fmaf(h[c].x[e] * inv, w[c].x[e], b[c].x[e]);
+            for (int e = 0; e < V; ++e) h[c].x[e] = fmaf(h[c].x[e] * inv, by.x[e], to.x[e]);
             h[c].store(reinterpret_cast<T*>(a.y) + row * a.n, (c * LANES + lane) * V, n);
         }
     }
 }
 
 // a.x is the stream h.  part: [work-groups][dw, db][n].
-template <class T, int LANES, int C>
+template <class T, int LANES, int C, bool TINY>
 __global__ __launch_bounds__(row_threads<LANES>()) void layer_norm_backward_kernel(LayerNormCall a) {
     constexpr int V = RowPiece<T>::V, ROWS = row_threads<LANES>() / LANES, WIDTH = LANES * C * V;
     __shared__ float slots[2][2][16];
@@ -218,10 +270,12 @@ __global__ __launch_bounds__(row_threads<LANES>()) void layer_norm_backward_kern
     float dw[C][V], db[C][V];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        w[c].load(reinterpret_cast<const T*>(a.w), (c * LANES + lane) * V, a.n);
+        w[c].template load<TINY>(reinterpret_cast<const T*>(a.w), (c * LANES + lane) * V, a.n);
+        if (!TINY && a.n % V) w[c].down((c * LANES + lane) * V, a.n);
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[c][e] = db[c][e] = 0.f;
     }
+    const bool whole = TINY || a.n % V == 0;
     const float rn = 1.f / a.n;
     for (long long r0 = (long long)blockIdx.x * ROWS; r0 < a.rows; r0 += (long long)gridDim.x * ROWS) {
         const long long row = r0 + sub;
@@ -230,10 +284,18 @@ __global__ __launch_bounds__(row_threads<LANES>()) void layer_norm_backward_kern
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int i = (c * LANES + lane) * V;
-            h[c].load(reinterpret_cast<const T*>(a.x) + row * a.xs, i, n);
-            g[c].load(reinterpret_cast<const T*>(a.dy) + row * a.dys, i, n);
-            dh[c].load(reinterpret_cast<const T*>(a.dh) + row * a.dhs, i, a.dh ? n : 0);
+            h[c].template load<TINY>(reinterpret_cast<const T*>(a.x) + row * a.xs, i, n);
+            g[c].template load<TINY>(reinterpret_cast<const T*>(a.dy) + row * a.dys, i, n);
+            dh[c].template load<TINY>(reinterpret_cast<const T*>(a.dh) + row * a.dhs, i, a.dh ? n : 0);
         }
+        if (!whole)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int i = (c * LANES + lane) * V;
+                h[c].down(i, n);
+                g[c].down(i, n);
+                if (a.dh) dh[c].down(i, n);
+            }
         float s = 0.f, sg = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -453,7 +515,7 @@ struct RowShape {
     int lanes, pieces;  // 0: longer than the registers of a work-group
 };
 static RowShape row_shape(const LayerNorm& c, bool backward) {
-    static const RowShape of[] = {{16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}};
+    static const RowShape of[] = {{8, 1}, {16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}};
     for (const RowShape& s : of)
         if (c.width <= (long long)s.lanes * s.pieces * (c.bf16 ? 8 : 4) && !(backward && c.bf16 && s.lanes == 1024 && s.pieces == 4)) return s;
     return {0, 0};
@@ -462,19 +524,21 @@ static int rows_at_once(const RowShape& s) { return s.lanes == 0 || s.lanes >= 2
 static long long row_groups(long long rows, int at_a_time, int per_cu) {
     return std::max(1LL, std::min((rows + at_a_time - 1) / at_a_time, (long long)per_cu * device_cus()));
 }
-// Work-groups of a backward.  Each leaves partial sums of 2 n floats, so beyond one for each CU no more than one for eight rows.
+// Work-groups of a backward.  Each leaves partial sums of 2 n floats, so beyond one for each CU no more than one for eight rows.  Three to a CU, four
+// where a row has few lanes (a step with 2 / 3 / 4, us: 8192 x 4096 bf16 118 / 118 / 124, 16384 x 1000 58 / 55 / 60, 262144 x 64 90 / 76 / 69).
 static long long layer_norm_groups(const LayerNorm& c) {
-    return std::min(row_groups(c.rows, rows_at_once(row_shape(c, true)), 4), std::max<long long>(device_cus(), c.rows / 8));
+    const RowShape s = row_shape(c, true);
+    return std::min(row_groups(c.rows, rows_at_once(s), s.lanes > 0 && s.lanes < 64 ? 4 : 3), std::max<long long>(device_cus(), c.rows / 8));
 }
 
-template <class T, int LANES, int C>
+template <class T, int LANES, int C, bool TINY = false>
 static bool run_rows(const LayerNormCall& a, bool backward, long long groups, hipStream_t stream) {
     const dim3 grid((unsigned)groups), block(row_threads<LANES>());
     if (!backward) {
-        hipLaunchKernelGGL((layer_norm_forward_kernel<T, LANES, C>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((layer_norm_forward_kernel<T, LANES, C, TINY>), grid, block, 0, stream, a);
         return check_launch("layer_norm_forward_kernel");
     }
-    if constexpr (sizeof(T) == 4 || LANES * C < 4096) hipLaunchKernelGGL((layer_norm_backward_kernel<T, LANES, C>), grid, block, 0, stream, a);
+    if constexpr (sizeof(T) == 4 || LANES * C < 4096) hipLaunchKernelGGL((layer_norm_backward_kernel<T, LANES, C, TINY>), grid, block, 0, stream, a);
     return check_launch("layer_norm_backward_kernel");
 }
 template <class T>
@@ -488,6 +552,9 @@ static bool run_layer_norm(const LayerNorm& c, bool backward, hipStream_t stream
     const long long groups = backward ? layer_norm_groups(c) : row_groups(c.rows, rows_at_once(s), s.lanes == 0 || s.lanes >= 256 ? 8 : 16);
     bool ok = false;
     switch (s.lanes * 8 + s.pieces) {
+        case 8 * 8 + 1:
+            ok = c.width < RowPiece<T>::V ? run_rows<T, 8, 1, true>(a, backward, groups, stream) : run_rows<T, 8, 1>(a, backward, groups, stream);
+            break;
         case 16 * 8 + 1: ok = run_rows<T, 16, 1>(a, backward, groups, stream); break;
         case 16 * 8 + 2: ok = run_rows<T, 16, 2>(a, backward, groups, stream); break;
         case 64 * 8 + 1: ok = run_rows<T, 64, 1>(a, backward, groups, stream); break;
