@@ -23,7 +23,7 @@ struct CrossWalk {
     int strips, splits, per_split;  // tiles of 32 to a piece
 };
 // All rows of a group in one strip of 32: the backward is one pass over the keys.
-static bool cross_one_strip(const Cross& c) { return rows_of(c) <= 32 && (c.bf16 || c.head_dim < 128); }
+static bool cross_one_strip(const Cross& c) { return rows_of(c) <= 32; }
 
 // Which, by an estimate of the launch's time, us.  A CU's work-groups share it: it takes as long for them as for one after the other, within a
 // fifth (bf16, d = 64: 0.49 us a tile of 32 keys and 128 rows alone, 0.41 with four of them).  So a launch takes the most work-groups that a CU
@@ -34,7 +34,7 @@ static bool cross_one_strip(const Cross& c) { return rows_of(c) <= 32 && (c.bf16
 //   16 of 1024 x 4096: 63 / 37, 41;  d = 128 97 / 60, 93;  fp32 199 / 96, 159;  64 of 256 x 1024, fp32, d = 32: 35 / 25, 23
 // At most eight work-groups to a CU where there are pieces, so the workspace is bounded.
 static double cross_tile_us(const Cross& c, CrossPass pass, bool few) {
-    static const double wide_us[2][3] = {{0.85, 1.5, 3.2}, {0.25, 0.45, 0.75}}, few_us[2][3] = {{1.05, 2.4, 0.}, {0.4, 0.6, 1.35}};
+    static const double wide_us[2][3] = {{0.85, 1.5, 3.2}, {0.25, 0.45, 0.75}}, few_us[2][3] = {{1.05, 2.4, 6.}, {0.4, 0.6, 1.35}};
     const int d = c.head_dim == 32 ? 0 : c.head_dim == 64 ? 1 : 2, bf16 = c.bf16 ? 1 : 0;
     const double us = (few ? few_us : wide_us)[bf16][d] * (pass == CrossPass::FORWARD ? 1. : pass == CrossPass::ROW ? 1.3 : 1.75);
     return few && pass != CrossPass::COL && cross_one_strip(c) ? std::max(us, 4 * 64 * c.head_dim * (c.bf16 ? 2 : 4) / 20e3) : us;
@@ -42,11 +42,10 @@ static double cross_tile_us(const Cross& c, CrossPass pass, bool few) {
 static CrossWalk cross_walk_of(const Cross& c, CrossPass pass, bool can_split) {
     const long long own = pass == CrossPass::COL ? c.k_len : rows_of(c), other = pass == CrossPass::COL ? rows_of(c) : c.k_len;
     const long long groups = (long long)c.batch * c.key_heads, tiles = tiles_of(other), cus = device_cus();
-    const bool fits = c.bf16 || c.head_dim < 128;  // (tiles of 128 fp32 features for four wavefronts do not fit a CU)
-    const bool must = pass == CrossPass::ROW && cross_one_strip(c);
+    const bool must = pass != CrossPass::COL && cross_one_strip(c);
     CrossWalk w{};
     double least = 0;
-    for (int few = must; few <= (int)fits; ++few) {
+    for (int few = must; few <= 1; ++few) {
         const int rows = few ? 32 : 128, unit = few ? 1 : 2;
         const long long strips = tiles_of(own, rows), steps = tiles_of(tiles, few ? 4 : unit);
         const double us = cross_tile_us(c, pass, few) * (few ? 1 : unit);
@@ -183,7 +182,6 @@ static bool cross_join(const char* name, K few, K many, long long groups, long l
 template <class T, int D>
 struct CrossRun {
     static constexpr size_t STAGES = cross_stages_bytes<T, D>() + sizeof(CrossLds);
-    static constexpr bool FEW = sizeof(T) == 2 || D < 128;
     static bool forward(const Cross& c, hipStream_t stream) {
         CrossCall a = cross_device_call(c);
         const long long groups = (long long)a.B * a.G;
@@ -193,12 +191,14 @@ struct CrossRun {
         const long long n = groups * w.strips * w.splits;
         bool ok = false;
         if (w.rows == 128) ok = cross_launch("cross_forward_kernel", cross_forward_kernel<T, D>, n, STAGES, stream, a);
-        if constexpr (FEW)
-            if (w.rows == 32)
-                ok = cross_launch("cross_forward_few_kernel", cross_forward_few_kernel<T, D>, n, cross_tiles_bytes<T, D>(), stream, a);
+        if (w.rows == 32) ok = cross_launch("cross_forward_few_kernel", cross_forward_few_kernel<T, D>, n, cross_tiles_bytes<T, D>(), stream, a);
         return ok && (w.splits == 1 || cross_join<D>("cross_merge_kernel", cross_merge_kernel<T, D, false>, cross_merge_kernel<T, D, true>, groups, a.rows, stream, a));
     }
     static bool backward(const Cross& c, hipStream_t stream) {
+        constexpr bool BF16 = sizeof(T) == 2;
+        // dS in two bf16 numbers up to 256 keys, where the rounding of O in D shows (128 heads of 1024 x 256: d = 64 81 us, and 77 without; d = 128 137 and
+        // 128; of 512, where it shows no more, 121 and 109)
+        const bool fine = BF16 && c.k_len <= 256;
         CrossCall a = cross_device_call(c);
         const long long groups = (long long)a.B * a.G;
         const CrossWalk row = cross_walk_of(c, CrossPass::ROW, true), col = cross_walk_of(c, CrossPass::COL, true);
@@ -207,12 +207,10 @@ struct CrossRun {
         cross_take(a, row);
         long long n = groups * row.strips * row.splits;
         bool ok = false;
-        if (row.rows == 128) ok = cross_launch("cross_backward_row_kernel", cross_backward_row_kernel<T, D>, n, STAGES, stream, a);
-        if constexpr (FEW) {
-            if (cross_one_strip(c)) ok = cross_launch("cross_backward_few_kernel", cross_backward_few_kernel<T, D>, n, cross_few_bytes<T, D>(), stream, a);
-            else if (row.rows == 32)
-                ok = cross_launch("cross_backward_row_few_kernel", cross_backward_row_few_kernel<T, D>, n, cross_tiles_bytes<T, D>(), stream, a);
-        }
+        if (row.rows == 128) ok = cross_launch("cross_backward_row_kernel", fine ? cross_backward_row_kernel<T, D, BF16> : cross_backward_row_kernel<T, D, false>, n, STAGES, stream, a);
+        if (cross_one_strip(c)) ok = cross_launch("cross_backward_few_kernel", cross_backward_few_kernel<T, D>, n, cross_few_bytes<T, D>(), stream, a);
+        else if (row.rows == 32)
+            ok = cross_launch("cross_backward_row_few_kernel", cross_backward_row_few_kernel<T, D>, n, cross_tiles_bytes<T, D>() + cross_shared_bytes<T, D>(), stream, a);
         if (!ok) return false;
         if (row.splits > 1 &&
             !cross_join<D>("cross_merge_row_kernel", cross_merge_row_kernel<T, D, false>, cross_merge_row_kernel<T, D, true>, groups, a.rows, stream, a))
@@ -220,10 +218,10 @@ struct CrossRun {
         if (cross_one_strip(c)) return true;  // (with all three gradients)
         cross_take(a, col);
         n = groups * col.strips * col.splits;
-        if (col.rows == 128) ok = cross_launch("cross_backward_col_kernel", cross_backward_col_kernel<T, D>, n, STAGES + 1024, stream, a);
-        if constexpr (FEW)
-            if (col.rows == 32)
-                ok = cross_launch("cross_backward_col_few_kernel", cross_backward_col_few_kernel<T, D>, n, cross_col_few_bytes<T, D>(), stream, a);
+        if (col.rows == 128)
+            ok = cross_launch("cross_backward_col_kernel", fine ? cross_backward_col_kernel<T, D, BF16> : cross_backward_col_kernel<T, D, false>, n, STAGES + 1024, stream, a);
+        if (col.rows == 32)
+            ok = cross_launch("cross_backward_col_few_kernel", cross_backward_col_few_kernel<T, D>, n, cross_col_few_bytes<T, D>(), stream, a);
         if (!ok) return false;
         return col.splits == 1 ||
                cross_join<D>("cross_merge_col_kernel", cross_merge_col_kernel<T, D, false>, cross_merge_col_kernel<T, D, true>, groups, a.Lk, stream, a);

@@ -330,17 +330,6 @@ __device__ __forceinline__ void cross_walk(const CrossCall& a, CrossLds& sc, con
     }
 }
 
-// PRODUCTS matrix instructions of a block, and behind each VECTORS vector instructions and READS LDS reads of the same block.
-template <int PRODUCTS, int VECTORS, int READS>
-__device__ __forceinline__ void cross_beside() {
-#pragma unroll
-    for (int i = 0; i < PRODUCTS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, VECTORS, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-    }
-}
-
 // A wavefront's 32 x D result acc[c][r] (lane (li, h): row li, feature 32 c + acc_row(r, h)), scaled by the lane's f, through its part of
 // red; out(row, eighth, values).
 template <int D, class Out>
@@ -516,14 +505,17 @@ __device__ __forceinline__ void cross_add_fine(const Columns& xt, const float (&
 // Few rows: 32 of them to a work-group, and its wavefronts take every fourth tile of the keys, each through its own part of LDS, so that
 // nothing waits for a barrier inside the walk.
 template <class T, int D>
+constexpr int cross_own_tiles() { return sizeof(T) == 4 && D == 128 ? 1 : 2; }  // (two fp32 tiles of 128 features for four wavefronts do not fit a CU)
+template <class T, int D>
 constexpr int cross_tiles_bytes() {
-    const int tiles = 4 * 2 * BiasTile<T, D>::BYTES, merge = merge_floats<D>() * 4;
+    const int tiles = 4 * cross_own_tiles<T, D>() * BiasTile<T, D>::BYTES, merge = merge_floats<D>() * 4;
     return tiles > merge ? tiles : merge;
 }
 // Wavefront w of piece s has tiles 4 s + w, 4 (s + splits) + w, ...: what padding leaves is dealt evenly (in ranges of tiles, a piece could have
 // none).  It makes the words of its tiles itself, from mask values that were asked for two tiles ahead; K and V are one tile ahead.
-// body(tile's first key, word): for all tiles, those without a key (a word of 0) among them if EVERY.
-template <class T, int D, bool EVERY, class Body>
+// body(tile's first key, word, put_k, put_v): for all tiles, those without a key (a word of 0) among them if EVERY; put_k() and put_v(), once each
+// for tiles with a key (with one tile: V_FIRST or not), bring the tiles to LDS and ask for the next.
+template <class T, int D, bool EVERY, bool V_FIRST, class Body>
 __device__ __forceinline__ void cross_few_walk(const CrossCall& a, const CrossItem& it, char* tk, char* tv, int w, int l, Body&& body) {
     const HeadBuf kh = HeadBuf::of<T, D>(a.k, it.b, it.g, a.Lk), vh = HeadBuf::of<T, D>(a.v, it.b, it.g, a.Lk);
     const int tiles = (a.Lk + 31) / 32, step = 4 * a.splits;
@@ -537,10 +529,13 @@ __device__ __forceinline__ void cross_few_walk(const CrossCall& a, const CrossIt
         if (tile >= tiles) return 0u;
         return a.mask ? (unsigned)__ballot(asked != 0) : tail_word(a.Lk - tile * 32);
     };
-    TileInFlight<T, D> fk, fv;
+    // With one tile (ONE) the tensors take turns: what is put second is asked for when the first one has been put, so that one of them is in flight.
+    constexpr bool ONE = cross_own_tiles<T, D>() == 1;
+    TileInFlight<T, D> fk, other;
+    TileInFlight<T, D>& fv = ONE ? fk : other;
     auto fetch = [&](int tile) __attribute__((always_inline)) {
-        fk.load(kh, tile * 32, l);
-        fv.load(vh, tile * 32, l);
+        if (!ONE || !V_FIRST) fk.load(kh, tile * 32, l);
+        if (!ONE || V_FIRST) fv.load(vh, tile * 32, l);
     };
     int tile = 4 * it.split + w;
     unsigned asked = ask(tile), next = ask(tile + step), word = word_of(tile, asked);
@@ -549,14 +544,24 @@ __device__ __forceinline__ void cross_few_walk(const CrossCall& a, const CrossIt
         const unsigned now = word;
         word = word_of(tile + step, next);
         next = ask(tile + 2 * step);
-        if (now) {
+        auto put_k = [&]() __attribute__((always_inline)) {
             wave_lds_order();
             fk.store(tk, now, l);
+            wave_lds_order();
+            if (ONE && !V_FIRST) fv.load(vh, tile * 32, l);
+            else if (word && ONE) fv.load(vh, (tile + step) * 32, l);
+            else if (word) fk.load(kh, (tile + step) * 32, l);
+        };
+        auto put_v = [&]() __attribute__((always_inline)) {
+            wave_lds_order();
             fv.store(tv, now, l);
             wave_lds_order();
-        }
-        if (word) fetch(tile + step);
-        if (EVERY || now) body(tile * 32, now);
+            if (ONE && V_FIRST) fk.load(kh, tile * 32, l);
+            else if (word && ONE) fk.load(kh, (tile + step) * 32, l);
+            else if (word) fv.load(vh, (tile + step) * 32, l);
+        };
+        if (!now && word) fetch(tile + step);
+        if (EVERY || now) body(tile * 32, now, put_k, put_v);
     }
 }
 
@@ -570,12 +575,15 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_for
     const int q0 = it.strip * 32;
     const typename TL::Row q = TL::load(a.row(a.q, it.b, it.g, min(q0 + li, a.rows - 1)), h, q0 + li < a.rows);
     const typename TL::At at = TL::at(l);
-    char* tk = lds + w * 2 * TL::BYTES;
-    char* tv = tk + TL::BYTES;
+    constexpr int TILES = cross_own_tiles<T, D>();
+    char* tk = lds + w * TILES * TL::BYTES;
+    char* tv = tk + (TILES - 1) * TL::BYTES;
     const float c2 = a.scale * LOG2E;
     q.settled();
     CrossSoftmax<T, D> x;
-    cross_few_walk<T, D, false>(a, it, tk, tv, w, l, [&](int, unsigned word) __attribute__((always_inline)) {
+    cross_few_walk<T, D, false, false>(a, it, tk, tv, w, l, [&](int, unsigned word, auto&& put_k, auto&& put_v) __attribute__((always_inline)) {
+        put_k();
+        if (TILES == 2) put_v();
         const typename TL::Row kr = TL::rows(tk, at);
         typename TL::Columns vt;
         if (TL::EARLY) vt = TL::columns(tv, at);
@@ -585,6 +593,7 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_for
         x.raise(s, words, c2, h);
         float p[16];
         x.weights(s[0], c2, -x.base(), p);
+        if (TILES == 1) put_v();
         if (!TL::EARLY) vt = TL::columns(tv, at);
         cross_add_fine<TL>(vt, p, x.o);
     });
@@ -737,7 +746,10 @@ __device__ __forceinline__ void cross_ds(const f32x16& s, const f32x16& dp, floa
     }
 }
 
-template <class T, int D>
+// FINE (bf16): dS in two bf16 numbers (cross_add_fine).  D = dO . O, of an O that is rounded, is the further off against dP - D the fewer keys there are,
+// and with dS rounded too the gradients of a call of few keys are half as far off again as their own rounding (100 keys, d = 64: 0.0026 and
+// 0.0017; so 0.0020).
+template <class T, int D, bool FINE>
 __global__ __launch_bounds__(256, (cross_row_waves<T, D>())) void cross_backward_row_kernel(CrossCall a) {
     typedef BiasTile<T, D> TL;
     typedef CrossStage<T, D> ST;
@@ -784,7 +796,8 @@ __global__ __launch_bounds__(256, (cross_row_waves<T, D>())) void cross_backward
                 float ds[16];
                 cross_ds(s, dp, c2, minus_lse, word[u], h, ds);
                 if (!TL::EARLY || D == 128) kt = TL::columns(tk, at);
-                TL::add_t(kt, ds, dq);
+                if constexpr (FINE) cross_add_fine<TL>(kt, ds, dq);
+                else TL::add_t(kt, ds, dq);
             }
         });
     __syncthreads();  // the stages are done with
@@ -797,6 +810,36 @@ __global__ __launch_bounds__(256, (cross_row_waves<T, D>())) void cross_backward
     });
 }
 
+// A wavefront's tile of rows of Q or dO on its way to LDS (TileInFlight, which has the rows of one head).
+template <class T, int D>
+struct RowsInFlight {
+    typedef BiasTile<T, D> TL;
+    PieceInFlight<T> x[TL::CPR / 2];
+    template <class S>
+    __device__ __forceinline__ void load(const S& from, int first, int l) {
+#pragma unroll
+        for (int i = 0; i < TL::CPR / 2; ++i) x[i].load(from.r, from.at(first, (64 * i + l) / TL::CPR, 8 * (l % TL::CPR) * (int)sizeof(T)));
+    }
+    __device__ __forceinline__ void store(char* tile, unsigned word, int l) const {
+#pragma unroll
+        for (int i = 0; i < TL::CPR / 2; ++i) x[i].template store<D, false>(tile, (64 * i + l) / TL::CPR, l % TL::CPR, (word >> ((64 * i + l) / TL::CPR)) & 1u);
+    }
+};
+
+// Where the operands of 32 rows of their own are too many registers (fp32, 128 features: 192), a work-group's wavefronts read them from two tiles that
+// they share.
+template <class T, int D>
+constexpr int cross_shared_bytes() { return cross_own_tiles<T, D>() == 1 ? 2 * BiasTile<T, D>::BYTES : 0; }
+template <class T, int D, class S>
+__device__ __forceinline__ void cross_share(char* tiles, const S& xs, const S& ys, int first, int rows, int w, int l) {
+    if (w < 2) {
+        RowsInFlight<T, D> x;
+        x.load(w ? ys : xs, first, l);
+        x.store(tiles + w * BiasTile<T, D>::BYTES, tail_word(rows - first), l);
+    }
+    __syncthreads();
+}
+
 // Strips of 32 rows, as in cross_forward_few_kernel.
 template <class T, int D>
 __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_row_few_kernel(CrossCall a) {
@@ -806,29 +849,48 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     const CrossItem it(a, gridDim.x);
     const int q0 = it.strip * 32, qi = min(q0 + li, a.rows - 1);
     const bool there = q0 + li < a.rows;
-    const typename TL::Row q = TL::load(a.row(a.q, it.b, it.g, qi), h, there);
-    const typename TL::Row go = TL::load(a.row(a.dout, it.b, it.g, qi), h, there);
+    constexpr int TILES = cross_own_tiles<T, D>();
+    char* const shared = lds + cross_tiles_bytes<T, D>();
+    typename TL::Row q, go = TL::load(a.row(a.dout, it.b, it.g, qi), h, there);
     const size_t stat = (size_t)it.bg * a.rows + qi;
     const float minus_lse = there ? -a.lse[stat] : -__builtin_inff();
     const float delta = half_swap_sum(TL::dot(go, TL::load(a.row(a.o, it.b, it.g, qi), h, there)));
     if (it.split == 0 && tid < 32 && there) a.delta[stat] = delta;
     const typename TL::At at = TL::at(l);
-    char* tk = lds + w * 2 * TL::BYTES;
-    char* tv = tk + TL::BYTES;
+    char* tk = lds + w * TILES * TL::BYTES;
+    char* tv = tk + (TILES - 1) * TL::BYTES;
     const float c2 = a.scale * LOG2E;
     const f32x16 minus = splat16(-delta);
-    q.settled();
-    go.settled();
+    if constexpr (TILES == 1) {
+        typedef CrossSource<T, D, false> S;
+        cross_share<T, D>(shared, S(a, a.q, it.b, it.g), S(a, a.dout, it.b, it.g), q0, a.rows, w, l);
+    } else {
+        q = TL::load(a.row(a.q, it.b, it.g, qi), h, there);
+        q.settled();
+        go.settled();
+    }
     f32x16 dq[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
-    cross_few_walk<T, D, false>(a, it, tk, tv, w, l, [&](int, unsigned word) __attribute__((always_inline)) {
-        const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
+    cross_few_walk<T, D, false, true>(a, it, tk, tv, w, l, [&](int, unsigned word, auto&& put_k, auto&& put_v) __attribute__((always_inline)) {
+        f32x16 s, dp;
         typename TL::Columns kt;
-        if (TL::EARLY) kt = TL::columns(tk, at);
-        issue_order();
-        const f32x16 s = TL::feat(kr, q);
-        const f32x16 dp = TL::feat(vr, go, minus);
+        if constexpr (TILES == 1) {
+            int same = 0;  // (not so to the compiler, which would keep what the shared tiles hold in registers)
+            asm volatile("" : "+v"(same));
+            put_v();
+            dp = TL::feat(TL::rows(tv, at), TL::rows(shared + TL::BYTES + same, at), minus);
+            put_k();
+            s = TL::feat(TL::rows(tk, at), TL::rows(shared + same, at));
+        } else {
+            put_k();
+            put_v();
+            const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
+            if (TL::EARLY) kt = TL::columns(tk, at);
+            issue_order();
+            s = TL::feat(kr, q);
+            dp = TL::feat(vr, go, minus);
+        }
         float ds[16];
         cross_ds(s, dp, c2, minus_lse, word, h, ds);
         if (!TL::EARLY) kt = TL::columns(tk, at);
@@ -857,22 +919,6 @@ __global__ __launch_bounds__(256) void cross_merge_row_kernel(CrossCall a) {
     if (j.group == 0) cross_put4<T>(a.row(a.dq, bg / a.G, bg % a.G, r), j.col, x);
 }
 
-// A wavefront's tile of rows of Q or dO on its way to LDS (TileInFlight, which has the rows of one head).
-template <class T, int D>
-struct RowsInFlight {
-    typedef BiasTile<T, D> TL;
-    PieceInFlight<T> x[TL::CPR / 2];
-    template <class S>
-    __device__ __forceinline__ void load(const S& from, int first, int l) {
-#pragma unroll
-        for (int i = 0; i < TL::CPR / 2; ++i) x[i].load(from.r, from.at(first, (64 * i + l) / TL::CPR, 8 * (l % TL::CPR) * (int)sizeof(T)));
-    }
-    __device__ __forceinline__ void store(char* tile, unsigned word, int l) const {
-#pragma unroll
-        for (int i = 0; i < TL::CPR / 2; ++i) x[i].template store<D, false>(tile, (64 * i + l) / TL::CPR, l % TL::CPR, (word >> ((64 * i + l) / TL::CPR)) & 1u);
-    }
-};
-
 // -------------------------------------------------------------------------------------------------
 // Backward of few rows, in one pass over the keys
 // -------------------------------------------------------------------------------------------------
@@ -882,7 +928,7 @@ struct RowsInFlight {
 // lie in registers either way.  Every wavefront takes every fourth tile, leaves its dK and dV and keeps dQ; bound by memory.
 template <class T, int D>
 constexpr int cross_few_region() {  // a wavefront's tiles of K and V, then its results on their way out
-    const int tiles = 2 * BiasTile<T, D>::BYTES, out = 32 * (D + 4) * 4;
+    const int tiles = cross_own_tiles<T, D>() * BiasTile<T, D>::BYTES, out = 32 * (D + 4) * 4;
     return tiles > out ? tiles : out;
 }
 template <class T, int D>
@@ -891,6 +937,7 @@ constexpr int cross_few_bytes() { return 4 * cross_few_region<T, D>() + 2 * Bias
 template <class T, int D>
 __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_few_kernel(CrossCall a) {
     typedef BiasTile<T, D> TL;
+    constexpr int TILES = cross_own_tiles<T, D>();
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char* const tq = lds + 4 * cross_few_region<T, D>();
     char* const tg = tq + TL::BYTES;
@@ -914,33 +961,51 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     }
     const typename TL::At at = TL::at(l);
     char* const tk = lds + w * cross_few_region<T, D>();
-    char* const tv = tk + TL::BYTES;
+    char* const tv = tk + (TILES - 1) * TL::BYTES;
     const float c2 = a.scale * LOG2E;
     f32x16 dq[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = splat16(0.f);
     const char *const ok = a.dk.head(it.b, it.g), *const ov = a.dv.head(it.b, it.g);
     __syncthreads();  // the tiles of Q and dO, and the rows' numbers
-    cross_few_walk<T, D, true>(a, it, tk, tv, w, l, [&](int k0, unsigned word) __attribute__((always_inline)) {
+    cross_few_walk<T, D, true, true>(a, it, tk, tv, w, l, [&](int k0, unsigned word, auto&& put_k, auto&& put_v) __attribute__((always_inline)) {
         float p[16], ds[16];
         // (an offset that is not the same in every turn to the compiler, which would keep what the tiles of Q and dO hold in registers)
         int same = 0;
         asm volatile("" : "+v"(same));
         const float* const st = stats + same + 4 * h;
         if (word) {
-            cross_ds(TL::feat(TL::rows(tk, at), TL::rows(tq + same, at)), TL::feat(TL::rows(tv, at), TL::rows(tg + same, at), splat16(-delta)), c2,
-                     minus_lse, word, h, ds);
-            cross_add_fine<TL>(TL::columns(tk, at), ds, dq);
-            issue_order();
-            f32x16 dp;
+            // rows of K and V by the queries, for dQ, and the other way round, for dK and dV
+            f32x16 s, dp;
+            auto minus_d = [&]() __attribute__((always_inline)) {
+                f32x16 x;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 d = *reinterpret_cast<const f32x4*>(st + 32 + 8 * g);
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 d = *reinterpret_cast<const f32x4*>(st + 32 + 8 * g);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) dp[4 * g + j] = d[j];
+                    for (int j = 0; j < 4; ++j) x[4 * g + j] = d[j];
+                }
+                return x;
+            };
+            if constexpr (TILES == 1) {
+                put_v();
+                const f32x16 dp_t = TL::feat(TL::rows(tv, at), TL::rows(tg + same, at), splat16(-delta));
+                dp = TL::feat(TL::rows(tg + same, at), TL::rows(tv, at), minus_d());
+                put_k();
+                cross_ds(TL::feat(TL::rows(tk, at), TL::rows(tq + same, at)), dp_t, c2, minus_lse, word, h, ds);
+                cross_add_fine<TL>(TL::columns(tk, at), ds, dq);
+                issue_order();
+                s = TL::feat(TL::rows(tq + same, at), TL::rows(tk, at));
+            } else {
+                put_k();
+                put_v();
+                cross_ds(TL::feat(TL::rows(tk, at), TL::rows(tq + same, at)), TL::feat(TL::rows(tv, at), TL::rows(tg + same, at), splat16(-delta)), c2,
+                         minus_lse, word, h, ds);
+                cross_add_fine<TL>(TL::columns(tk, at), ds, dq);
+                issue_order();
+                s = TL::feat(TL::rows(tq + same, at), TL::rows(tk, at));
+                dp = TL::feat(TL::rows(tg + same, at), TL::rows(tv, at), minus_d());
             }
-            const f32x16 s = TL::feat(TL::rows(tq + same, at), TL::rows(tk, at));
-            dp = TL::feat(TL::rows(tg + same, at), TL::rows(tv, at), dp);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 e = *reinterpret_cast<const f32x4*>(st + 8 * g);
@@ -1010,7 +1075,7 @@ struct CrossRowStats {
 
 // At D = 128 dK and dV are 128 registers beside the 64 of K and V, so one wavefront a SIMD.  (In a pass each, two wavefronts a SIMD, five products for
 // four: 813 us against 767, 32 heads of 2048 x 8192.)
-template <class T, int D>
+template <class T, int D, bool FINE>
 __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_col_kernel(CrossCall a) {
     typedef BiasTile<T, D> TL;
     typedef CrossStage<T, D> ST;
@@ -1057,7 +1122,7 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
         cross_walk<T, D, false>(a, sc, it, S(a, a.q, it.b, it.g), S(a, a.dout, it.b, it.g), lds, tid, rs,
             [&](const unsigned (&word)[SUBS], const char* buf, auto which) __attribute__((always_inline)) {
                 if (!some) return;
-                if constexpr (sizeof(T) == 2 && D == 128) {
+                if constexpr (sizeof(T) == 2 && D == 128 && !FINE) {
                     if (word[SUBS - 1] != 0) {
                         // One wavefront a SIMD: two tiles, the arithmetic of each beside the products of the other.
                         const float* st = stats + 128 * which + 4 * h;
@@ -1106,7 +1171,8 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
                     if (!TL::EARLY || D == 128) gt = TL::columns(tg, at);
                     TL::add_t(gt, p, dv);
                     if (!TL::EARLY || D == 128) qt = TL::columns(tq, at);
-                    TL::add_t(qt, ds, dk);
+                    if constexpr (FINE) cross_add_fine<TL>(qt, ds, dk);
+                    else TL::add_t(qt, ds, dk);
                 }
             });
     __syncthreads();  // the stages are done with
@@ -1128,36 +1194,45 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
 
 // Strips of 32 keys, and a work-group's wavefronts take every fourth tile of the rows.
 template <class T, int D>
-constexpr int cross_col_few_bytes() { return cross_tiles_bytes<T, D>() + 4 * 64 * 4; }
+constexpr int cross_col_few_bytes() { return cross_tiles_bytes<T, D>() + cross_shared_bytes<T, D>() + 4 * 64 * 4; }
 template <class T, int D>
 __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_col_few_kernel(CrossCall a) {
     typedef BiasTile<T, D> TL;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, li = l & 31, h = l >> 5;
-    float* const stats = reinterpret_cast<float*>(lds + cross_tiles_bytes<T, D>()) + 64 * w;
+    constexpr int TILES = cross_own_tiles<T, D>();
+    char* const shared = lds + cross_tiles_bytes<T, D>();
+    float* const stats = reinterpret_cast<float*>(shared + cross_shared_bytes<T, D>()) + 64 * w;
     const CrossItem it(a, gridDim.x);
     const int k0 = it.strip * 32, ki = min(k0 + li, a.Lk - 1);
     const bool key = cross_key(a, it.b, k0 + li);
-    const typename TL::Row k = TL::load(a.k.head(it.b, it.g) + ki * a.k.row, h, k0 + li < a.Lk);
-    const typename TL::Row v = TL::load(a.v.head(it.b, it.g) + ki * a.v.row, h, k0 + li < a.Lk);
+    typename TL::Row k, v;
+    if constexpr (TILES == 1) {
+        typedef CrossSource<T, D, true> S;
+        cross_share<T, D>(shared, S(a, a.k, it.b, it.g), S(a, a.v, it.b, it.g), k0, a.Lk, w, l);
+    } else {
+        k = TL::load(a.k.head(it.b, it.g) + ki * a.k.row, h, k0 + li < a.Lk);
+        v = TL::load(a.v.head(it.b, it.g) + ki * a.v.row, h, k0 + li < a.Lk);
+        k.settled();
+        v.settled();
+    }
     const typename TL::At at = TL::at(l);
-    char* const tq = lds + w * 2 * TL::BYTES;
-    char* const tg = tq + TL::BYTES;
+    char* const tq = lds + w * TILES * TL::BYTES;
+    char* const tg = tq + (TILES - 1) * TL::BYTES;
     const float c2 = a.scale * LOG2E;
     f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = splat16(0.f);
-    k.settled();
-    v.settled();
     typedef CrossSource<T, D, false> S;
     const S qs(a, a.q, it.b, it.g), gs(a, a.dout, it.b, it.g);
     const float *lse = a.lse + (size_t)it.bg * a.rows, *delta = a.delta + (size_t)it.bg * a.rows;
     const int tiles = __any(key) ? (a.rows + 31) / 32 : 0, step = 4 * a.splits;
-    RowsInFlight<T, D> fq, fg;
+    RowsInFlight<T, D> fq, other;
+    RowsInFlight<T, D>& fg = TILES == 1 ? fq : other;  // (one tensor in flight, as in cross_few_walk)
     float e = 0.f, d = 0.f;
     auto fetch = [&](int tile) __attribute__((always_inline)) {
         fq.load(qs, tile * 32, l);
-        fg.load(gs, tile * 32, l);
+        if (TILES == 2) fg.load(gs, tile * 32, l);
         const int r = min(tile * 32 + li, a.rows - 1);
         e = lse[r], d = delta[r];
     };
@@ -1166,37 +1241,62 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
     for (; tile < tiles; tile += step) {
         const unsigned word = tail_word(a.rows - tile * 32);
         const bool there = (word >> li) & 1u;
-        wave_lds_order();
-        fq.store(tq, word, l);
-        fg.store(tg, word, l);
+        const bool more = tile + step < tiles;
+        auto put = [&](auto& rows, char* to) __attribute__((always_inline)) {
+            wave_lds_order();
+            rows.store(to, word, l);
+            wave_lds_order();
+        };
         if (l < 32) {
             stats[li] = there ? -e : -__builtin_inff();  // (rows behind the last have P = 0)
             stats[32 + li] = there ? -d : 0.f;
         }
-        wave_lds_order();
-        if (tile + step < tiles) fetch(tile + step);
-        const float* const st = stats + 4 * h;
-        f32x16 dp;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(st + 32 + 8 * g);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) dp[4 * g + j] = x[j];
+        put(fq, tq);
+        if (TILES == 2) {
+            put(fg, tg);
+            if (more) fetch(tile + step);
         }
-        const typename TL::Row qr = TL::rows(tq, at), gr = TL::rows(tg, at);
-        issue_order();
-        const f32x16 s = TL::feat(qr, k);
-        dp = TL::feat(gr, v, dp);  // dP - D
+        const float* const st = stats + 4 * h;
+        auto stat = [&](int first) __attribute__((always_inline)) {
+            f32x16 y;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(st + first + 8 * g);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[4 * g + j] = x[j];
+            }
+            return y;
+        };
+        f32x16 s, dp;
+        int same = 0;
+        asm volatile("" : "+v"(same));
+        if constexpr (TILES == 1) {
+            fg.load(gs, tile * 32, l);
+            s = TL::feat(TL::rows(tq, at), TL::rows(shared + same, at));
+            issue_order();
+            put(fg, tg);
+            fq.load(qs, tile * 32, l);  // (once more, for dK)
+            dp = TL::feat(TL::rows(tg, at), TL::rows(shared + TL::BYTES + same, at), stat(32));  // dP - D
+            issue_order();
+        } else {
+            const f32x16 minus_d = stat(32);
+            const typename TL::Row qr = TL::rows(tq, at), gr = TL::rows(tg, at);
+            issue_order();
+            s = TL::feat(qr, k);
+            dp = TL::feat(gr, v, minus_d);
+        }
+        const f32x16 minus_lse = stat(0);
         float p[16], ds[16];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(st + 8 * g);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], c2, x[j]));
+        for (int r = 0; r < 16; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, minus_lse[r]));
+            ds[r] = p[r] * dp[r];
         }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ds[r] = p[r] * dp[r];
         cross_add_fine<TL>(TL::columns(tg, at), p, dv);
+        if (TILES == 1) {
+            put(fq, tq);
+            if (more) fetch(tile + step);
+        }
         cross_add_fine<TL>(TL::columns(tq, at), ds, dk);
     }
     const unsigned keys = (unsigned)__ballot(key);
