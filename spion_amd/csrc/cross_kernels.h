@@ -484,6 +484,15 @@ __global__ __launch_bounds__(256, (cross_forward_waves<T, D>())) void cross_forw
     });
 }
 
+// what rounding to bf16 takes from p
+__device__ __forceinline__ void cross_rest(float (&p)[16]) {
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+        const unsigned hi = pack_bf16(p[r], p[r + 1]);
+        p[r] -= bf16_lo(hi);
+        p[r + 1] -= bf16_hi(hi);
+    }
+}
 // out += X^T . W of bf16 tiles with W as the sum of two bf16 numbers (fp32: of three, as everywhere).  Calls of few rows wait for memory, so that
 // the second product and its 40 vector instructions cost nothing there (one token over 2048 keys 8.6 us with either), and the
 // rounding of the weights is gone from their results: errors of 0.0017, that of the result's own rounding, against 0.0025.
@@ -493,11 +502,8 @@ __device__ __forceinline__ void cross_add_fine(const Columns& xt, const float (&
     if constexpr (TL::IM == 1) {
         float rest[16];
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            const unsigned hi = pack_bf16(p[r], p[r + 1]);
-            rest[r] = p[r] - bf16_lo(hi);
-            rest[r + 1] = p[r + 1] - bf16_hi(hi);
-        }
+        for (int r = 0; r < 16; ++r) rest[r] = p[r];
+        cross_rest(rest);
         TL::add_t(xt, rest, out);
     }
 }
@@ -1073,10 +1079,45 @@ struct CrossRowStats {
     }
 };
 
-// At D = 128 dK and dV are 128 registers beside the 64 of K and V, so one wavefront a SIMD.  (In a pass each, two wavefronts a SIMD, five products for
-// four: 813 us against 767, 32 heads of 2048 x 8192.)
+// The column pass's products with a tile of the stage, whose operands are read as they are needed: `row`, `col` are the lane's places for the first
+// 16 features of a row and the first 32 columns, from which the others differ in bits, and are made anew each time (kept, they would be
+// 24 registers at D = 128).
+template <int D>
+__device__ __forceinline__ f32x16 cross_feat(const char* t, int row, const typename BiasTile<__bf16, D>::Row& b, f32x16 acc) {
+    asm volatile("" : "+v"(row));
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) acc = mfma_bf16(__builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(t + (row ^ 16 * i))), b.x[0][i], acc);
+    return acc;
+}
+template <int D, bool FINE>
+__device__ __forceinline__ void cross_add_t(const char* t, const int (&col)[2], float (&p)[16], f32x16 (&out)[D / 32]) {
+    typedef s16x4 __attribute__((address_space(3))) * lds_ptr;
+    int at[2] = {col[0], col[1]};
+    asm volatile("" : "+v"(at[0]), "+v"(at[1]));
+    bf16x8 w[2], rest[2];
+    pack16(p, w);
+    if (FINE) {
+        cross_rest(p);
+        pack16(p, rest);
+    }
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + (at[0] ^ 64 * c) + 16 * i * BiasTile<__bf16, D>::ROW));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(t + (at[1] ^ 64 * c) + 16 * i * BiasTile<__bf16, D>::ROW));
+            const bf16x8 x = __builtin_shufflevector(__builtin_bit_cast(bf16x4, lo), __builtin_bit_cast(bf16x4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
+            out[c] = mfma_bf16(x, w[i], out[c]);
+            if (FINE) out[c] = mfma_bf16(x, rest[i], out[c]);
+        }
+}
+// Wavefronts a SIMD.  Of bf16, D = 128, dK and dV are 128 registers beside the 64 of K and V; what is left of 256 is enough if nothing else is kept
+// (2 x 16 heads over 4 of 2048 x 8192: 711 us with one wavefront and operands read ahead, 556 with two).  D = 64: 256 heads of 2048 x 2048 take 705 us
+// with two, 656 with three.
+template <class T, int D>
+constexpr int cross_col_waves() { return sizeof(T) == 2 ? (D == 32 ? 4 : D == 64 ? 3 : 2) : D == 32 ? 2 : 1; }
 template <class T, int D, bool FINE>
-__global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_backward_col_kernel(CrossCall a) {
+__global__ __launch_bounds__(256, (cross_col_waves<T, D>())) void cross_backward_col_kernel(CrossCall a) {
     typedef BiasTile<T, D> TL;
     typedef CrossStage<T, D> ST;
     constexpr int SUBS = ST::SUBS;
@@ -1109,70 +1150,47 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
         }
         return x;
     };
-    auto weights = [&](const f32x16& s, const f32x16& dp, const f32x16& e, float (&p)[16], float (&ds)[16]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, e[r]));
-            ds[r] = p[r] * dp[r];
-        }
-    };
     if (l == 0) sc.seg[w] = some;
     __syncthreads();
     if (sc.seg[0] | sc.seg[1] | sc.seg[2] | sc.seg[3])
         cross_walk<T, D, false>(a, sc, it, S(a, a.q, it.b, it.g), S(a, a.dout, it.b, it.g), lds, tid, rs,
             [&](const unsigned (&word)[SUBS], const char* buf, auto which) __attribute__((always_inline)) {
                 if (!some) return;
-                if constexpr (sizeof(T) == 2 && D == 128 && !FINE) {
-                    if (word[SUBS - 1] != 0) {
-                        // One wavefront a SIMD: two tiles, the arithmetic of each beside the products of the other.
-                        const float* st = stats + 128 * which + 4 * h;
-                        const typename TL::Row q0 = TL::rows(buf, at), g0 = TL::rows(buf + SUBS * TL::BYTES, at);
-                        const f32x16 d0 = stat(st + 64);
-                        issue_order();
-                        const f32x16 s0 = TL::feat(q0, k), dp0 = TL::feat(g0, v, d0);
-                        const typename TL::Row q1 = TL::rows(buf + TL::BYTES, at), g1 = TL::rows(buf + (SUBS + 1) * TL::BYTES, at);
-                        const f32x16 d1 = stat(st + 96);
-                        read_behind_products<D / 8, 2>();
-                        issue_order();
-                        float p0[16], ds0[16], p1[16], ds1[16];
-                        const f32x16 s1 = TL::feat(q1, k), dp1 = TL::feat(g1, v, d1);
-                        weights(s0, dp0, stat(st), p0, ds0);
-                        const typename TL::Columns gt0 = TL::columns(buf + SUBS * TL::BYTES, at), qt0 = TL::columns(buf, at);
-                        issue_order();
-                        TL::add_t(gt0, p0, dv);
-                        TL::add_t(qt0, ds0, dk);
-                        weights(s1, dp1, stat(st + 32), p1, ds1);
-                        const typename TL::Columns gt1 = TL::columns(buf + (SUBS + 1) * TL::BYTES, at), qt1 = TL::columns(buf + TL::BYTES, at);
-                        issue_order();
-                        TL::add_t(gt1, p1, dv);
-                        TL::add_t(qt1, ds1, dk);
-                        return;
-                    }
-                }
 #pragma unroll
                 for (int u = 0; u < SUBS; ++u) {
                     if (word[u] == 0) continue;
                     const char *tq = buf + u * TL::BYTES, *tg = buf + (SUBS + u) * TL::BYTES;
                     const float* st = stats + 128 * which + 32 * u + 4 * h;
-                    const f32x16 d = stat(st + 64);
-                    const typename TL::Row qr = TL::rows(tq, at), gr = TL::rows(tg, at);
-                    typename TL::Columns qt, gt;
-                    if (D < 128) issue_order();
-                    const f32x16 s = TL::feat(qr, k);
-                    if (D == 128) issue_order();
-                    const f32x16 dp = TL::feat(gr, v, d);  // dP - D
-                    if (D == 128) issue_order();
-                    if (TL::EARLY && D < 128) {
-                        gt = TL::columns(tg, at), qt = TL::columns(tq, at);
-                        read_behind_products<D / 8, 2 * D / 8>();
+                    float x[16];  // P, then dS
+                    if constexpr (sizeof(T) == 2) {
+                        issue_order();
+                        const f32x16 s = cross_feat<D>(tq, at.row[0], k, splat16(0.f));
+                        issue_order();
+                        const f32x16 e = stat(st);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, e[r]));
+                        issue_order();
+                        cross_add_t<D, false>(tg, at.col[0], x, dv);
+                        issue_order();
+                        const f32x16 dp = cross_feat<D>(tg, at.row[0], v, stat(st + 64));  // dP - D
+                        issue_order();
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[r] *= dp[r];
+                        cross_add_t<D, FINE>(tq, at.col[0], x, dk);
+                        issue_order();
+                    } else {
+                        const f32x16 s = TL::feat(TL::rows(tq, at), k);
+                        if (D == 128) issue_order();
+                        const f32x16 dp = TL::feat(TL::rows(tg, at), v, stat(st + 64));
+                        if (D == 128) issue_order();
+                        const f32x16 e = stat(st);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c2, e[r]));
+                        TL::add_t(TL::columns(tg, at), x, dv);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[r] *= dp[r];
+                        TL::add_t(TL::columns(tq, at), x, dk);
                     }
-                    float p[16], ds[16];
-                    weights(s, dp, stat(st), p, ds);
-                    if (!TL::EARLY || D == 128) gt = TL::columns(tg, at);
-                    TL::add_t(gt, p, dv);
-                    if (!TL::EARLY || D == 128) qt = TL::columns(tq, at);
-                    if constexpr (FINE) cross_add_fine<TL>(qt, ds, dk);
-                    else TL::add_t(qt, ds, dk);
                 }
             });
     __syncthreads();  // the stages are done with
