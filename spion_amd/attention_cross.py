@@ -205,10 +205,11 @@ class _FusedKV(torch.autograd.Function):
             g2 = torch.as_strided(dk, (B * L, 2 * n), (2 * n, 1))
         else:
             g2 = torch.stack([g.transpose(1, 2) for g in (dk, dv)], 2).reshape(B * L, 2 * n)
-        dX = (g2 @ w).view(B, L, dim) if ctx.needs_input_grad[0] else None
-        dW = g2.t() @ X2
-        db = g2.sum(0)
-        return dX, dW[:n], dW[n:], db[:n], db[n:], None, None
+        needs = ctx.needs_input_grad
+        dX = (g2 @ w).view(B, L, dim) if needs[0] else None
+        dW = (g2.t() @ X2).split(n) if needs[1] or needs[2] else (None, None)
+        db = g2.sum(0).split(n) if needs[3] or needs[4] else (None, None)
+        return dX, *dW, *db, None, None
 
 
 class CrossAttention(nn.Module):

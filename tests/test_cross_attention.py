@@ -150,3 +150,22 @@ def test_the_layer_refuses_what_its_core_does_not_take():
     for change in (dict(num_key_head=3), dict(num_key_head=0), dict(num_key_head=8), dict(head_dim=48)):
         with pytest.raises(ValueError):
             spion_amd.CrossAttention({**ok, **change})
+
+
+@pytest.mark.parametrize("frozen", [(), (1, 2), (3, 4), (0,)])
+def test_projections_of_keys_and_values_as_one(frozen):
+    """The product of the stacked weights against the two products, in 64 bits; inputs without a gradient get none."""
+    from spion_amd.attention_cross import _FusedKV
+
+    g = torch.Generator().manual_seed(3)
+    B, L, dim, G, d = 2, 5, 7, 3, 4
+    states, wk, wv, bk, bv = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((B, L, dim), (G * d, dim), (G * d, dim), (G * d,), (G * d,)))
+    ins = [t.requires_grad_(i not in frozen) for i, t in enumerate((states, wk, wv, bk, bv))]
+    want = [(states @ w.t() + b).view(B, L, G, d).transpose(1, 2) for w, b in ((wk, bk), (wv, bv))]
+    got = _FusedKV.apply(*ins, G, d)
+    grads = [torch.randn(t.shape, generator=g, dtype=torch.float64) for t in want]
+    leaves = [t for t in ins if t.requires_grad]
+    for a, b in zip(got, want):
+        assert torch.allclose(a, b, atol=1e-12)
+    for a, b in zip(torch.autograd.grad(got, leaves, grads), torch.autograd.grad(want, leaves, grads)):
+        assert torch.allclose(a, b, atol=1e-12)
