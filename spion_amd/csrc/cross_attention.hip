@@ -25,16 +25,17 @@ struct CrossWalk {
 // All rows of a group in one strip of 32: the backward is one pass over the keys.
 static bool cross_one_strip(const Cross& c) { return rows_of(c) <= 32; }
 
-// Which, by an estimate of the launch's time, us.  A CU's work-groups share it: it takes as long for them as for one after the other, within a
-// fifth (bf16, d = 64: 0.49 us a tile of 32 keys and 128 rows alone, 0.41 with four of them).  So a launch takes the most work-groups that a CU
-// has, times a piece's tiles, times what a tile (strips of 32: four tiles, one to a wavefront) takes, measured with one work-group to
-// a CU in the forward; the row pass takes 1.3 times, the column pass 1.75 times that.  All rows in one strip: K and V come from memory
+// Which, by an estimate of the launch's time, us.  A CU's work-groups share it: a launch takes the most work-groups that a CU has, times a piece's
+// tiles, times what a tile (strips of 32: four tiles, one to a wavefront) takes, measured with one work-group to a CU in the forward; the row
+// pass takes 1.3 times, the column pass 1.75 times that; and where the registers of two fit a CU, several take 0.8 of that (bf16, d = 64: 0.49 us
+// a tile of 32 keys and 128 rows alone, 0.41 with four of them; 64 fp32 heads of 16 rows, 4096 padded keys, d = 32, training: 66 us in four pieces
+// each, 57 in eight).  All rows in one strip: K and V come from memory
 // once, at 20 bytes a ns to a CU.  Pieces cost a second launch, and their sums are written and read at some 4 TB/s.
 //   us, forward, one launch / its best cut in strips of 128, strips of 32:  64 heads of 512 x 512, bf16, d = 64: 14 / 22, 17;  32 of 256 x 256: 9 / 14, 7
 //   16 of 1024 x 4096: 63 / 37, 41;  d = 128 97 / 60, 93;  fp32 199 / 96, 159;  64 of 256 x 1024, fp32, d = 32: 35 / 25, 23
 // At most eight work-groups to a CU where there are pieces, so the workspace is bounded.
 static double cross_tile_us(const Cross& c, CrossPass pass, bool few) {
-    static const double wide_us[2][3] = {{0.85, 1.5, 3.2}, {0.25, 0.45, 0.75}}, few_us[2][3] = {{1.05, 2.4, 6.}, {0.4, 0.6, 1.35}};
+    static const double wide_us[2][3] = {{0.85, 1.5, 3.2}, {0.25, 0.45, 0.75}}, few_us[2][3] = {{1.15, 2.4, 6.}, {0.4, 0.6, 1.35}};
     const int d = c.head_dim == 32 ? 0 : c.head_dim == 64 ? 1 : 2, bf16 = c.bf16 ? 1 : 0;
     const double us = (few ? few_us : wide_us)[bf16][d] * (pass == CrossPass::FORWARD ? 1. : pass == CrossPass::ROW ? 1.3 : 1.75);
     return few && pass != CrossPass::COL && cross_one_strip(c) ? std::max(us, 4 * 64 * c.head_dim * (c.bf16 ? 2 : 4) / 20e3) : us;
@@ -49,9 +50,10 @@ static CrossWalk cross_walk_of(const Cross& c, CrossPass pass, bool can_split) {
         const int rows = few ? 32 : 128, unit = few ? 1 : 2;
         const long long strips = tiles_of(own, rows), steps = tiles_of(tiles, few ? 4 : unit);
         const double us = cross_tile_us(c, pass, few) * (few ? 1 : unit);
+        const bool two = c.bf16 ? !few || c.head_dim < 128 : c.head_dim == 32;  // (two work-groups' registers fit a CU)
         for (long long n = 1; n == 1 || (can_split && n <= std::min(steps / 2, 64LL) && groups * strips * n <= 8 * cus); ++n) {
             const long long rounds = tiles_of(groups * strips * n, cus), each = tiles_of(steps, n);
-            double cost = 3 + rounds * each * us;
+            double cost = 3 + rounds * each * us * (rounds > 1 && two ? 0.8 : 1.);
             if (n > 1) cost += 3 + (pass == CrossPass::COL ? 2 : 1) * groups * own * n * c.head_dim * 8 / 4e6;
             if (w.rows && cost >= least) continue;
             least = cost;

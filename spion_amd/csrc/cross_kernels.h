@@ -519,8 +519,8 @@ constexpr int cross_tiles_bytes() {
 }
 // Wavefront w of piece s has tiles 4 s + w, 4 (s + splits) + w, ...: what padding leaves is dealt evenly (in ranges of tiles, a piece could have
 // none).  It makes the words of its tiles itself, from mask values that were asked for two tiles ahead; K and V are one tile ahead.
-// body(tile's first key, word, put_k, put_v): for all tiles, those without a key (a word of 0) among them if EVERY; put_k() and put_v(), once each
-// for tiles with a key (with one tile: V_FIRST or not), bring the tiles to LDS and ask for the next.
+// body(tile's first key, word, put_k, put_v): for all tiles, those without a key (a word of 0) among them if EVERY; put_k(), once for tiles with a
+// key, brings K and V to LDS and asks for the next; with one tile it brings K, and put_v(), which comes first or not (V_FIRST), V.
 template <class T, int D, bool EVERY, bool V_FIRST, class Body>
 __device__ __forceinline__ void cross_few_walk(const CrossCall& a, const CrossItem& it, char* tk, char* tv, int w, int l, Body&& body) {
     const HeadBuf kh = HeadBuf::of<T, D>(a.k, it.b, it.g, a.Lk), vh = HeadBuf::of<T, D>(a.v, it.b, it.g, a.Lk);
@@ -553,18 +553,18 @@ __device__ __forceinline__ void cross_few_walk(const CrossCall& a, const CrossIt
         auto put_k = [&]() __attribute__((always_inline)) {
             wave_lds_order();
             fk.store(tk, now, l);
+            if (!ONE) fv.store(tv, now, l);
             wave_lds_order();
             if (ONE && !V_FIRST) fv.load(vh, tile * 32, l);
             else if (word && ONE) fv.load(vh, (tile + step) * 32, l);
-            else if (word) fk.load(kh, (tile + step) * 32, l);
+            else if (word) fetch(tile + step);
         };
-        auto put_v = [&]() __attribute__((always_inline)) {
+        auto put_v = [&]() __attribute__((always_inline)) {  // (ONE)
             wave_lds_order();
             fv.store(tv, now, l);
             wave_lds_order();
-            if (ONE && V_FIRST) fk.load(kh, tile * 32, l);
-            else if (word && ONE) fk.load(kh, (tile + step) * 32, l);
-            else if (word) fv.load(vh, (tile + step) * 32, l);
+            if (V_FIRST) fk.load(kh, tile * 32, l);
+            else if (word) fk.load(kh, (tile + step) * 32, l);
         };
         if (!now && word) fetch(tile + step);
         if (EVERY || now) body(tile * 32, now, put_k, put_v);
@@ -589,7 +589,6 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_for
     CrossSoftmax<T, D> x;
     cross_few_walk<T, D, false, false>(a, it, tk, tv, w, l, [&](int, unsigned word, auto&& put_k, auto&& put_v) __attribute__((always_inline)) {
         put_k();
-        if (TILES == 2) put_v();
         const typename TL::Row kr = TL::rows(tk, at);
         typename TL::Columns vt;
         if (TL::EARLY) vt = TL::columns(tv, at);
@@ -890,7 +889,6 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
             s = TL::feat(TL::rows(tk, at), TL::rows(shared + same, at));
         } else {
             put_k();
-            put_v();
             const typename TL::Row kr = TL::rows(tk, at), vr = TL::rows(tv, at);
             if (TL::EARLY) kt = TL::columns(tk, at);
             issue_order();
@@ -929,7 +927,7 @@ __global__ __launch_bounds__(256) void cross_merge_row_kernel(CrossCall a) {
 // Backward of few rows, in one pass over the keys
 // -------------------------------------------------------------------------------------------------
 // All rows of a group in one strip of 32: a tile's dK and dV are then whole after its own products, and K and V are read once for
-// all three gradients (the two passes read them twice: 64 fp32 heads of 4096 padded keys, 16 rows, d = 32: 61 us, this one 30).  dQ wants the
+// all three gradients (the two passes read them twice: 64 fp32 heads of 4096 padded keys, 16 rows, d = 32: the training step 82 us, so 66).  dQ wants the
 // rows as lanes and dK, dV the keys, so both products over the head dimension are formed twice, with their operands exchanged: they
 // lie in registers either way.  Every wavefront takes every fourth tile, leaves its dK and dV and keeps dQ; bound by memory.
 template <class T, int D>
@@ -1004,7 +1002,6 @@ __global__ __launch_bounds__(256, (cross_backward_waves<T, D>())) void cross_bac
                 s = TL::feat(TL::rows(tq + same, at), TL::rows(tk, at));
             } else {
                 put_k();
-                put_v();
                 cross_ds(TL::feat(TL::rows(tk, at), TL::rows(tq + same, at)), TL::feat(TL::rows(tv, at), TL::rows(tg + same, at), splat16(-delta)), c2,
                          minus_lse, word, h, ds);
                 cross_add_fine<TL>(TL::columns(tk, at), ds, dq);
