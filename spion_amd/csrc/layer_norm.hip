@@ -9,7 +9,9 @@
 // only what is left of a row behind its last whole piece goes element by element.  The backward forms mu and s again (8 bytes a row
 // less to keep) in two reductions of two sums each.  Rows longer than the registers are read again for each step (from L2).  Statistics
 // and sums are fp32.  Work-groups walk several rows each: the weight is read once, and the backward leaves one partial dw and db a
-// work-group, which a second launch adds up in a fixed order.
+// work-group, which a second launch adds up in a fixed order.  With a residual, us (bytes moved to the time, TB/s): 262144 x 64 fp32 forward 44
+// (6.1, part of it from the cache), backward 45 + 4 for dw and db; 8192 x 4096 bf16 47 (5.7) and 61 + 9; 16384 x 1001 bf16, forward alone,
+// 17 (3.9); one row of 768 3.3, the launch.
 #include "common.h"
 #include "tile_ops.h"
 #include "../../include/spion_hip.h"
@@ -509,13 +511,14 @@ __global__ __launch_bounds__(1024) void layer_norm_weight_kernel(const float* __
 // ---------------------------------------------------------------------------------------------------------------------
 typedef spion_layer_norm LayerNorm;
 
-// Lanes to a row and pieces to a lane: the fewest lanes whose registers hold it.  (bf16 rows past 16384 would spill in the backward, with
+// Lanes to a row and pieces to a lane: the fewest lanes whose registers hold it.  (Three pieces beside two and four, bf16, a step: 16352 x 1026 85 us
+// without, 74 with them; 14475 x 1159 70 and 60; 2653 x 5000 70 and 64.  bf16 rows past 16384 would spill in the backward, with
 // six tensors' pieces of eight floats.)
 struct RowShape {
     int lanes, pieces;  // 0: longer than the registers of a work-group
 };
 static RowShape row_shape(const LayerNorm& c, bool backward) {
-    static const RowShape of[] = {{8, 1}, {16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}};
+    static const RowShape of[] = {{8, 1}, {16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 3}, {64, 4}, {256, 2}, {256, 3}, {256, 4}, {1024, 2}, {1024, 4}};
     for (const RowShape& s : of)
         if (c.width <= (long long)s.lanes * s.pieces * (c.bf16 ? 8 : 4) && !(backward && c.bf16 && s.lanes == 1024 && s.pieces == 4)) return s;
     return {0, 0};
@@ -559,8 +562,10 @@ static bool run_layer_norm(const LayerNorm& c, bool backward, hipStream_t stream
         case 16 * 8 + 2: ok = run_rows<T, 16, 2>(a, backward, groups, stream); break;
         case 64 * 8 + 1: ok = run_rows<T, 64, 1>(a, backward, groups, stream); break;
         case 64 * 8 + 2: ok = run_rows<T, 64, 2>(a, backward, groups, stream); break;
+        case 64 * 8 + 3: ok = run_rows<T, 64, 3>(a, backward, groups, stream); break;
         case 64 * 8 + 4: ok = run_rows<T, 64, 4>(a, backward, groups, stream); break;
         case 256 * 8 + 2: ok = run_rows<T, 256, 2>(a, backward, groups, stream); break;
+        case 256 * 8 + 3: ok = run_rows<T, 256, 3>(a, backward, groups, stream); break;
         case 256 * 8 + 4: ok = run_rows<T, 256, 4>(a, backward, groups, stream); break;
         case 1024 * 8 + 2: ok = run_rows<T, 1024, 2>(a, backward, groups, stream); break;
         case 1024 * 8 + 4: ok = run_rows<T, 1024, 4>(a, backward, groups, stream); break;
