@@ -315,3 +315,11 @@ def test_rows_wider_than_a_launch_has_threads_for():
     assert float((dx.double() - want).abs().max()) <= 64 * U
     assert float((dw.double() - (G * xh).sum(0)).abs().max()) <= 64 * U
     assert torch.equal(db.double(), G.sum(0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [769, 1026, 1159, 1535, 1536, 1537, 2500, 3071, 3073, 5000, 6143, 6144, 6145])
+def test_three_pieces_a_lane(n, dtype):
+    x, w, b, res, dy, dh = _inputs(n, (300, n), dtype)
+    _check(x, w, b, res, dy, dh, *_train(x, w, b, res, dy, dh))
+    _check(x, w, None, None, dy, None, *_train(x, w, None, None, dy, None))
