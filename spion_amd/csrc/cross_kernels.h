@@ -7,6 +7,9 @@
 // r % Lq of its head r / Lq.  K and V of a group are then read once for all of them, a single token of four heads is four rows of
 // one strip, and dK and dV are summed over the group by the products themselves.
 // P is never written: the forward leaves lse, and the backward, in a pass over rows (dQ) and one over keys (dK, dV), forms P again.
+// Long calls are bound by issue and power (matrix units 41 to 48 % busy at 1.9 GHz; TFLOP/s of forward / rows / keys, bf16: d = 32 530 / 740 / 735, d = 64
+// 755 / 910 / 862, d = 128 940 / 1080 / 950; fp32, six bf16 products counted as one: 163 to 197), calls of few rows by memory (one token of
+// 4 x 16 heads over 4, 32768 keys, d = 128: 268 MB in 46 us), small ones by the latency of a strip: some 0.5 us a step, 2 to 3 us to start and end.
 #pragma once
 #include "bias_tile.h"
 
@@ -270,7 +273,7 @@ __device__ __forceinline__ void cross_walk(const CrossCall& a, CrossLds& sc, con
         const int n = listed ? cross_scan<ST::SUBS>(a, sc, it.b, first, count, tid) : (count + ST::SUBS - 1) / ST::SUBS;
         ST st;
         // A stage's place and words are read from the list while the one two before it is worked on: read where they are needed, they cost a padded
-        // call a third of its time (128 heads of 1024 x 2048, three quarters of the keys: forward 90 us, and 88 of all of them).
+        // call a tenth of its time (128 heads of 1024 x 2048, three quarters of the keys: forward 90 us, so 82).
         struct Entry {
             int unit;
             unsigned word[ST::SUBS];

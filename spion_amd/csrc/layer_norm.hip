@@ -11,7 +11,7 @@
 // and sums are fp32.  Work-groups walk several rows each: the weight is read once, and the backward leaves one partial dw and db a
 // work-group, which a second launch adds up in a fixed order.  With a residual, us (bytes moved to the time, TB/s): 262144 x 64 fp32 forward 44
 // (6.1, part of it from the cache), backward 45 + 4 for dw and db; 8192 x 4096 bf16 47 (5.7) and 61 + 9; 16384 x 1001 bf16, forward alone,
-// 17 (3.9); one row of 768 3.3, the launch.
+// 17 (3.9); one row of 768 2.8, the launch.
 #include "common.h"
 #include "tile_ops.h"
 #include "../../include/spion_hip.h"
