@@ -255,11 +255,13 @@ class CrossAttention(nn.Module):
     def attend(self, X, keys_values, mask=None):
         if self.norm is not None:  # (fp16 rows, as autocast leaves them, in fp32: what follows casts for itself)
             X = self.norm(X.float() if X.dtype == torch.float16 else X)
-        heads = (self._split(self.W_q(X), self.num_head), *keys_values)
+        q = self._split(self.W_q(X), self.num_head)
+        heads = (q, *keys_values)
         if any(t.dtype == torch.float16 for t in heads):
             heads = tuple(t.float() for t in heads)
+        # kept on the other side of autocast: the queries, which are the shorter, come to the type of the keys, and the output goes back
         with torch.autocast(device_type=X.device.type, enabled=False):
-            out = cross_attention(*heads, mask)
+            out = cross_attention(heads[0].to(heads[1].dtype), *heads[1:], mask).to(q.dtype)
         return self.ff(out.transpose(1, 2).reshape(X.shape[0], X.shape[1], self.num_head * self.head_dim))
 
     def forward(self, X, states, mask=None):

@@ -1,0 +1,68 @@
+"""What the layer around the attention to an encoder's states hands to its core, without a GPU: the core is stated in torch's
+operations here, and takes one type of heads as the kernels do."""
+import pytest
+import torch
+
+import spion_amd
+from spion_amd import attention_cross as ac
+
+
+@pytest.fixture
+def core(monkeypatch):
+    """The types of the heads that the core was given, call by call."""
+    seen = []
+
+    def plain(query, key, value, key_mask=None):
+        if not query.dtype == key.dtype == value.dtype:
+            raise TypeError("heads of one type expected")
+        if query.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("fp32 or bf16 heads expected")
+        seen.append(query.dtype)
+        n = query.shape[1] // key.shape[1]
+        q, k, v = query.double(), key.double().repeat_interleave(n, 1), value.double().repeat_interleave(n, 1)
+        t = q @ k.transpose(-1, -2) / q.shape[-1] ** 0.5
+        if key_mask is not None:
+            t = t.masked_fill((key_mask == 0)[:, None, None, :], float("-inf"))
+        return (torch.softmax(t, -1) @ v).to(query.dtype)
+
+    monkeypatch.setattr(ac, "cross_attention", plain)
+    return seen
+
+
+def _layer(**more):
+    torch.manual_seed(0)
+    return spion_amd.CrossAttention(dict(transformer_dim=48, head_dim=32, num_head=4, num_key_head=2, **more))
+
+
+def _rand(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("half", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kept_under", [False, True])
+def test_states_kept_on_the_other_side_of_autocast(core, kept_under, half):
+    """Keys and values that were projected outside autocast serve a call under it, and the other way round; they stay as they are where the
+    core takes their type.  Off the fp32 layer by the roundings of a few values to the half type: 8 of them, of sums of sizes up to 4."""
+    layer = _layer()
+    X, states = _rand(1, 2, 3, 48), _rand(2, 2, 20, 48)
+    want = layer(X, states)
+    with torch.autocast("cpu", dtype=half, enabled=kept_under):
+        # (the layer asks for the GPU's autocast: as it projects under that)
+        kept = tuple(layer._split(w(states), 2) for w in (layer.W_k, layer.W_v))
+    assert kept[0].dtype == (half if kept_under else torch.float32)
+    core.clear()
+    with torch.autocast("cpu", dtype=half, enabled=not kept_under):
+        y = layer.attend(X, kept)
+    assert core == [torch.float32 if half == torch.float16 else kept[0].dtype]
+    assert y.dtype == (torch.float32 if kept_under else half)
+    assert float((y.float() - want).detach().abs().max()) <= 8 * torch.finfo(half).eps / 2 * 4
+
+
+def test_gradients_pass_the_change_of_type(core):
+    layer = _layer()
+    X, states = _rand(3, 2, 3, 48).requires_grad_(), _rand(4, 2, 20, 48)
+    kept = layer.keys_values(states)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        y = layer.attend(X, kept)
+    y.float().sum().backward()
+    assert X.grad.dtype == torch.float32 and bool(X.grad.any()) and bool(layer.W_k.weight.grad.any())
