@@ -99,6 +99,13 @@ def _observed(d):
         or "forward" in d
 
 
+def plain_projections(*modules):
+    """Whether the modules are linear layers with a bias that nobody has changed or watches, so that a product of their
+    weights is what they give (an adapter or a hook that makes the weight, as weight_norm's, is not in ``weight``)."""
+    return not _nn_module._has_any_global_hook() and all(
+        type(m) is nn.Linear and not _observed(m.__dict__) and m.bias is not None for m in modules)
+
+
 class Attention(nn.Module):
     def __init__(self, config, inference=False):
         super().__init__()

@@ -21,6 +21,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .attention import plain_projections
 from .relative_bias import _Heads, _heads
 
 
@@ -247,8 +248,10 @@ class CrossAttention(nn.Module):
         return X.reshape(X.shape[0], X.shape[1], heads, self.head_dim).transpose(1, 2)
 
     def keys_values(self, states):
-        """(key, value) [B, num_key_head, Lk, head_dim] of an encoder's states."""
-        if states.dtype == self.W_k.weight.dtype and not torch.is_autocast_enabled():
+        """(key, value) [B, num_key_head, Lk, head_dim] of an encoder's states: one product where the projections are linear layers as they
+        are, else what the modules give."""
+        if plain_projections(self.W_k, self.W_v) and states.dtype == self.W_k.weight.dtype == self.W_v.weight.dtype \
+                and not torch.is_autocast_enabled():
             return _FusedKV.apply(states, self.W_k.weight, self.W_v.weight, self.W_k.bias, self.W_v.bias, self.num_key_head, self.head_dim)
         return self._split(self.W_k(states), self.num_key_head), self._split(self.W_v(states), self.num_key_head)
 

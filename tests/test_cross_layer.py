@@ -66,3 +66,53 @@ def test_gradients_pass_the_change_of_type(core):
         y = layer.attend(X, kept)
     y.float().sum().backward()
     assert X.grad.dtype == torch.float32 and bool(X.grad.any()) and bool(layer.W_k.weight.grad.any())
+
+
+class _Adapted(torch.nn.Linear):
+    """A projection with a term of its own, and a ``weight`` that is only part of it."""
+
+    def forward(self, x):
+        return super().forward(x) + x.sum(-1, keepdim=True)
+
+
+def _replaced(layer, how):
+    """What a program does to a projection of keys or values; returns the projection."""
+    old = layer.W_v
+    if how == "adapter":
+        layer.W_v = _Adapted(old.in_features, old.out_features)
+    elif how == "no bias":
+        layer.W_v = torch.nn.Linear(old.in_features, old.out_features, bias=False)
+    elif how == "weight norm":
+        torch.nn.utils.weight_norm(old)  # (its weight is made by a hook ahead of the module's forward)
+        with torch.no_grad():
+            old.weight_g.mul_(3.0)
+    elif how == "parametrized":
+        torch.nn.utils.parametrizations.orthogonal(old)
+    elif how == "hook":
+        old.register_forward_hook(lambda m, i, o: 2 * o)
+    elif how == "own forward":
+        old.forward = lambda x: torch.nn.functional.linear(x, old.weight) - 1
+    return layer.W_v
+
+
+@pytest.mark.filterwarnings("ignore:.*weight_norm.*")
+@pytest.mark.parametrize("how", ["plain", "adapter", "no bias", "weight norm", "parametrized", "hook", "own forward"])
+def test_projections_are_the_modules_own(how):
+    """keys_values is what the layer's projections give, whatever a program has made of them (64-bit states: no rounding to speak of)."""
+    layer = _layer().double()
+    of_values = _replaced(layer, how).double()
+    states = _rand(5, 2, 20, 48).double()
+    k, v = layer.keys_values(states)
+    for got, module in ((k, layer.W_k), (v, of_values)):
+        assert torch.allclose(got, module(states).view(2, 20, 2, 32).transpose(1, 2), atol=1e-12)
+
+
+def test_global_hooks_see_the_projections():
+    layer = _layer()
+    seen = []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, i, o: seen.append(m) and None)
+    try:
+        layer.keys_values(_rand(6, 2, 20, 48))
+    finally:
+        handle.remove()
+    assert layer.W_k in seen and layer.W_v in seen
