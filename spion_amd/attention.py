@@ -174,7 +174,8 @@ class Attention(nn.Module):
                 return done
         if node is not None:
             Q, K, V = self._in_node(node.project_heads, X, *weights[:6], self.num_head, self.head_dim)
-        elif self.fused_qkv and X.dtype == torch.float32 and not torch.is_autocast_enabled():
+        elif self.fused_qkv and X.dtype == torch.float32 and not torch.is_autocast_enabled() \
+                and plain_projections(self.W_q, self.W_k, self.W_v):
             Q, K, V = _FusedQKV.apply(X, self.W_q.weight, self.W_k.weight, self.W_v.weight, self.W_q.bias,
                                       self.W_k.bias, self.W_v.bias, self.num_head, self.head_dim)
         else:
