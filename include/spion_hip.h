@@ -577,6 +577,8 @@ int spion_rms_norm_backward(const spion_rms_norm* call, void* stream);
  *   heads        Q, Out, dO, dQ [B][heads][q_len][d], K, V, dK, dV [B][key_heads][k_len][d]: tensors or views, strides in elements,
  *                multiples of 16 bytes; pointers 16-byte aligned; d = 32, 64 or 128.  The strides of tensors that are only read may
  *                be 0.  Rows lie up to 2^24 bytes apart, a head of keys and the heads of queries that share it within 2^31 bytes.
+ *   sizes        up to 2^29 keys, and queries of the heads that share them; batch * key_heads strips of 128 of either, fewer than 2^24
+ *                in all (a launch holds no more).
  *   key_mask     null, or [batch][k_len] floats (mask_bytes 4) or bytes (1): keys with a 0 are left out, and nothing of their K and V
  *                is used.  A row without any key has an Out of 0 and no gradients.
  *   Lse          [batch * heads][q_len] fp32, out of the forward and into the backward: log2 Z_i, +infinity for empty rows, NaN

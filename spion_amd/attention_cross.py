@@ -157,8 +157,8 @@ def _check(query, key, value, key_mask):
 def cross_attention(query, key, value, key_mask=None):
     """Attention of query [B, H, Lq, d] to key and value [B, G, Lk, d]; gradients for all three.
 
-    fp32 or bf16, d 32, 64 or 128, any lengths, tensors or views (views of projections, and expanded ones, are read in place).  H is a
-    multiple of G: heads g H/G .. (g + 1) H/G - 1 of the query share head g of key and value.  key_mask [B, Lk]: keys with a 0 are
+    fp32 or bf16, d 32, 64 or 128, lengths up to 2^29 (the header has the limits of a launch), tensors or views (views of projections, and
+    expanded ones, are read in place).  H is a multiple of G: heads g H/G .. (g + 1) H/G - 1 of the query share head g of key and value.  key_mask [B, Lk]: keys with a 0 are
     left out, whatever they hold (bool, or any type, compared with 0); a row without keys gives zeros.  Infinities among fp32
     operands that take part, and values of 2^127 and more, give NaN."""
     node = _lib.autograd_node()

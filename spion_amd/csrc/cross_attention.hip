@@ -15,6 +15,9 @@ static long long tiles_of(long long rows, long long tile = 32) { return (rows + 
 static int each_of(const Cross& c) { return c.heads / c.key_heads; }
 static long long rows_of(const Cross& c) { return (long long)each_of(c) * c.q_len; }
 
+// Work-groups of 256 threads that a launch holds (2^32 threads and more are refused by the runtime, in the middle of a call).
+constexpr long long CROSS_MOST_GROUPS = (1 << 24) - 1;
+
 // How one side of a call is walked: in strips of 128 rows over shared stages, or of 32 with the tiles dealt to the wavefronts, and the
 // other side in `splits` pieces.
 enum class CrossPass { FORWARD, ROW, COL };
@@ -51,6 +54,7 @@ static CrossWalk cross_walk_of(const Cross& c, CrossPass pass, bool can_split) {
         const long long strips = tiles_of(own, rows), steps = tiles_of(tiles, few ? 4 : unit);
         const double us = cross_tile_us(c, pass, few) * (few ? 1 : unit);
         const bool two = c.bf16 ? !few || c.head_dim < 128 : c.head_dim == 32;  // (two work-groups' registers fit a CU)
+        if (groups * strips > CROSS_MOST_GROUPS) continue;  // (strips of 128 are few enough: cross_sizes_ok)
         for (long long n = 1; n == 1 || (can_split && n <= std::min(steps / 2, 64LL) && groups * strips * n <= 8 * cus); ++n) {
             const long long rounds = tiles_of(groups * strips * n, cus), each = tiles_of(steps, n);
             double cost = 3 + rounds * each * us * (rounds > 1 && two ? 0.8 : 1.);
@@ -78,9 +82,6 @@ static long long cross_floats(const Cross& c, bool backward) {
     return ((groups * rows + 3) & ~3LL) + std::max(a, b);  // D, rounded up to whole pieces of 16 bytes, and the pieces
 }
 
-// Work-groups of 256 threads that a launch holds (2^32 threads and more are refused by the runtime, in the middle of a call).
-constexpr long long CROSS_MOST_GROUPS = (1 << 24) - 1;
-
 static bool cross_sizes_ok(const char* who, const Cross& c) {
     if (c.batch < 1 || c.heads < 1 || c.key_heads < 1 || c.q_len < 1 || c.k_len < 1) {
         set_error("%s: sizes are positive", who);
@@ -99,8 +100,8 @@ static bool cross_sizes_ok(const char* who, const Cross& c) {
         return false;
     }
     const long long groups = (long long)c.batch * c.key_heads;
-    if (groups > CROSS_MOST_GROUPS || groups * tiles_of(std::max<long long>(rows_of(c), c.k_len)) > CROSS_MOST_GROUPS) {
-        set_error("%s: too many heads and rows for one launch", who);
+    if (groups > CROSS_MOST_GROUPS || groups * tiles_of(std::max<long long>(rows_of(c), c.k_len), 128) > CROSS_MOST_GROUPS) {
+        set_error("%s: too many heads and rows for one launch: 2^24 strips of 128 rows, or of 128 keys", who);
         return false;
     }
     if (c.key_mask && c.mask_bytes != 1 && c.mask_bytes != 4) {
