@@ -45,10 +45,13 @@ def _lib_typed():
 
 
 def _fits(t, together):
-    """Whether the kernels read ``t`` in place; ``together`` heads of it are reached from one address."""
-    if _lib.head_layout(t) is None or t.stride(2) * t.element_size() > 1 << 24:
+    """Whether the kernels read ``t`` in place (strides and address of 16 bytes, rows up to 2^24 bytes apart); ``together`` heads of it, within
+    2^31 bytes, are reached from one address."""
+    sb, sh, sl, sf = t.stride()
+    e = t.element_size()
+    if sf != 1 or t.data_ptr() % 16 or any(s < 0 or s * e % 16 for s in (sb, sh, sl)) or not t.shape[3] <= sl <= (1 << 24) // e:
         return False
-    return ((together - 1) * t.stride(1) + (t.shape[2] - 1) * t.stride(2) + t.shape[3]) * t.element_size() < 1 << 31
+    return ((together - 1) * sh + (t.shape[2] - 1) * sl + t.shape[3]) * e < 1 << 31
 
 
 def _readable(t, together=1):

@@ -476,13 +476,15 @@ std::vector<Tensor> layer_norm(const Tensor& x, const Tensor& weight, const c10:
 }
 
 // ---- attention to keys of another length ------------------------------------------------------------------------------
-// Heads as the kernels read them: themselves, or a copy where their strides or address are not theirs.  `together` heads are reached
-// from one address.
+// Heads as the kernels read them: themselves, or a copy where their strides or address are not theirs (multiples of 16 bytes, rows up to
+// 2^24 bytes apart).  `together` heads, within 2^31 bytes, are reached from one address.
 Tensor readable_group(const Tensor& t, int64_t together) {
-    spion_head_layout lay{};
     const auto fits = [&](const Tensor& x) {
-        return head_layout(x, lay) && x.stride(2) * x.element_size() <= 1 << 24 &&
-               ((together - 1) * x.stride(1) + (x.size(2) - 1) * x.stride(2) + x.size(3)) * (int64_t)x.element_size() < int64_t(1) << 31;
+        const int64_t sb = x.stride(0), sh = x.stride(1), sl = x.stride(2), d = x.size(3), e = x.element_size();
+        if (x.stride(3) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 || sb < 0 || sh < 0 || sb * e % 16 || sh * e % 16 || sl * e % 16 ||
+            sl < d || sl * e > 1 << 24)
+            return false;
+        return ((together - 1) * sh + (x.size(2) - 1) * sl + d) * e < int64_t(1) << 31;
     };
     if (fits(t)) return t;
     const Tensor c = t.contiguous();

@@ -2,6 +2,7 @@
 import ctypes
 
 import pytest
+import torch
 
 from spion_amd import _lib
 from spion_amd import attention_cross as ac
@@ -29,3 +30,14 @@ def test_calls_of_as_many_strips_of_128_are_refused(sizes):
         assert _workspace(backward, batch=1 << 17, **sizes) == -1
         with pytest.raises(_lib.SpionLibraryError, match="strips"):
             _lib.check_error()
+
+
+@pytest.mark.parametrize("dtype,H,d", [(torch.bfloat16, 8, 128), (torch.float32, 4, 128), (torch.bfloat16, 2, 32), (torch.float32, 1, 64)])
+def test_long_heads_are_read_in_place(dtype, H, d):
+    """Heads within 2^31 bytes, in either order: what the library takes is not copied ahead of it."""
+    most = (1 << 31) // (H * d * dtype.itemsize)
+    for L, fits in ((most // 2, True), (most - 1, True), (most + 1, False)):
+        assert ac._fits(torch.empty(1, L, H, d, dtype=dtype, device="meta").transpose(1, 2), 1) == fits, L
+    most = (1 << 31) // (d * dtype.itemsize)
+    for L, together, fits in ((most // 2, 1, True), (most - 1, 1, True), (most + 1, 1, False), (most // 2 + 1, 2, False)):
+        assert ac._fits(torch.empty(1, 2 * H, L, d, dtype=dtype, device="meta"), together) == fits, L
