@@ -581,6 +581,9 @@ int spion_rms_norm_backward(const spion_rms_norm* call, void* stream);
  *                in all (a launch holds no more).
  *   key_mask     null, or [batch][k_len] floats (mask_bytes 4) or bytes (1): keys with a 0 are left out, and nothing of their K and V
  *                is used.  A row without any key has an Out of 0 and no gradients.
+ *   roundings    bf16 results are rounded once.  P and dS are rounded to bf16 for their products, which leaves results off by some 1.4 of their
+ *                own rounding.  They go as the sum of two bf16 numbers, and leave that rounding alone, where up to 32 queries share a head
+ *                of keys; so does dS (for dQ and dK) in calls with a k_len up to 256, however many keys a mask leaves.
  *   Lse          [batch * heads][q_len] fp32, out of the forward and into the backward: log2 Z_i, +infinity for empty rows, NaN
  *                where a logit that takes part is one.
  *   workspace    spion_cross_workspace(call, backward) floats, 16-byte aligned, contents unspecified; a forward without it walks

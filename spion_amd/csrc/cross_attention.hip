@@ -200,7 +200,8 @@ struct CrossRun {
     static bool backward(const Cross& c, hipStream_t stream) {
         constexpr bool BF16 = sizeof(T) == 2;
         // dS in two bf16 numbers up to 256 keys, where the rounding of O in D shows (128 heads of 1024 x 256: d = 64 81 us, and 77 without; d = 128 137 and
-        // 128; of 512, where it shows no more, 121 and 109)
+        // 128; of 512, where it shows no more, 121 and 109).  By the keys there are: the host does not know how many a mask leaves.  dV has no D in it
+        // and takes P in one number.
         const bool fine = BF16 && c.k_len <= 256;
         CrossCall a = cross_device_call(c);
         const long long groups = (long long)a.B * a.G;
