@@ -496,9 +496,9 @@ __device__ __forceinline__ void cross_rest(float (&p)[16]) {
         p[r + 1] -= bf16_hi(hi);
     }
 }
-// out += X^T . W of bf16 tiles with W as the sum of two bf16 numbers (fp32: of three, as everywhere).  Calls of few rows wait for memory, so that
-// the second product and its 40 vector instructions cost nothing there (one token over 2048 keys 8.6 us with either), and the
-// rounding of the weights is gone from their results: errors of 0.0017, that of the result's own rounding, against 0.0025.
+// out += X^T . W of bf16 tiles with W as the sum of two bf16 numbers (fp32 tiles have three images, and no second product here).  bf16 calls of a token
+// wait for memory, so that the second product and its 40 vector instructions cost nothing there (2048 keys 8.6 us with either); it goes with every
+// strip of 32, and the rounding of the weights is gone from their results: errors of 0.0017, that of the result's own rounding, against 0.0024.
 template <class TL, class Columns, int N>
 __device__ __forceinline__ void cross_add_fine(const Columns& xt, const float (&p)[16], f32x16 (&out)[N]) {
     TL::add_t(xt, p, out);
@@ -930,9 +930,10 @@ __global__ __launch_bounds__(256) void cross_merge_row_kernel(CrossCall a) {
 // Backward of few rows, in one pass over the keys
 // -------------------------------------------------------------------------------------------------
 // All rows of a group in one strip of 32: a tile's dK and dV are then whole after its own products, and K and V are read once for
-// all three gradients (the two passes read them twice: 64 fp32 heads of 4096 padded keys, 16 rows, d = 32: the training step 82 us, so 66).  dQ wants the
+// all three gradients (the two passes read them twice: 64 fp32 heads of 4096 padded keys, 16 rows, d = 32: the training step 82 us then, and 66).  dQ wants the
 // rows as lanes and dK, dV the keys, so both products over the head dimension are formed twice, with their operands exchanged: they
-// lie in registers either way.  Every wavefront takes every fourth tile, leaves its dK and dV and keeps dQ; bound by memory.
+// lie in registers either way.  Every wavefront takes every fourth tile, leaves its dK and dV and keeps dQ.  Bound by a tile's work, seven products of 32 rows
+// however many there are, rather than by memory: those heads take 34 us, 3.4 TB/s, and in bf16 20 us for half of the bytes.
 template <class T, int D>
 constexpr int cross_few_region() {  // a wavefront's tiles of K and V, then its results on their way out
     const int tiles = cross_own_tiles<T, D>() * BiasTile<T, D>::BYTES, out = 32 * (D + 4) * 4;

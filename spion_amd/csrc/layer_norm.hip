@@ -10,8 +10,8 @@
 // less to keep) in two reductions of two sums each.  Rows longer than the registers are read again for each step (from L2).  Statistics
 // and sums are fp32.  Work-groups walk several rows each: the weight is read once, and the backward leaves one partial dw and db a
 // work-group, which a second launch adds up in a fixed order.  With a residual, us (bytes moved to the time, TB/s): 262144 x 64 fp32 forward 44
-// (6.1, part of it from the cache), backward 45 + 4 for dw and db; 8192 x 4096 bf16 47 (5.7) and 61 + 9; 16384 x 1001 bf16, forward alone,
-// 17 (3.9); one row of 768 2.8, the launch.
+// (6.1, part of it from the cache), backward 44 + 4 for dw and db; 8192 x 4096 bf16 46 (5.8) and 58 to 61 + 9; 16384 x 1001 bf16, forward alone,
+// 15 to 17 (3.9 to 4.3); one row of 768 3, the launch.
 #include "common.h"
 #include "tile_ops.h"
 #include "../../include/spion_hip.h"
@@ -39,7 +39,7 @@ typedef unsigned word_anywhere __attribute__((aligned(2)));
 
 // Elements i .. i + V - 1 of a row of n, those behind its end zeros: the words as they come from memory, so that nothing waits for them
 // before all of a row's pieces are asked for, and then as floats.  (Converted where they are loaded, each piece waited for its own: backward
-// of 8192 x 4096 bf16 107 us against 52.)
+// of 8192 x 4096 bf16 107 us against 60.)
 template <class T>
 struct RowWords {
     static constexpr int V = 16 / sizeof(T);
